@@ -198,6 +198,117 @@ int mako_attn_decode_noalloc(const mako_decode_args* a, mako_dtype in, mako_dtyp
                              const void* v, const uint32_t* ctx_len, void* o, float* lse, void* stream);
 
 /*
+ * Attention of drafted tokens over a cache (speculative decoding): each sequence attends n_draft rows at once, the nodes
+ * of a tree of drafts, before any of them is in the cache. No counterpart in the reference (it decodes one token of one
+ * sequence at a time). Row b * n_draft + r is node r of sequence b, the rows mako_heads writes for the drafts of all
+ * sequences one after another: q [heads][q_pad][dim], kd, vd [kv_heads][d_pad][dim], o [batch * n_draft][width],
+ * lse [heads][batch * n_draft] (may be NULL); k, v [batch][kv_heads][cap][dim], the cache of mako_attn_decode.
+ * Node r of sequence b sees the cache rows [0, min(ctx_len[b], max_ctx)) and the drafts j < n_nodes[b] with bit j of
+ * mask[b * n_draft + r] set (its ancestors and itself, where the caller sets its bit; mask NULL: the drafts j <= r, a
+ * chain). A node that sees nothing gives 0 and lse = -inf. n_nodes (u32 [batch], NULL: n_draft each): rows of o and lse
+ * from n_nodes[b] on are left as they were. ctx_len, n_nodes and mask are in device memory. A key that a node does
+ * not see has no part in its row, whatever its k and v hold (infinities and NaN too), nor has a cache row past ctx_len.
+ * dim 64, 128 or 256, n_draft at most 64, width a multiple of 4. o must not overlap the inputs.
+ * Precision: scores, sums and lse in f32; the probabilities meet V in V's own type, f16 with 11 bits for f16 tiles and
+ * f16 output, else as the sum of two values of the type (bf16: 16 bits; f16: 21), so that the output's rounding is the
+ * one that counts. workspace: at least mako_attn_tree_workspace(a) bytes, 16-byte aligned; its contents do not matter,
+ * and calls that overlap in time need separate ones.
+ */
+typedef struct mako_tree_args {
+    uint32_t batch;   /* sequences */
+    uint32_t n_draft; /* rows a sequence: at most 64 */
+    uint32_t q_pad;   /* rows of a query head in q (>= batch * n_draft) */
+    uint32_t d_pad;   /* rows of a kv head in kd and vd (>= batch * n_draft) */
+    uint32_t heads, kv_heads;
+    uint32_t dim;     /* 64, 128 or 256 */
+    uint32_t cap;     /* rows of a kv head of one sequence in the cache */
+    uint32_t max_ctx; /* an upper bound on every ctx_len[b] (<= cap) */
+    uint32_t width;   /* o row length in elements (>= heads * dim) */
+    float scale;
+} mako_tree_args;
+
+size_t mako_attn_tree_workspace(const mako_tree_args* a);
+int mako_attn_tree(const mako_tree_args* a, mako_dtype in, mako_dtype out, const void* q, const void* k, const void* v,
+                   const void* kd, const void* vd, const uint32_t* ctx_len, const uint32_t* n_nodes,
+                   const uint64_t* mask, void* o, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Appends rows to the cache: of sequence b, the draft rows path[b * n_draft + i], i < n_path[b], in that order (the
+ * accepted path of a tree; path NULL: rows 0, 1, ...; n_path NULL: n_draft rows each) become the cache rows
+ * ctx_len[b] + i of k and v, for every kv head; an entry at or past n_draft appends a row of zeros, and rows past cap are
+ * dropped. ctx_out[b] is the number of rows afterwards. Where given, w [batch][kv_heads][cap] (the rows' gathered
+ * weights) is 0 and pos [batch][kv_heads][cap] (their token positions) is seen[b] + i on the new rows, and seen_out[b]
+ * = seen[b] + the rows appended: seen counts a sequence's tokens, as ctx_len its rows, which fall behind once rows are
+ * evicted. ctx_out may be ctx_len and seen_out seen. kd and vd are not in k or v. No counterpart in the reference.
+ */
+typedef struct mako_append_args {
+    uint32_t batch, n_draft;
+    uint32_t d_pad; /* rows of a kv head in kd and vd (>= batch * n_draft) */
+    uint32_t kv_heads;
+    uint32_t dim;   /* 64, 128 or 256 */
+    uint32_t cap;
+} mako_append_args;
+
+int mako_cache_append(const mako_append_args* a, mako_dtype in, const void* kd, const void* vd, const uint32_t* path,
+                      const uint32_t* n_path, const uint32_t* ctx_len, uint32_t* ctx_out, const uint32_t* seen,
+                      uint32_t* seen_out, float* w, uint32_t* pos, void* k, void* v, void* stream);
+
+/*
+ * The attention weight that each cache row gathers, summed over queries and over the heads of a group:
+ *   w_out[b][kvh][j] = decay * w[b][kvh][j] + sum over h, i of exp(scale * q_i . k_j - lse_i),  j < ctx_len[b]
+ * over the n = n_path[b] queries of sequence b (n_path NULL: n_q each) that see row j: query i sits at cache row
+ * ctx_len[b] - n + i and sees the rows up to it (a whole prompt, a chunk, one token, an accepted path after its append).
+ * Query i of the sequence is row b * n_q + path[b * n_q + i] of q (path NULL: i; an entry at or past n_q is no query, the
+ * same entry twice is two), q [heads][q_pad][dim] and lse [heads][batch * n_q], the natural-log sums of the attention's
+ * call over the same rows (mako_attn_fwd's for one sequence, mako_attn_tree's for a tree); or with q_pad = 0
+ * q [batch][heads][n_q][dim] and lse [batch][heads][n_q], with n_q = 1 mako_attn_decode's. A query with lse = -inf saw
+ * nothing and adds nothing. k [batch][kv_heads][cap][dim]; w and w_out [batch][kv_heads][cap] (w NULL or decay 0: the
+ * sum alone; w_out may be w); rows of w_out from ctx_len[b] on are left as they were, and k's are not read as keys.
+ * dim 64, 128 or 256. Sums in f32, in an order that the arguments fix. workspace: mako_cache_weights_workspace(a) bytes,
+ * 16-byte aligned. No counterpart in the reference.
+ */
+typedef struct mako_weights_args {
+    uint32_t batch, n_q;
+    uint32_t q_pad;   /* rows of a query head in q (>= batch * n_q); 0: q and lse by sequence */
+    uint32_t heads, kv_heads;
+    uint32_t dim;     /* 64, 128 or 256 */
+    uint32_t cap;
+    uint32_t max_ctx; /* an upper bound on every ctx_len[b] (<= cap) */
+    float scale;
+    float decay;      /* finite, >= 0 */
+} mako_weights_args;
+
+size_t mako_cache_weights_workspace(const mako_weights_args* a);
+int mako_cache_weights(const mako_weights_args* a, mako_dtype in, const void* q, const float* lse, const void* k,
+                       const uint32_t* ctx_len, const uint32_t* path, const uint32_t* n_path, const float* w,
+                       float* w_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Evicts cache rows down to a budget. Of each (sequence, kv head) with more than `budget` rows, budget rows stay: first
+ * the protected ones, of tokens pos < sinks or pos >= seen[b] - recent, then by w, the largest first; ties go to the
+ * lower row, and NaN counts as -inf. Rows move as little as possible: the i-th kept row at or past `budget` goes into
+ * the i-th row below it that is given up, so the order of rows is not that of tokens afterwards (the cached keys carry
+ * their rotation, and attention over a cache takes its rows in any order); pos tells each row's token. k and v
+ * [batch][kv_heads][cap][dim] in place; w_out and pos_out [batch][kv_heads][cap] get rows below min(ctx_len[b], budget),
+ * ctx_out[b] is that number. The rows behind are left as they were, so a call whose outputs are not its inputs can be
+ * made again. pos and seen NULL: row j is token j, seen[b] = ctx_len[b]. w_out may be w, pos_out pos, ctx_out ctx_len.
+ * recent + sinks at most budget. workspace: mako_cache_evict_workspace(a) bytes, 16-byte aligned. No counterpart in the
+ * reference.
+ */
+typedef struct mako_evict_args {
+    uint32_t batch, kv_heads;
+    uint32_t dim;     /* 64, 128 or 256 */
+    uint32_t cap;
+    uint32_t max_ctx; /* an upper bound on every ctx_len[b] (<= cap) */
+    uint32_t budget, recent, sinks;
+} mako_evict_args;
+
+size_t mako_cache_evict_workspace(const mako_evict_args* a);
+int mako_cache_evict(const mako_evict_args* a, mako_dtype in, void* k, void* v, const float* w, const uint32_t* pos,
+                     const uint32_t* seen, const uint32_t* ctx_len, float* w_out, uint32_t* pos_out, uint32_t* ctx_out,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Head tiles from fp32 rows: head h of token t, x[t][col0 + h * stride .. + dim), written as y row
  * [h][row0 + t][dim] in f16 (the reference's half tiles) or bf16, optionally RMS-normed (times w) and then rotated by
  * the angle table cs. One call stands for each of the reference's tile producers (src/kernels/ops.metal:11-52,

@@ -21,7 +21,8 @@ EXPORTS = ("mako_attn_abi_version", "mako_last_error", "mako_attn_fwd", "mako_cu
            "mako_proj_bf16_workspace", "mako_proj_bf16_ws", "mako_kda_scan", "mako_kda_scan_workspace",
            "mako_kda_scan_ws", "mako_attn_fwd_workspace", "mako_attn_fwd_ws", "mako_attn_sparse_workspace",
            "mako_attn_sparse_ws", "mako_attn_fwd_rows_workspace", "mako_attn_fwd_rows_ws", "mako_attn_release",
-           "mako_attn_held_bytes")
+           "mako_attn_held_bytes", "mako_attn_tree_workspace", "mako_attn_tree", "mako_cache_append",
+           "mako_cache_weights_workspace", "mako_cache_weights", "mako_cache_evict_workspace", "mako_cache_evict")
 
 
 class AttnArgs(ctypes.Structure):
@@ -38,6 +39,25 @@ class SparseArgs(ctypes.Structure):
 class DecodeArgs(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint32) for n in ("batch", "heads", "kv_heads", "dim", "cap", "max_ctx", "split")] + \
         [("scale", ctypes.c_float)]
+
+
+class TreeArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("batch", "n_draft", "q_pad", "d_pad", "heads", "kv_heads", "dim", "cap",
+                                               "max_ctx", "width")] + [("scale", ctypes.c_float)]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("batch", "n_draft", "d_pad", "kv_heads", "dim", "cap")]
+
+
+class WeightsArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("batch", "n_q", "q_pad", "heads", "kv_heads", "dim", "cap",
+                                               "max_ctx")] + [("scale", ctypes.c_float), ("decay", ctypes.c_float)]
+
+
+class EvictArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("batch", "kv_heads", "dim", "cap", "max_ctx", "budget", "recent",
+                                               "sinks")]
 
 
 class HeadsArgs(ctypes.Structure):
@@ -121,7 +141,18 @@ def lib():
         L.mako_attn_release.argtypes = [P]
         L.mako_attn_held_bytes.argtypes = []
         L.mako_attn_held_bytes.restype = SZ
-        for name in ("mako_attn_fwd", "mako_cube_select", "mako_attn_sparse", "mako_attn_decode",
+        L.mako_attn_tree_workspace.argtypes = [ctypes.POINTER(TreeArgs)]
+        L.mako_attn_tree_workspace.restype = SZ
+        L.mako_attn_tree.argtypes = [ctypes.POINTER(TreeArgs), I, I] + [P] * 11 + [SZ, P]
+        L.mako_cache_append.argtypes = [ctypes.POINTER(AppendArgs), I] + [P] * 13
+        L.mako_cache_weights_workspace.argtypes = [ctypes.POINTER(WeightsArgs)]
+        L.mako_cache_weights_workspace.restype = SZ
+        L.mako_cache_weights.argtypes = [ctypes.POINTER(WeightsArgs), I] + [P] * 9 + [SZ, P]
+        L.mako_cache_evict_workspace.argtypes = [ctypes.POINTER(EvictArgs)]
+        L.mako_cache_evict_workspace.restype = SZ
+        L.mako_cache_evict.argtypes = [ctypes.POINTER(EvictArgs), I] + [P] * 10 + [SZ, P]
+        for name in ("mako_attn_tree", "mako_cache_append", "mako_cache_weights", "mako_cache_evict",
+                     "mako_attn_fwd", "mako_cube_select", "mako_attn_sparse", "mako_attn_decode",
                      "mako_attn_decode_noalloc", "mako_heads", "mako_attn_fwd_rows", "mako_attn_fwd_ws",
                      "mako_attn_sparse_ws", "mako_attn_fwd_rows_ws", "mako_attn_release",
                      "mako_attn_pv", "mako_attn_gather_scores", "mako_attn_gather_pv", "mako_idx_dots",
@@ -256,6 +287,75 @@ def attn_decode_noalloc(a, q, k, v, ctx_len, o, *, lse=None, stream=None):
 
 
 DECODE_SCRATCH_BYTES = 16 << 20  # MAKO_DECODE_SCRATCH_BYTES
+
+
+def tree_args(*, batch, n_draft, heads, kv_heads, dim, cap, max_ctx, q_pad=None, d_pad=None, width=None, scale=None):
+    rows = batch * n_draft
+    return TreeArgs(batch, n_draft, rows if q_pad is None else q_pad, rows if d_pad is None else d_pad, heads, kv_heads,
+                    dim, cap, max_ctx, heads * dim if width is None else width,
+                    1.0 / dim ** 0.5 if scale is None else scale)
+
+
+def attn_tree_workspace(a):
+    return lib().mako_attn_tree_workspace(ctypes.byref(a))
+
+
+def attn_tree(a, q, k, v, kd, vd, ctx_len, o, workspace, *, n_nodes=None, mask=None, lse=None, stream=None):
+    """mako_attn_tree on torch tensors: q [heads][q_pad][dim], k, v [batch][kv_heads][cap][dim], kd, vd
+    [kv_heads][d_pad][dim], ctx_len / n_nodes int32 [batch] (read as u32), mask int64 [batch][n_draft] (read as u64),
+    o [batch * n_draft][width], lse float32 [heads][batch * n_draft]."""
+    _check(lib().mako_attn_tree(ctypes.byref(a), dtype_code(q), dtype_code(o), _ptr(q), _ptr(k), _ptr(v), _ptr(kd),
+                                _ptr(vd), _ptr(ctx_len), _ptr(n_nodes), _ptr(mask), _ptr(o), _ptr(lse),
+                                _ptr(workspace), _nbytes(workspace), _stream(stream)))
+
+
+def append_args(*, batch, n_draft, kv_heads, dim, cap, d_pad=None):
+    return AppendArgs(batch, n_draft, batch * n_draft if d_pad is None else d_pad, kv_heads, dim, cap)
+
+
+def cache_append(a, kd, vd, k, v, ctx_len, ctx_out, *, path=None, n_path=None, seen=None, seen_out=None, w=None,
+                 pos=None, stream=None):
+    """mako_cache_append on torch tensors: kd, vd [kv_heads][d_pad][dim], k, v [batch][kv_heads][cap][dim], path int32
+    [batch][n_draft], n_path, ctx_len, ctx_out, seen, seen_out int32 [batch], w float32 and pos int32
+    [batch][kv_heads][cap]."""
+    _check(lib().mako_cache_append(ctypes.byref(a), dtype_code(k), _ptr(kd), _ptr(vd), _ptr(path), _ptr(n_path),
+                                   _ptr(ctx_len), _ptr(ctx_out), _ptr(seen), _ptr(seen_out), _ptr(w), _ptr(pos),
+                                   _ptr(k), _ptr(v), _stream(stream)))
+
+
+def weights_args(*, batch, n_q, heads, kv_heads, dim, cap, max_ctx, q_pad=None, decode=False, scale=None, decay=1.0):
+    """decode: q [batch][heads][n_q][dim] and lse [batch][heads][n_q] (q_pad 0)."""
+    return WeightsArgs(batch, n_q, 0 if decode else batch * n_q if q_pad is None else q_pad, heads, kv_heads, dim, cap,
+                       max_ctx, 1.0 / dim ** 0.5 if scale is None else scale, decay)
+
+
+def cache_weights_workspace(a):
+    return lib().mako_cache_weights_workspace(ctypes.byref(a))
+
+
+def cache_weights(a, q, lse, k, ctx_len, w_out, workspace, *, w=None, path=None, n_path=None, stream=None):
+    """mako_cache_weights on torch tensors: q [heads][q_pad][dim] and lse float32 [heads][batch * n_q] (or by sequence,
+    as weights_args says), k [batch][kv_heads][cap][dim], ctx_len / n_path int32 [batch], path int32 [batch][n_q], w and
+    w_out float32 [batch][kv_heads][cap]."""
+    _check(lib().mako_cache_weights(ctypes.byref(a), dtype_code(q), _ptr(q), _ptr(lse), _ptr(k), _ptr(ctx_len),
+                                    _ptr(path), _ptr(n_path), _ptr(w), _ptr(w_out), _ptr(workspace),
+                                    _nbytes(workspace), _stream(stream)))
+
+
+def evict_args(*, batch, kv_heads, dim, cap, max_ctx, budget, recent=0, sinks=0):
+    return EvictArgs(batch, kv_heads, dim, cap, max_ctx, budget, recent, sinks)
+
+
+def cache_evict_workspace(a):
+    return lib().mako_cache_evict_workspace(ctypes.byref(a))
+
+
+def cache_evict(a, k, v, w, ctx_len, w_out, pos_out, ctx_out, workspace, *, pos=None, seen=None, stream=None):
+    """mako_cache_evict on torch tensors: k, v [batch][kv_heads][cap][dim] in place, w and w_out float32, pos and pos_out
+    int32 [batch][kv_heads][cap], ctx_len, ctx_out and seen int32 [batch]."""
+    _check(lib().mako_cache_evict(ctypes.byref(a), dtype_code(k), _ptr(k), _ptr(v), _ptr(w), _ptr(pos), _ptr(seen),
+                                  _ptr(ctx_len), _ptr(w_out), _ptr(pos_out), _ptr(ctx_out), _ptr(workspace),
+                                  _nbytes(workspace), _stream(stream)))
 
 
 def window_random_blocks(n_blocks, lists, window=8, n_random=8, seed=0):
