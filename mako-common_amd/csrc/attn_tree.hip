@@ -3,118 +3,659 @@
 //
 // Mathematics: row r of sequence b, head h, with S the cache rows below ctx[b] and the drafts j < n_nodes[b] that r sees:
 //   o = sum_{j in S} exp(s_j - m) v_j / sum_{j in S} exp(s_j - m),  s_j = scale q.k_j,  lse = m + ln(sum),  m any bound
+// Sums over parts of S join by their maxima, so the keys are split over workgroups.
 //
-// tree_rows: one workgroup a row and head. Each wave takes every fourth key, its lanes the head dims, with a running
-// maximum; the waves meet in LDS. Every row reads its keys for itself.
-#include "device.hpp"
+// Bound: the read of K and V, once for all the rows and heads that share a kv head: the (row, head of the group) pairs
+// are the columns of S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16, 32 a wave. Past a few hundred columns the
+// matrix products bind.
+//
+// * A tile is 32 keys: of the cache, or of the drafts, whose tiles follow the cache's. A workgroup is NG column groups
+//   times KW key ways: wave w takes columns 32 (w % NG) .. and every KW-th tile; the NG waves of a way share its tiles,
+//   each staging 1 / NG of them. A step is KW tiles. More columns than 32 NG go to further workgroups (column blocks) on
+//   the same keys, next to each other on an XCD so that the second read hits its L2.
+// * Tiles come raw by LDS DMA into a ring of DEPTH steps, DEPTH - 1 of them in flight; one barrier a step (none with one
+//   column group, whose waves share nothing). K rows lie in slot order (bits 2 and 3 of the row swapped: the
+//   exponentiated scores are then the B operand of the P V product) with their 16-byte chunks XORed by the row, V rows
+//   with their 32-byte units permuted; V^T comes from transpose reads. Rows past the context or the tree lie outside the
+//   buffer descriptors and load zeros.
+// * Each row's mask word masks the draft tiles alone. Infinities and NaN of a draft's V must not reach the rows that do
+//   not see it (0 times them is NaN): a draft tile's are zeroed in LDS, and added to the rows that do at the end.
+// * The steps of all (sequence, kv head) segments, end to end, are cut into equal ranges, one a workgroup. Each overlap of
+//   a range and a segment is a piece; its ways join through LDS and leave one f32 partial a column at index range +
+//   segment (unique: pieces are intervals between consecutive boundaries), which tree_merge joins. Short contexts take a
+//   segment a workgroup and no merge.
+#include <algorithm>
+
+#include "lds_tiles.hpp"
 
 namespace mako {
 namespace {
+
+constexpr int kTK = 32;  // keys a tile
+constexpr float kRescale = 8.0f;
 
 struct TreeParams {
     const void *q, *k, *v, *kd, *vd;
     const uint32_t *ctx, *nodes;
     const uint64_t* mask;
+    float* part_o;   // [pieces][nc][D]
+    float* part_ml;  // [pieces][nc][2]: maximum (base 2), sum
+    uint32_t* part_odd;  // [pieces]: a draft's V holds what is not finite
     uint32_t batch, n_draft, q_pad, d_pad, heads, kv_heads, group, cap, max_ctx, width;
+    uint32_t nc, ncb;   // columns (n_draft x group), column blocks
+    uint32_t ways;      // tiles a step
+    uint32_t n_ranges;  // 0: a segment a workgroup
     float scale_log2;
 };
 
-constexpr int kRowWaves = 4;
+__device__ __forceinline__ uint32_t ctx_of(const TreeParams& p, uint32_t b) { return min(p.ctx[b], p.max_ctx); }
+__device__ __forceinline__ uint32_t nodes_of(const TreeParams& p, uint32_t b)
+{
+    return p.nodes ? min(p.nodes[b], p.n_draft) : p.n_draft;
+}
+// The drafts that node r of a tree of `nodes` sees.
+__device__ __forceinline__ uint64_t sees_of(const TreeParams& p, uint32_t b, uint32_t r, uint32_t nodes)
+{
+    return (p.mask ? p.mask[(size_t)b * p.n_draft + r] : (2ull << r) - 1) & (~0ull >> (64 - nodes));
+}
+__device__ __forceinline__ uint32_t steps_of(const TreeParams& p, uint32_t ctx, uint32_t nodes)
+{
+    return ((ctx + kTK - 1) / kTK + (nodes + kTK - 1) / kTK + p.ways - 1) / p.ways;
+}
+
+// A value the whole wave holds, in a scalar register.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane(x); }
+
+// The steps of a segment of sequences [0, n), summed; 64 sequences at a time.
+__device__ __forceinline__ uint32_t steps_before(const TreeParams& p, uint32_t n, uint32_t lane)
+{
+    uint32_t s = 0;
+    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+        const uint32_t i = i0 + lane;
+        uint32_t v = i < n ? steps_of(p, ctx_of(p, i), nodes_of(p, i)) : 0u;
+        #pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            v += __shfl_xor(v, o);
+        s += v;
+    }
+    return s;
+}
+
+// The sequence whose segments hold step x of all of them end to end (x below their sum), and its first step.
+__device__ __forceinline__ void seq_of(const TreeParams& p, uint32_t x, uint32_t lane, uint32_t& b, uint32_t& first)
+{
+    uint32_t base = 0;
+    for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
+        const uint32_t i = i0 + lane;
+        const uint32_t len = i < p.batch ? steps_of(p, ctx_of(p, i), nodes_of(p, i)) * p.kv_heads : 0u;
+        uint32_t inc = len;
+        #pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t t = __shfl_up(inc, o);
+            inc += lane >= (uint32_t)o ? t : 0u;
+        }
+        const uint64_t hit = __ballot(i < p.batch && x < base + inc);
+        if (hit) {
+            const uint32_t at = (uint32_t)__builtin_ctzll(hit);
+            b = i0 + at;
+            first = base + __shfl(inc - len, at);
+            return;
+        }
+        base += __shfl(inc, 63);
+    }
+    b = p.batch;
+    first = base;
+}
+
+// T steps cut into n equal ranges: range w starts at floor(w T / n), without a 64-bit division (w r < n^2 fits 32 bits).
+struct Ranges {
+    uint32_t T, n, q, r;
+    __device__ Ranges(uint32_t total, uint32_t ranges) : T(total), n(ranges), q(total / ranges), r(total % ranges) {}
+    __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * q + (w * r) / n; }
+    // The range that holds step x.
+    __device__ __forceinline__ uint32_t of(uint32_t x) const
+    {
+        uint32_t w = (uint32_t)(((uint64_t)x * n) / T);
+        while (w + 1 < n && start(w + 1) <= x)
+            ++w;
+        while (w > 0 && start(w) > x)
+            --w;
+        return w;
+    }
+};
+
+// The key in slot s of a tile's K image (its own inverse).
+__device__ __forceinline__ uint32_t slot_of(uint32_t s) { return (s & ~12u) | ((s & 4u) << 1) | ((s & 8u) >> 1); }
+
+// Where 16-byte chunk c of K row s sits in its LDS row: XORed so that the 16 rows a ds_read_b128 spans start in distinct
+// banks (rows of 128 bytes: two fill the 64 banks).
+template <int D>
+__device__ __forceinline__ uint32_t k_xor(uint32_t s)
+{
+    return D == 64 ? (s >> 1) & 7u : s & 15u;
+}
+
+// Where 32-byte unit u of V row k sits in its LDS row: the two units of the four rows that a transpose read's 32 lanes
+// address cover the 64 banks once (a bijection of the units; its own inverse up to the parity term).
+template <int D>
+__device__ __forceinline__ uint32_t v_unit(uint32_t u, uint32_t k)
+{
+    return D == 64 ? u ^ (k & 2u) : u ^ (k & 3u) ^ (4u * (u & 1u));
+}
+template <int D>
+__device__ __forceinline__ uint32_t v_unit_at(uint32_t pos, uint32_t k)
+{
+    if (D == 64)
+        return pos ^ (k & 2u);
+    const uint32_t x = pos ^ (k & 3u);
+    return x ^ (4u * (x & 1u));
+}
+
+// The exponent bits of a value of T: all set in an infinity or NaN.
+template <class T>
+constexpr uint32_t kExp = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+
+// What the drafts' infinities and NaN add to head dim d of row r: p v is v for p > 0.
+template <class T, int D>
+__device__ float odd_sum(const TreeParams& p, uint32_t b, uint32_t kvh, uint32_t r, uint32_t nodes, uint32_t d)
+{
+    const uint64_t sees = sees_of(p, b, r, nodes);
+    const T* v = static_cast<const T*>(p.vd) + ((size_t)kvh * p.d_pad + (size_t)b * p.n_draft) * D + d;
+    float x = 0.0f;
+    for (uint32_t j = 0; j < nodes; ++j) {
+        const T y = v[(size_t)j * D];
+        if (sees >> j & 1 && (__builtin_bit_cast(uint16_t, y) & kExp<T>) == kExp<T>)
+            x += (float)y;
+    }
+    return x;
+}
+
+// Waves, ways and ring depth by head dims and column groups: at most 128 KiB of tiles, one workgroup a CU.
+template <int D, int NG>
+struct Shape {
+    static constexpr int kSlot = 2 * kTK * 2 * D;  // a tile's K and V
+    static constexpr int kKW = D == 64 ? (NG == 1 ? 8 : NG == 2 ? 4 : 2) : D == 128 ? (NG == 4 ? 2 : 4) : NG == 4 ? 1 : 2;
+    static constexpr int kDepth = 128 * 1024 / (kSlot * kKW);
+    static constexpr int kWaves = NG * kKW;
+    static constexpr int kLds = kDepth * kKW * kSlot;
+    static_assert(kDepth >= 2 && kLds >= kWaves * 32 * D * 4, "a ring of two steps, and room for the waves' sums");
+};
+
+// Zeros the infinities and NaN of a V image of `bytes` in LDS (waves that share the tile may do so side by side: they
+// write the same); whether the wave found one.
+template <class T, int bytes>
+__device__ __forceinline__ bool finite_only(unsigned char* v, uint32_t lane)
+{
+    constexpr uint32_t e = kExp<T>;
+    bool found = false;
+    #pragma unroll 1
+    for (int i = 0; i < bytes; i += 1024) {
+        u32x4* at = reinterpret_cast<u32x4*>(v + i + 16 * lane);
+        u32x4 x = *at;
+        bool hit = false;
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool lo = (x[j] & e) == e, hi = (x[j] & e << 16) == e << 16;
+            hit = hit || lo || hi;
+            x[j] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+        }
+        if (hit)
+            *at = x;
+        found = found || hit;
+    }
+    return __any(found);
+}
+
+template <class T>
+__device__ __forceinline__ float value_of(uint32_t x, int i)
+{
+    const uint16_t h = (uint16_t)(i ? x >> 16 : x);
+    return (float)__builtin_bit_cast(T, h);
+}
+
+template <class T, class TO, int D, int NG>
+__global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves + 3) / 4)) void tree_split(
+    const TreeParams p, TO* __restrict__ o, float* __restrict__ lse)
+{
+    using S = Shape<D, NG>;
+    using E = Elem<T>;
+    using V8 = typename E::vec8;
+    constexpr bool kSplitP = __is_same(T, __bf16) || __is_same(TO, float);  // P as the sum of two values of T
+    constexpr int KW = S::kKW, ND = D / 32, NK = D / 16, W = S::kWaves;
+    constexpr int kRow = 2 * D, kHalf = kTK * kRow, kPieces = kHalf / 1024 / NG;  // 1 KiB pieces of K (of V) a wave
+    static_assert(kPieces >= 1, "every wave stages some");
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[S::kLds];
+    __shared__ float2 s_ml[W][32];
+    __shared__ uint32_t s_odd;  // a draft's V holds what is not finite
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c32 = lane & 31;
+    const uint32_t wl = uniform(tid >> 6), cg = wl % NG, kw = wl / NG;
+    uint32_t range = blockIdx.x, cb = 0;
+    if (p.ncb > 1) {  // the column blocks of a range 8 apart: one XCD
+        const uint32_t in = blockIdx.x % (8 * p.ncb);
+        range = blockIdx.x / (8 * p.ncb) * 8 + in % 8;
+        cb = in / 8;
+    }
+    const uint32_t n_seg = p.batch * p.kv_heads;
+    if (range >= (p.n_ranges ? p.n_ranges : n_seg))
+        return;
+
+    // This wave's DMA pieces: the bytes of the tile's rows that the lane's 16 LDS bytes hold.
+    uint32_t kd[kPieces], vd[kPieces];
+    #pragma unroll
+    for (int m = 0; m < kPieces; ++m) {
+        const uint32_t at = 1024 * (cg * kPieces + m) + 16 * lane, r = at / kRow, pos = at % kRow;
+        kd[m] = slot_of(r) * kRow + 16 * ((pos / 16) ^ k_xor<D>(r));
+        vd[m] = r * kRow + 32 * v_unit_at<D>(pos / 32, r) + (pos & 16);
+    }
+    const uint32_t lbase = uniform((uint32_t)reinterpret_cast<uintptr_t>(lds));
+    // K operand: row c32, chunk (2 kk + g) at its place; V^T operand: see v_unit (lane 4 j + y of a group of 16: head
+    // dims 16 (group % 2) + 4 y .. of key 8 g + j).
+    const uint32_t ka = c32 * kRow + 16 * (g ^ k_xor<D>(c32));
+    const uint32_t gj = (lane >> 2) & 3u, gy = lane & 3u, gg = (lane >> 4) & 1u;
+    constexpr int NV = D == 64 ? 2 : 4;
+    uint32_t va[NV];
+    #pragma unroll
+    for (int i = 0; i < NV; ++i)
+        va[i] = kHalf + (8 * g + gj) * kRow + 32 * v_unit<D>(2 * i + gg, gj) + 8 * gy;
+
+    // The first piece of the range (or the segment).
+    uint32_t b, kvh, s0, s1, left = 0;  // steps [s0, s1) of the segment; steps of the range behind them
+    if (p.n_ranges) {
+        const Ranges rg(uniform(steps_before(p, p.batch, lane) * p.kv_heads), p.n_ranges);
+        const uint32_t x0 = rg.start(range), x1 = rg.start(range + 1);
+        if (x0 >= x1)
+            return;
+        uint32_t first;
+        seq_of(p, x0, lane, b, first);
+        b = uniform(b);
+        const uint32_t len = uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b)));
+        kvh = (x0 - uniform(first)) / len;
+        s0 = (x0 - uniform(first)) % len;
+        s1 = min(len, s0 + (x1 - x0));
+        left = x1 - x0 - (s1 - s0);
+    } else {
+        b = range / p.kv_heads, kvh = range % p.kv_heads, s0 = 0;
+        s1 = uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b)));
+    }
+
+    for (;;) {
+        const uint32_t ctx = uniform(ctx_of(p, b)), nodes = uniform(nodes_of(p, b)), tc = (ctx + kTK - 1) / kTK;
+        // The lane's column: row r, head h; its mask, cut to the tree.
+        const uint32_t col = 32 * (cb * NG + cg) + c32, r = col / p.group, h = kvh * p.group + col % p.group;
+        const bool has = col < p.nc && r < nodes;
+        uint64_t sees = has ? sees_of(p, b, r, nodes) : 0;
+        asm volatile("" : "+v"(sees));  // arrived before the tiles' loads
+        V8 qreg[NK];
+        {
+            const T* src = static_cast<const T*>(p.q) + ((size_t)h * p.q_pad + (size_t)b * p.n_draft + r) * D + 8 * g;
+            #pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+                qreg[kk] = has ? *reinterpret_cast<const V8*>(src + 16 * kk) : V8{};
+        }
+        const size_t cache = ((size_t)b * p.kv_heads + kvh) * p.cap * D;
+        const size_t draft = ((size_t)kvh * p.d_pad + (size_t)b * p.n_draft) * D;
+        const u32x4 rs[4] = {tile_rsrc(static_cast<const T*>(p.k) + cache, ctx * kRow),
+                             tile_rsrc(static_cast<const T*>(p.v) + cache, ctx * kRow),
+                             tile_rsrc(static_cast<const T*>(p.kd) + draft, nodes * kRow),
+                             tile_rsrc(static_cast<const T*>(p.vd) + draft, nodes * kRow)};
+        // The tile of way kw in step s into its ring slot (past the segment's tiles: rows past the tree, zeros).
+        auto stage = [&](uint32_t s) __attribute__((always_inline)) {
+            const uint32_t t = s * KW + kw, dst = lbase + (s % S::kDepth * KW + kw) * S::kSlot + 1024 * cg * kPieces;
+            if (t < tc) {
+                #pragma unroll
+                for (int m = 0; m < kPieces; ++m)
+                    dma16_at(dst + 1024 * m, kd[m] + t * kHalf, 0, rs[0]);
+                #pragma unroll
+                for (int m = 0; m < kPieces; ++m)
+                    dma16_at(dst + kHalf + 1024 * m, vd[m] + t * kHalf, 0, rs[1]);
+            } else {
+                #pragma unroll
+                for (int m = 0; m < kPieces; ++m)
+                    dma16_at(dst + 1024 * m, kd[m] + (t - tc) * kHalf, 0, rs[2]);
+                #pragma unroll
+                for (int m = 0; m < kPieces; ++m)
+                    dma16_at(dst + kHalf + 1024 * m, vd[m] + (t - tc) * kHalf, 0, rs[3]);
+            }
+        };
+        f32x16 acc[ND];
+        #pragma unroll
+        for (int db = 0; db < ND; ++db)
+            acc[db] = f32x16{};
+        float m = -INFINITY, l = 0.0f;
+        bool odd = false;
+        const float c = p.scale_log2;
+        if (tid == 0)
+            s_odd = 0;
+        #pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+            settle(qreg[kk]);
+        for (uint32_t s = s0; s < min(s1, s0 + S::kDepth - 1); ++s)
+            stage(s);
+        for (uint32_t s = s0; s < s1; ++s) {
+            // Step s has landed; every wave is done with step s - 1, whose slots take step s + DEPTH - 1.
+            if (s + S::kDepth - 1 <= s1)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::kDepth - 2) * 2 * kPieces) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            if (NG > 1)
+                asm volatile("s_barrier" ::: "memory");
+            if (s + S::kDepth - 1 < s1)
+                stage(s + S::kDepth - 1);
+            const uint32_t t = s * KW + kw;
+            unsigned char* tile = lds + (s % S::kDepth * KW + kw) * S::kSlot;
+            if (t * kTK < tc * kTK + nodes) {
+                f32x16 x = f32x16{};
+                #pragma unroll
+                for (int kk = 0; kk < NK; ++kk)
+                    x = E::mfma32(*reinterpret_cast<const V8*>(tile + (ka ^ (32 * kk))), qreg[kk], x);
+                // Register i holds key 16 (i / 8) + 8 g + i % 8 of the tile.
+                #pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    x[i] *= c;
+                const bool drafts = t >= tc;
+                const uint32_t word = drafts ? (uint32_t)(sees >> (32 * (t - tc))) : 0u;
+                if (drafts) {
+                    #pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        x[i] = word >> (16 * (i >> 3) + (i & 7) + 8 * g) & 1 ? x[i] : -INFINITY;
+                } else if ((t + 1) * kTK > ctx) {
+                    #pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        x[i] = t * kTK + 16 * (i >> 3) + 8 * g + (i & 7) < ctx ? x[i] : -INFINITY;
+                }
+                float mx = x[0];
+                #pragma unroll
+                for (int i = 1; i < 16; ++i)
+                    mx = fmaxf(mx, x[i]);
+                mx = pair_max(mx);
+                float f = 1.0f;
+                if (mx > m + kRescale) {
+                    f = exp2_fast(m - mx);
+                    m = mx;
+                }
+                if (__any(f != 1.0f)) {
+                    l *= f;
+                    #pragma unroll
+                    for (int db = 0; db < ND; ++db)
+                        #pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            acc[db][i] *= f;
+                }
+                const float mu = m == -INFINITY ? 0.0f : m;
+                #pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    x[i] = exp2_fast(x[i] - mu);
+                    l += x[i];
+                }
+                if (drafts)
+                    odd |= finite_only<T, kHalf>(tile + kHalf, lane);
+                #pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    u32x4 hi, lo;
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float e0 = x[8 * a + 2 * i], e1 = x[8 * a + 2 * i + 1];
+                        hi[i] = E::pack2(e0, e1);
+                        if (kSplitP)
+                            lo[i] = E::pack2(e0 - value_of<T>(hi[i], 0), e1 - value_of<T>(hi[i], 1));
+                    }
+                    #pragma unroll
+                    for (int db = 0; db < ND; ++db) {
+                        const unsigned char* at = tile + va[db % NV] + db / NV * 256 + 16 * a * kRow;
+                        const s16x4 v0 = tr_read(at), v1 = tr_read(at + 4 * kRow);
+                        const V8 vv =
+                            __builtin_bit_cast(V8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                        acc[db] = E::mfma32(vv, __builtin_bit_cast(V8, hi), acc[db]);
+                        if (kSplitP)
+                            acc[db] = E::mfma32(vv, __builtin_bit_cast(V8, lo), acc[db]);
+                    }
+                }
+            }
+        }
+        // The piece's ways join: every wave's columns into LDS (the ring is idle: nothing is in flight), column c32 a row of
+        // D floats, its 16-byte chunks XORed by the column.
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        {
+            f32x4* row = reinterpret_cast<f32x4*>(lds) + (wl * 32 + c32) * (D / 4);
+            #pragma unroll
+            for (int q = 0; q < D / 8; ++q)
+                row[(8 * (q / 4) + 2 * (q % 4) + g) ^ (c32 & 15)] =
+                    f32x4{acc[q / 4][4 * (q % 4)], acc[q / 4][4 * (q % 4) + 1], acc[q / 4][4 * (q % 4) + 2],
+                          acc[q / 4][4 * (q % 4) + 3]};
+            const float lt = pair_sum(l);
+            if (g == 0)
+                s_ml[wl][c32] = float2{m, lt};
+            if (odd)
+                s_odd = 1;
+        }
+        __syncthreads();
+        const size_t part = (size_t)range + (size_t)b * p.kv_heads + kvh;
+        const bool any_odd = s_odd != 0;
+        if (p.n_ranges && tid == 0 && cb == 0)
+            p.part_odd[part] = any_odd;
+        for (uint32_t it = tid; it < NG * 32 * (D / 4); it += W * 64) {
+            const uint32_t q = it % (D / 4), cc = it / (D / 4) % 32, gi = it / (D / 4) / 32;
+            const uint32_t ccol = 32 * (cb * NG + gi) + cc, rr = ccol / p.group;
+            if (ccol >= p.nc || rr >= nodes)
+                continue;
+            float mx = -INFINITY, sum = 0.0f;
+            #pragma unroll
+            for (int y = 0; y < KW; ++y)
+                mx = fmaxf(mx, s_ml[gi + NG * y][cc].x);
+            f32x4 a = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            #pragma unroll
+            for (int y = 0; y < KW; ++y) {
+                const uint32_t w = gi + NG * y;
+                const float2 ml = s_ml[w][cc];
+                const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mx);
+                sum += ml.y * f;
+                a += reinterpret_cast<const f32x4*>(lds)[(w * 32 + cc) * (D / 4) + (q ^ (cc & 15))] * f;
+            }
+            if (p.n_ranges) {
+                *reinterpret_cast<f32x4*>(p.part_o + (part * p.nc + ccol) * D + 4 * q) = a;
+                if (q == 0)
+                    *reinterpret_cast<float2*>(p.part_ml + (part * p.nc + ccol) * 2) = float2{mx, sum};
+            } else {
+                const uint32_t hh = kvh * p.group + ccol % p.group;
+                const size_t row = (size_t)b * p.n_draft + rr;
+                a *= sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (any_odd)
+                    #pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        a[y] += odd_sum<T, D>(p, b, kvh, rr, nodes, 4 * q + y);
+                store4<TO>(o + row * p.width + (size_t)hh * D + 4 * q, a[0], a[1], a[2], a[3]);
+                if (lse && q == 0)
+                    lse[(size_t)hh * p.batch * p.n_draft + row] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * kLn2;
+            }
+        }
+        if (left == 0)
+            return;
+        __syncthreads();  // the ring is free again
+        do {
+            if (++kvh == p.kv_heads) {
+                kvh = 0;
+                ++b;
+            }
+            s1 = b < p.batch ? uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b))) : 0u;
+        } while (b < p.batch && s1 == 0);
+        if (b >= p.batch)
+            return;
+        s0 = 0;
+        s1 = min(s1, left);
+        left -= s1;
+    }
+}
+
+// One workgroup a row and head: each wave every kMergeWaves-th piece of its segment, up to 4 loads in flight, a running
+// maximum; the waves join in LDS.
+constexpr int kMergeWaves = 4;
 
 template <class T, class TO, int D>
-__global__ __launch_bounds__(kRowWaves * 64) void tree_rows(const TreeParams p, TO* __restrict__ o,
-                                                             float* __restrict__ lse)
+__global__ __launch_bounds__(kMergeWaves * 64) void tree_merge(const TreeParams p, TO* __restrict__ o,
+                                                                float* __restrict__ lse)
 {
-    constexpr int E = D / 64;  // head dims a lane
-    __shared__ float s_m[kRowWaves], s_l[kRowWaves], s_o[kRowWaves][D];
-    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const uint32_t row = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
-    const uint32_t b = row / p.n_draft, r = row % p.n_draft, kvh = h / p.group;
-    const uint32_t nodes = p.nodes ? min(p.nodes[b], p.n_draft) : p.n_draft;
+    constexpr int E = D / 64;
+    __shared__ float s_m[kMergeWaves], s_l[kMergeWaves], s_o[kMergeWaves][D];
+    const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const uint32_t row = blockIdx.x / p.heads, h = blockIdx.x % p.heads, b = row / p.n_draft, r = row % p.n_draft;
+    const uint32_t nodes = nodes_of(p, b);
     if (r >= nodes)
         return;
-    const uint32_t ctx = min(p.ctx[b], p.max_ctx);
-    const uint64_t mask = p.mask ? p.mask[row] : (2ull << r) - 1;
-    const T* q = static_cast<const T*>(p.q) + ((size_t)h * p.q_pad + row) * D;
-    const size_t cache = ((size_t)b * p.kv_heads + kvh) * p.cap * D;
-    const size_t draft = ((size_t)kvh * p.d_pad + (size_t)b * p.n_draft) * D;
-    float qr[E], acc[E], m = -INFINITY, l = 0.0f;
+    const uint32_t kvh = h / p.group, col = r * p.group + h % p.group, seg = b * p.kv_heads + kvh;
+    const uint32_t len = steps_of(p, ctx_of(p, b), nodes);
+    const uint32_t first = steps_before(p, b, lane) * p.kv_heads + kvh * len;
+    const Ranges rg(steps_before(p, p.batch, lane) * p.kv_heads, p.n_ranges);
+    const uint32_t w0 = rg.of(first), w1 = rg.of(first + len - 1);
+    float m = -INFINITY, l = 0.0f, acc[E];
     #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        qr[e] = (float)q[lane + 64 * e];
+    for (int e = 0; e < E; ++e)
         acc[e] = 0.0f;
-    }
-    for (uint32_t j = w; j < ctx + nodes; j += kRowWaves) {
-        if (j >= ctx && !(mask >> (j - ctx) & 1))
-            continue;
-        const T* kr = j < ctx ? static_cast<const T*>(p.k) + cache + (size_t)j * D
-                              : static_cast<const T*>(p.kd) + draft + (size_t)(j - ctx) * D;
-        const T* vr = j < ctx ? static_cast<const T*>(p.v) + cache + (size_t)j * D
-                              : static_cast<const T*>(p.vd) + draft + (size_t)(j - ctx) * D;
-        float s = 0.0f;
+    constexpr int U = 4;
+    for (uint32_t x0 = w0 + wv; x0 <= w1; x0 += U * kMergeWaves) {
+        float2 ml[U];
+        float v[U][E];
         #pragma unroll
-        for (int e = 0; e < E; ++e)
-            s = fmaf(qr[e], (float)kr[lane + 64 * e], s);
+        for (int u = 0; u < U; ++u) {
+            const uint32_t x = x0 + u * kMergeWaves;
+            const bool live = x <= w1 && rg.start(x) < rg.start(x + 1);  // (an empty range wrote nothing)
+            const size_t at = ((size_t)(live ? x : w0) + seg) * p.nc + col;
+            ml[u] = live ? *reinterpret_cast<const float2*>(p.part_ml + at * 2) : float2{-INFINITY, 0.0f};
+            #pragma unroll
+            for (int e = 0; e < E; ++e)
+                v[u][e] = live ? p.part_o[at * D + 64 * e + lane] : 0.0f;
+        }
         #pragma unroll
-        for (int x = 32; x > 0; x >>= 1)
-            s += __shfl_xor(s, x);
-        s *= p.scale_log2;
-        const float nm = fmaxf(m, s), f = m == -INFINITY ? 0.0f : exp2_fast(m - nm), e0 = exp2_fast(s - nm);
-        l = l * f + e0;
-        #pragma unroll
-        for (int e = 0; e < E; ++e)
-            acc[e] = acc[e] * f + e0 * (float)vr[lane + 64 * e];
-        m = nm;
+        for (int u = 0; u < U; ++u) {
+            const float nm = fmaxf(m, ml[u].x);
+            const float f = m == -INFINITY ? 0.0f : exp2_fast(m - nm), g = ml[u].x == -INFINITY ? 0.0f : exp2_fast(ml[u].x - nm);
+            l = l * f + ml[u].y * g;
+            #pragma unroll
+            for (int e = 0; e < E; ++e)
+                acc[e] = acc[e] * f + v[u][e] * g;
+            m = nm;
+        }
     }
     if (lane == 0) {
-        s_m[w] = m;
-        s_l[w] = l;
+        s_m[wv] = m;
+        s_l[wv] = l;
     }
     #pragma unroll
     for (int e = 0; e < E; ++e)
-        s_o[w][lane + 64 * e] = acc[e];
+        s_o[wv][64 * e + lane] = acc[e];
     __syncthreads();
-    if (w != 0)
+    if (wv != 0)
         return;
     float mx = s_m[0];
-    for (int i = 1; i < kRowWaves; ++i)
+    #pragma unroll
+    for (int i = 1; i < kMergeWaves; ++i)
         mx = fmaxf(mx, s_m[i]);
-    float sum = 0.0f, f[kRowWaves];
-    for (int i = 0; i < kRowWaves; ++i) {
+    float sum = 0.0f, f[kMergeWaves];
+    #pragma unroll
+    for (int i = 0; i < kMergeWaves; ++i) {
         f[i] = s_m[i] == -INFINITY ? 0.0f : exp2_fast(s_m[i] - mx);
         sum += s_l[i] * f[i];
     }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    bool odd = false;
+    for (uint32_t x = w0 + lane; x <= w1; x += 64)
+        odd = odd || (rg.start(x) < rg.start(x + 1) && p.part_odd[x + seg]);
+    odd = __any(odd);
     TO* orow = o + (size_t)row * p.width + (size_t)h * D;
     #pragma unroll
     for (int e = 0; e < E; ++e) {
         float x = 0.0f;
-        for (int i = 0; i < kRowWaves; ++i)
-            x += s_o[i][lane + 64 * e] * f[i];
-        orow[lane + 64 * e] = (TO)(sum == 0.0f ? 0.0f : x / sum);
+        #pragma unroll
+        for (int i = 0; i < kMergeWaves; ++i)
+            x += s_o[i][64 * e + lane] * f[i];
+        x *= inv;
+        if (odd)
+            x += odd_sum<T, D>(p, b, kvh, r, nodes, 64 * e + lane);
+        orow[64 * e + lane] = (TO)x;
     }
     if (lse && lane == 0)
         lse[(size_t)h * p.batch * p.n_draft + row] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * kLn2;
 }
 
-template <class T, int D>
-void launch(const TreeParams& p, mako_dtype out, void* o, float* lse, hipStream_t s)
+// A call's split, from its sizes alone (contexts are known on the device only).
+struct Plan {
+    uint32_t ng, ways, ncb, n_ranges;  // n_ranges 0: a segment a workgroup
+    size_t pieces;
+};
+
+template <int D>
+uint32_t ways_of(uint32_t ng)
 {
-    const dim3 grid(p.batch * p.n_draft * p.heads), block(kRowWaves * 64);
-    if (out == MAKO_F32)
-        hipLaunchKernelGGL((tree_rows<T, float, D>), grid, block, 0, s, p, static_cast<float*>(o), lse);
-    else
-        hipLaunchKernelGGL((tree_rows<T, T, D>), grid, block, 0, s, p, static_cast<T*>(o), lse);
+    return ng == 1 ? Shape<D, 1>::kKW : ng == 2 ? Shape<D, 2>::kKW : Shape<D, 4>::kKW;
 }
 
-template <class T>
-void launch_dim(const TreeParams& p, uint32_t dim, mako_dtype out, void* o, float* lse, hipStream_t s)
+constexpr uint32_t kDirectSteps = 5;
+
+Plan plan_of(const mako_tree_args* a, uint32_t cus)
+{
+    const uint32_t nc = a->n_draft * (a->heads / a->kv_heads);
+    Plan pl{};
+    pl.ng = nc <= 32 ? 1 : nc <= 64 ? 2 : 4;
+    pl.ncb = (nc + 32 * pl.ng - 1) / (32 * pl.ng);
+    pl.ways = a->dim == 64 ? ways_of<64>(pl.ng) : a->dim == 128 ? ways_of<128>(pl.ng) : ways_of<256>(pl.ng);
+    const uint32_t tiles = (a->max_ctx + kTK - 1) / kTK + (a->n_draft + kTK - 1) / kTK;
+    const uint32_t steps = (tiles + pl.ways - 1) / pl.ways;
+    if (steps > kDirectSteps) {
+        const uint64_t segs = (uint64_t)a->batch * a->kv_heads;
+        pl.n_ranges = (uint32_t)std::min<uint64_t>(std::max(1u, cus / pl.ncb), segs * steps);
+        pl.pieces = pl.n_ranges + segs;
+    }
+    return pl;
+}
+
+size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+
+// The partials' parts: outputs, maxima and sums, flags.
+size_t part_o_bytes(const Plan& pl, const mako_tree_args* a)
+{
+    return round256(pl.pieces * a->n_draft * (a->heads / a->kv_heads) * a->dim * sizeof(float));
+}
+size_t part_ml_bytes(const Plan& pl, const mako_tree_args* a)
+{
+    return round256(pl.pieces * a->n_draft * (a->heads / a->kv_heads) * 2 * sizeof(float));
+}
+size_t workspace_for(const Plan& pl, const mako_tree_args* a)
+{
+    return part_o_bytes(pl, a) + part_ml_bytes(pl, a) + pl.pieces * sizeof(uint32_t);
+}
+
+template <class T, class TO, int D, int NG>
+void launch_split(const TreeParams& p, void* o, float* lse, hipStream_t s)
+{
+    const uint32_t units = p.n_ranges ? p.n_ranges : p.batch * p.kv_heads;
+    const dim3 grid(p.ncb > 1 ? (units + 7) / 8 * 8 * p.ncb : units), block(Shape<D, NG>::kWaves * 64);
+    hipLaunchKernelGGL((tree_split<T, TO, D, NG>), grid, block, 0, s, p, static_cast<TO*>(o), lse);
+}
+
+template <class T, class TO, int D>
+void launch(const TreeParams& p, uint32_t ng, void* o, float* lse, hipStream_t s)
+{
+    if (ng == 1)
+        launch_split<T, TO, D, 1>(p, o, lse, s);
+    else if (ng == 2)
+        launch_split<T, TO, D, 2>(p, o, lse, s);
+    else
+        launch_split<T, TO, D, 4>(p, o, lse, s);
+    if (p.n_ranges)
+        hipLaunchKernelGGL((tree_merge<T, TO, D>), dim3(p.batch * p.n_draft * p.heads), dim3(kMergeWaves * 64), 0, s, p,
+                           static_cast<TO*>(o), lse);
+}
+
+template <class T, class TO>
+void launch_dim(const TreeParams& p, uint32_t dim, uint32_t ng, void* o, float* lse, hipStream_t s)
 {
     if (dim == 64)
-        launch<T, 64>(p, out, o, lse, s);
+        launch<T, TO, 64>(p, ng, o, lse, s);
     else if (dim == 128)
-        launch<T, 128>(p, out, o, lse, s);
+        launch<T, TO, 128>(p, ng, o, lse, s);
     else
-        launch<T, 256>(p, out, o, lse, s);
+        launch<T, TO, 256>(p, ng, o, lse, s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -164,23 +705,48 @@ int check_args(const mako_tree_args* a, mako_dtype in, mako_dtype out, const voi
 
 using namespace mako;
 
-extern "C" size_t mako_attn_tree_workspace(const mako_tree_args*) { return 0; }
+extern "C" size_t mako_attn_tree_workspace(const mako_tree_args* a)
+{
+    const uint32_t cus = device_cus();
+    if (!a || !cus || !a->heads || !a->kv_heads || a->heads % a->kv_heads || !a->batch || !a->n_draft || a->n_draft > 64 ||
+        (a->dim != 64 && a->dim != 128 && a->dim != 256))
+        return 0;
+    return workspace_for(plan_of(a, cus), a);
+}
 
 extern "C" int mako_attn_tree(const mako_tree_args* a, mako_dtype in, mako_dtype out, const void* q, const void* k,
                               const void* v, const void* kd, const void* vd, const uint32_t* ctx_len,
-                              const uint32_t* n_nodes, const uint64_t* mask, void* o, float* lse, void*, size_t,
-                              void* stream)
+                              const uint32_t* n_nodes, const uint64_t* mask, void* o, float* lse, void* workspace,
+                              size_t workspace_bytes, void* stream)
 {
+    const char* what = "attention_tree";
     if (const int rc = check_args(a, in, out, q, k, v, kd, vd, ctx_len, mask, o))
         return rc;
     if (a->batch == 0 || a->n_draft == 0)
         return ok();
-    const TreeParams p{q, k, v, kd, vd, ctx_len, n_nodes, mask, a->batch, a->n_draft, a->q_pad, a->d_pad, a->heads,
-                       a->kv_heads, a->heads / a->kv_heads, a->cap, a->max_ctx, a->width, a->scale * kLog2e};
+    const uint32_t cus = device_cus();
+    if (!cus)
+        return fail(MAKO_EHIP, "%s: no device to size the split for", what);
+    const Plan pl = plan_of(a, cus);
+    const size_t need = workspace_for(pl, a);
+    if (workspace_bytes < need || (need && !workspace) || !aligned16(workspace))
+        return fail(MAKO_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, workspace_bytes,
+                    need);
+    const uint32_t group = a->heads / a->kv_heads;
+    const auto at = [&](size_t off) { return need ? static_cast<char*>(workspace) + off : nullptr; };
+    const size_t ob = part_o_bytes(pl, a), mb = part_ml_bytes(pl, a);
+    const TreeParams p{q, k, v, kd, vd, ctx_len, n_nodes, mask, reinterpret_cast<float*>(at(0)),
+                       reinterpret_cast<float*>(at(ob)), reinterpret_cast<uint32_t*>(at(ob + mb)),
+                       a->batch, a->n_draft, a->q_pad, a->d_pad, a->heads, a->kv_heads, group, a->cap, a->max_ctx,
+                       a->width, a->n_draft * group, pl.ncb, pl.ways, pl.n_ranges, a->scale * kLog2e};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (in == MAKO_BF16)
-        launch_dim<__bf16>(p, a->dim, out, o, lse, s);
+    if (in == MAKO_BF16 && out == MAKO_F32)
+        launch_dim<__bf16, float>(p, a->dim, pl.ng, o, lse, s);
+    else if (in == MAKO_BF16)
+        launch_dim<__bf16, __bf16>(p, a->dim, pl.ng, o, lse, s);
+    else if (out == MAKO_F32)
+        launch_dim<_Float16, float>(p, a->dim, pl.ng, o, lse, s);
     else
-        launch_dim<_Float16>(p, a->dim, out, o, lse, s);
-    return check_launch("attention_tree");
+        launch_dim<_Float16, _Float16>(p, a->dim, pl.ng, o, lse, s);
+    return check_launch(what);
 }
