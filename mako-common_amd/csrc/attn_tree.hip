@@ -27,6 +27,7 @@
 #include <algorithm>
 
 #include "lds_tiles.hpp"
+#include "split_ranges.hpp"
 
 namespace mako {
 namespace {
@@ -63,77 +64,14 @@ __device__ __forceinline__ uint32_t steps_of(const TreeParams& p, uint32_t ctx, 
     return ((ctx + kTK - 1) / kTK + (nodes + kTK - 1) / kTK + p.ways - 1) / p.ways;
 }
 
-// A value the whole wave holds, in a scalar register.
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane(x); }
-
-// The steps of a segment of sequences [0, n), summed; 64 sequences at a time.
-__device__ __forceinline__ uint32_t steps_before(const TreeParams& p, uint32_t n, uint32_t lane)
-{
-    uint32_t s = 0;
-    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
-        const uint32_t i = i0 + lane;
-        uint32_t v = i < n ? steps_of(p, ctx_of(p, i), nodes_of(p, i)) : 0u;
-        #pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            v += __shfl_xor(v, o);
-        s += v;
-    }
-    return s;
-}
-
-// The sequence whose segments hold step x of all of them end to end (x below their sum), and its first step.
-__device__ __forceinline__ void seq_of(const TreeParams& p, uint32_t x, uint32_t lane, uint32_t& b, uint32_t& first)
-{
-    uint32_t base = 0;
-    for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
-        const uint32_t i = i0 + lane;
-        const uint32_t len = i < p.batch ? steps_of(p, ctx_of(p, i), nodes_of(p, i)) * p.kv_heads : 0u;
-        uint32_t inc = len;
-        #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t t = __shfl_up(inc, o);
-            inc += lane >= (uint32_t)o ? t : 0u;
-        }
-        const uint64_t hit = __ballot(i < p.batch && x < base + inc);
-        if (hit) {
-            const uint32_t at = (uint32_t)__builtin_ctzll(hit);
-            b = i0 + at;
-            first = base + __shfl(inc - len, at);
-            return;
-        }
-        base += __shfl(inc, 63);
-    }
-    b = p.batch;
-    first = base;
-}
-
-// T steps cut into n equal ranges: range w starts at floor(w T / n), without a 64-bit division (w r < n^2 fits 32 bits).
-struct Ranges {
-    uint32_t T, n, q, r;
-    __device__ Ranges(uint32_t total, uint32_t ranges) : T(total), n(ranges), q(total / ranges), r(total % ranges) {}
-    __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * q + (w * r) / n; }
-    // The range that holds step x.
-    __device__ __forceinline__ uint32_t of(uint32_t x) const
-    {
-        uint32_t w = (uint32_t)(((uint64_t)x * n) / T);
-        while (w + 1 < n && start(w + 1) <= x)
-            ++w;
-        while (w > 0 && start(w) > x)
-            --w;
-        return w;
-    }
+// The steps of a segment of sequence i.
+struct SegSteps {
+    const TreeParams& p;
+    __device__ __forceinline__ uint32_t operator()(uint32_t i) const { return steps_of(p, ctx_of(p, i), nodes_of(p, i)); }
 };
 
 // The key in slot s of a tile's K image (its own inverse).
 __device__ __forceinline__ uint32_t slot_of(uint32_t s) { return (s & ~12u) | ((s & 4u) << 1) | ((s & 8u) >> 1); }
-
-// Where 16-byte chunk c of K row s sits in its LDS row: XORed so that the 16 rows a ds_read_b128 spans start in distinct
-// banks (rows of 128 bytes: two fill the 64 banks).
-template <int D>
-__device__ __forceinline__ uint32_t k_xor(uint32_t s)
-{
-    return D == 64 ? (s >> 1) & 7u : s & 15u;
-}
 
 // Where 32-byte unit u of V row k sits in its LDS row: the two units of the four rows that a transpose read's 32 lanes
 // address cover the 64 banks once (a bijection of the units; its own inverse up to the parity term).
@@ -262,12 +200,12 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
     // The first piece of the range (or the segment).
     uint32_t b, kvh, s0, s1, left = 0;  // steps [s0, s1) of the segment; steps of the range behind them
     if (p.n_ranges) {
-        const Ranges rg(uniform(steps_before(p, p.batch, lane) * p.kv_heads), p.n_ranges);
+        const Ranges rg(uniform(sum_of(p.batch, lane, SegSteps{p}) * p.kv_heads), p.n_ranges);
         const uint32_t x0 = rg.start(range), x1 = rg.start(range + 1);
         if (x0 >= x1)
             return;
         uint32_t first;
-        seq_of(p, x0, lane, b, first);
+        seq_of(p.batch, x0, lane, SegSteps{p}, p.kv_heads, b, first);
         b = uniform(b);
         const uint32_t len = uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b)));
         kvh = (x0 - uniform(first)) / len;
@@ -505,8 +443,8 @@ __global__ __launch_bounds__(kMergeWaves * 64) void tree_merge(const TreeParams 
         return;
     const uint32_t kvh = h / p.group, col = r * p.group + h % p.group, seg = b * p.kv_heads + kvh;
     const uint32_t len = steps_of(p, ctx_of(p, b), nodes);
-    const uint32_t first = steps_before(p, b, lane) * p.kv_heads + kvh * len;
-    const Ranges rg(steps_before(p, p.batch, lane) * p.kv_heads, p.n_ranges);
+    const uint32_t first = sum_of(b, lane, SegSteps{p}) * p.kv_heads + kvh * len;
+    const Ranges rg(sum_of(p.batch, lane, SegSteps{p}) * p.kv_heads, p.n_ranges);
     const uint32_t w0 = rg.of(first), w1 = rg.of(first + len - 1);
     float m = -INFINITY, l = 0.0f, acc[E];
     #pragma unroll

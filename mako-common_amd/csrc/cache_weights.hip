@@ -2,52 +2,447 @@
 //
 // Mathematics: w_out[j] = decay w[j] + sum over the group's heads h and the queries i that see row j of
 //   exp(scale q_i.k_j - lse_i)
-// No maximum is needed: lse bounds every score it was summed from.
+// No maximum is needed: lse bounds every score it was summed from. The scores come from v_mfma_f32_32x32x16; a query that
+// adds nothing (past the sequence's, lse = -inf) is a row of zeros with an offset of -inf.
 //
-// weights_keys: one thread a key, its row of K in registers eight head dims at a time, every query in turn.
-#include "device.hpp"
+// weights_few, up to 64 (query, head of the group) rows a kv head. Bound: the read of K. The rows are the A operand, in
+// registers, and 32 keys a tile the B operand: a lane holds one key's scores, so the sum over the rows is lane-local but
+// for one exchange of halves. K comes raw by LDS DMA into a ring of each wave's own (chunks XORed by row), w beside it;
+// the tiles of all (sequence, kv head) segments, end to end, are cut into equal ranges, one a wave. No wave waits for
+// another, and every key's sum is its wave's alone.
+//
+// weights_many, any number of rows. Bound: an exponential a pair beside 2 D operations of its product. A workgroup holds
+// 4 x 32 KB keys in registers as the A operand, and the queries come in tiles of 32 through an LDS ring that the four
+// waves share: a lane holds one query's scores, so its offset is one register, and the sums stay in registers, a lane's
+// queries apart, until the end. Queries are cut into chunks where keys alone leave CUs idle; each chunk's sums go to the
+// workspace and weights_join adds them in order.
+#include <algorithm>
+
+#include "lds_tiles.hpp"
+#include "split_ranges.hpp"
 
 namespace mako {
 namespace {
+
+constexpr int kTK = 32;     // keys, or queries, a tile
+constexpr int kFewRows = 64;
 
 struct WeightsParams {
     const void *q, *k;
     const float *lse, *w;
     float* w_out;
     const uint32_t *ctx, *path, *n_path;
-    uint32_t batch, n_q, heads, kv_heads, group, dim, cap, max_ctx;
+    float* part;          // [chunks][lists][max_ctx]
+    uint32_t batch, n_q, heads, kv_heads, group, cap, max_ctx;
+    uint32_t n_ranges;    // weights_few: waves
+    uint32_t chunk, n_chunks, n_blocks;  // weights_many: queries a chunk, chunks, key blocks
     uint64_t qs_b, qs_h;  // q strides (elements) of a sequence and a head
     uint64_t ls_b, ls_h;  // lse strides
     float scale_log2, decay;
 };
 
-template <class T>
-__global__ __launch_bounds__(256) void weights_keys(const WeightsParams p)
+__device__ __forceinline__ uint32_t ctx_of(const WeightsParams& p, uint32_t b) { return min(p.ctx[b], p.max_ctx); }
+__device__ __forceinline__ uint32_t n_of(const WeightsParams& p, uint32_t b)
 {
-    const uint32_t b = blockIdx.x / p.kv_heads, kvh = blockIdx.x % p.kv_heads;
-    const uint32_t ctx = min(p.ctx[b], p.max_ctx), n = p.n_path ? min(p.n_path[b], p.n_q) : p.n_q;
-    const size_t list = (size_t)b * p.kv_heads + kvh;
-    for (uint32_t j = threadIdx.x; j < ctx; j += 256) {
-        const T* kr = static_cast<const T*>(p.k) + (list * p.cap + j) * p.dim;
-        float sum = 0.0f;
-        for (uint32_t i = 0; i < n; ++i) {
-            const uint32_t r = p.path ? p.path[(size_t)b * p.n_q + i] : i;
-            if (r >= p.n_q || (uint64_t)j + n > (uint64_t)ctx + i)
-                continue;
-            for (uint32_t h = kvh * p.group; h < (kvh + 1) * p.group; ++h) {
-                const float l = p.lse[b * p.ls_b + h * p.ls_h + r];
-                if (l == -INFINITY)
-                    continue;
-                const T* qr = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + (size_t)r * p.dim;
-                float s = 0.0f;
-                for (uint32_t d = 0; d < p.dim; ++d)
-                    s = fmaf((float)qr[d], (float)kr[d], s);
-                sum += exp2_fast(fmaf(s, p.scale_log2, -l * kLog2e));
+    return p.n_path ? min(p.n_path[b], p.n_q) : p.n_q;
+}
+struct KeyTiles {
+    const WeightsParams& p;
+    __device__ __forceinline__ uint32_t operator()(uint32_t i) const { return (ctx_of(p, i) + kTK - 1) / kTK; }
+};
+
+// Query i of sequence b: its row of q (n_q: none) for head h, and its offset, lse in base 2 (inf: adds nothing).
+__device__ __forceinline__ uint32_t query(const WeightsParams& p, uint32_t b, uint32_t h, uint32_t i, bool has, float& off)
+{
+    uint32_t r = has ? i : p.n_q;
+    if (has && p.path)
+        r = p.path[(size_t)b * p.n_q + i];
+    off = INFINITY;
+    if (r >= p.n_q)
+        return p.n_q;
+    const float l = p.lse[b * p.ls_b + h * p.ls_h + r];
+    if (l == -INFINITY)
+        return p.n_q;
+    off = l * kLog2e;
+    return r;
+}
+
+// Four bytes a lane from rsrc + voff to LDS m0 + 4 lane.
+__device__ __forceinline__ void dma4_at(uint32_t m0, uint32_t voff, u32x4 rsrc)
+{
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(m0), "v"(voff), "s"(rsrc)
+                 : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
+template <int D>
+struct Few {
+    static constexpr int kWaves = 4;
+    static constexpr int kRow = 2 * D, kTile = kTK * kRow, kPieces = kTile / 1024;
+    static constexpr int kDepth = D == 64 ? 8 : D == 128 ? 4 : 2;
+    static constexpr int kSlot = kTile + 256;  // K, and 64 lanes' weights
+    static constexpr int kLds = kWaves * kDepth * kSlot;
+};
+
+template <class T, int D, int NCG>
+__global__ __launch_bounds__(256, 1) void weights_few(const WeightsParams p)
+{
+    using S = Few<D>;
+    using E = Elem<T>;
+    using V8 = typename E::vec8;
+    constexpr int NK = D / 16, kRow = S::kRow;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[S::kLds];
+    __shared__ __attribute__((aligned(16))) float s_off[S::kWaves][32 * NCG];
+    __shared__ __attribute__((aligned(16))) uint32_t s_lim[S::kWaves][32 * NCG];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c32 = lane & 31, wl = uniform(tid >> 6);
+    const Ranges rg(uniform(sum_of(p.batch, lane, KeyTiles{p}) * p.kv_heads), p.n_ranges);
+    const uint32_t wave = blockIdx.x * S::kWaves + wl, x0 = rg.start(wave), x1 = rg.start(wave + 1);
+    if (x0 >= x1)
+        return;
+    uint32_t b, first;
+    seq_of(p.batch, x0, lane, KeyTiles{p}, p.kv_heads, b, first);
+    b = uniform(b);
+    first = uniform(first);
+    uint32_t len = uniform(KeyTiles{p}(b)), kvh = (x0 - first) / len, t0 = (x0 - first) % len, left = x1 - x0;
+
+    uint32_t kd[S::kPieces];
+    #pragma unroll
+    for (int m = 0; m < S::kPieces; ++m) {
+        const uint32_t at = 1024 * m + 16 * lane, r = at / kRow, pos = at % kRow;
+        kd[m] = r * kRow + 16 * ((pos / 16) ^ k_xor<D>(r));
+    }
+    const uint32_t lbase = uniform((uint32_t)reinterpret_cast<uintptr_t>(lds)) + wl * S::kDepth * S::kSlot;
+    unsigned char* ring = lds + wl * S::kDepth * S::kSlot;
+    const uint32_t ka = c32 * kRow + 16 * (g ^ k_xor<D>(c32));
+
+    for (;;) {
+        const uint32_t ctx = uniform(ctx_of(p, b)), n = uniform(n_of(p, b)), t1 = min(len, t0 + left);
+        const size_t list = (size_t)b * p.kv_heads + kvh;
+        const u32x4 krs = tile_rsrc(static_cast<const T*>(p.k) + list * p.cap * D, ctx * kRow);
+        const u32x4 wrs = tile_rsrc(p.w + list * p.cap, p.w ? ctx * 4 : 0u);
+        auto stage = [&](uint32_t t) __attribute__((always_inline)) {
+            const uint32_t dst = lbase + t % S::kDepth * S::kSlot;
+            #pragma unroll
+            for (int m = 0; m < S::kPieces; ++m)
+                dma16_at(dst + 1024 * m, kd[m] + t * S::kTile, 0, krs);
+            dma4_at(dst + S::kTile, (t * kTK + c32) * 4, wrs);
+        };
+        // The rows: lane l looks up row l's offset and how many keys it sees; the A operand holds row c32 of each group.
+        V8 qreg[NCG][NK];
+        #pragma unroll
+        for (int cg = 0; cg < NCG; ++cg) {
+            const uint32_t row = 32 * cg + c32, i = row / p.group, h = kvh * p.group + row % p.group;
+            float off;
+            const uint32_t r = query(p, b, h, i, i < n, off);
+            const T* src = static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h + (size_t)r * D + 8 * g;
+            #pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+                qreg[cg][kk] = r < p.n_q ? *reinterpret_cast<const V8*>(src + 16 * kk) : V8{};
+            s_off[wl][row] = off;
+            s_lim[wl][row] = r < p.n_q && ctx + i >= n ? ctx + i - n + 1 : 0u;
+            #pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+                settle(qreg[cg][kk]);
+        }
+        for (uint32_t t = t0; t < min(t1, t0 + S::kDepth - 1); ++t)
+            stage(t);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        f32x4 off[NCG][4];
+        #pragma unroll
+        for (int cg = 0; cg < NCG; ++cg)
+            #pragma unroll
+            for (int i = 0; i < 4; ++i)
+                off[cg][i] = *reinterpret_cast<const f32x4*>(&s_off[wl][32 * cg + 8 * i + 4 * g]);
+        for (uint32_t t = t0; t < t1; ++t) {
+            if (t + S::kDepth - 1 <= t1)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::kDepth - 2) * (S::kPieces + 1)) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            if (t + S::kDepth - 1 < t1)
+                stage(t + S::kDepth - 1);
+            const unsigned char* tile = ring + t % S::kDepth * S::kSlot;
+            const uint32_t j = t * kTK + c32;
+            bool masked = (t + 1) * kTK + n > ctx + 1;  // some row does not see all of the tile
+            f32x16 x[NCG];
+            #pragma unroll
+            for (int cg = 0; cg < NCG; ++cg)
+                x[cg] = f32x16{};
+            #pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                const V8 kf = *reinterpret_cast<const V8*>(tile + (ka ^ (32 * kk)));
+                #pragma unroll
+                for (int cg = 0; cg < NCG; ++cg)
+                    x[cg] = E::mfma32(qreg[cg][kk], kf, x[cg]);
+            }
+            const float w = *reinterpret_cast<const float*>(tile + S::kTile + 4 * c32);
+            // Register i: row 8 (i / 4) + 4 g + i % 4. A key that is not finite gives NaN against the rows that are no
+            // query too: then those are masked.
+            float sum;
+            for (;;) {
+                sum = 0.0f;
+                #pragma unroll
+                for (int cg = 0; cg < NCG; ++cg)
+                    #pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) {
+                        f32x4 e;
+                        #pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            e[i] = exp2_fast(fmaf(x[cg][4 * i4 + i], p.scale_log2, -off[cg][i4][i]));
+                        if (masked) {
+                            const u32x4 lim = *reinterpret_cast<const u32x4*>(&s_lim[wl][32 * cg + 8 * i4 + 4 * g]);
+                            #pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                e[i] = j < lim[i] ? e[i] : 0.0f;
+                        }
+                        sum += (e[0] + e[1]) + (e[2] + e[3]);
+                    }
+                if (masked || !__any(sum != sum))
+                    break;
+                masked = true;
+            }
+            sum = pair_sum(sum);
+            if (g == 0 && j < ctx)
+                p.w_out[list * p.cap + j] = p.w ? fmaf(p.decay, w, sum) : sum;
+        }
+        left -= t1 - t0;
+        if (left == 0)
+            return;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        t0 = 0;
+        if (++kvh == p.kv_heads) {
+            kvh = 0;
+            do {
+                if (++b >= p.batch)
+                    return;
+                len = uniform(KeyTiles{p}(b));
+            } while (len == 0);
+        }
+    }
+}
+
+template <int D>
+struct Many {
+    static constexpr int kKB = D == 256 ? 1 : 2;             // blocks of 32 keys a wave
+    static constexpr int kKeys = 4 * 32 * kKB;               // keys a workgroup
+    static constexpr int kRow = 2 * D, kTile = kTK * kRow;   // a tile of queries
+    static constexpr int kPieces = kTile / 1024 / 4;         // 1 KiB pieces of it a wave
+    static constexpr int kDepth = D == 64 ? 8 : 4;
+    static constexpr int kTable = 2048;                      // rows whose place and offset are looked up at a time
+};
+
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
+{
+    using S = Many<D>;
+    using E = Elem<T>;
+    using V8 = typename E::vec8;
+    constexpr int NK = D / 16, kRow = S::kRow, KB = S::kKB;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[S::kDepth * S::kTile];
+    __shared__ float s_off[S::kTable];
+    __shared__ uint32_t s_row[S::kTable];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c32 = lane & 31, wl = uniform(tid >> 6);
+    // lists first, so that with a multiple of 8 of them a list's workgroups share an XCD
+    const uint32_t lists = p.batch * p.kv_heads, list = blockIdx.x % lists, rest = blockIdx.x / lists;
+    const uint32_t block = rest % p.n_blocks, chunk = rest / p.n_blocks, b = list / p.kv_heads, kvh = list % p.kv_heads;
+    const uint32_t ctx = uniform(ctx_of(p, b)), n = uniform(n_of(p, b)), k0 = block * S::kKeys;
+    if (k0 >= ctx)
+        return;
+    // Queries [ia, ib): the chunk's that see a key of the block (query i sees ctx - n + i and what is before).
+    const uint32_t ib = min(n, (chunk + 1) * p.chunk);
+    const uint32_t see0 = k0 + n > ctx ? k0 + n - ctx : 0u;  // the first query that sees k0
+    const uint32_t ia = max(chunk * p.chunk, see0 & ~31u);
+    const uint32_t nt = ib > ia ? (ib - ia + kTK - 1) / kTK : 0u;  // tiles a head
+    if (nt == 0 && p.n_chunks > 1)
+        return;
+
+    uint32_t qr[S::kPieces], qc[S::kPieces];  // the row and byte of a tile that the lane's 16 LDS bytes hold
+    #pragma unroll
+    for (int m = 0; m < S::kPieces; ++m) {
+        const uint32_t at = 1024 * (wl * S::kPieces + m) + 16 * lane, pos = at % kRow;
+        qr[m] = at / kRow;
+        qc[m] = 16 * ((pos / 16) ^ k_xor<D>(qr[m]));
+    }
+    const uint32_t lbase = uniform((uint32_t)reinterpret_cast<uintptr_t>(lds));
+    const uint32_t qa = c32 * kRow + 16 * (g ^ k_xor<D>(c32));
+    const uint32_t kw = k0 + wl * 32 * KB;  // the wave's first key
+    V8 kreg[KB][NK];
+    #pragma unroll
+    for (int i = 0; i < KB; ++i) {
+        const uint32_t j = kw + 32 * i + c32;
+        const T* src = static_cast<const T*>(p.k) + ((size_t)list * p.cap + j) * D + 8 * g;
+        #pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+            kreg[i][kk] = j < ctx ? *reinterpret_cast<const V8*>(src + 16 * kk) : V8{};
+    }
+    f32x16 acc[KB];
+    #pragma unroll
+    for (int i = 0; i < KB; ++i)
+        acc[i] = f32x16{};
+    const uint32_t tiles = nt * p.group;
+    for (uint32_t tb = 0; tb < tiles; tb += S::kTable / kTK) {
+        const uint32_t te = min(tiles, tb + S::kTable / kTK);
+        __syncthreads();
+        for (uint32_t x = tid; x < (te - tb) * kTK; x += 256) {
+            const uint32_t t = tb + x / kTK, h = kvh * p.group + t / nt, i = ia + t % nt * kTK + x % kTK;
+            float off;
+            const uint32_t r = query(p, b, h, i, i < ib, off);
+            s_off[x] = off;
+            s_row[x] = r < p.n_q ? r * kRow : 0x80000000u;  // (past the descriptor: zeros)
+        }
+        #pragma unroll
+        for (int i = 0; i < KB; ++i)
+            #pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+                settle(kreg[i][kk]);
+        __syncthreads();
+        auto stage = [&](uint32_t t) __attribute__((always_inline)) {
+            const uint32_t dst = lbase + t % S::kDepth * S::kTile + 1024 * wl * S::kPieces, h = kvh * p.group + t / nt;
+            const u32x4 rs = tile_rsrc(static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h, p.n_q * kRow);
+            #pragma unroll
+            for (int m = 0; m < S::kPieces; ++m)
+                dma16_at(dst + 1024 * m, s_row[(t - tb) * kTK + qr[m]] + qc[m], 0, rs);
+        };
+        for (uint32_t t = tb; t < min(te, tb + S::kDepth - 1); ++t)
+            stage(t);
+        for (uint32_t t = tb; t < te; ++t) {
+            if (t + S::kDepth - 1 <= te)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::kDepth - 2) * S::kPieces) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (t + S::kDepth - 1 < te)
+                stage(t + S::kDepth - 1);
+            const unsigned char* tile = lds + t % S::kDepth * S::kTile;
+            f32x16 x[KB];
+            #pragma unroll
+            for (int i = 0; i < KB; ++i)
+                x[i] = f32x16{};
+            #pragma unroll
+            for (int kk = 0; kk < NK; ++kk) {
+                const V8 qf = *reinterpret_cast<const V8*>(tile + (qa ^ (32 * kk)));
+                #pragma unroll
+                for (int i = 0; i < KB; ++i)
+                    x[i] = E::mfma32(kreg[i][kk], qf, x[i]);
+            }
+            const float off = s_off[(t - tb) * kTK + c32];
+            const uint32_t i0 = ia + t % nt * kTK;
+            const bool none = off == INFINITY;  // no query: 0 against a key that is not finite too
+            if (kw + 32 * KB + n > ctx + i0 + 1 || __any(none)) {  // some row does not see all of the wave's keys
+                const uint32_t lim = !none && ctx + i0 + c32 >= n ? ctx + i0 + c32 - n + 1 : 0u;
+                #pragma unroll
+                for (int i = 0; i < KB; ++i)
+                    #pragma unroll
+                    for (int y = 0; y < 16; ++y) {
+                        const uint32_t j = kw + 32 * i + 8 * (y >> 2) + 4 * g + (y & 3);
+                        const float e = exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
+                        acc[i][y] += j < lim ? e : 0.0f;
+                    }
+            } else {
+                #pragma unroll
+                for (int i = 0; i < KB; ++i)
+                    #pragma unroll
+                    for (int y = 0; y < 16; ++y)
+                        acc[i][y] += exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
             }
         }
-        const size_t at = list * p.cap + j;
-        p.w_out[at] = p.w ? fmaf(p.decay, p.w[at], sum) : sum;
     }
+    // A key's sum over the 32 lanes of its half: halving exchanges, 16 registers to 1. Lane bit s then picked register
+    // bit s, so lane (g, c32) ends with register c32 % 16 summed over all lanes but bit 4, which the last one adds.
+    #pragma unroll
+    for (int i = 0; i < KB; ++i) {
+        #pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const bool up = lane >> s & 1;
+            #pragma unroll
+            for (int y = 0; y < 8 >> s; ++y) {
+                const float keep = up ? acc[i][2 * y + 1] : acc[i][2 * y], give = up ? acc[i][2 * y] : acc[i][2 * y + 1];
+                acc[i][y] = keep + __shfl_xor(give, 1 << s);
+            }
+        }
+        const float sum = acc[i][0] + __shfl_xor(acc[i][0], 16);
+        const uint32_t y = c32 & 15, j = kw + 32 * i + 8 * (y >> 2) + 4 * g + (y & 3);
+        if (c32 < 16 && j < ctx) {
+            if (p.n_chunks > 1)
+                p.part[((size_t)chunk * lists + list) * p.max_ctx + j] = sum;
+            else
+                p.w_out[(size_t)list * p.cap + j] =
+                    p.w ? fmaf(p.decay, p.w[(size_t)list * p.cap + j], sum) : sum;
+        }
+    }
+}
+
+// The chunks' sums of each key, in order (those that saw a key of its block wrote one).
+__global__ __launch_bounds__(256) void weights_join(const WeightsParams p, uint32_t keys, uint32_t per_list)
+{
+    const uint32_t lists = p.batch * p.kv_heads, list = blockIdx.x / per_list, b = list / p.kv_heads;
+    const uint32_t ctx = ctx_of(p, b), n = n_of(p, b), j = blockIdx.x % per_list * 256 + threadIdx.x;
+    if (j >= ctx)
+        return;
+    const uint32_t k0 = j / keys * keys, see0 = k0 + n > ctx ? k0 + n - ctx : 0u;
+    float sum = 0.0f;
+    for (uint32_t c = min(see0, n) / p.chunk; c < p.n_chunks && max(c * p.chunk, see0) < n; ++c)
+        sum += p.part[((size_t)c * lists + list) * p.max_ctx + j];
+    const size_t at = (size_t)list * p.cap + j;
+    p.w_out[at] = p.w ? fmaf(p.decay, p.w[at], sum) : sum;
+}
+
+// A call's shape, from its sizes alone.
+struct Plan {
+    bool few;
+    uint32_t keys, n_blocks, chunk, n_chunks;
+};
+
+Plan plan_of(const mako_weights_args* a, uint32_t cus)
+{
+    const uint64_t rows = (uint64_t)a->n_q * (a->heads / a->kv_heads);
+    Plan pl{rows <= kFewRows, 0, 0, 0, 1};
+    if (pl.few)
+        return pl;
+    pl.keys = a->dim == 256 ? Many<256>::kKeys : Many<128>::kKeys;
+    pl.n_blocks = (a->max_ctx + pl.keys - 1) / pl.keys;
+    const uint64_t units = std::max<uint64_t>(1, (uint64_t)a->batch * a->kv_heads * pl.n_blocks);
+    const uint32_t want = (uint32_t)std::min<uint64_t>(64, (8ull * cus + units - 1) / units);
+    const uint32_t most = (a->n_q + 63) / 64;  // at least 64 queries a chunk
+    pl.n_chunks = std::max(1u, std::min(want, most));
+    pl.chunk = (a->n_q + pl.n_chunks * 32 - 1) / (pl.n_chunks * 32) * 32;
+    pl.n_chunks = (a->n_q + pl.chunk - 1) / pl.chunk;
+    return pl;
+}
+
+size_t workspace_for(const Plan& pl, const mako_weights_args* a)
+{
+    return pl.n_chunks > 1 ? (size_t)pl.n_chunks * a->batch * a->kv_heads * a->max_ctx * sizeof(float) : 0;
+}
+
+template <class T, int D>
+void launch(const WeightsParams& p, const Plan& pl, hipStream_t s)
+{
+    if (pl.few) {
+        const dim3 grid(p.n_ranges / Few<D>::kWaves);
+        if (p.n_q * p.group <= 32)
+            hipLaunchKernelGGL((weights_few<T, D, 1>), grid, dim3(256), 0, s, p);
+        else
+            hipLaunchKernelGGL((weights_few<T, D, 2>), grid, dim3(256), 0, s, p);
+        return;
+    }
+    const uint32_t lists = p.batch * p.kv_heads;
+    hipLaunchKernelGGL((weights_many<T, D>), dim3(lists * p.n_blocks * p.n_chunks), dim3(256), 0, s, p);
+    if (p.n_chunks > 1) {
+        const uint32_t per_list = (p.max_ctx + 255) / 256;
+        hipLaunchKernelGGL(weights_join, dim3(lists * per_list), dim3(256), 0, s, p, pl.keys, per_list);
+    }
+}
+
+template <class T>
+void launch_dim(const WeightsParams& p, uint32_t dim, const Plan& pl, hipStream_t s)
+{
+    if (dim == 64)
+        launch<T, 64>(p, pl, s);
+    else if (dim == 128)
+        launch<T, 128>(p, pl, s);
+    else
+        launch<T, 256>(p, pl, s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -88,18 +483,36 @@ int check_args(const mako_weights_args* a, mako_dtype in, const void* q, const f
 
 using namespace mako;
 
-extern "C" size_t mako_cache_weights_workspace(const mako_weights_args*) { return 0; }
+extern "C" size_t mako_cache_weights_workspace(const mako_weights_args* a)
+{
+    const uint32_t cus = device_cus();
+    if (!a || !cus || !a->heads || !a->kv_heads || a->heads % a->kv_heads)
+        return 0;
+    return workspace_for(plan_of(a, cus), a);
+}
 
 extern "C" int mako_cache_weights(const mako_weights_args* a, mako_dtype in, const void* q, const float* lse,
                                   const void* k, const uint32_t* ctx_len, const uint32_t* path, const uint32_t* n_path,
-                                  const float* w, float* w_out, void*, size_t, void* stream)
+                                  const float* w, float* w_out, void* workspace, size_t workspace_bytes, void* stream)
 {
+    const char* what = "cache_weights";
     if (const int rc = check_args(a, in, q, lse, k, ctx_len, w_out))
         return rc;
     if (a->batch == 0 || a->max_ctx == 0)
         return ok();
-    WeightsParams p{q, k, lse, a->decay == 0.0f ? nullptr : w, w_out, ctx_len, path, n_path, a->batch, a->n_q, a->heads,
-                    a->kv_heads, a->heads / a->kv_heads, a->dim, a->cap, a->max_ctx, 0, 0, 0, 0, a->scale * kLog2e,
+    const uint32_t cus = device_cus();
+    if (!cus)
+        return fail(MAKO_EHIP, "%s: no device to size the split for", what);
+    const Plan pl = plan_of(a, cus);
+    const size_t need = workspace_for(pl, a);
+    if (workspace_bytes < need || (need && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 16)
+        return fail(MAKO_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, workspace_bytes,
+                    need);
+    if ((uint64_t)a->batch * a->kv_heads * std::max(1u, pl.n_blocks) * pl.n_chunks > 0x7fffffffu)
+        return fail(MAKO_EINVAL, "%s: %u x %u lists exceed the grid", what, a->batch, a->kv_heads);
+    WeightsParams p{q, k, lse, a->decay == 0.0f ? nullptr : w, w_out, ctx_len, path, n_path,
+                    static_cast<float*>(workspace), a->batch, a->n_q, a->heads, a->kv_heads, a->heads / a->kv_heads,
+                    a->cap, a->max_ctx, 4 * cus, pl.chunk, pl.n_chunks, pl.n_blocks, 0, 0, 0, 0, a->scale * kLog2e,
                     a->decay};
     if (a->q_pad) {
         p.qs_b = (uint64_t)a->n_q * a->dim, p.qs_h = (uint64_t)a->q_pad * a->dim;
@@ -109,10 +522,9 @@ extern "C" int mako_cache_weights(const mako_weights_args* a, mako_dtype in, con
         p.ls_b = (uint64_t)a->heads * a->n_q, p.ls_h = a->n_q;
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const dim3 grid(a->batch * a->kv_heads);
     if (in == MAKO_BF16)
-        hipLaunchKernelGGL(weights_keys<__bf16>, grid, dim3(256), 0, s, p);
+        launch_dim<__bf16>(p, a->dim, pl, s);
     else
-        hipLaunchKernelGGL(weights_keys<_Float16>, grid, dim3(256), 0, s, p);
-    return check_launch("cache_weights");
+        launch_dim<_Float16>(p, a->dim, pl, s);
+    return check_launch(what);
 }

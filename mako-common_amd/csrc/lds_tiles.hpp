@@ -23,6 +23,14 @@ __device__ __forceinline__ u32x4 tile_rsrc(const void* base, uint32_t bytes)
     return u32x4{(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, bytes, 0x00020000u};
 }
 
+// Where 16-byte chunk c of row s (16-bit heads of D) sits in its LDS row: XORed so that the 16 rows a ds_read_b128 spans start in distinct
+// banks (rows of 128 bytes: two fill the 64 banks).
+template <int D>
+__device__ __forceinline__ uint32_t k_xor(uint32_t s)
+{
+    return D == 64 ? (s >> 1) & 7u : s & 15u;
+}
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 

@@ -374,6 +374,33 @@ def test_weights_queries_that_saw_nothing():
     run_weights(dt=F16, dim=128, heads=2, kv=1, ctx=[150], n=30, form="rows", lse_set=some, seed=41)
 
 
+@pytest.mark.parametrize("n", [4, 200])
+def test_weights_of_keys_that_hold_anything(n):
+    """A key that is not finite: its weight is NaN where a query sees it, its old weight where none does, and no other
+    key's changes."""
+    heads, kv, dim, ctx = 2, 1, 64, 300
+    g = gen(43)
+    k, q = randn(g, (1, kv, ctx, dim), F16), randn(g, (heads, n, dim), F16)
+    lse = torch.full((heads, n), 4.0, device="cuda")
+    lse[:, n - 2:] = -float("inf")  # the last two queries, and so the last two keys, are out
+    w = torch.rand((1, kv, ctx), generator=g, device="cuda")
+    a = M.weights_args(batch=1, n_q=n, heads=heads, kv_heads=kv, dim=dim, cap=ctx, max_ctx=ctx)
+    ws, outs = buffer(M.cache_weights_workspace(a)), []
+    for bad in (None, NAN, float("inf")):
+        if bad is not None:
+            k[:, :, [5, ctx - 40, ctx - 1], ::9] = bad
+        out = torch.zeros_like(w)
+        M.cache_weights(a, q, lse, k, i32([ctx]), out, ws, w=w)
+        torch.cuda.synchronize()
+        outs.append(out)
+    for out in outs[1:]:
+        assert torch.isnan(out[..., 5]).all() or torch.isinf(out[..., 5]).all()
+        assert torch.equal(out[..., ctx - 1], w[..., ctx - 1])
+        fine = torch.ones(ctx, dtype=torch.bool, device="cuda")
+        fine[[5, ctx - 40, ctx - 1]] = False
+        assert torch.equal(out[..., fine], outs[0][..., fine])
+
+
 def test_weights_sum_to_the_queries():
     """A whole prompt's weights sum to its queries times the heads of a group, over mako_attn_fwd's lse."""
     n, heads, kv = 1000, 8, 2
