@@ -25,6 +25,7 @@
 //   segment (unique: pieces are intervals between consecutive boundaries), which tree_merge joins. Short contexts take a
 //   segment a workgroup and no merge.
 #include <algorithm>
+#include <type_traits>
 
 #include "lds_tiles.hpp"
 #include "split_ranges.hpp"
@@ -42,6 +43,7 @@ struct TreeParams {
     float* part_o;   // [pieces][nc][D]
     float* part_ml;  // [pieces][nc][2]: maximum (base 2), sum
     uint32_t* part_odd;  // [pieces]: a draft's V holds what is not finite
+    uint32_t* seg_ends;  // [segments][2]: the first and the last range of each
     uint32_t batch, n_draft, q_pad, d_pad, heads, kv_heads, group, cap, max_ctx, width;
     uint32_t nc, ncb;   // columns (n_draft x group), column blocks
     uint32_t ways;      // tiles a step
@@ -198,32 +200,62 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
         va[i] = kHalf + (8 * g + gj) * kRow + 32 * v_unit<D>(2 * i + gg, gj) + 8 * gy;
 
     // The first piece of the range (or the segment).
-    uint32_t b, kvh, s0, s1, left = 0;  // steps [s0, s1) of the segment; steps of the range behind them
+    uint32_t b, kvh, len, s0, s1, left = 0;  // steps [s0, s1) of the segment's len; steps of the range behind them
     if (p.n_ranges) {
-        const Ranges rg(uniform(sum_of(p.batch, lane, SegSteps{p}) * p.kv_heads), p.n_ranges);
-        const uint32_t x0 = rg.start(range), x1 = rg.start(range + 1);
-        if (x0 >= x1)
+        const uint32_t total = uniform(sum_of(p.batch, lane, SegSteps{p}) * p.kv_heads);
+        if (range >= total)
             return;
+        const Ranges rg(total, min(total, p.n_ranges));  // (none is empty)
+        const uint32_t x0 = rg.start(range), x1 = rg.start(range + 1);
         uint32_t first;
         seq_of(p.batch, x0, lane, SegSteps{p}, p.kv_heads, b, first);
         b = uniform(b);
-        const uint32_t len = uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b)));
+        len = uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b)));
         kvh = (x0 - uniform(first)) / len;
         s0 = (x0 - uniform(first)) % len;
         s1 = min(len, s0 + (x1 - x0));
         left = x1 - x0 - (s1 - s0);
     } else {
         b = range / p.kv_heads, kvh = range % p.kv_heads, s0 = 0;
-        s1 = uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b)));
+        s1 = len = uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b)));
     }
 
     for (;;) {
         const uint32_t ctx = uniform(ctx_of(p, b)), nodes = uniform(nodes_of(p, b)), tc = (ctx + kTK - 1) / kTK;
-        // The lane's column: row r, head h; its mask, cut to the tree.
+        const size_t cache = ((size_t)b * p.kv_heads + kvh) * p.cap * D;
+        const size_t draft = ((size_t)kvh * p.d_pad + (size_t)b * p.n_draft) * D;
+        const u32x4 rs[4] = {tile_rsrc(static_cast<const T*>(p.k) + cache, ctx * kRow),
+                             tile_rsrc(static_cast<const T*>(p.v) + cache, ctx * kRow),
+                             tile_rsrc(static_cast<const T*>(p.kd) + draft, nodes * kRow),
+                             tile_rsrc(static_cast<const T*>(p.vd) + draft, nodes * kRow)};
+        // The tile of way kw in step s into its ring slot (past the segment's tiles: rows past the tree, zeros). Streaming
+        // loads where no other workgroup reads the keys.
+        auto stage = [&](uint32_t s) __attribute__((always_inline)) {
+            const uint32_t t = s * KW + kw, dst = lbase + (s % S::kDepth * KW + kw) * S::kSlot + 1024 * cg * kPieces;
+            const uint32_t off = (t < tc ? t : t - tc) * kHalf;
+            const u32x4 k = t < tc ? rs[0] : rs[2], v = t < tc ? rs[1] : rs[3];
+            if (NG < 4 || p.ncb == 1) {
+                #pragma unroll
+                for (int m = 0; m < kPieces; ++m)
+                    dma16_nt(dst + 1024 * m, kd[m] + off, k);
+                #pragma unroll
+                for (int m = 0; m < kPieces; ++m)
+                    dma16_nt(dst + kHalf + 1024 * m, vd[m] + off, v);
+            } else {
+                #pragma unroll
+                for (int m = 0; m < kPieces; ++m)
+                    dma16_at(dst + 1024 * m, kd[m] + off, 0, k);
+                #pragma unroll
+                for (int m = 0; m < kPieces; ++m)
+                    dma16_at(dst + kHalf + 1024 * m, vd[m] + off, 0, v);
+            }
+        };
+        for (uint32_t s = s0; s < min(s1, s0 + S::kDepth - 1); ++s)
+            stage(s);
+        // The lane's column: row r, head h; its mask, cut to the tree; Q, beside the first tiles' loads.
         const uint32_t col = 32 * (cb * NG + cg) + c32, r = col / p.group, h = kvh * p.group + col % p.group;
         const bool has = col < p.nc && r < nodes;
         uint64_t sees = has ? sees_of(p, b, r, nodes) : 0;
-        asm volatile("" : "+v"(sees));  // arrived before the tiles' loads
         V8 qreg[NK];
         {
             const T* src = static_cast<const T*>(p.q) + ((size_t)h * p.q_pad + (size_t)b * p.n_draft + r) * D + 8 * g;
@@ -231,31 +263,7 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
             for (int kk = 0; kk < NK; ++kk)
                 qreg[kk] = has ? *reinterpret_cast<const V8*>(src + 16 * kk) : V8{};
         }
-        const size_t cache = ((size_t)b * p.kv_heads + kvh) * p.cap * D;
-        const size_t draft = ((size_t)kvh * p.d_pad + (size_t)b * p.n_draft) * D;
-        const u32x4 rs[4] = {tile_rsrc(static_cast<const T*>(p.k) + cache, ctx * kRow),
-                             tile_rsrc(static_cast<const T*>(p.v) + cache, ctx * kRow),
-                             tile_rsrc(static_cast<const T*>(p.kd) + draft, nodes * kRow),
-                             tile_rsrc(static_cast<const T*>(p.vd) + draft, nodes * kRow)};
-        // The tile of way kw in step s into its ring slot (past the segment's tiles: rows past the tree, zeros).
-        auto stage = [&](uint32_t s) __attribute__((always_inline)) {
-            const uint32_t t = s * KW + kw, dst = lbase + (s % S::kDepth * KW + kw) * S::kSlot + 1024 * cg * kPieces;
-            if (t < tc) {
-                #pragma unroll
-                for (int m = 0; m < kPieces; ++m)
-                    dma16_at(dst + 1024 * m, kd[m] + t * kHalf, 0, rs[0]);
-                #pragma unroll
-                for (int m = 0; m < kPieces; ++m)
-                    dma16_at(dst + kHalf + 1024 * m, vd[m] + t * kHalf, 0, rs[1]);
-            } else {
-                #pragma unroll
-                for (int m = 0; m < kPieces; ++m)
-                    dma16_at(dst + 1024 * m, kd[m] + (t - tc) * kHalf, 0, rs[2]);
-                #pragma unroll
-                for (int m = 0; m < kPieces; ++m)
-                    dma16_at(dst + kHalf + 1024 * m, vd[m] + (t - tc) * kHalf, 0, rs[3]);
-            }
-        };
+        asm volatile("" : "+v"(sees));
         f32x16 acc[ND];
         #pragma unroll
         for (int db = 0; db < ND; ++db)
@@ -268,10 +276,8 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
         #pragma unroll
         for (int kk = 0; kk < NK; ++kk)
             settle(qreg[kk]);
-        for (uint32_t s = s0; s < min(s1, s0 + S::kDepth - 1); ++s)
-            stage(s);
-        for (uint32_t s = s0; s < s1; ++s) {
-            // Step s has landed; every wave is done with step s - 1, whose slots take step s + DEPTH - 1.
+        // Step s has landed; every wave is done with step s - 1, whose slots take step s + DEPTH - 1.
+        auto arrive = [&](uint32_t s) __attribute__((always_inline)) {
             if (s + S::kDepth - 1 <= s1)
                 asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::kDepth - 2) * 2 * kPieces) : "memory");
             else
@@ -280,76 +286,96 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                 asm volatile("s_barrier" ::: "memory");
             if (s + S::kDepth - 1 < s1)
                 stage(s + S::kDepth - 1);
+        };
+        // The wave's tile of step s; CUT: one that not every column sees all of.
+        auto tile_step = [&](auto cut, uint32_t s) __attribute__((always_inline)) {
+            constexpr bool CUT = decltype(cut)::value;
             const uint32_t t = s * KW + kw;
             unsigned char* tile = lds + (s % S::kDepth * KW + kw) * S::kSlot;
-            if (t * kTK < tc * kTK + nodes) {
-                f32x16 x = f32x16{};
+            f32x16 x = f32x16{};
+            #pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+                x = E::mfma32(*reinterpret_cast<const V8*>(tile + (ka ^ (32 * kk))), qreg[kk], x);
+            if (CUT && t >= tc)
+                odd |= finite_only<T, kHalf>(tile + kHalf, lane);
+            // V^T's operands come while the exponentials are made.
+            V8 vf[2][ND];
+            #pragma unroll
+            for (int a = 0; a < 2; ++a)
                 #pragma unroll
-                for (int kk = 0; kk < NK; ++kk)
-                    x = E::mfma32(*reinterpret_cast<const V8*>(tile + (ka ^ (32 * kk))), qreg[kk], x);
-                // Register i holds key 16 (i / 8) + 8 g + i % 8 of the tile.
+                for (int db = 0; db < ND; ++db) {
+                    const unsigned char* at = tile + va[db % NV] + db / NV * 256 + 16 * a * kRow;
+                    const s16x4 v0 = tr_read(at), v1 = tr_read(at + 4 * kRow);
+                    vf[a][db] = __builtin_bit_cast(V8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            // Register i holds key 16 (i / 8) + 8 g + i % 8 of the tile.
+            #pragma unroll
+            for (int i = 0; i < 16; ++i)
+                x[i] *= c;
+            if (CUT) {
+                uint32_t word;
+                if (t >= tc)
+                    word = (uint32_t)(sees >> (32 * (t - tc)));
+                else
+                    word = (t + 1) * kTK <= ctx ? ~0u : (1u << (ctx - t * kTK)) - 1;
+                word >>= 8 * g;
                 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    x[i] *= c;
-                const bool drafts = t >= tc;
-                const uint32_t word = drafts ? (uint32_t)(sees >> (32 * (t - tc))) : 0u;
-                if (drafts) {
-                    #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        x[i] = word >> (16 * (i >> 3) + (i & 7) + 8 * g) & 1 ? x[i] : -INFINITY;
-                } else if ((t + 1) * kTK > ctx) {
-                    #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        x[i] = t * kTK + 16 * (i >> 3) + 8 * g + (i & 7) < ctx ? x[i] : -INFINITY;
-                }
-                float mx = x[0];
-                #pragma unroll
-                for (int i = 1; i < 16; ++i)
-                    mx = fmaxf(mx, x[i]);
-                mx = pair_max(mx);
+                    x[i] = word >> (16 * (i >> 3) + (i & 7)) & 1 ? x[i] : -INFINITY;
+            }
+            float mx = fmaxf(x[0], x[1]);
+            #pragma unroll
+            for (int i = 2; i < 16; i += 2)
+                mx = fmaxf(fmaxf(mx, x[i]), x[i + 1]);
+            mx = pair_max(mx);
+            if (__any(mx > m + kRescale)) {
                 float f = 1.0f;
                 if (mx > m + kRescale) {
                     f = exp2_fast(m - mx);
                     m = mx;
                 }
-                if (__any(f != 1.0f)) {
-                    l *= f;
+                l *= f;
+                #pragma unroll
+                for (int db = 0; db < ND; ++db)
+                    #pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        acc[db][i] *= f;
+            }
+            const float mu = m == -INFINITY ? 0.0f : m;
+            #pragma unroll
+            for (int i = 0; i < 16; ++i)
+                x[i] = exp2_fast(x[i] - mu);
+            l += ((x[0] + x[1]) + (x[2] + x[3]) + ((x[4] + x[5]) + (x[6] + x[7]))) +
+                 ((x[8] + x[9]) + (x[10] + x[11]) + ((x[12] + x[13]) + (x[14] + x[15])));
+            #pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                u32x4 hi, lo;
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e0 = x[8 * a + 2 * i], e1 = x[8 * a + 2 * i + 1];
+                    hi[i] = E::pack2(e0, e1);
+                    if (kSplitP)
+                        lo[i] = E::pack2(e0 - value_of<T>(hi[i], 0), e1 - value_of<T>(hi[i], 1));
+                }
+                #pragma unroll
+                for (int db = 0; db < ND; ++db)
+                    acc[db] = E::mfma32(vf[a][db], __builtin_bit_cast(V8, hi), acc[db]);
+                if (kSplitP)
                     #pragma unroll
                     for (int db = 0; db < ND; ++db)
-                        #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            acc[db][i] *= f;
-                }
-                const float mu = m == -INFINITY ? 0.0f : m;
-                #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    x[i] = exp2_fast(x[i] - mu);
-                    l += x[i];
-                }
-                if (drafts)
-                    odd |= finite_only<T, kHalf>(tile + kHalf, lane);
-                #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    u32x4 hi, lo;
-                    #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e0 = x[8 * a + 2 * i], e1 = x[8 * a + 2 * i + 1];
-                        hi[i] = E::pack2(e0, e1);
-                        if (kSplitP)
-                            lo[i] = E::pack2(e0 - value_of<T>(hi[i], 0), e1 - value_of<T>(hi[i], 1));
-                    }
-                    #pragma unroll
-                    for (int db = 0; db < ND; ++db) {
-                        const unsigned char* at = tile + va[db % NV] + db / NV * 256 + 16 * a * kRow;
-                        const s16x4 v0 = tr_read(at), v1 = tr_read(at + 4 * kRow);
-                        const V8 vv =
-                            __builtin_bit_cast(V8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-                        acc[db] = E::mfma32(vv, __builtin_bit_cast(V8, hi), acc[db]);
-                        if (kSplitP)
-                            acc[db] = E::mfma32(vv, __builtin_bit_cast(V8, lo), acc[db]);
-                    }
-                }
+                        acc[db] = E::mfma32(vf[a][db], __builtin_bit_cast(V8, lo), acc[db]);
             }
+        };
+        uint32_t s = s0;
+        for (const uint32_t whole = min(s1, ctx / kTK / KW); s < whole; ++s) {
+            arrive(s);
+            tile_step(std::false_type{}, s);
+        }
+        for (; s < s1; ++s) {
+            arrive(s);
+            if ((s * KW + kw) * kTK < tc * kTK + nodes)
+                tile_step(std::true_type{}, s);
         }
         // The piece's ways join: every wave's columns into LDS (the ring is idle: nothing is in flight), column c32 a row of
         // D floats, its 16-byte chunks XORed by the column.
@@ -371,8 +397,13 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
         __syncthreads();
         const size_t part = (size_t)range + (size_t)b * p.kv_heads + kvh;
         const bool any_odd = s_odd != 0;
-        if (p.n_ranges && tid == 0 && cb == 0)
+        if (p.n_ranges && tid == 0 && cb == 0) {
             p.part_odd[part] = any_odd;
+            if (s0 == 0)
+                p.seg_ends[2 * (b * p.kv_heads + kvh)] = range;
+            if (s1 == len)
+                p.seg_ends[2 * (b * p.kv_heads + kvh) + 1] = range;
+        }
         for (uint32_t it = tid; it < NG * 32 * (D / 4); it += W * 64) {
             const uint32_t q = it % (D / 4), cc = it / (D / 4) % 32, gi = it / (D / 4) / 32;
             const uint32_t ccol = 32 * (cb * NG + gi) + cc, rr = ccol / p.group;
@@ -416,104 +447,91 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                 kvh = 0;
                 ++b;
             }
-            s1 = b < p.batch ? uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b))) : 0u;
-        } while (b < p.batch && s1 == 0);
+            len = b < p.batch ? uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b))) : 0u;
+        } while (b < p.batch && len == 0);
         if (b >= p.batch)
             return;
         s0 = 0;
-        s1 = min(s1, left);
+        s1 = min(len, left);
         left -= s1;
     }
 }
 
-// One workgroup a row and head: each wave every kMergeWaves-th piece of its segment, up to 4 loads in flight, a running
-// maximum; the waves join in LDS.
-constexpr int kMergeWaves = 4;
-
-template <class T, class TO, int D>
-__global__ __launch_bounds__(kMergeWaves * 64) void tree_merge(const TreeParams p, TO* __restrict__ o,
-                                                                float* __restrict__ lse)
+// NW waves a row and head, each every NW-th piece of its segment: a running maximum, 8 pieces' loads in flight, and with
+// more than one wave a join in LDS.
+template <class T, class TO, int D, int NW>
+__global__ __launch_bounds__(256) void tree_merge(const TreeParams p, TO* __restrict__ o, float* __restrict__ lse)
 {
-    constexpr int E = D / 64;
-    __shared__ float s_m[kMergeWaves], s_l[kMergeWaves], s_o[kMergeWaves][D];
-    const uint32_t lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    const uint32_t row = blockIdx.x / p.heads, h = blockIdx.x % p.heads, b = row / p.n_draft, r = row % p.n_draft;
-    const uint32_t nodes = nodes_of(p, b);
+    constexpr int E = D / 64, U = 8;
+    typedef float fE __attribute__((ext_vector_type(E)));
+    __shared__ float s_m[4], s_l[4];
+    __shared__ fE s_o[4][64];
+    const uint32_t lane = threadIdx.x & 63, wl = uniform(threadIdx.x >> 6), wv = wl % NW;
+    const uint32_t item = blockIdx.x * (4 / NW) + wl / NW, row = item / p.heads, h = item % p.heads;
+    const uint32_t b = row / p.n_draft, r = row % p.n_draft;
+    if (row >= p.batch * p.n_draft)
+        return;  // (with NW = 4 the whole workgroup)
+    const uint32_t nodes = uniform(nodes_of(p, b));
     if (r >= nodes)
         return;
     const uint32_t kvh = h / p.group, col = r * p.group + h % p.group, seg = b * p.kv_heads + kvh;
-    const uint32_t len = steps_of(p, ctx_of(p, b), nodes);
-    const uint32_t first = sum_of(b, lane, SegSteps{p}) * p.kv_heads + kvh * len;
-    const Ranges rg(sum_of(p.batch, lane, SegSteps{p}) * p.kv_heads, p.n_ranges);
-    const uint32_t w0 = rg.of(first), w1 = rg.of(first + len - 1);
-    float m = -INFINITY, l = 0.0f, acc[E];
-    #pragma unroll
-    for (int e = 0; e < E; ++e)
-        acc[e] = 0.0f;
-    constexpr int U = 4;
-    for (uint32_t x0 = w0 + wv; x0 <= w1; x0 += U * kMergeWaves) {
+    const uint32_t w0 = uniform(p.seg_ends[2 * seg]), w1 = uniform(p.seg_ends[2 * seg + 1]);
+    bool odd = false;
+    for (uint32_t x = w0 + lane; x <= w1; x += 64)
+        odd = odd || p.part_odd[x + seg];
+    float m = -INFINITY, l = 0.0f;
+    fE acc = fE(0.0f);
+    for (uint32_t x0 = w0 + wv; x0 <= w1; x0 += U * NW) {
         float2 ml[U];
-        float v[U][E];
+        fE v[U];
         #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t x = x0 + u * kMergeWaves;
-            const bool live = x <= w1 && rg.start(x) < rg.start(x + 1);  // (an empty range wrote nothing)
-            const size_t at = ((size_t)(live ? x : w0) + seg) * p.nc + col;
-            ml[u] = live ? *reinterpret_cast<const float2*>(p.part_ml + at * 2) : float2{-INFINITY, 0.0f};
-            #pragma unroll
-            for (int e = 0; e < E; ++e)
-                v[u][e] = live ? p.part_o[at * D + 64 * e + lane] : 0.0f;
+            const uint32_t x = x0 + u * NW;
+            const size_t at = ((size_t)min(x, w1) + seg) * p.nc + col;
+            ml[u] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+            v[u] = *reinterpret_cast<const fE*>(p.part_o + at * D + E * lane);
+            if (x > w1)
+                ml[u].x = -INFINITY;
         }
         #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float nm = fmaxf(m, ml[u].x);
-            const float f = m == -INFINITY ? 0.0f : exp2_fast(m - nm), g = ml[u].x == -INFINITY ? 0.0f : exp2_fast(ml[u].x - nm);
-            l = l * f + ml[u].y * g;
-            #pragma unroll
-            for (int e = 0; e < E; ++e)
-                acc[e] = acc[e] * f + v[u][e] * g;
+            const float f = m == -INFINITY ? 0.0f : exp2_fast(m - nm);
+            const float e = ml[u].x == -INFINITY ? 0.0f : exp2_fast(ml[u].x - nm);
+            l = l * f + ml[u].y * e;
+            acc = acc * f + v[u] * e;
             m = nm;
         }
     }
-    if (lane == 0) {
-        s_m[wv] = m;
-        s_l[wv] = l;
+    if (NW > 1) {
+        if (lane == 0) {
+            s_m[wl] = m;
+            s_l[wl] = l;
+        }
+        s_o[wl][lane] = acc;
+        __syncthreads();
+        if (wv != 0)
+            return;
+        #pragma unroll
+        for (int i = 1; i < NW; ++i) {
+            const float mi = s_m[i], nm = fmaxf(m, mi);
+            const float f = m == -INFINITY ? 0.0f : exp2_fast(m - nm), e = mi == -INFINITY ? 0.0f : exp2_fast(mi - nm);
+            l = l * f + s_l[i] * e;
+            acc = acc * f + s_o[i][lane] * e;
+            m = nm;
+        }
     }
+    acc *= l == 0.0f ? 0.0f : 1.0f / l;
+    if (__any(odd))
+        #pragma unroll
+        for (int e = 0; e < E; ++e)
+            acc[e] += odd_sum<T, D>(p, b, kvh, r, nodes, E * lane + e);
+    TO* orow = o + (size_t)row * p.width + (size_t)h * D + E * lane;
     #pragma unroll
     for (int e = 0; e < E; ++e)
-        s_o[wv][64 * e + lane] = acc[e];
-    __syncthreads();
-    if (wv != 0)
-        return;
-    float mx = s_m[0];
-    #pragma unroll
-    for (int i = 1; i < kMergeWaves; ++i)
-        mx = fmaxf(mx, s_m[i]);
-    float sum = 0.0f, f[kMergeWaves];
-    #pragma unroll
-    for (int i = 0; i < kMergeWaves; ++i) {
-        f[i] = s_m[i] == -INFINITY ? 0.0f : exp2_fast(s_m[i] - mx);
-        sum += s_l[i] * f[i];
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    bool odd = false;
-    for (uint32_t x = w0 + lane; x <= w1; x += 64)
-        odd = odd || (rg.start(x) < rg.start(x + 1) && p.part_odd[x + seg]);
-    odd = __any(odd);
-    TO* orow = o + (size_t)row * p.width + (size_t)h * D;
-    #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        float x = 0.0f;
-        #pragma unroll
-        for (int i = 0; i < kMergeWaves; ++i)
-            x += s_o[i][64 * e + lane] * f[i];
-        x *= inv;
-        if (odd)
-            x += odd_sum<T, D>(p, b, kvh, r, nodes, 64 * e + lane);
-        orow[64 * e + lane] = (TO)x;
-    }
+        orow[e] = (TO)acc[e];
     if (lse && lane == 0)
-        lse[(size_t)h * p.batch * p.n_draft + row] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * kLn2;
+        lse[(size_t)h * p.batch * p.n_draft + row] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
 // A call's split, from its sizes alone (contexts are known on the device only).
@@ -560,7 +578,9 @@ size_t part_ml_bytes(const Plan& pl, const mako_tree_args* a)
 }
 size_t workspace_for(const Plan& pl, const mako_tree_args* a)
 {
-    return part_o_bytes(pl, a) + part_ml_bytes(pl, a) + pl.pieces * sizeof(uint32_t);
+    return pl.pieces ? part_o_bytes(pl, a) + part_ml_bytes(pl, a) + round256(pl.pieces * sizeof(uint32_t)) +
+                           (size_t)a->batch * a->kv_heads * 2 * sizeof(uint32_t)
+                     : 0;
 }
 
 template <class T, class TO, int D, int NG>
@@ -580,9 +600,14 @@ void launch(const TreeParams& p, uint32_t ng, void* o, float* lse, hipStream_t s
         launch_split<T, TO, D, 2>(p, o, lse, s);
     else
         launch_split<T, TO, D, 4>(p, o, lse, s);
-    if (p.n_ranges)
-        hipLaunchKernelGGL((tree_merge<T, TO, D>), dim3(p.batch * p.n_draft * p.heads), dim3(kMergeWaves * 64), 0, s, p,
-                           static_cast<TO*>(o), lse);
+    if (!p.n_ranges)
+        return;
+    // a wave an item where segments have few pieces (n_ranges of them over all, and a cut one more each)
+    const uint32_t items = p.batch * p.n_draft * p.heads;
+    if (p.n_ranges / (p.batch * p.kv_heads) < 8)
+        hipLaunchKernelGGL((tree_merge<T, TO, D, 1>), dim3((items + 3) / 4), dim3(256), 0, s, p, static_cast<TO*>(o), lse);
+    else
+        hipLaunchKernelGGL((tree_merge<T, TO, D, 4>), dim3(items), dim3(256), 0, s, p, static_cast<TO*>(o), lse);
 }
 
 template <class T, class TO>
@@ -672,9 +697,10 @@ extern "C" int mako_attn_tree(const mako_tree_args* a, mako_dtype in, mako_dtype
                     need);
     const uint32_t group = a->heads / a->kv_heads;
     const auto at = [&](size_t off) { return need ? static_cast<char*>(workspace) + off : nullptr; };
-    const size_t ob = part_o_bytes(pl, a), mb = part_ml_bytes(pl, a);
+    const size_t ob = part_o_bytes(pl, a), mb = part_ml_bytes(pl, a), fb = round256(pl.pieces * sizeof(uint32_t));
     const TreeParams p{q, k, v, kd, vd, ctx_len, n_nodes, mask, reinterpret_cast<float*>(at(0)),
                        reinterpret_cast<float*>(at(ob)), reinterpret_cast<uint32_t*>(at(ob + mb)),
+                       reinterpret_cast<uint32_t*>(at(ob + mb + fb)),
                        a->batch, a->n_draft, a->q_pad, a->d_pad, a->heads, a->kv_heads, group, a->cap, a->max_ctx,
                        a->width, a->n_draft * group, pl.ncb, pl.ways, pl.n_ranges, a->scale * kLog2e};
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -16,6 +16,17 @@ __device__ __forceinline__ void dma16_at(uint32_t m0, uint32_t voff, uint32_t so
 #pragma clang diagnostic pop
 }
 
+// The same as a streaming (non-temporal) load, for bytes that one workgroup reads once.
+__device__ __forceinline__ void dma16_nt(uint32_t m0, uint32_t voff, u32x4 rsrc)
+{
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(m0), "v"(voff),
+                 "s"(rsrc)
+                 : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
 // A buffer descriptor over `bytes` bytes at base, for dma16_at: rows past them load zeros.
 __device__ __forceinline__ u32x4 tile_rsrc(const void* base, uint32_t bytes)
 {
