@@ -6,16 +6,17 @@
 //
 // Eviction, per list (sequence, kv head) of n > budget rows, in two launches:
 // * evict_select, one workgroup a list. A row's key is its weight as an integer in the same order (protected rows the
-//   largest key, NaN that of -inf, -0 that of 0). The budget-th largest key T comes from four histograms of 8 bits, the
-//   highest first; rows above T stay, of those at T the first `need` do. Each wave then counts its run of rows, the
-//   counts before it give every row its rank among the kept, and from ranks follow the rows' places: a row j below the
-//   budget that is given up is hole j - (kept before j), a kept row past the budget source (kept before it) - (kept
-//   below the budget). The lists of holes and sources go into the workspace.
+//   largest key, NaN that of -inf, -0 that of 0), held in LDS. The budget-th largest key T comes from histograms of
+//   11, 11 and 10 bits, the highest first; rows above T stay, of those at T the first `need` do. Counts of the runs of
+//   64 rows give every row its rank among the kept, and from ranks follow the rows' places: a row j below the budget that
+//   is given up is hole j - (kept before j), a kept row past the budget source (kept before it) - (kept below the
+//   budget). The lists of holes and sources go into the workspace.
 // * evict_move copies source i over hole i, K, V, weight and position. Sources lie past the budget and holes below it,
 //   so no row is read and written.
 #include <algorithm>
 
 #include "device.hpp"
+#include "split_ranges.hpp"
 
 namespace mako {
 namespace {
@@ -88,127 +89,203 @@ __device__ __forceinline__ uint32_t order_of(float x)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-struct EvictList {
-    const float* w;
-    const uint32_t* pos;
-    uint32_t sinks, late;  // positions below sinks, and from late on, are protected
-    __device__ __forceinline__ uint32_t key(uint32_t j) const
-    {
-        const uint32_t at = pos ? pos[j] : j;
-        return at < sinks || at >= late ? 0xffffffffu : order_of(w[j]);
-    }
-};
+constexpr int kDigits = 2048;  // of 11, 11 and 10 bits
+constexpr int kCopies = 2;     // counters a digit, by lane
 
-__global__ __launch_bounds__(kThreads) void evict_select(const EvictParams p)
+// The inclusive sum of x over the workgroup's threads up to this one (s: a word a wave; two barriers).
+template <int W>
+__device__ __forceinline__ uint32_t scan_threads(uint32_t x, uint32_t (&s)[W], uint32_t lane, uint32_t wv)
 {
-    __shared__ uint32_t hist[kWaves][256], s_digit, s_above, s_gt[kWaves], s_eq[kWaves];
-    const uint32_t list = blockIdx.x, b = list / p.kv_heads, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    #pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t t = __shfl_up(x, o);
+        x += lane >= (uint32_t)o ? t : 0u;
+    }
+    if (lane == 63)
+        s[wv] = x;
+    __syncthreads();
+    uint32_t sums[W];
+    #pragma unroll
+    for (int i = 0; i < W; ++i)
+        sums[i] = s[i];
+    #pragma unroll
+    for (int i = 0; i < W; ++i)
+        x += i < (int)wv ? sums[i] : 0u;
+    __syncthreads();
+    return x;
+}
+
+// A workgroup of TH threads; the keys of ROWS rows in LDS (registers would hold them too, but unrolled over them the code
+// outgrows the instruction cache, and each line of it runs once). A longer list goes through in blocks of ROWS, read again
+// in each pass.
+template <int TH, int ROWS>
+__global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
+{
+    constexpr int W = TH / 64, kPer = kDigits / TH, kRuns = ROWS / TH;  // digits a thread sums; runs of 64 a wave
+    static_assert(ROWS <= 32768 && kRuns * W <= TH && kRuns % 8 == 0, "counts of a block fit 16 bits, a run's count has a thread");
+    __shared__ uint32_t keys[ROWS];
+    __shared__ __attribute__((aligned(16))) uint32_t hist[kDigits * kCopies];
+    __shared__ __attribute__((aligned(16))) uint32_t s_scan[W];
+    __shared__ uint32_t s_digit, s_above, s_total, s_cnt[kRuns * W];
+    const uint32_t list = blockIdx.x, b = list / p.kv_heads, tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
     const uint32_t n = min(p.ctx[b], p.max_ctx), seen = p.seen ? p.seen[b] : n;
     const size_t base = (size_t)list * p.cap;
-    const EvictList a{p.w + base, p.pos ? p.pos + base : nullptr, p.sinks, seen > p.recent ? seen - p.recent : 0u};
+    const float* w_in = p.w + base;
+    const uint32_t* pos_in = p.pos ? p.pos + base : nullptr;
     float* w_out = p.w_out + base;
     uint32_t* pos_out = p.pos_out + base;
-    if (n <= p.budget) {
-        for (uint32_t j = tid; j < n; j += kThreads) {
-            w_out[j] = a.w[j];
-            pos_out[j] = a.pos ? a.pos[j] : j;
-        }
+    const bool copies = p.w_out != p.w || p.pos_out != p.pos;
+    if (n <= p.budget || p.budget == 0) {
+        if (copies && p.budget)
+            for (uint32_t j = tid; j < n; j += TH) {
+                w_out[j] = w_in[j];
+                pos_out[j] = pos_in ? pos_in[j] : j;
+            }
         if (tid == 0)
             p.count[list] = 0;
         return;
     }
-    // The budget-th largest key, 8 bits at a time: `need` rows are still to be found among those with the prefix.
+    const uint32_t late = seen > p.recent ? seen - p.recent : 0u;  // positions from here on, and below sinks, are protected
+    const uint32_t blocks = (n + ROWS - 1) / ROWS;
+    // Block blk's keys (rows past the list: key 0, below every row's); thread t reads and writes entries t, t + TH, ...
+    auto load = [&](uint32_t blk) __attribute__((always_inline)) {
+        const uint32_t j0 = blk * ROWS, runs = (min(n - j0, (uint32_t)ROWS) + TH - 1) / TH;
+        #pragma unroll 1
+        for (uint32_t e = 0; e < runs; e += 8) {  // eight loads in flight (ROWS is a multiple of 8 TH)
+            float w[8];
+            uint32_t at[8];
+            #pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                at[i] = min(j0 + (e + i) * TH + tid, n - 1);
+                w[i] = w_in[at[i]];
+            }
+            if (pos_in)
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    at[i] = pos_in[at[i]];
+            #pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const uint32_t x = at[i] < p.sinks || at[i] >= late ? 0xffffffffu : order_of(w[i]);
+                keys[(e + i) * TH + tid] = j0 + (e + i) * TH + tid < n ? x : 0u;
+            }
+        }
+        return runs;
+    };
+    uint32_t runs = load(0);
+    // The budget-th largest key, a digit at a time: `need` rows are still to be found among those with the prefix.
     uint32_t prefix = 0, need = p.budget;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (uint32_t i = tid; i < kWaves * 256; i += kThreads)
-            hist[i / 256][i % 256] = 0;
+    #pragma unroll 1
+    for (uint32_t shift = 21, bits = 11, d = 0; d < 3; ++d) {
+        for (uint32_t i = tid; i < kDigits * kCopies / 4; i += TH)
+            reinterpret_cast<u32x4*>(hist)[i] = u32x4{};
         __syncthreads();
-        for (uint32_t j = tid; j < n; j += kThreads) {
-            const uint32_t key = a.key(j);
-            if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8))
-                atomicAdd(&hist[wv][key >> shift & 255], 1u);
-        }
-        __syncthreads();
-        if (wv == 0) {  // lane l: digits 255 - 4 l down to 252 - 4 l
-            uint32_t c[4], sum = 0;
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                c[i] = 0;
-                for (int x = 0; x < kWaves; ++x)
-                    c[i] += hist[x][255 - 4 * lane - i];
-                sum += c[i];
-            }
-            uint32_t inc = sum;
-            #pragma unroll
-            for (int x = 1; x < 64; x <<= 1) {
-                const uint32_t t = __shfl_up(inc, x);
-                inc += lane >= (uint32_t)x ? t : 0u;
-            }
-            uint32_t above = inc - sum;
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (above < need && above + c[i] >= need) {
-                    s_digit = 255 - 4 * lane - i;
-                    s_above = above;
-                }
-                above += c[i];
+        for (uint32_t blk = 0; blk < blocks; ++blk) {
+            if (blocks > 1)
+                runs = load(blk);
+            // (the first digit compares its keys' bits above 32: none)
+            #pragma unroll 1
+            for (uint32_t e = 0; e < runs; e += 8) {
+                uint32_t key[8];
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    key[i] = keys[(e + i) * TH + tid];
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    if ((uint64_t)(key[i] ^ prefix) >> (shift + bits) == 0)
+                        atomicAdd(&hist[(key[i] >> shift & ((1u << bits) - 1)) * kCopies + (lane & (kCopies - 1))], 1u);
             }
         }
         __syncthreads();
-        if (need) {  // (a budget of 0 keeps nothing)
-            prefix |= s_digit << shift;
-            need -= s_above;
+        // Thread t: kPer digits from the largest down.
+        uint32_t c[kPer], sum = 0;
+        #pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const u32x2 x = reinterpret_cast<const u32x2*>(hist)[kDigits - 1 - (kPer * tid + i)];
+            c[i] = x[0] + x[1];
+            sum += c[i];
+        }
+        uint32_t above = scan_threads(sum, s_scan, lane, wv) - sum;
+        #pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (above < need && above + c[i] >= need) {
+                s_digit = kDigits - 1 - (kPer * tid + i);
+                s_above = above;
+            }
+            above += c[i];
         }
         __syncthreads();
+        prefix |= uniform(s_digit) << shift;
+        need -= uniform(s_above);
+        bits = d == 0 ? 11 : 10;
+        shift -= bits;
     }
-    const uint32_t T = p.budget ? prefix : 0xffffffffu;
-    const bool none = p.budget == 0;
-    // Each wave's run of rows: how many above T, and at T, in it.
-    const uint32_t run = (n + kWaves * 64 - 1) / (kWaves * 64) * 64, j0 = wv * run, j1 = min(n, j0 + run);
-    uint32_t gt = 0, eq = 0;
-    for (uint32_t j = j0; j < j1; j += 64) {
-        const uint32_t key = j + lane < n ? a.key(j + lane) : 0u;
-        gt += __popcll(__ballot(j + lane < n && !none && key > T));
-        eq += __popcll(__ballot(j + lane < n && !none && key == T));
-    }
-    if (lane == 0) {
-        s_gt[wv] = gt;
-        s_eq[wv] = eq;
-    }
-    __syncthreads();
-    gt = eq = 0;
-    for (uint32_t x = 0; x < wv; ++x) {
-        gt += s_gt[x];
-        eq += s_eq[x];
-    }
-    // The ranks: the rows below the budget first (their number sets the sources' ranks).
+    const uint32_t T = prefix;
+    // The kept rows before each: of the blocks before, then of the runs of 64 before (the counts above T in the low half,
+    // at T in the high), then in the run.
     uint32_t* hole = p.hole + (size_t)list * p.most;
     uint32_t* src = p.src + (size_t)list * p.most;
-    __shared__ uint32_t s_low;
-    for (uint32_t j = j0; j < j1; j += 64) {
-        const uint32_t x = j + lane;
-        const uint32_t key = x < n ? a.key(x) : 0u;
-        const uint64_t g = __ballot(x < n && !none && key > T), e = __ballot(x < n && !none && key == T);
-        const uint64_t below = (1ull << lane) - 1;
-        const uint32_t eb = eq + __popcll(e & below);
-        const uint32_t before = gt + __popcll(g & below) + min(eb, need);  // kept rows before x
-        const bool kept = x < n && !none && (key > T || (key == T && eb < need));
-        if (x == p.budget)
-            s_low = before;
-        if (x < p.budget && !kept)
-            hole[x - before] = x;
-        if (x < p.budget && kept) {
-            w_out[x] = a.w[x];
-            pos_out[x] = a.pos ? a.pos[x] : x;
+    uint32_t gt0 = 0, eq0 = 0;
+    for (uint32_t blk = 0; blk < blocks; ++blk) {
+        if (blocks > 1)
+            runs = load(blk);
+        const uint32_t j0 = blk * ROWS;
+        #pragma unroll 1
+        for (uint32_t e = 0; e < runs; e += 8) {
+            uint32_t key[8], mine = 0;  // (lane i keeps run e + i's count)
+            #pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                key[i] = keys[(e + i) * TH + tid];
+            #pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const uint32_t c = (uint32_t)__popcll(__ballot(key[i] > T)) | (uint32_t)__popcll(__ballot(key[i] == T)) << 16;
+                mine = lane == i ? c : mine;
+            }
+            if (lane < 8)
+                s_cnt[(e + lane) * W + wv] = mine;
         }
-        if (x >= p.budget && kept)  // counted from the end: the last kept row is source 0 here
-            src[p.budget - 1 - before] = x;
-        gt += __popcll(g);
-        eq += __popcll(e);
+        __syncthreads();
+        const uint32_t mine = tid < runs * W ? s_cnt[tid] : 0u;  // (the runs past the block's: key 0, no count)
+        const uint32_t inc = scan_threads(mine, s_scan, lane, wv);
+        if (tid < runs * W)
+            s_cnt[tid] = inc - mine;
+        if (tid == TH - 1)
+            s_total = inc;
+        __syncthreads();
+        const uint32_t total = s_total;
+        const uint64_t below = (1ull << lane) - 1;
+        #pragma unroll 1
+        for (uint32_t e0 = 0; e0 < runs; e0 += 8) {
+            uint32_t key[8], run[8];
+            #pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                key[i] = keys[(e0 + i) * TH + tid];
+                run[i] = s_cnt[(e0 + i) * W + wv];
+            }
+            #pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const uint32_t x = j0 + (e0 + i) * TH + tid;
+                const uint64_t g = __ballot(key[i] > T), q = __ballot(key[i] == T);
+                if ((g | q) == 0 && j0 + (e0 + i) * TH > p.budget)
+                    continue;  // none of the run stays, nor lies below the budget
+                const uint32_t eq = eq0 + (run[i] >> 16) + __popcll(q & below);
+                const uint32_t before = gt0 + (run[i] & 0xffffu) + __popcll(g & below) + min(eq, need);
+                const bool kept = key[i] > T || (key[i] == T && eq < need);
+                if (x == p.budget)
+                    p.count[list] = p.budget - before;
+                if (x < p.budget && !kept)
+                    hole[x - before] = x;
+                if (x >= p.budget && kept)
+                    src[p.budget - 1 - before] = x;  // from the end: the first source comes last
+                if (copies && x < p.budget && kept) {
+                    w_out[x] = w_in[x];
+                    pos_out[x] = pos_in ? pos_in[x] : x;
+                }
+            }
+        }
+        gt0 += total & 0xffffu;
+        eq0 += total >> 16;
+        __syncthreads();
     }
-    __syncthreads();
-    if (tid == 0)
-        p.count[list] = p.budget - s_low;
 }
 
 constexpr int kMoveRows = 16;  // rows of K and V a workgroup of evict_move
@@ -341,7 +418,10 @@ extern "C" int mako_cache_evict(const mako_evict_args* a, mako_dtype in, void* k
                         reinterpret_cast<uint32_t*>(ws + at), reinterpret_cast<uint32_t*>(ws + at + bytes), a->kv_heads,
                         a->dim, a->cap, a->max_ctx, a->budget, a->recent, a->sinks, most};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(evict_select, dim3((uint32_t)lists), dim3(kThreads), 0, s, p);
+    if (a->max_ctx <= 4096)
+        hipLaunchKernelGGL((evict_select<512, 4096>), dim3((uint32_t)lists), dim3(512), 0, s, p);
+    else
+        hipLaunchKernelGGL((evict_select<1024, 32768>), dim3((uint32_t)lists), dim3(1024), 0, s, p);
     hipLaunchKernelGGL(evict_move, dim3((uint32_t)(lists * chunks)), dim3(256), 0, s, p);
     return check_launch(what);
 }
