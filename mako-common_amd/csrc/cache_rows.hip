@@ -7,10 +7,10 @@
 // Eviction, per list (sequence, kv head) of n > budget rows, in two launches:
 // * evict_select, one workgroup a list. A row's key is its weight as an integer in the same order (protected rows the
 //   largest key, NaN that of -inf, -0 that of 0), held in LDS. The budget-th largest key T comes from histograms of
-//   11, 11 and 10 bits, the highest first; rows above T stay, of those at T the first `need` do. Counts of the runs of
-//   64 rows give every row its rank among the kept, and from ranks follow the rows' places: a row j below the budget that
-//   is given up is hole j - (kept before j), a kept row past the budget source (kept before it) - (kept below the
-//   budget). The lists of holes and sources go into the workspace.
+//   11, 11 and 10 bits, the highest first; rows above T stay, of those at T the first `need` do. A sum over the threads of
+//   their rows' counts gives every row its rank among the kept, and from ranks follow the rows' places: a row j below the
+//   budget that is given up is hole j - (kept before j), a kept row past the budget source (kept before it) - (kept below
+//   the budget). The lists of holes and sources go into the workspace.
 // * evict_move copies source i over hole i, K, V, weight and position. Sources lie past the budget and holes below it,
 //   so no row is read and written.
 #include <algorithm>
@@ -92,54 +92,63 @@ __device__ __forceinline__ uint32_t order_of(float x)
 constexpr int kDigits = 2048;  // of 11, 11 and 10 bits
 constexpr int kCopies = 2;     // counters a digit, by lane
 
-// The inclusive sum of x over the workgroup's threads up to this one (s: a word a wave; two barriers).
-template <int W>
-__device__ __forceinline__ uint32_t scan_threads(uint32_t x, uint32_t (&s)[W], uint32_t lane, uint32_t wv)
+// The inclusive sum of x over a wave's lanes up to this one, by row shifts and broadcasts.
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t x)
 {
-    #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t t = __shfl_up(x, o);
-        x += lane >= (uint32_t)o ? t : 0u;
-    }
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, false);  // row_shr 1
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false);  // lane 15 of rows 0 and 2 to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
+    return x;
+}
+
+// The same over the workgroup's threads; total: over all of them (s: a word a wave; two barriers).
+template <int W>
+__device__ __forceinline__ uint32_t scan_threads(uint32_t x, u32x4 (&s)[W / 4], uint32_t lane, uint32_t wv, uint32_t& total)
+{
+    x = scan_lanes(x);
     if (lane == 63)
-        s[wv] = x;
+        reinterpret_cast<uint32_t*>(s)[wv] = x;
     __syncthreads();
-    uint32_t sums[W];
+    total = 0;
     #pragma unroll
-    for (int i = 0; i < W; ++i)
-        sums[i] = s[i];
-    #pragma unroll
-    for (int i = 0; i < W; ++i)
-        x += i < (int)wv ? sums[i] : 0u;
+    for (int i = 0; i < W / 4; ++i) {
+        const u32x4 y = s[i];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x += 4 * i + j < (int)wv ? y[j] : 0u;
+            total += y[j];
+        }
+    }
     __syncthreads();
     return x;
 }
 
 // A workgroup of TH threads; the keys of ROWS rows in LDS (registers would hold them too, but unrolled over them the code
-// outgrows the instruction cache, and each line of it runs once). A longer list goes through in blocks of ROWS, read again
-// in each pass.
+// outgrows the instruction cache, and each line of it runs once). Thread t has R consecutive rows, its first at t R, in
+// LDS rows of R + 1 words (R even: no bank conflicts). A longer list goes through in blocks of ROWS, read again in each
+// pass. Bound by one CU: about 40 VALU operations a row, and an LDS atomic a row for the first digit.
 template <int TH, int ROWS>
 __global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
 {
-    constexpr int W = TH / 64, kPer = kDigits / TH, kRuns = ROWS / TH;  // digits a thread sums; runs of 64 a wave
-    static_assert(ROWS <= 32768 && kRuns * W <= TH && kRuns % 8 == 0, "counts of a block fit 16 bits, a run's count has a thread");
-    __shared__ uint32_t keys[ROWS];
-    __shared__ __attribute__((aligned(16))) uint32_t hist[kDigits * kCopies];
-    __shared__ __attribute__((aligned(16))) uint32_t s_scan[W];
-    __shared__ uint32_t s_digit, s_above, s_total, s_cnt[kRuns * W];
+    constexpr int W = TH / 64, kPer = kDigits / TH;  // digits a thread sums
+    static_assert(ROWS <= 32768 && ROWS / TH % 8 == 0, "counts of a block fit 16 bits, rows go eight at a time");
+    __shared__ uint32_t keys[ROWS + TH];
+    __shared__ u32x4 hist[kDigits * kCopies / 4], s_scan[W / 4];
+    __shared__ uint32_t s_digit, s_above;
     const uint32_t list = blockIdx.x, b = list / p.kv_heads, tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
-    const uint32_t n = min(p.ctx[b], p.max_ctx), seen = p.seen ? p.seen[b] : n;
+    const uint32_t n = min(p.ctx[b], p.max_ctx), seen = p.seen ? p.seen[b] : n, budget = p.budget;
     const size_t base = (size_t)list * p.cap;
-    const float* w_in = p.w + base;
-    const uint32_t* pos_in = p.pos ? p.pos + base : nullptr;
-    float* w_out = p.w_out + base;
-    uint32_t* pos_out = p.pos_out + base;
+    const char* w_in = reinterpret_cast<const char*>(p.w + base);  // (byte offsets of 32 bits: scalar base addressing)
+    const char* pos_in = p.pos ? reinterpret_cast<const char*>(p.pos + base) : nullptr;
     const bool copies = p.w_out != p.w || p.pos_out != p.pos;
-    if (n <= p.budget || p.budget == 0) {
-        if (copies && p.budget)
+    if (n <= budget || budget == 0) {
+        if (copies && budget)
             for (uint32_t j = tid; j < n; j += TH) {
-                w_out[j] = w_in[j];
-                pos_out[j] = pos_in ? pos_in[j] : j;
+                p.w_out[base + j] = p.w[base + j];
+                p.pos_out[base + j] = p.pos ? p.pos[base + j] : j;
             }
         if (tid == 0)
             p.count[list] = 0;
@@ -147,55 +156,91 @@ __global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
     }
     const uint32_t late = seen > p.recent ? seen - p.recent : 0u;  // positions from here on, and below sinks, are protected
     const uint32_t blocks = (n + ROWS - 1) / ROWS;
-    // Block blk's keys (rows past the list: key 0, below every row's); thread t reads and writes entries t, t + TH, ...
-    auto load = [&](uint32_t blk) __attribute__((always_inline)) {
-        const uint32_t j0 = blk * ROWS, runs = (min(n - j0, (uint32_t)ROWS) + TH - 1) / TH;
+    const uint32_t lg = blocks > 1 ? 31 - __builtin_clz(ROWS / TH) : max(3, 32 - __builtin_clz((n - 1) / TH | 1)), R = 1u << lg;
+    // Block blk's keys (rows past the list: key 0, below every row's); `first`: with the copies below the budget (the rows
+    // that are given up get theirs from evict_move).
+    auto load = [&](uint32_t blk, bool first) __attribute__((always_inline)) {
         #pragma unroll 1
-        for (uint32_t e = 0; e < runs; e += 8) {  // eight loads in flight (ROWS is a multiple of 8 TH)
+        for (uint32_t e = 0; e < R; e += 8) {
+            const uint32_t x0 = e * TH + tid, j0 = blk * ROWS + x0;
+            const uint32_t lo = blk * ROWS + e * TH, hi = lo + 8 * TH;  // the rows of all threads
             float w[8];
             uint32_t at[8];
             #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
-                at[i] = min(j0 + (e + i) * TH + tid, n - 1);
-                w[i] = w_in[at[i]];
+                at[i] = min(j0 + i * TH, n - 1);
+                w[i] = *reinterpret_cast<const float*>(w_in + 4 * at[i]);
             }
             if (pos_in)
                 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i)
-                    at[i] = pos_in[at[i]];
+                    at[i] = *reinterpret_cast<const uint32_t*>(pos_in + 4 * at[i]);
+            uint32_t key[8];
             #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const uint32_t x = at[i] < p.sinks || at[i] >= late ? 0xffffffffu : order_of(w[i]);
-                keys[(e + i) * TH + tid] = j0 + (e + i) * TH + tid < n ? x : 0u;
-            }
+            for (uint32_t i = 0; i < 8; ++i)
+                key[i] = order_of(w[i]);
+            if (pos_in || lo < p.sinks || hi > late)
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    key[i] = at[i] < p.sinks || at[i] >= late ? 0xffffffffu : key[i];
+            if (hi > n)
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    key[i] = j0 + i * TH < n ? key[i] : 0u;
+            #pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                keys[x0 + i * TH + ((x0 + i * TH) >> lg)] = key[i];
+            if (first && copies && lo < budget)
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    if (j0 + i * TH < budget) {
+                        p.w_out[base + j0 + i * TH] = w[i];
+                        p.pos_out[base + j0 + i * TH] = at[i];
+                    }
         }
-        return runs;
     };
-    uint32_t runs = load(0);
-    // The budget-th largest key, a digit at a time: `need` rows are still to be found among those with the prefix.
-    uint32_t prefix = 0, need = p.budget;
+    load(0, true);
+    const uint32_t mine = tid * (R + 1);  // this thread's keys
+    // The budget-th largest key, a digit at a time: `need` rows are still to be found among those with the prefix. Protected
+    // rows are counted apart (they would all meet in one counter): where they alone reach the budget, theirs is the key.
+    uint32_t prefix = 0, known = 0, need = budget, total, safe = 0;
     #pragma unroll 1
-    for (uint32_t shift = 21, bits = 11, d = 0; d < 3; ++d) {
+    for (uint32_t shift = 21, d = 0; d < 3; ++d) {
+        const uint32_t mask = d < 2 ? 2047u : 1023u;
         for (uint32_t i = tid; i < kDigits * kCopies / 4; i += TH)
-            reinterpret_cast<u32x4*>(hist)[i] = u32x4{};
-        __syncthreads();
+            hist[i] = u32x4{};
         for (uint32_t blk = 0; blk < blocks; ++blk) {
-            if (blocks > 1)
-                runs = load(blk);
-            // (the first digit compares its keys' bits above 32: none)
+            if (blocks > 1) {
+                __syncthreads();
+                load(blk, blk > 0 && d == 0);
+            }
+            __syncthreads();
             #pragma unroll 1
-            for (uint32_t e = 0; e < runs; e += 8) {
+            for (uint32_t e = 0; e < R; e += 8) {
                 uint32_t key[8];
                 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i)
-                    key[i] = keys[(e + i) * TH + tid];
+                    key[i] = keys[mine + e + i];
+                if (d == 0)
+                    #pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        safe += key[i] == 0xffffffffu;
                 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i)
-                    if ((uint64_t)(key[i] ^ prefix) >> (shift + bits) == 0)
-                        atomicAdd(&hist[(key[i] >> shift & ((1u << bits) - 1)) * kCopies + (lane & (kCopies - 1))], 1u);
+                    if ((key[i] & known) == prefix && key[i] + 1 > 1)  // (not 0, not a protected row's)
+                        atomicAdd(reinterpret_cast<uint32_t*>(hist) + (key[i] >> shift & mask) * kCopies +
+                                      (lane & (kCopies - 1)), 1u);
             }
         }
         __syncthreads();
+        if (d == 0) {
+            scan_threads<W>(safe, s_scan, lane, wv, total);
+            if (total >= budget) {
+                prefix = 0xffffffffu;
+                break;
+            }
+            need -= total;
+        }
         // Thread t: kPer digits from the largest down.
         uint32_t c[kPer], sum = 0;
         #pragma unroll
@@ -204,7 +249,7 @@ __global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
             c[i] = x[0] + x[1];
             sum += c[i];
         }
-        uint32_t above = scan_threads(sum, s_scan, lane, wv) - sum;
+        uint32_t above = scan_threads<W>(sum, s_scan, lane, wv, total) - sum;
         #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             if (above < need && above + c[i] >= need) {
@@ -215,76 +260,71 @@ __global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
         }
         __syncthreads();
         prefix |= uniform(s_digit) << shift;
+        known |= mask << shift;
         need -= uniform(s_above);
-        bits = d == 0 ? 11 : 10;
-        shift -= bits;
+        shift -= d == 0 ? 11 : 10;
     }
-    const uint32_t T = prefix;
-    // The kept rows before each: of the blocks before, then of the runs of 64 before (the counts above T in the low half,
-    // at T in the high), then in the run.
+    const uint32_t T = uniform(prefix);
+    // The kept rows before each, in row order: of the blocks before, of the threads before (the counts above T in the low
+    // half, at T in the high), and the thread's own.
     uint32_t* hole = p.hole + (size_t)list * p.most;
     uint32_t* src = p.src + (size_t)list * p.most;
     uint32_t gt0 = 0, eq0 = 0;
     for (uint32_t blk = 0; blk < blocks; ++blk) {
-        if (blocks > 1)
-            runs = load(blk);
-        const uint32_t j0 = blk * ROWS;
-        #pragma unroll 1
-        for (uint32_t e = 0; e < runs; e += 8) {
-            uint32_t key[8], mine = 0;  // (lane i keeps run e + i's count)
-            #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i)
-                key[i] = keys[(e + i) * TH + tid];
-            #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const uint32_t c = (uint32_t)__popcll(__ballot(key[i] > T)) | (uint32_t)__popcll(__ballot(key[i] == T)) << 16;
-                mine = lane == i ? c : mine;
-            }
-            if (lane < 8)
-                s_cnt[(e + lane) * W + wv] = mine;
+        if (blocks > 1) {
+            __syncthreads();
+            load(blk, false);
+            __syncthreads();
         }
-        __syncthreads();
-        const uint32_t mine = tid < runs * W ? s_cnt[tid] : 0u;  // (the runs past the block's: key 0, no count)
-        const uint32_t inc = scan_threads(mine, s_scan, lane, wv);
-        if (tid < runs * W)
-            s_cnt[tid] = inc - mine;
-        if (tid == TH - 1)
-            s_total = inc;
-        __syncthreads();
-        const uint32_t total = s_total;
-        const uint64_t below = (1ull << lane) - 1;
+        uint32_t c = 0;
         #pragma unroll 1
-        for (uint32_t e0 = 0; e0 < runs; e0 += 8) {
-            uint32_t key[8], run[8];
+        for (uint32_t e = 0; e < R; e += 8)
             #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
-                key[i] = keys[(e0 + i) * TH + tid];
-                run[i] = s_cnt[(e0 + i) * W + wv];
+                const uint32_t key = keys[mine + e + i];
+                c += key > T ? 1u : key == T ? 0x10000u : 0u;
             }
-            #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const uint32_t x = j0 + (e0 + i) * TH + tid;
-                const uint64_t g = __ballot(key[i] > T), q = __ballot(key[i] == T);
-                if ((g | q) == 0 && j0 + (e0 + i) * TH > p.budget)
-                    continue;  // none of the run stays, nor lies below the budget
-                const uint32_t eq = eq0 + (run[i] >> 16) + __popcll(q & below);
-                const uint32_t before = gt0 + (run[i] & 0xffffu) + __popcll(g & below) + min(eq, need);
-                const bool kept = key[i] > T || (key[i] == T && eq < need);
-                if (x == p.budget)
-                    p.count[list] = p.budget - before;
-                if (x < p.budget && !kept)
-                    hole[x - before] = x;
-                if (x >= p.budget && kept)
-                    src[p.budget - 1 - before] = x;  // from the end: the first source comes last
-                if (copies && x < p.budget && kept) {
-                    w_out[x] = w_in[x];
-                    pos_out[x] = pos_in ? pos_in[x] : x;
+        const uint32_t before = scan_threads<W>(c, s_scan, lane, wv, total) - c;
+        uint32_t gt = gt0 + (before & 0xffffu), eq = eq0 + (before >> 16);
+        uint32_t x = blk * ROWS + tid * R;
+        if (blk * ROWS + wv * 64 * R > budget && !__any(c >> 16)) {
+            // Sources alone, none of them at T.
+            uint32_t at = budget - 1 - gt - min(eq, need);
+            #pragma unroll 1
+            for (uint32_t e = 0; e < R; e += 8) {
+                uint32_t key[8];
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    key[i] = keys[mine + e + i];
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    if (key[i] > T)
+                        src[at--] = x + e + i;
+            }
+        } else {
+            #pragma unroll 1
+            for (uint32_t e = 0; e < R; e += 8) {
+                uint32_t key[8];
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    key[i] = keys[mine + e + i];
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i, ++x) {
+                    const uint32_t kept_before = gt + min(eq, need);
+                    const bool kept = key[i] > T || (key[i] == T && eq < need);
+                    if (x == budget)
+                        p.count[list] = budget - kept_before;
+                    if (x < budget && !kept)
+                        hole[x - kept_before] = x;
+                    if (x >= budget && kept)
+                        src[budget - 1 - kept_before] = x;  // from the end: the first source comes last
+                    gt += key[i] > T;
+                    eq += key[i] == T;
                 }
             }
         }
         gt0 += total & 0xffffu;
         eq0 += total >> 16;
-        __syncthreads();
     }
 }
 
