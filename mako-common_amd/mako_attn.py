@@ -169,15 +169,22 @@ def _check(rc):
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
+
+
+_current = None  # how the current stream is asked for: torch.cuda.current_stream() builds a Stream object, 3 us a call
 
 
 def _stream(stream):
-    if stream is None:
+    if stream is not None:
+        return stream
+    global _current
+    if _current is None:
         import torch
 
-        return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-    return ctypes.c_void_p(stream)
+        torch.cuda.current_stream()  # initialises the device
+        _current = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    return _current[1](_current[0]())
 
 
 def dtype_code(t):
