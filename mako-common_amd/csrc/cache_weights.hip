@@ -32,10 +32,11 @@ struct WeightsParams {
     const float *lse, *w;
     float* w_out;
     const uint32_t *ctx, *path, *n_path;
-    float* part;          // [chunks][lists][max_ctx]
+    float* part;          // [range + block][keys]: sums of the ranges' share of a key block
+    uint32_t* ends;       // [lists][n_blocks][2]: the first and the last range of each block
     uint32_t batch, n_q, heads, kv_heads, group, cap, max_ctx;
-    uint32_t n_ranges;    // weights_few: waves
-    uint32_t chunk, n_chunks, n_blocks;  // weights_many: queries a chunk, chunks, key blocks
+    uint32_t n_ranges;    // waves (weights_few), workgroups (weights_many)
+    uint32_t n_blocks;    // weights_many: key blocks of max_ctx
     uint64_t qs_b, qs_h;  // q strides (elements) of a sequence and a head
     uint64_t ls_b, ls_h;  // lse strides
     float scale_log2, decay;
@@ -229,7 +230,49 @@ struct Many {
     static constexpr int kRow = 2 * D, kTile = kTK * kRow;   // a tile of queries
     static constexpr int kPieces = kTile / 1024 / 4;         // 1 KiB pieces of it a wave
     static constexpr int kDepth = D == 64 ? 8 : 4;
-    static constexpr int kTable = 2048;                      // rows whose place and offset are looked up at a time
+    static constexpr int kTable = D == 256 ? 2048 : 4096;    // rows whose place and offset are looked up at a time
+};
+
+// The query tiles of a list's key blocks. Block i's keys start at i keys; the first query that sees them is the (i keys -
+// (ctx - n))-th, in tile i per - a, so block i has count - max(0, i per - a) tiles a head, at least one where n > 0.
+struct BlockTiles {
+    int per, a, count, group;  // 32-key tiles a block; ctx - n in tiles, rounded up; tiles of n; heads
+    uint32_t blocks;
+    __device__ __forceinline__ BlockTiles(const WeightsParams& p, uint32_t b, uint32_t keys)
+    {
+        const uint32_t ctx = ctx_of(p, b), n = n_of(p, b);
+        per = keys / kTK;
+        a = ctx >= n ? (int)((ctx - n + kTK - 1) / kTK) : -(int)((n - ctx) / kTK);
+        count = (n + kTK - 1) / kTK;
+        group = p.group;
+        blocks = n ? (ctx + keys - 1) / keys : 0u;
+    }
+    __device__ __forceinline__ uint32_t first_tile(uint32_t i) const { return max(0, (int)i * per - a); }
+    __device__ __forceinline__ uint32_t tiles(uint32_t i) const { return count - first_tile(i); }  // of a head
+    // The tiles of blocks [0, i), over the heads.
+    __device__ __forceinline__ uint32_t before(uint32_t i) const
+    {
+        const uint32_t i0 = a < 0 ? 0u : min(i, (uint32_t)(a / per) + 1);  // blocks below see every query's tile
+        const uint32_t m = i - i0;
+        // i0 per - a, then per more each
+        return group * (i * count - m * (uint32_t)((int)i0 * per - a) - per * (m * (m - 1) / 2));
+    }
+    __device__ __forceinline__ uint32_t total() const { return before(blocks); }
+    // The block that holds tile x of them.
+    __device__ __forceinline__ uint32_t of(uint32_t x) const
+    {
+        uint32_t lo = 0, hi = blocks;  // before(lo) <= x < before(hi)
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            (before(mid) <= x ? lo : hi) = mid;
+        }
+        return lo;
+    }
+};
+struct ListTiles {
+    const WeightsParams& p;
+    uint32_t keys;
+    __device__ __forceinline__ uint32_t operator()(uint32_t i) const { return BlockTiles(p, i, keys).total(); }
 };
 
 template <class T, int D>
@@ -243,19 +286,26 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
     __shared__ float s_off[S::kTable];
     __shared__ uint32_t s_row[S::kTable];
     const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c32 = lane & 31, wl = uniform(tid >> 6);
-    // lists first, so that with a multiple of 8 of them a list's workgroups share an XCD
-    const uint32_t lists = p.batch * p.kv_heads, list = blockIdx.x % lists, rest = blockIdx.x / lists;
-    const uint32_t block = rest % p.n_blocks, chunk = rest / p.n_blocks, b = list / p.kv_heads, kvh = list % p.kv_heads;
-    const uint32_t ctx = uniform(ctx_of(p, b)), n = uniform(n_of(p, b)), k0 = block * S::kKeys;
-    if (k0 >= ctx)
+    const uint32_t total = uniform(sum_of(p.batch, lane, ListTiles{p, S::kKeys}) * p.kv_heads);
+    // An XCD's workgroups take neighbouring ranges: they share queries and keys in its L2.
+    const uint32_t per_xcd = (p.n_ranges + 7) / 8, range = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
+    const Ranges rg(total, min(total, p.n_ranges));
+    if (blockIdx.x / 8 >= per_xcd || range >= rg.n)
         return;
-    // Queries [ia, ib): the chunk's that see a key of the block (query i sees ctx - n + i and what is before).
-    const uint32_t ib = min(n, (chunk + 1) * p.chunk);
-    const uint32_t see0 = k0 + n > ctx ? k0 + n - ctx : 0u;  // the first query that sees k0
-    const uint32_t ia = max(chunk * p.chunk, see0 & ~31u);
-    const uint32_t nt = ib > ia ? (ib - ia + kTK - 1) / kTK : 0u;  // tiles a head
-    if (nt == 0 && p.n_chunks > 1)
-        return;
+    const uint32_t x0 = rg.start(range);
+    uint32_t left = rg.start(range + 1) - x0, b, first;
+    seq_of(p.batch, x0, lane, ListTiles{p, S::kKeys}, p.kv_heads, b, first);
+    b = uniform(b);
+    first = uniform(first);
+    uint32_t kvh, block, tb;  // tiles from tb of the block on
+    {
+        const BlockTiles bt(p, b, S::kKeys);
+        const uint32_t len = uniform(bt.total());
+        kvh = (x0 - first) / len;
+        const uint32_t x = (x0 - first) % len;
+        block = uniform(bt.of(x));
+        tb = x - uniform(bt.before(block));
+    }
 
     uint32_t qr[S::kPieces], qc[S::kPieces];  // the row and byte of a tile that the lane's 16 LDS bytes hold
     #pragma unroll
@@ -266,153 +316,202 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
     }
     const uint32_t lbase = uniform((uint32_t)reinterpret_cast<uintptr_t>(lds));
     const uint32_t qa = c32 * kRow + 16 * (g ^ k_xor<D>(c32));
-    const uint32_t kw = k0 + wl * 32 * KB;  // the wave's first key
-    V8 kreg[KB][NK];
-    #pragma unroll
-    for (int i = 0; i < KB; ++i) {
-        const uint32_t j = kw + 32 * i + c32;
-        const T* src = static_cast<const T*>(p.k) + ((size_t)list * p.cap + j) * D + 8 * g;
-        #pragma unroll
-        for (int kk = 0; kk < NK; ++kk)
-            kreg[i][kk] = j < ctx ? *reinterpret_cast<const V8*>(src + 16 * kk) : V8{};
-    }
-    f32x16 acc[KB];
-    #pragma unroll
-    for (int i = 0; i < KB; ++i)
-        acc[i] = f32x16{};
-    const uint32_t tiles = nt * p.group;
-    for (uint32_t tb = 0; tb < tiles; tb += S::kTable / kTK) {
-        const uint32_t te = min(tiles, tb + S::kTable / kTK);
-        __syncthreads();
-        for (uint32_t x = tid; x < (te - tb) * kTK; x += 256) {
-            const uint32_t t = tb + x / kTK, h = kvh * p.group + t / nt, i = ia + t % nt * kTK + x % kTK;
-            float off;
-            const uint32_t r = query(p, b, h, i, i < ib, off);
-            s_off[x] = off;
-            s_row[x] = r < p.n_q ? r * kRow : 0x80000000u;  // (past the descriptor: zeros)
+    for (;;) {
+        const BlockTiles bt(p, b, S::kKeys);
+        const uint32_t ctx = uniform(ctx_of(p, b)), n = uniform(n_of(p, b)), list = b * p.kv_heads + kvh;
+        const uint32_t nt = uniform(bt.tiles(block)), ia = uniform(bt.first_tile(block)) * kTK, all = nt * p.group;
+        const uint32_t t_end = min(all, tb + left), kw = block * S::kKeys + wl * 32 * KB;  // the wave's first key
+        const bool whole = tb == 0 && t_end == all;
+        if (tid == 0) {
+            uint32_t* ends = p.ends + 2 * ((size_t)list * p.n_blocks + block);
+            if (tb == 0)
+                ends[0] = range;
+            if (t_end == all)
+                ends[1] = range;
         }
+        V8 kreg[KB][NK];
         #pragma unroll
-        for (int i = 0; i < KB; ++i)
+        for (int i = 0; i < KB; ++i) {
+            const uint32_t j = kw + 32 * i + c32;
+            const T* src = static_cast<const T*>(p.k) + ((size_t)list * p.cap + j) * D + 8 * g;
             #pragma unroll
             for (int kk = 0; kk < NK; ++kk)
-                settle(kreg[i][kk]);
-        __syncthreads();
-        auto stage = [&](uint32_t t) __attribute__((always_inline)) {
-            const uint32_t dst = lbase + t % S::kDepth * S::kTile + 1024 * wl * S::kPieces, h = kvh * p.group + t / nt;
-            const u32x4 rs = tile_rsrc(static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h, p.n_q * kRow);
-            #pragma unroll
-            for (int m = 0; m < S::kPieces; ++m)
-                dma16_at(dst + 1024 * m, s_row[(t - tb) * kTK + qr[m]] + qc[m], 0, rs);
-        };
-        for (uint32_t t = tb; t < min(te, tb + S::kDepth - 1); ++t)
-            stage(t);
-        for (uint32_t t = tb; t < te; ++t) {
-            if (t + S::kDepth - 1 <= te)
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::kDepth - 2) * S::kPieces) : "memory");
-            else
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (t + S::kDepth - 1 < te)
-                stage(t + S::kDepth - 1);
-            const unsigned char* tile = lds + t % S::kDepth * S::kTile;
-            f32x16 x[KB];
+                kreg[i][kk] = j < ctx ? *reinterpret_cast<const V8*>(src + 16 * kk) : V8{};
+        }
+        f32x16 acc[KB];
+        #pragma unroll
+        for (int i = 0; i < KB; ++i)
+            acc[i] = f32x16{};
+        left -= t_end - tb;
+        while (tb < t_end) {
+            const uint32_t te = min(t_end, tb + S::kTable / kTK);
+            __syncthreads();
+            for (uint32_t x = tid; x < (te - tb) * kTK; x += 256) {
+                const uint32_t t = tb + x / kTK, h = kvh * p.group + t / nt, i = ia + t % nt * kTK + x % kTK;
+                float off;
+                const uint32_t r = query(p, b, h, i, i < n, off);
+                s_off[x] = off;
+                s_row[x] = r < p.n_q ? r * kRow : 0x80000000u;  // (past the descriptor: zeros)
+            }
             #pragma unroll
             for (int i = 0; i < KB; ++i)
-                x[i] = f32x16{};
-            #pragma unroll
-            for (int kk = 0; kk < NK; ++kk) {
-                const V8 qf = *reinterpret_cast<const V8*>(tile + (qa ^ (32 * kk)));
+                #pragma unroll
+                for (int kk = 0; kk < NK; ++kk)
+                    settle(kreg[i][kk]);
+            __syncthreads();
+            // Tile t's head and place in it, as t goes on.
+            uint32_t sh = tb / nt, st = tb % nt, ch = sh, ct = st;
+            auto stage = [&](uint32_t t) __attribute__((always_inline)) {
+                const uint32_t dst = lbase + t % S::kDepth * S::kTile + 1024 * wl * S::kPieces;
+                const u32x4 rs = tile_rsrc(
+                    static_cast<const T*>(p.q) + b * p.qs_b + (uint64_t)(kvh * p.group + sh) * p.qs_h, p.n_q * kRow);
+                #pragma unroll
+                for (int m = 0; m < S::kPieces; ++m)
+                    dma16_at(dst + 1024 * m, s_row[(t - tb) * kTK + qr[m]] + qc[m], 0, rs);
+                if (++st == nt) {
+                    st = 0;
+                    ++sh;
+                }
+            };
+            for (uint32_t t = tb; t < min(te, tb + S::kDepth - 1); ++t)
+                stage(t);
+            for (uint32_t t = tb; t < te; ++t) {
+                if (t + S::kDepth - 1 <= te)
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::kDepth - 2) * S::kPieces)
+                                 : "memory");
+                else
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (t + S::kDepth - 1 < te)
+                    stage(t + S::kDepth - 1);
+                const unsigned char* tile = lds + t % S::kDepth * S::kTile;
+                const float off = s_off[(t - tb) * kTK + c32];
+                f32x16 x[KB];
                 #pragma unroll
                 for (int i = 0; i < KB; ++i)
-                    x[i] = E::mfma32(kreg[i][kk], qf, x[i]);
-            }
-            const float off = s_off[(t - tb) * kTK + c32];
-            const uint32_t i0 = ia + t % nt * kTK;
-            const bool none = off == INFINITY;  // no query: 0 against a key that is not finite too
-            if (kw + 32 * KB + n > ctx + i0 + 1 || __any(none)) {  // some row does not see all of the wave's keys
-                const uint32_t lim = !none && ctx + i0 + c32 >= n ? ctx + i0 + c32 - n + 1 : 0u;
+                    x[i] = f32x16{};
                 #pragma unroll
-                for (int i = 0; i < KB; ++i)
+                for (int kk = 0; kk < NK; ++kk) {
+                    const V8 qf = *reinterpret_cast<const V8*>(tile + (qa ^ (32 * kk)));
                     #pragma unroll
-                    for (int y = 0; y < 16; ++y) {
-                        const uint32_t j = kw + 32 * i + 8 * (y >> 2) + 4 * g + (y & 3);
-                        const float e = exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
-                        acc[i][y] += j < lim ? e : 0.0f;
-                    }
-            } else {
-                #pragma unroll
-                for (int i = 0; i < KB; ++i)
+                    for (int i = 0; i < KB; ++i)
+                        x[i] = E::mfma32(kreg[i][kk], qf, x[i]);
+                }
+                const uint32_t i0 = ia + ct * kTK;
+                if (++ct == nt) {
+                    ct = 0;
+                    ++ch;
+                }
+                const bool none = off == INFINITY;  // no query: 0 against a key that is not finite too
+                if (kw + 32 * KB + n > ctx + i0 + 1 || __any(none)) {  // some row does not see all of the wave's keys
+                    const uint32_t lim = !none && ctx + i0 + c32 >= n ? ctx + i0 + c32 - n + 1 : 0u;
                     #pragma unroll
-                    for (int y = 0; y < 16; ++y)
-                        acc[i][y] += exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
+                    for (int i = 0; i < KB; ++i)
+                        #pragma unroll
+                        for (int y = 0; y < 16; ++y) {
+                            const uint32_t j = kw + 32 * i + 8 * (y >> 2) + 4 * g + (y & 3);
+                            const float e = exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
+                            acc[i][y] += j < lim ? e : 0.0f;
+                        }
+                } else {
+                    #pragma unroll
+                    for (int i = 0; i < KB; ++i)
+                        #pragma unroll
+                        for (int y = 0; y < 16; ++y)
+                            acc[i][y] += exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
+                }
             }
+            tb = te;
         }
-    }
-    // A key's sum over the 32 lanes of its half: halving exchanges, 16 registers to 1. Lane bit s then picked register
-    // bit s, so lane (g, c32) ends with register c32 % 16 summed over all lanes but bit 4, which the last one adds.
-    #pragma unroll
-    for (int i = 0; i < KB; ++i) {
+        // A key's sum over the 32 lanes of its half: halving exchanges, 16 registers to 1. Lane bit s picks register bit s,
+        // so lane (g, c32) ends with register c32 % 16 summed over all lanes but bit 4, which the last one adds.
         #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const bool up = lane >> s & 1;
+        for (int i = 0; i < KB; ++i) {
             #pragma unroll
-            for (int y = 0; y < 8 >> s; ++y) {
-                const float keep = up ? acc[i][2 * y + 1] : acc[i][2 * y], give = up ? acc[i][2 * y] : acc[i][2 * y + 1];
-                acc[i][y] = keep + __shfl_xor(give, 1 << s);
+            for (int s = 0; s < 4; ++s) {
+                const bool up = lane >> s & 1;
+                #pragma unroll
+                for (int y = 0; y < 8 >> s; ++y) {
+                    const float keep = up ? acc[i][2 * y + 1] : acc[i][2 * y];
+                    const float give = up ? acc[i][2 * y] : acc[i][2 * y + 1];
+                    acc[i][y] = keep + __shfl_xor(give, 1 << s);
+                }
+            }
+            const float sum = acc[i][0] + __shfl_xor(acc[i][0], 16);
+            const uint32_t y = c32 & 15, j = kw + 32 * i + 8 * (y >> 2) + 4 * g + (y & 3);
+            if (c32 < 16 && j < ctx) {
+                const size_t at = (size_t)list * p.cap + j;
+                if (whole)
+                    p.w_out[at] = p.w ? fmaf(p.decay, p.w[at], sum) : sum;
+                else
+                    p.part[((size_t)range + (size_t)list * p.n_blocks + block) * S::kKeys + j % S::kKeys] = sum;
             }
         }
-        const float sum = acc[i][0] + __shfl_xor(acc[i][0], 16);
-        const uint32_t y = c32 & 15, j = kw + 32 * i + 8 * (y >> 2) + 4 * g + (y & 3);
-        if (c32 < 16 && j < ctx) {
-            if (p.n_chunks > 1)
-                p.part[((size_t)chunk * lists + list) * p.max_ctx + j] = sum;
-            else
-                p.w_out[(size_t)list * p.cap + j] =
-                    p.w ? fmaf(p.decay, p.w[(size_t)list * p.cap + j], sum) : sum;
+        if (left == 0)
+            return;
+        tb = 0;
+        if (++block == bt.blocks) {
+            block = 0;
+            if (++kvh == p.kv_heads) {
+                kvh = 0;
+                do {
+                    if (++b >= p.batch)
+                        return;
+                } while (uniform(BlockTiles(p, b, S::kKeys).blocks) == 0);
+            }
         }
     }
 }
 
-// The chunks' sums of each key, in order (those that saw a key of its block wrote one).
+// The blocks that more than one range met: their sums, in order (one range: weights_many wrote the result; no query at all:
+// the old weights).
 __global__ __launch_bounds__(256) void weights_join(const WeightsParams p, uint32_t keys, uint32_t per_list)
 {
-    const uint32_t lists = p.batch * p.kv_heads, list = blockIdx.x / per_list, b = list / p.kv_heads;
-    const uint32_t ctx = ctx_of(p, b), n = n_of(p, b), j = blockIdx.x % per_list * 256 + threadIdx.x;
+    const uint32_t list = blockIdx.x / per_list, b = list / p.kv_heads;
+    const uint32_t ctx = ctx_of(p, b), j = blockIdx.x % per_list * 256 + threadIdx.x;
     if (j >= ctx)
         return;
-    const uint32_t k0 = j / keys * keys, see0 = k0 + n > ctx ? k0 + n - ctx : 0u;
+    const size_t at = (size_t)list * p.cap + j, block = (size_t)list * p.n_blocks + j / keys;
     float sum = 0.0f;
-    for (uint32_t c = min(see0, n) / p.chunk; c < p.n_chunks && max(c * p.chunk, see0) < n; ++c)
-        sum += p.part[((size_t)c * lists + list) * p.max_ctx + j];
-    const size_t at = (size_t)list * p.cap + j;
+    if (n_of(p, b)) {
+        const uint32_t r0 = p.ends[2 * block], r1 = p.ends[2 * block + 1];
+        if (r0 == r1)
+            return;
+        for (uint32_t r = r0; r <= r1; ++r)
+            sum += p.part[(r + block) * keys + j % keys];
+    }
     p.w_out[at] = p.w ? fmaf(p.decay, p.w[at], sum) : sum;
 }
 
 // A call's shape, from its sizes alone.
 struct Plan {
     bool few;
-    uint32_t keys, n_blocks, chunk, n_chunks;
+    uint32_t keys, n_blocks, n_ranges;
 };
 
 Plan plan_of(const mako_weights_args* a, uint32_t cus)
 {
     const uint64_t rows = (uint64_t)a->n_q * (a->heads / a->kv_heads);
-    Plan pl{rows <= kFewRows, 0, 0, 0, 1};
+    Plan pl{rows <= kFewRows, 0, 0, 4 * cus};
     if (pl.few)
         return pl;
     pl.keys = a->dim == 256 ? Many<256>::kKeys : Many<128>::kKeys;
     pl.n_blocks = (a->max_ctx + pl.keys - 1) / pl.keys;
-    const uint64_t units = std::max<uint64_t>(1, (uint64_t)a->batch * a->kv_heads * pl.n_blocks);
-    const uint32_t want = (uint32_t)std::min<uint64_t>(64, (8ull * cus + units - 1) / units);
-    const uint32_t most = (a->n_q + 63) / 64;  // at least 64 queries a chunk
-    pl.n_chunks = std::max(1u, std::min(want, most));
-    pl.chunk = (a->n_q + pl.n_chunks * 32 - 1) / (pl.n_chunks * 32) * 32;
-    pl.n_chunks = (a->n_q + pl.chunk - 1) / pl.chunk;
+    pl.n_ranges = 2 * cus;
     return pl;
 }
 
+size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+
+// The ranges' ends of the blocks, then the shares.
+size_t ends_bytes(const Plan& pl, const mako_weights_args* a)
+{
+    return round256((size_t)a->batch * a->kv_heads * pl.n_blocks * 2 * sizeof(uint32_t));
+}
 size_t workspace_for(const Plan& pl, const mako_weights_args* a)
 {
-    return pl.n_chunks > 1 ? (size_t)pl.n_chunks * a->batch * a->kv_heads * a->max_ctx * sizeof(float) : 0;
+    if (pl.few)
+        return 0;
+    return ends_bytes(pl, a) + (pl.n_ranges + (size_t)a->batch * a->kv_heads * pl.n_blocks) * pl.keys * sizeof(float);
 }
 
 template <class T, int D>
@@ -426,12 +525,9 @@ void launch(const WeightsParams& p, const Plan& pl, hipStream_t s)
             hipLaunchKernelGGL((weights_few<T, D, 2>), grid, dim3(256), 0, s, p);
         return;
     }
-    const uint32_t lists = p.batch * p.kv_heads;
-    hipLaunchKernelGGL((weights_many<T, D>), dim3(lists * p.n_blocks * p.n_chunks), dim3(256), 0, s, p);
-    if (p.n_chunks > 1) {
-        const uint32_t per_list = (p.max_ctx + 255) / 256;
-        hipLaunchKernelGGL(weights_join, dim3(lists * per_list), dim3(256), 0, s, p, pl.keys, per_list);
-    }
+    hipLaunchKernelGGL((weights_many<T, D>), dim3((p.n_ranges + 7) / 8 * 8), dim3(256), 0, s, p);
+    const uint32_t per_list = (p.max_ctx + 255) / 256;
+    hipLaunchKernelGGL(weights_join, dim3(p.batch * p.kv_heads * per_list), dim3(256), 0, s, p, pl.keys, per_list);
 }
 
 template <class T>
@@ -508,12 +604,14 @@ extern "C" int mako_cache_weights(const mako_weights_args* a, mako_dtype in, con
     if (workspace_bytes < need || (need && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 16)
         return fail(MAKO_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, workspace_bytes,
                     need);
-    if ((uint64_t)a->batch * a->kv_heads * std::max(1u, pl.n_blocks) * pl.n_chunks > 0x7fffffffu)
-        return fail(MAKO_EINVAL, "%s: %u x %u lists exceed the grid", what, a->batch, a->kv_heads);
+    // (the query tiles of all key blocks, counted in 32 bits)
+    if (!pl.few && (uint64_t)a->batch * a->heads * pl.n_blocks * ((a->n_q + kTK - 1) / kTK) >= (1ull << 32))
+        return fail(MAKO_EINVAL, "%s: %u x %u heads of %u queries over %u rows exceed 2^32 tiles", what, a->batch, a->heads,
+                    a->n_q, a->max_ctx);
     WeightsParams p{q, k, lse, a->decay == 0.0f ? nullptr : w, w_out, ctx_len, path, n_path,
-                    static_cast<float*>(workspace), a->batch, a->n_q, a->heads, a->kv_heads, a->heads / a->kv_heads,
-                    a->cap, a->max_ctx, 4 * cus, pl.chunk, pl.n_chunks, pl.n_blocks, 0, 0, 0, 0, a->scale * kLog2e,
-                    a->decay};
+                    need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + ends_bytes(pl, a)) : nullptr,
+                    static_cast<uint32_t*>(workspace), a->batch, a->n_q, a->heads, a->kv_heads, a->heads / a->kv_heads,
+                    a->cap, a->max_ctx, pl.n_ranges, pl.n_blocks, 0, 0, 0, 0, a->scale * kLog2e, a->decay};
     if (a->q_pad) {
         p.qs_b = (uint64_t)a->n_q * a->dim, p.qs_h = (uint64_t)a->q_pad * a->dim;
         p.ls_b = a->n_q, p.ls_h = (uint64_t)a->batch * a->n_q;
