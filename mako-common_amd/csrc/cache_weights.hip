@@ -229,8 +229,8 @@ struct Many {
     static constexpr int kKeys = 4 * 32 * kKB;               // keys a workgroup
     static constexpr int kRow = 2 * D, kTile = kTK * kRow;   // a tile of queries
     static constexpr int kPieces = kTile / 1024 / 4;         // 1 KiB pieces of it a wave
-    static constexpr int kDepth = D == 64 ? 8 : 4;
-    static constexpr int kTable = D == 256 ? 2048 : 4096;    // rows whose place and offset are looked up at a time
+    static constexpr int kStep = D == 256 ? 2 : 4;           // tiles a step: a barrier and a ring slot of two
+    static constexpr int kTable = 2048;                      // rows whose place and offset are looked up at a time
 };
 
 // The query tiles of a list's key blocks. Block i's keys start at i keys; the first query that sees them is the (i keys -
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
     using E = Elem<T>;
     using V8 = typename E::vec8;
     constexpr int NK = D / 16, kRow = S::kRow, KB = S::kKB;
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[S::kDepth * S::kTile];
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * S::kStep * S::kTile];
     __shared__ float s_off[S::kTable];
     __shared__ uint32_t s_row[S::kTable];
     const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c32 = lane & 31, wl = uniform(tid >> 6);
@@ -338,10 +338,12 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
             for (int kk = 0; kk < NK; ++kk)
                 kreg[i][kk] = j < ctx ? *reinterpret_cast<const V8*>(src + 16 * kk) : V8{};
         }
-        f32x16 acc[KB];
+        float acc[KB][16];  // (scalars: 16-register tuples would be copied where the loop's two branches meet)
         #pragma unroll
         for (int i = 0; i < KB; ++i)
-            acc[i] = f32x16{};
+            #pragma unroll
+            for (int y = 0; y < 16; ++y)
+                acc[i][y] = 0.0f;
         left -= t_end - tb;
         while (tb < t_end) {
             const uint32_t te = min(t_end, tb + S::kTable / kTK);
@@ -360,64 +362,79 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
                     settle(kreg[i][kk]);
             __syncthreads();
             // Tile t's head and place in it, as t goes on.
-            uint32_t sh = tb / nt, st = tb % nt, ch = sh, ct = st;
+            uint32_t sh = tb / nt, st = tb % nt, ct = st;
+            // The step from tile t on (the steps of a table start at tb).
             auto stage = [&](uint32_t t) __attribute__((always_inline)) {
-                const uint32_t dst = lbase + t % S::kDepth * S::kTile + 1024 * wl * S::kPieces;
-                const u32x4 rs = tile_rsrc(
-                    static_cast<const T*>(p.q) + b * p.qs_b + (uint64_t)(kvh * p.group + sh) * p.qs_h, p.n_q * kRow);
+                const uint32_t dst = lbase + ((t - tb) / S::kStep & 1) * S::kStep * S::kTile + 1024 * wl * S::kPieces;
                 #pragma unroll
-                for (int m = 0; m < S::kPieces; ++m)
-                    dma16_at(dst + 1024 * m, s_row[(t - tb) * kTK + qr[m]] + qc[m], 0, rs);
-                if (++st == nt) {
-                    st = 0;
-                    ++sh;
+                for (int i = 0; i < S::kStep; ++i) {
+                    if (t + i >= te)
+                        break;
+                    const u32x4 rs = tile_rsrc(
+                        static_cast<const T*>(p.q) + b * p.qs_b + (uint64_t)(kvh * p.group + sh) * p.qs_h, p.n_q * kRow);
+                    #pragma unroll
+                    for (int m = 0; m < S::kPieces; ++m)
+                        dma16_at(dst + i * S::kTile + 1024 * m, s_row[(t + i - tb) * kTK + qr[m]] + qc[m], 0, rs);
+                    if (++st == nt) {
+                        st = 0;
+                        ++sh;
+                    }
                 }
             };
-            for (uint32_t t = tb; t < min(te, tb + S::kDepth - 1); ++t)
-                stage(t);
-            for (uint32_t t = tb; t < te; ++t) {
-                if (t + S::kDepth - 1 <= te)
-                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::kDepth - 2) * S::kPieces)
-                                 : "memory");
-                else
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                if (t + S::kDepth - 1 < te)
-                    stage(t + S::kDepth - 1);
-                const unsigned char* tile = lds + t % S::kDepth * S::kTile;
-                const float off = s_off[(t - tb) * kTK + c32];
-                f32x16 x[KB];
-                #pragma unroll
-                for (int i = 0; i < KB; ++i)
-                    x[i] = f32x16{};
-                #pragma unroll
-                for (int kk = 0; kk < NK; ++kk) {
-                    const V8 qf = *reinterpret_cast<const V8*>(tile + (qa ^ (32 * kk)));
+            stage(tb);
+            for (uint32_t t0 = tb; t0 < te; t0 += S::kStep) {
+                // The step has landed, and every wave is done with the one before, whose slot takes the next.
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (t0 + S::kStep < te)
+                    stage(t0 + S::kStep);
+                const unsigned char* step = lds + ((t0 - tb) / S::kStep & 1) * S::kStep * S::kTile;
+                const uint32_t t1 = min(te, t0 + S::kStep);
+                // A tile's operands are read a tile ahead, beside the exponentials of the one before.
+                V8 qf[NK];
+                float off_next;
+                auto read = [&](uint32_t t) __attribute__((always_inline)) {
+                    off_next = s_off[(t - tb) * kTK + c32];
+                    #pragma unroll
+                    for (int kk = 0; kk < NK; ++kk)
+                        qf[kk] = *reinterpret_cast<const V8*>(step + (t - t0) * S::kTile + (qa ^ (32 * kk)));
+                };
+                read(t0);
+                #pragma unroll 1
+                for (uint32_t t = t0; t < t1; ++t) {
+                    const float off = off_next;
+                    f32x16 x[KB];
                     #pragma unroll
                     for (int i = 0; i < KB; ++i)
-                        x[i] = E::mfma32(kreg[i][kk], qf, x[i]);
-                }
-                const uint32_t i0 = ia + ct * kTK;
-                if (++ct == nt) {
-                    ct = 0;
-                    ++ch;
-                }
-                const bool none = off == INFINITY;  // no query: 0 against a key that is not finite too
-                if (kw + 32 * KB + n > ctx + i0 + 1 || __any(none)) {  // some row does not see all of the wave's keys
-                    const uint32_t lim = !none && ctx + i0 + c32 >= n ? ctx + i0 + c32 - n + 1 : 0u;
+                        x[i] = f32x16{};
                     #pragma unroll
-                    for (int i = 0; i < KB; ++i)
+                    for (int kk = 0; kk < NK; ++kk)
                         #pragma unroll
-                        for (int y = 0; y < 16; ++y) {
-                            const uint32_t j = kw + 32 * i + 8 * (y >> 2) + 4 * g + (y & 3);
-                            const float e = exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
-                            acc[i][y] += j < lim ? e : 0.0f;
-                        }
-                } else {
-                    #pragma unroll
-                    for (int i = 0; i < KB; ++i)
+                        for (int i = 0; i < KB; ++i)
+                            x[i] = E::mfma32(kreg[i][kk], qf[kk], x[i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    read(min(t + 1, t1 - 1));
+                    __builtin_amdgcn_sched_barrier(0);
+                    const uint32_t i0 = ia + ct * kTK;
+                    if (++ct == nt)
+                        ct = 0;
+                    const bool none = off == INFINITY;  // no query: 0 against a key that is not finite too
+                    if (kw + 32 * KB + n > ctx + i0 + 1 || __any(none)) {  // some row does not see all of the wave's keys
+                        // the lane's keys kw + 4 g + .. that it sees
+                        const int lim = none ? -1 : (int)(ctx + i0 + c32 + 1) - (int)(n + kw + 4 * g);
                         #pragma unroll
-                        for (int y = 0; y < 16; ++y)
-                            acc[i][y] += exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
+                        for (int i = 0; i < KB; ++i)
+                            #pragma unroll
+                            for (int y = 0; y < 16; ++y) {
+                                const float e = exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
+                                acc[i][y] += 32 * i + 8 * (y >> 2) + (y & 3) < lim ? e : 0.0f;
+                            }
+                    } else {
+                        #pragma unroll
+                        for (int i = 0; i < KB; ++i)
+                            #pragma unroll
+                            for (int y = 0; y < 16; ++y)
+                                acc[i][y] += exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
+                    }
                 }
             }
             tb = te;
