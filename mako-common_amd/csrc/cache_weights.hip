@@ -230,7 +230,7 @@ struct Many {
     static constexpr int kRow = 2 * D, kTile = kTK * kRow;   // a tile of queries
     static constexpr int kPieces = kTile / 1024 / 4;         // 1 KiB pieces of it a wave
     static constexpr int kStep = D == 256 ? 2 : 4;           // tiles a step: a barrier and a ring slot of two
-    static constexpr int kTable = 2048;                      // rows whose place and offset are looked up at a time
+    static constexpr int kTable = 1024;                      // rows of a path looked up at a time
 };
 
 // The query tiles of a list's key blocks. Block i's keys start at i keys; the first query that sees them is the (i keys -
@@ -275,16 +275,19 @@ struct ListTiles {
     __device__ __forceinline__ uint32_t operator()(uint32_t i) const { return BlockTiles(p, i, keys).total(); }
 };
 
-template <class T, int D>
+template <class T, int D, bool PATH>
 __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
 {
     using S = Many<D>;
     using E = Elem<T>;
     using V8 = typename E::vec8;
     constexpr int NK = D / 16, kRow = S::kRow, KB = S::kKB;
+    constexpr int kKPieces = KB * 32 * kRow / 1024;  // 1 KiB pieces of a wave's keys
+    static_assert(4 * kKPieces * 1024 <= 2 * S::kStep * S::kTile, "the keys pass through the ring");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * S::kStep * S::kTile];
-    __shared__ float s_off[S::kTable];
-    __shared__ uint32_t s_row[S::kTable];
+    // lse of the ring's tiles (64 words each, the DMA's), or with a path the offsets and places of kTable rows
+    __shared__ float s_off[PATH ? 2 * S::kTable : 2 * S::kStep * 64];
+    uint32_t* const s_row = reinterpret_cast<uint32_t*>(s_off) + (PATH ? S::kTable : 0);
     const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c32 = lane & 31, wl = uniform(tid >> 6);
     const uint32_t total = uniform(sum_of(p.batch, lane, ListTiles{p, S::kKeys}) * p.kv_heads);
     // An XCD's workgroups take neighbouring ranges: they share queries and keys in its L2.
@@ -315,6 +318,7 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
         qc[m] = 16 * ((pos / 16) ^ k_xor<D>(qr[m]));
     }
     const uint32_t lbase = uniform((uint32_t)reinterpret_cast<uintptr_t>(lds));
+    const uint32_t obase = uniform((uint32_t)reinterpret_cast<uintptr_t>(s_off));
     const uint32_t qa = c32 * kRow + 16 * (g ^ k_xor<D>(c32));
     for (;;) {
         const BlockTiles bt(p, b, S::kKeys);
@@ -322,6 +326,16 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
         const uint32_t nt = uniform(bt.tiles(block)), ia = uniform(bt.first_tile(block)) * kTK, all = nt * p.group;
         const uint32_t t_end = min(all, tb + left), kw = block * S::kKeys + wl * 32 * KB;  // the wave's first key
         const bool whole = tb == 0 && t_end == all;
+        left -= t_end - tb;
+        // The wave's keys, through its part of the ring.
+        {
+            const u32x4 rs = tile_rsrc(static_cast<const T*>(p.k) + (size_t)list * p.cap * D, ctx * kRow);
+            #pragma unroll
+            for (int m = 0; m < kKPieces; ++m) {
+                const uint32_t at = 1024 * m + 16 * lane, r = at / kRow, pos = at % kRow;
+                dma16_at(lbase + 1024 * (wl * kKPieces + m), (kw + r) * kRow + 16 * ((pos / 16) ^ k_xor<D>(r)), 0, rs);
+            }
+        }
         if (tid == 0) {
             uint32_t* ends = p.ends + 2 * ((size_t)list * p.n_blocks + block);
             if (tb == 0)
@@ -329,55 +343,62 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
             if (t_end == all)
                 ends[1] = range;
         }
-        V8 kreg[KB][NK];
-        #pragma unroll
-        for (int i = 0; i < KB; ++i) {
-            const uint32_t j = kw + 32 * i + c32;
-            const T* src = static_cast<const T*>(p.k) + ((size_t)list * p.cap + j) * D + 8 * g;
-            #pragma unroll
-            for (int kk = 0; kk < NK; ++kk)
-                kreg[i][kk] = j < ctx ? *reinterpret_cast<const V8*>(src + 16 * kk) : V8{};
-        }
-        float acc[KB][16];  // (scalars: 16-register tuples would be copied where the loop's two branches meet)
+        float acc[KB][16];  // (scalars: 16-register tuples would be copied where the loop's branches meet)
         #pragma unroll
         for (int i = 0; i < KB; ++i)
             #pragma unroll
             for (int y = 0; y < 16; ++y)
                 acc[i][y] = 0.0f;
-        left -= t_end - tb;
-        while (tb < t_end) {
-            const uint32_t te = min(t_end, tb + S::kTable / kTK);
-            __syncthreads();
-            for (uint32_t x = tid; x < (te - tb) * kTK; x += 256) {
-                const uint32_t t = tb + x / kTK, h = kvh * p.group + t / nt, i = ia + t % nt * kTK + x % kTK;
-                float off;
-                const uint32_t r = query(p, b, h, i, i < n, off);
-                s_off[x] = off;
-                s_row[x] = r < p.n_q ? r * kRow : 0x80000000u;  // (past the descriptor: zeros)
-            }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        V8 kreg[KB][NK];
+        #pragma unroll
+        for (int i = 0; i < KB; ++i)
             #pragma unroll
-            for (int i = 0; i < KB; ++i)
-                #pragma unroll
-                for (int kk = 0; kk < NK; ++kk)
-                    settle(kreg[i][kk]);
-            __syncthreads();
+            for (int kk = 0; kk < NK; ++kk)
+                kreg[i][kk] = *reinterpret_cast<const V8*>(lds + 1024 * wl * kKPieces + 32 * i * kRow + (qa ^ (32 * kk)));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        while (tb < t_end) {
+            const uint32_t te = PATH ? min(t_end, tb + S::kTable / kTK) : t_end;
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the ring and the tables are free
+            if (PATH) {
+                for (uint32_t x = tid; x < (te - tb) * kTK; x += 256) {
+                    const uint32_t t = tb + x / kTK, h = kvh * p.group + t / nt, i = ia + t % nt * kTK + x % kTK;
+                    float off;
+                    const uint32_t r = query(p, b, h, i, i < n, off);
+                    s_off[x] = off;
+                    s_row[x] = r * kRow;  // (n_q: past the descriptor, zeros)
+                }
+                __syncthreads();
+            }
             // Tile t's head and place in it, as t goes on.
-            uint32_t sh = tb / nt, st = tb % nt, ct = st;
-            // The step from tile t on (the steps of a table start at tb).
+            uint32_t sh = uniform(tb / nt), st = uniform(tb % nt), ct = st;
+            u32x4 qrs, lrs;
+            auto head = [&]() __attribute__((always_inline)) {
+                const uint64_t h = kvh * p.group + sh;
+                qrs = tile_rsrc(static_cast<const T*>(p.q) + b * p.qs_b + h * p.qs_h, p.n_q * kRow);
+                lrs = tile_rsrc(p.lse + b * p.ls_b + h * p.ls_h, p.n_q * 4);
+            };
+            head();
+            // The step from tile t on (the steps start at tb). Without a path, rows past the last query are another's, or past
+            // the descriptor: masked.
             auto stage = [&](uint32_t t) __attribute__((always_inline)) {
-                const uint32_t dst = lbase + ((t - tb) / S::kStep & 1) * S::kStep * S::kTile + 1024 * wl * S::kPieces;
+                const uint32_t slot = ((t - tb) / S::kStep & 1) * S::kStep;
                 #pragma unroll
                 for (int i = 0; i < S::kStep; ++i) {
                     if (t + i >= te)
                         break;
-                    const u32x4 rs = tile_rsrc(
-                        static_cast<const T*>(p.q) + b * p.qs_b + (uint64_t)(kvh * p.group + sh) * p.qs_h, p.n_q * kRow);
+                    const uint32_t dst = lbase + (slot + i) * S::kTile + 1024 * wl * S::kPieces;
                     #pragma unroll
-                    for (int m = 0; m < S::kPieces; ++m)
-                        dma16_at(dst + i * S::kTile + 1024 * m, s_row[(t + i - tb) * kTK + qr[m]] + qc[m], 0, rs);
+                    for (int m = 0; m < S::kPieces; ++m) {
+                        const uint32_t at = PATH ? s_row[(t + i - tb) * kTK + qr[m]] : (ia + st * kTK + qr[m]) * kRow;
+                        dma16_at(dst + 1024 * m, at + qc[m], 0, qrs);
+                    }
+                    if (!PATH && wl == i % 4)
+                        dma4_at(obase + (slot + i) * 256, (ia + st * kTK + c32) * 4, lrs);
                     if (++st == nt) {
                         st = 0;
                         ++sh;
+                        head();
                     }
                 }
             };
@@ -387,21 +408,25 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 if (t0 + S::kStep < te)
                     stage(t0 + S::kStep);
-                const unsigned char* step = lds + ((t0 - tb) / S::kStep & 1) * S::kStep * S::kTile;
-                const uint32_t t1 = min(te, t0 + S::kStep);
+                const uint32_t slot = ((t0 - tb) / S::kStep & 1) * S::kStep, t1 = min(te, t0 + S::kStep);
                 // A tile's operands are read a tile ahead, beside the exponentials of the one before.
                 V8 qf[NK];
                 float off_next;
                 auto read = [&](uint32_t t) __attribute__((always_inline)) {
-                    off_next = s_off[(t - tb) * kTK + c32];
+                    off_next = PATH ? s_off[(t - tb) * kTK + c32] : s_off[(slot + t - t0) * 64 + c32];
                     #pragma unroll
                     for (int kk = 0; kk < NK; ++kk)
-                        qf[kk] = *reinterpret_cast<const V8*>(step + (t - t0) * S::kTile + (qa ^ (32 * kk)));
+                        qf[kk] = *reinterpret_cast<const V8*>(lds + (slot + t - t0) * S::kTile + (qa ^ (32 * kk)));
                 };
                 read(t0);
                 #pragma unroll 1
                 for (uint32_t t = t0; t < t1; ++t) {
-                    const float off = off_next;
+                    const uint32_t i0 = ia + ct * kTK;
+                    if (++ct == nt)
+                        ct = 0;
+                    // No query: -inf as lse, or past the last. (With 0 for a row, against a key that is not finite, NaN: masked.)
+                    const bool none = PATH ? off_next == INFINITY : off_next == -INFINITY || i0 + c32 >= n;
+                    const float off = PATH ? off_next : off_next * kLog2e;
                     f32x16 x[KB];
                     #pragma unroll
                     for (int i = 0; i < KB; ++i)
@@ -414,26 +439,25 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
                     __builtin_amdgcn_sched_barrier(0);
                     read(min(t + 1, t1 - 1));
                     __builtin_amdgcn_sched_barrier(0);
-                    const uint32_t i0 = ia + ct * kTK;
-                    if (++ct == nt)
-                        ct = 0;
-                    const bool none = off == INFINITY;  // no query: 0 against a key that is not finite too
-                    if (kw + 32 * KB + n > ctx + i0 + 1 || __any(none)) {  // some row does not see all of the wave's keys
-                        // the lane's keys kw + 4 g + .. that it sees
-                        const int lim = none ? -1 : (int)(ctx + i0 + c32 + 1) - (int)(n + kw + 4 * g);
-                        #pragma unroll
-                        for (int i = 0; i < KB; ++i)
-                            #pragma unroll
-                            for (int y = 0; y < 16; ++y) {
-                                const float e = exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
-                                acc[i][y] += 32 * i + 8 * (y >> 2) + (y & 3) < lim ? e : 0.0f;
-                            }
-                    } else {
-                        #pragma unroll
-                        for (int i = 0; i < KB; ++i)
+                    const bool some = __any(none);
+                    #pragma unroll
+                    for (int i = 0; i < KB; ++i) {
+                        // The first query sees `seen` of the block's keys, the last 31 more.
+                        const int seen = (int)(ctx + i0 + 1) - (int)(n + kw + 32 * i);
+                        if (seen + 31 <= 0)
+                            continue;
+                        if (seen >= 32 && !some) {
                             #pragma unroll
                             for (int y = 0; y < 16; ++y)
                                 acc[i][y] += exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
+                        } else {
+                            const int lim = none ? -1 : seen + (int)c32 - 4 * (int)g;
+                            #pragma unroll
+                            for (int y = 0; y < 16; ++y) {
+                                const float e = exp2_fast(fmaf(x[i][y], p.scale_log2, -off));
+                                acc[i][y] += 8 * (y >> 2) + (y & 3) < lim ? e : 0.0f;
+                            }
+                        }
                     }
                 }
             }
@@ -465,6 +489,7 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
         }
         if (left == 0)
             return;
+        __syncthreads();  // the ring is free
         tb = 0;
         if (++block == bt.blocks) {
             block = 0;
@@ -542,7 +567,11 @@ void launch(const WeightsParams& p, const Plan& pl, hipStream_t s)
             hipLaunchKernelGGL((weights_few<T, D, 2>), grid, dim3(256), 0, s, p);
         return;
     }
-    hipLaunchKernelGGL((weights_many<T, D>), dim3((p.n_ranges + 7) / 8 * 8), dim3(256), 0, s, p);
+    const dim3 grid((p.n_ranges + 7) / 8 * 8);
+    if (p.path)
+        hipLaunchKernelGGL((weights_many<T, D, true>), grid, dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((weights_many<T, D, false>), grid, dim3(256), 0, s, p);
     const uint32_t per_list = (p.max_ctx + 255) / 256;
     hipLaunchKernelGGL(weights_join, dim3(p.batch * p.kv_heads * per_list), dim3(256), 0, s, p, pl.keys, per_list);
 }
