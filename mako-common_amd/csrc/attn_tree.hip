@@ -343,29 +343,43 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                         acc[db][i] *= f;
             }
             const float mu = m == -INFINITY ? 0.0f : m;
-            #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                x[i] = exp2_fast(x[i] - mu);
-            l += ((x[0] + x[1]) + (x[2] + x[3]) + ((x[4] + x[5]) + (x[6] + x[7]))) +
-                 ((x[8] + x[9]) + (x[10] + x[11]) + ((x[12] + x[13]) + (x[14] + x[15])));
-            #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                u32x4 hi, lo;
+            // 16 keys at a time: the second half's exponentials run beside the first half's products.
+            u32x4 hi[2], lo[2];
+            auto half = [&](int a) __attribute__((always_inline)) {
+                #pragma unroll
+                for (int i = 8 * a; i < 8 * a + 8; ++i)
+                    x[i] = exp2_fast(x[i] - mu);
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float e0 = x[8 * a + 2 * i], e1 = x[8 * a + 2 * i + 1];
-                    hi[i] = E::pack2(e0, e1);
+                    hi[a][i] = E::pack2(e0, e1);
                     if (kSplitP)
-                        lo[i] = E::pack2(e0 - value_of<T>(hi[i], 0), e1 - value_of<T>(hi[i], 1));
+                        lo[a][i] = E::pack2(e0 - value_of<T>(hi[a][i], 0), e1 - value_of<T>(hi[a][i], 1));
                 }
+                l += (x[8 * a] + x[8 * a + 1]) + (x[8 * a + 2] + x[8 * a + 3]) +
+                     ((x[8 * a + 4] + x[8 * a + 5]) + (x[8 * a + 6] + x[8 * a + 7]));
+            };
+            auto products = [&](int a) __attribute__((always_inline)) {
                 #pragma unroll
                 for (int db = 0; db < ND; ++db)
-                    acc[db] = E::mfma32(vf[a][db], __builtin_bit_cast(V8, hi), acc[db]);
+                    acc[db] = E::mfma32(vf[a][db], __builtin_bit_cast(V8, hi[a]), acc[db]);
                 if (kSplitP)
                     #pragma unroll
                     for (int db = 0; db < ND; ++db)
-                        acc[db] = E::mfma32(vf[a][db], __builtin_bit_cast(V8, lo), acc[db]);
+                        acc[db] = E::mfma32(vf[a][db], __builtin_bit_cast(V8, lo[a]), acc[db]);
+            };
+            half(0);
+            __builtin_amdgcn_sched_barrier(0);
+            products(0);
+            half(1);
+            constexpr int kMf = ND * (kSplitP ? 2 : 1);  // products of a half
+            #pragma unroll
+            for (int i = 0; i < kMf; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, (kSplitP ? 40 : 20) / kMf + 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x400, 8 / kMf + 1, 0);
             }
+            products(1);
         };
         uint32_t s = s0;
         for (const uint32_t whole = min(s1, ctx / kTK / KW); s < whole; ++s) {
