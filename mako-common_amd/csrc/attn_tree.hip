@@ -48,6 +48,7 @@ struct TreeParams {
     uint32_t nc, ncb;   // columns (n_draft x group), column blocks
     uint32_t ways;      // tiles a step
     uint32_t n_ranges;  // 0: a segment a workgroup
+    uint32_t lead;      // units of a segment in front of its steps
     float scale_log2;
 };
 
@@ -66,10 +67,15 @@ __device__ __forceinline__ uint32_t steps_of(const TreeParams& p, uint32_t ctx, 
     return ((ctx + kTK - 1) / kTK + (nodes + kTK - 1) / kTK + p.ways - 1) / p.ways;
 }
 
-// The steps of a segment of sequence i.
-struct SegSteps {
+// The units of a segment of sequence i: its steps, and `lead` more in front of them for what a piece costs beside its
+// steps, so that ranges that meet two segments get fewer.
+struct SegUnits {
     const TreeParams& p;
-    __device__ __forceinline__ uint32_t operator()(uint32_t i) const { return steps_of(p, ctx_of(p, i), nodes_of(p, i)); }
+    __device__ __forceinline__ uint32_t operator()(uint32_t i) const
+    {
+        const uint32_t steps = steps_of(p, ctx_of(p, i), nodes_of(p, i));
+        return steps ? steps + p.lead : 0u;
+    }
 };
 
 // The key in slot s of a tile's K image (its own inverse).
@@ -199,26 +205,39 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
     for (int i = 0; i < NV; ++i)
         va[i] = kHalf + (8 * g + gj) * kRow + 32 * v_unit<D>(2 * i + gg, gj) + 8 * gy;
 
-    // The first piece of the range (or the segment).
-    uint32_t b, kvh, len, s0, s1, left = 0;  // steps [s0, s1) of the segment's len; steps of the range behind them
+    // The first piece of the range (or the segment): steps [s0, s1) of the segment's len; units of the range behind them.
+    uint32_t b, kvh, len, s0, s1, left = 0;
     if (p.n_ranges) {
-        const uint32_t total = uniform(sum_of(p.batch, lane, SegSteps{p}) * p.kv_heads);
-        if (range >= total)
+        const Place at = place_of(p.batch, p.kv_heads, range, p.n_ranges, lane, SegUnits{p});
+        if (at.x0 == at.x1)
             return;
-        const Ranges rg(total, min(total, p.n_ranges));  // (none is empty)
-        const uint32_t x0 = rg.start(range), x1 = rg.start(range + 1);
-        uint32_t first;
-        seq_of(p.batch, x0, lane, SegSteps{p}, p.kv_heads, b, first);
-        b = uniform(b);
-        len = uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b)));
-        kvh = (x0 - uniform(first)) / len;
-        s0 = (x0 - uniform(first)) % len;
-        s1 = min(len, s0 + (x1 - x0));
-        left = x1 - x0 - (s1 - s0);
+        b = at.b;
+        len = at.len - p.lead;
+        kvh = (at.x0 - at.first) / at.len;
+        const uint32_t u0 = (at.x0 - at.first) % at.len, u1 = min(at.len, u0 + (at.x1 - at.x0));
+        s0 = max(u0, p.lead) - p.lead;
+        s1 = max(u1, p.lead) - p.lead;
+        left = at.x1 - at.x0 - (u1 - u0);
     } else {
         b = range / p.kv_heads, kvh = range % p.kv_heads, s0 = 0;
         s1 = len = uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b)));
     }
+    // On to the segment behind; whether the range has a piece of it.
+    const auto next = [&]() __attribute__((always_inline)) {
+        do {
+            if (++kvh == p.kv_heads) {
+                kvh = 0;
+                ++b;
+            }
+            len = b < p.batch ? uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b))) : 0u;
+        } while (b < p.batch && len == 0);
+        s0 = 0;
+        s1 = max(min(len + p.lead, left), p.lead) - p.lead;
+        left -= min(len + p.lead, left);
+        return b < p.batch && s1 > 0;
+    };
+    if (p.n_ranges && s0 == s1 && !(left && next()))
+        return;
 
     for (;;) {
         const uint32_t ctx = uniform(ctx_of(p, b)), nodes = uniform(nodes_of(p, b)), tc = (ctx + kTK - 1) / kTK;
@@ -418,29 +437,36 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
             if (s1 == len)
                 p.seg_ends[2 * (b * p.kv_heads + kvh) + 1] = range;
         }
-        for (uint32_t it = tid; it < NG * 32 * (D / 4); it += W * 64) {
-            const uint32_t q = it % (D / 4), cc = it / (D / 4) % 32, gi = it / (D / 4) / 32;
+        constexpr int kItems = NG * 32 * (D / 4) / (W * 64);  // quads of a column a thread
+        constexpr int kUnroll = D == 256 || (W > 4 && KW >= 4) ? 1 : 4;  // (as registers allow)
+        #pragma unroll kUnroll
+        for (int i = 0; i < kItems; ++i) {
+            const uint32_t it = i * (W * 64) + tid, q = it % (D / 4), cc = it / (D / 4) % 32, gi = it / (D / 4) / 32;
             const uint32_t ccol = 32 * (cb * NG + gi) + cc, rr = ccol / p.group;
-            if (ccol >= p.nc || rr >= nodes)
-                continue;
             float mx = -INFINITY, sum = 0.0f;
-            #pragma unroll
-            for (int y = 0; y < KW; ++y)
-                mx = fmaxf(mx, s_ml[gi + NG * y][cc].x);
             f32x4 a = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            float2 ml[KW];
+            f32x4 v[KW];
             #pragma unroll
             for (int y = 0; y < KW; ++y) {
                 const uint32_t w = gi + NG * y;
-                const float2 ml = s_ml[w][cc];
-                const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - mx);
-                sum += ml.y * f;
-                a += reinterpret_cast<const f32x4*>(lds)[(w * 32 + cc) * (D / 4) + (q ^ (cc & 15))] * f;
+                ml[y] = s_ml[w][cc];
+                v[y] = reinterpret_cast<const f32x4*>(lds)[(w * 32 + cc) * (D / 4) + (q ^ (cc & 15))];
+                mx = fmaxf(mx, ml[y].x);
             }
+            #pragma unroll
+            for (int y = 0; y < KW; ++y) {
+                const float f = ml[y].x == -INFINITY ? 0.0f : exp2_fast(ml[y].x - mx);
+                sum += ml[y].y * f;
+                a += v[y] * f;
+            }
+            const bool live = ccol < p.nc && rr < nodes;
             if (p.n_ranges) {
-                *reinterpret_cast<f32x4*>(p.part_o + (part * p.nc + ccol) * D + 4 * q) = a;
-                if (q == 0)
+                if (live)
+                    *reinterpret_cast<f32x4*>(p.part_o + (part * p.nc + ccol) * D + 4 * q) = a;
+                if (live && q == 0)
                     *reinterpret_cast<float2*>(p.part_ml + (part * p.nc + ccol) * 2) = float2{mx, sum};
-            } else {
+            } else if (live) {
                 const uint32_t hh = kvh * p.group + ccol % p.group;
                 const size_t row = (size_t)b * p.n_draft + rr;
                 a *= sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -453,21 +479,9 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                     lse[(size_t)hh * p.batch * p.n_draft + row] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * kLn2;
             }
         }
-        if (left == 0)
+        if (left == 0 || !next())
             return;
         __syncthreads();  // the ring is free again
-        do {
-            if (++kvh == p.kv_heads) {
-                kvh = 0;
-                ++b;
-            }
-            len = b < p.batch ? uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b))) : 0u;
-        } while (b < p.batch && len == 0);
-        if (b >= p.batch)
-            return;
-        s0 = 0;
-        s1 = min(len, left);
-        left -= s1;
     }
 }
 
@@ -663,7 +677,7 @@ int check_args(const mako_tree_args* a, mako_dtype in, mako_dtype out, const voi
         return fail(MAKO_EINVAL, "%s: max_ctx %u over the cache's %u rows", what, a->max_ctx, a->cap);
     if ((uint64_t)a->cap * a->dim * 2 > 0x7fffffffu)
         return fail(MAKO_EINVAL, "%s: %u cache rows exceed 2 GiB a head", what, a->cap);
-    if ((uint64_t)a->batch * a->kv_heads * (a->max_ctx + 64ull) >= (1ull << 32))
+    if ((uint64_t)a->batch * a->kv_heads * (a->max_ctx + 512ull) >= (1ull << 32))
         return fail(MAKO_EINVAL, "%s: %u x %u x %u rows exceed 2^32", what, a->batch, a->kv_heads, a->max_ctx);
     if ((uint64_t)a->heads * a->dim > a->width || a->width % 4)
         return fail(MAKO_EINVAL, "%s: o rows of %u for %u heads of %u (a multiple of 4, at least their width)", what,
@@ -716,7 +730,7 @@ extern "C" int mako_attn_tree(const mako_tree_args* a, mako_dtype in, mako_dtype
                        reinterpret_cast<float*>(at(ob)), reinterpret_cast<uint32_t*>(at(ob + mb)),
                        reinterpret_cast<uint32_t*>(at(ob + mb + fb)),
                        a->batch, a->n_draft, a->q_pad, a->d_pad, a->heads, a->kv_heads, group, a->cap, a->max_ctx,
-                       a->width, a->n_draft * group, pl.ncb, pl.ways, pl.n_ranges, a->scale * kLog2e};
+                       a->width, a->n_draft * group, pl.ncb, pl.ways, pl.n_ranges, a->dim == 256 ? 6u : 3u, a->scale * kLog2e};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (in == MAKO_BF16 && out == MAKO_F32)
         launch_dim<__bf16, float>(p, a->dim, pl.ng, o, lse, s);

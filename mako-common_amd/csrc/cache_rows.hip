@@ -92,19 +92,7 @@ __device__ __forceinline__ uint32_t order_of(float x)
 constexpr int kDigits = 2048;  // of 11, 11 and 10 bits
 constexpr int kCopies = 2;     // counters a digit, by lane
 
-// The inclusive sum of x over a wave's lanes up to this one, by row shifts and broadcasts.
-__device__ __forceinline__ uint32_t scan_lanes(uint32_t x)
-{
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, false);  // row_shr 1
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false);  // lane 15 of rows 0 and 2 to rows 1 and 3
-    x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
-    return x;
-}
-
-// The same over the workgroup's threads; total: over all of them (s: a word a wave; two barriers).
+// The inclusive sum of x over the workgroup's threads up to this one; total: over all of them (s: a word a wave; two barriers).
 template <int W>
 __device__ __forceinline__ uint32_t scan_threads(uint32_t x, u32x4 (&s)[W / 4], uint32_t lane, uint32_t wv, uint32_t& total)
 {

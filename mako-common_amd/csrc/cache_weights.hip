@@ -98,15 +98,10 @@ __global__ __launch_bounds__(256, 1) void weights_few(const WeightsParams p)
     __shared__ __attribute__((aligned(16))) float s_off[S::kWaves][32 * NCG];
     __shared__ __attribute__((aligned(16))) uint32_t s_lim[S::kWaves][32 * NCG];
     const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c32 = lane & 31, wl = uniform(tid >> 6);
-    const Ranges rg(uniform(sum_of(p.batch, lane, KeyTiles{p}) * p.kv_heads), p.n_ranges);
-    const uint32_t wave = blockIdx.x * S::kWaves + wl, x0 = rg.start(wave), x1 = rg.start(wave + 1);
-    if (x0 >= x1)
+    const Place at = place_of(p.batch, p.kv_heads, blockIdx.x * S::kWaves + wl, p.n_ranges, lane, KeyTiles{p});
+    if (at.x0 == at.x1)
         return;
-    uint32_t b, first;
-    seq_of(p.batch, x0, lane, KeyTiles{p}, p.kv_heads, b, first);
-    b = uniform(b);
-    first = uniform(first);
-    uint32_t len = uniform(KeyTiles{p}(b)), kvh = (x0 - first) / len, t0 = (x0 - first) % len, left = x1 - x0;
+    uint32_t b = at.b, len = at.len, kvh = (at.x0 - at.first) / len, t0 = (at.x0 - at.first) % len, left = at.x1 - at.x0;
 
     uint32_t kd[S::kPieces];
     #pragma unroll
@@ -289,23 +284,15 @@ __global__ __launch_bounds__(256, 2) void weights_many(const WeightsParams p)
     __shared__ float s_off[PATH ? 2 * S::kTable : 2 * S::kStep * 64];
     uint32_t* const s_row = reinterpret_cast<uint32_t*>(s_off) + (PATH ? S::kTable : 0);
     const uint32_t tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c32 = lane & 31, wl = uniform(tid >> 6);
-    const uint32_t total = uniform(sum_of(p.batch, lane, ListTiles{p, S::kKeys}) * p.kv_heads);
     // An XCD's workgroups take neighbouring ranges: they share queries and keys in its L2.
     const uint32_t per_xcd = (p.n_ranges + 7) / 8, range = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
-    const Ranges rg(total, min(total, p.n_ranges));
-    if (blockIdx.x / 8 >= per_xcd || range >= rg.n)
+    const Place at = place_of(p.batch, p.kv_heads, range, p.n_ranges, lane, ListTiles{p, S::kKeys});
+    if (at.x0 == at.x1)
         return;
-    const uint32_t x0 = rg.start(range);
-    uint32_t left = rg.start(range + 1) - x0, b, first;
-    seq_of(p.batch, x0, lane, ListTiles{p, S::kKeys}, p.kv_heads, b, first);
-    b = uniform(b);
-    first = uniform(first);
-    uint32_t kvh, block, tb;  // tiles from tb of the block on
+    uint32_t left = at.x1 - at.x0, b = at.b, kvh = (at.x0 - at.first) / at.len, block, tb;  // tiles from tb of the block on
     {
         const BlockTiles bt(p, b, S::kKeys);
-        const uint32_t len = uniform(bt.total());
-        kvh = (x0 - first) / len;
-        const uint32_t x = (x0 - first) % len;
+        const uint32_t x = (at.x0 - at.first) % at.len;
         block = uniform(bt.of(x));
         tb = x - uniform(bt.before(block));
     }
