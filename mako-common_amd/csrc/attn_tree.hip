@@ -438,7 +438,7 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                 p.seg_ends[2 * (b * p.kv_heads + kvh) + 1] = range;
         }
         constexpr int kItems = NG * 32 * (D / 4) / (W * 64);  // quads of a column a thread
-        constexpr int kUnroll = D == 256 || (W > 4 && KW >= 4) ? 1 : 4;  // (as registers allow)
+        constexpr int kUnroll = W > 4 && KW >= 4 ? 1 : 4;  // (as registers allow)
         #pragma unroll kUnroll
         for (int i = 0; i < kItems; ++i) {
             const uint32_t it = i * (W * 64) + tid, q = it % (D / 4), cc = it / (D / 4) % 32, gi = it / (D / 4) / 32;
