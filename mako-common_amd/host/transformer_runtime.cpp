@@ -18,6 +18,12 @@ std::string fmt(const char* f, A... a)
     return buf;
 }
 
+template <class T>
+T* ptr(gpu::Buffer* b)
+{
+    return b ? static_cast<T*>(b->ptr) : nullptr;
+}
+
 }  // namespace
 
 void TransformerRuntime::heads(gpu::Encoder*& enc, gpu::Buffer* x, uint32_t ld, uint32_t col0, uint32_t n_heads,
@@ -187,6 +193,72 @@ void TransformerRuntime::attention_decode(gpu::Encoder*& enc, gpu::Buffer* q, gp
                                o->ptr, opt.lse ? static_cast<float*>(opt.lse->ptr) : nullptr, ws->ptr, ws->bytes,
                                enc->stream));
     after(enc, "attn_decode");
+}
+
+void TransformerRuntime::attention_tree(gpu::Encoder*& enc, gpu::Buffer* q, gpu::Buffer* k, gpu::Buffer* v,
+                                        gpu::Buffer* kd, gpu::Buffer* vd, gpu::Buffer* ctx_len, gpu::Buffer* n_nodes,
+                                        gpu::Buffer* mask, gpu::Buffer* o, uint32_t batch, uint32_t n_draft,
+                                        uint32_t n_heads, uint32_t kv_heads, uint32_t cap, uint32_t max_ctx,
+                                        uint32_t dim, const AttnOptions& opt)
+{
+    const mako_tree_args a{batch, n_draft, batch * n_draft, batch * n_draft, n_heads, kv_heads, dim, cap, max_ctx,
+                           n_heads * dim, 1.0f / std::sqrt(float(dim))};
+    const size_t need = mako_attn_tree_workspace(&a);
+    gpu::Buffer* ws = need ? scratch("attn_tree", need) : nullptr;
+    before(enc);
+    for (int r = repeats("attn_tree"); r > 0; --r)
+        check(mako_attn_tree(&a, opt.in, opt.out, q->ptr, k->ptr, v->ptr, kd->ptr, vd->ptr, ptr<const uint32_t>(ctx_len),
+                             ptr<const uint32_t>(n_nodes), ptr<const uint64_t>(mask), o->ptr, ptr<float>(opt.lse),
+                             ptr<void>(ws), ws ? ws->bytes : 0, enc->stream));
+    after(enc, "attn_tree");
+}
+
+void TransformerRuntime::cache_append(gpu::Encoder*& enc, gpu::Buffer* kd, gpu::Buffer* vd, gpu::Buffer* path,
+                                      gpu::Buffer* n_path, gpu::Buffer* ctx_len, gpu::Buffer* seen, gpu::Buffer* w,
+                                      gpu::Buffer* pos, gpu::Buffer* k, gpu::Buffer* v, uint32_t batch,
+                                      uint32_t n_draft, uint32_t kv_heads, uint32_t cap, uint32_t dim, mako_dtype in)
+{
+    const mako_append_args a{batch, n_draft, batch * n_draft, kv_heads, dim, cap};
+    before(enc);
+    // (once: what it appends to has grown by then)
+    check(mako_cache_append(&a, in, kd->ptr, vd->ptr, ptr<const uint32_t>(path), ptr<const uint32_t>(n_path),
+                            ptr<const uint32_t>(ctx_len), ptr<uint32_t>(ctx_len), ptr<const uint32_t>(seen),
+                            ptr<uint32_t>(seen), ptr<float>(w), ptr<uint32_t>(pos), k->ptr, v->ptr, enc->stream));
+    after(enc, "cache_append");
+}
+
+void TransformerRuntime::cache_weights(gpu::Encoder*& enc, gpu::Buffer* q, gpu::Buffer* lse, gpu::Buffer* k,
+                                       gpu::Buffer* ctx_len, gpu::Buffer* path, gpu::Buffer* n_path, gpu::Buffer* w,
+                                       uint32_t batch, uint32_t n_q, uint32_t n_heads, uint32_t kv_heads, uint32_t cap,
+                                       uint32_t max_ctx, float decay, bool by_sequence, uint32_t dim, mako_dtype in)
+{
+    const mako_weights_args a{batch, n_q, by_sequence ? 0u : batch * n_q, n_heads, kv_heads, dim, cap, max_ctx,
+                              1.0f / std::sqrt(float(dim)), decay};
+    const size_t need = mako_cache_weights_workspace(&a);
+    gpu::Buffer* ws = need ? scratch("cache_weights", need) : nullptr;
+    before(enc);
+    // (once: w gathers)
+    check(mako_cache_weights(&a, in, q->ptr, ptr<const float>(lse), k->ptr, ptr<const uint32_t>(ctx_len),
+                             ptr<const uint32_t>(path), ptr<const uint32_t>(n_path), ptr<const float>(w), ptr<float>(w),
+                             ptr<void>(ws), ws ? ws->bytes : 0, enc->stream));
+    after(enc, "cache_weights");
+}
+
+void TransformerRuntime::cache_evict(gpu::Encoder*& enc, gpu::Buffer* k, gpu::Buffer* v, gpu::Buffer* w,
+                                     gpu::Buffer* pos, gpu::Buffer* seen, gpu::Buffer* ctx_len, uint32_t batch,
+                                     uint32_t kv_heads, uint32_t cap, uint32_t max_ctx, uint32_t budget,
+                                     uint32_t recent, uint32_t sinks, uint32_t dim, mako_dtype in)
+{
+    const mako_evict_args a{batch, kv_heads, dim, cap, max_ctx, budget, recent, sinks};
+    const size_t need = mako_cache_evict_workspace(&a);
+    gpu::Buffer* ws = need ? scratch("cache_evict", need) : nullptr;
+    before(enc);
+    for (int r = repeats("cache_evict"); r > 0; --r)
+        check(mako_cache_evict(&a, in, k->ptr, v->ptr, ptr<const float>(w), ptr<const uint32_t>(pos),
+                               ptr<const uint32_t>(seen), ptr<const uint32_t>(ctx_len), ptr<float>(w),
+                               ptr<uint32_t>(pos), ptr<uint32_t>(ctx_len), ptr<void>(ws), ws ? ws->bytes : 0,
+                               enc->stream));
+    after(enc, "cache_evict");
 }
 
 }  // namespace mako::models

@@ -93,6 +93,35 @@ protected:
     void attention_decode(gpu::Encoder*& enc, gpu::Buffer* q, gpu::Buffer* k, gpu::Buffer* v, gpu::Buffer* ctx_len,
                           gpu::Buffer* o, uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t cap,
                           uint32_t max_ctx, const AttnOptions& opt = {});
+    // The cache of attention_decode with trees of drafted tokens (no counterparts in the reference). attention_tree: node r
+    // of sequence b is row b * n_draft + r of q [heads][rows][dim], kd and vd [kv_heads][rows][dim] (the tiles heads() and
+    // heads_partial() write for the drafts of all sequences one after another) and of o [rows][heads * dim], opt.lse
+    // [heads][rows]; it sees the cache rows below ctx_len[b] and the drafts of its mask (u64 [batch][n_draft], null: those
+    // up to it), n_nodes u32 [batch] of them (null: all). The split's partials are the Runtime-owned scratch "attn_tree".
+    void attention_tree(gpu::Encoder*& enc, gpu::Buffer* q, gpu::Buffer* k, gpu::Buffer* v, gpu::Buffer* kd,
+                        gpu::Buffer* vd, gpu::Buffer* ctx_len, gpu::Buffer* n_nodes, gpu::Buffer* mask, gpu::Buffer* o,
+                        uint32_t batch, uint32_t n_draft, uint32_t heads, uint32_t kv_heads, uint32_t cap,
+                        uint32_t max_ctx, uint32_t dim = kHeadDim, const AttnOptions& opt = {});
+    // Appends each sequence's accepted drafts (path u32 [batch][n_draft] and n_path u32 [batch], null: all in order) to the
+    // cache; ctx_len grows by their number, in place, as do seen (tokens so far) and, on the new rows, w (0) and pos (their
+    // tokens), where given.
+    void cache_append(gpu::Encoder*& enc, gpu::Buffer* kd, gpu::Buffer* vd, gpu::Buffer* path, gpu::Buffer* n_path,
+                      gpu::Buffer* ctx_len, gpu::Buffer* seen, gpu::Buffer* w, gpu::Buffer* pos, gpu::Buffer* k,
+                      gpu::Buffer* v, uint32_t batch, uint32_t n_draft, uint32_t kv_heads, uint32_t cap,
+                      uint32_t dim = kHeadDim, mako_dtype in = MAKO_F16);
+    // Adds to w [batch][kv_heads][cap], times decay first, the attention weight that each cache row gets from the last n_q
+    // rows' queries, or those of a path: q [heads][batch * n_q][dim] and lse [heads][batch * n_q] of the attention's call
+    // (by_sequence: attention_decode's [batch][heads][n_q]). Scratch "cache_weights".
+    void cache_weights(gpu::Encoder*& enc, gpu::Buffer* q, gpu::Buffer* lse, gpu::Buffer* k, gpu::Buffer* ctx_len,
+                       gpu::Buffer* path, gpu::Buffer* n_path, gpu::Buffer* w, uint32_t batch, uint32_t n_q,
+                       uint32_t heads, uint32_t kv_heads, uint32_t cap, uint32_t max_ctx, float decay = 1.0f,
+                       bool by_sequence = false, uint32_t dim = kHeadDim, mako_dtype in = MAKO_F16);
+    // Evicts rows down to `budget` a (sequence, kv head): tokens below sinks and the last `recent` ones stay, then the rows
+    // of the largest w. k, v, w, pos and ctx_len in place. Scratch "cache_evict".
+    void cache_evict(gpu::Encoder*& enc, gpu::Buffer* k, gpu::Buffer* v, gpu::Buffer* w, gpu::Buffer* pos,
+                     gpu::Buffer* seen, gpu::Buffer* ctx_len, uint32_t batch, uint32_t kv_heads, uint32_t cap,
+                     uint32_t max_ctx, uint32_t budget, uint32_t recent, uint32_t sinks, uint32_t dim = kHeadDim,
+                     mako_dtype in = MAKO_F16);
 };
 
 }  // namespace mako::models
