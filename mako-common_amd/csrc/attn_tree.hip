@@ -48,7 +48,6 @@ struct TreeParams {
     uint32_t nc, ncb;   // columns (n_draft x group), column blocks
     uint32_t ways;      // tiles a step
     uint32_t n_ranges;  // 0: a segment a workgroup
-    uint32_t lead;      // units of a segment in front of its steps
     float scale_log2;
 };
 
@@ -67,14 +66,16 @@ __device__ __forceinline__ uint32_t steps_of(const TreeParams& p, uint32_t ctx, 
     return ((ctx + kTK - 1) / kTK + (nodes + kTK - 1) / kTK + p.ways - 1) / p.ways;
 }
 
-// The units of a segment of sequence i: its steps, and `lead` more in front of them for what a piece costs beside its
-// steps, so that ranges that meet two segments get fewer.
+// The units of a segment of sequence i: its steps, and kLead more in front of them for what a piece costs beside its
+// steps, so that ranges that meet two segments get fewer (256 lists of 4096 keys, heads of 128: 94 us with 0 of them, 90
+// with 3, 89.6 with 6, 90 with 10; 40 lists of 5000: 37.1, 34.0, 33.2, 33.8).
+constexpr uint32_t kLead = 6;
 struct SegUnits {
     const TreeParams& p;
     __device__ __forceinline__ uint32_t operator()(uint32_t i) const
     {
         const uint32_t steps = steps_of(p, ctx_of(p, i), nodes_of(p, i));
-        return steps ? steps + p.lead : 0u;
+        return steps ? steps + kLead : 0u;
     }
 };
 
@@ -212,11 +213,11 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
         if (at.x0 == at.x1)
             return;
         b = at.b;
-        len = at.len - p.lead;
+        len = at.len - kLead;
         kvh = (at.x0 - at.first) / at.len;
         const uint32_t u0 = (at.x0 - at.first) % at.len, u1 = min(at.len, u0 + (at.x1 - at.x0));
-        s0 = max(u0, p.lead) - p.lead;
-        s1 = max(u1, p.lead) - p.lead;
+        s0 = max(u0, kLead) - kLead;
+        s1 = max(u1, kLead) - kLead;
         left = at.x1 - at.x0 - (u1 - u0);
     } else {
         b = range / p.kv_heads, kvh = range % p.kv_heads, s0 = 0;
@@ -232,8 +233,8 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
             len = b < p.batch ? uniform(steps_of(p, ctx_of(p, b), nodes_of(p, b))) : 0u;
         } while (b < p.batch && len == 0);
         s0 = 0;
-        s1 = max(min(len + p.lead, left), p.lead) - p.lead;
-        left -= min(len + p.lead, left);
+        s1 = max(min(len + kLead, left), kLead) - kLead;
+        left -= min(len + kLead, left);
         return b < p.batch && s1 > 0;
     };
     if (p.n_ranges && s0 == s1 && !(left && next()))
@@ -574,19 +575,31 @@ uint32_t ways_of(uint32_t ng)
     return ng == 1 ? Shape<D, 1>::kKW : ng == 2 ? Shape<D, 2>::kKW : Shape<D, 4>::kKW;
 }
 
-constexpr uint32_t kDirectSteps = 5;
+// A segment a workgroup, and no partials or second launch, up to this many steps: 5, and more the more segments there are to
+// fill the CUs and the more columns a partial has. A workgroup takes its segment's steps one after the other, whatever the
+// others' contexts, so the limit also bounds the loss where one is max_ctx long and the rest an eighth of it.
+// us direct / split, heads of 128: 32 columns, 8 segments of 5 steps 12.8 / 13.3, of 6 14.2 / 13.7; 64 of 17 29 / 24; 128 of
+// 9 21 / 25; 256 of 13 38 / 44. 128 columns: 64 of 9 23 / 27, of 17 32 / 31; 128 of 17 35 / 41; 256 of 25 57 / 78. One long
+// among short ones, 128 columns: 128 of 17 33 / 33; 256 of 17 34 / 45, of 33 55 / 49.
+uint32_t direct_steps(uint64_t segs, uint32_t nc, uint32_t cus)
+{
+    return 5 + (uint32_t)std::min<uint64_t>(28, segs * std::min(3u, (nc + 31) / 32) * 8 / cus);
+}
 
 Plan plan_of(const mako_tree_args* a, uint32_t cus)
 {
     const uint32_t nc = a->n_draft * (a->heads / a->kv_heads);
     Plan pl{};
+    // Column groups: as many as there are columns for. The other side, us at 64 lists (8 lists) of 8192 keys, heads of 128:
+    // 64 columns in 2 groups 57 (23), in 1 and two column blocks 61 (20), in 4 68 (26); 96 columns in 4 71 (28), in 2 80
+    // (24); 128 columns in 4 77 (30), in 2 81 (25); 32 columns, 32 lists, in 1 group 32, in 2 35, in 4 40.
     pl.ng = nc <= 32 ? 1 : nc <= 64 ? 2 : 4;
     pl.ncb = (nc + 32 * pl.ng - 1) / (32 * pl.ng);
     pl.ways = a->dim == 64 ? ways_of<64>(pl.ng) : a->dim == 128 ? ways_of<128>(pl.ng) : ways_of<256>(pl.ng);
     const uint32_t tiles = (a->max_ctx + kTK - 1) / kTK + (a->n_draft + kTK - 1) / kTK;
     const uint32_t steps = (tiles + pl.ways - 1) / pl.ways;
-    if (steps > kDirectSteps) {
-        const uint64_t segs = (uint64_t)a->batch * a->kv_heads;
+    const uint64_t segs = (uint64_t)a->batch * a->kv_heads;
+    if (steps > direct_steps(segs, nc, cus)) {
         pl.n_ranges = (uint32_t)std::min<uint64_t>(std::max(1u, cus / pl.ncb), segs * steps);
         pl.pieces = pl.n_ranges + segs;
     }
@@ -630,9 +643,11 @@ void launch(const TreeParams& p, uint32_t ng, void* o, float* lse, hipStream_t s
         launch_split<T, TO, D, 4>(p, o, lse, s);
     if (!p.n_ranges)
         return;
-    // a wave an item where segments have few pieces (n_ranges of them over all, and a cut one more each)
+    // A wave an item where segments have few pieces (n_ranges of them over all, and a cut one more each). The call's us with
+    // a wave and with four, 16 drafts, heads of 128: 4 pieces 37.9, 43.1; 8 pieces 37.4, 38.9; 32 pieces 41.9, 41.5; 64
+    // drafts, heads of 256, 128 pieces: 60.6, 58.3.
     const uint32_t items = p.batch * p.n_draft * p.heads;
-    if (p.n_ranges / (p.batch * p.kv_heads) < 8)
+    if (p.n_ranges / (p.batch * p.kv_heads) < 16)
         hipLaunchKernelGGL((tree_merge<T, TO, D, 1>), dim3((items + 3) / 4), dim3(256), 0, s, p, static_cast<TO*>(o), lse);
     else
         hipLaunchKernelGGL((tree_merge<T, TO, D, 4>), dim3(items), dim3(256), 0, s, p, static_cast<TO*>(o), lse);
@@ -730,7 +745,7 @@ extern "C" int mako_attn_tree(const mako_tree_args* a, mako_dtype in, mako_dtype
                        reinterpret_cast<float*>(at(ob)), reinterpret_cast<uint32_t*>(at(ob + mb)),
                        reinterpret_cast<uint32_t*>(at(ob + mb + fb)),
                        a->batch, a->n_draft, a->q_pad, a->d_pad, a->heads, a->kv_heads, group, a->cap, a->max_ctx,
-                       a->width, a->n_draft * group, pl.ncb, pl.ways, pl.n_ranges, a->dim == 256 ? 6u : 3u, a->scale * kLog2e};
+                       a->width, a->n_draft * group, pl.ncb, pl.ways, pl.n_ranges, a->scale * kLog2e};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (in == MAKO_BF16 && out == MAKO_F32)
         launch_dim<__bf16, float>(p, a->dim, pl.ng, o, lse, s);
