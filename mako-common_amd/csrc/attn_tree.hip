@@ -249,26 +249,18 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                              tile_rsrc(static_cast<const T*>(p.kd) + draft, nodes * kRow),
                              tile_rsrc(static_cast<const T*>(p.vd) + draft, nodes * kRow)};
         // The tile of way kw in step s into its ring slot (past the segment's tiles: rows past the tree, zeros). Streaming
-        // loads where no other workgroup reads the keys.
+        // loads: 128 lists of 8192 keys of 128 take 88 us with them, 103 without (with column blocks, which read the keys
+        // again from the L2, the same either way).
         auto stage = [&](uint32_t s) __attribute__((always_inline)) {
             const uint32_t t = s * KW + kw, dst = lbase + (s % S::kDepth * KW + kw) * S::kSlot + 1024 * cg * kPieces;
             const uint32_t off = (t < tc ? t : t - tc) * kHalf;
             const u32x4 k = t < tc ? rs[0] : rs[2], v = t < tc ? rs[1] : rs[3];
-            if (NG < 4 || p.ncb == 1) {
-                #pragma unroll
-                for (int m = 0; m < kPieces; ++m)
-                    dma16_nt(dst + 1024 * m, kd[m] + off, k);
-                #pragma unroll
-                for (int m = 0; m < kPieces; ++m)
-                    dma16_nt(dst + kHalf + 1024 * m, vd[m] + off, v);
-            } else {
-                #pragma unroll
-                for (int m = 0; m < kPieces; ++m)
-                    dma16_at(dst + 1024 * m, kd[m] + off, 0, k);
-                #pragma unroll
-                for (int m = 0; m < kPieces; ++m)
-                    dma16_at(dst + kHalf + 1024 * m, vd[m] + off, 0, v);
-            }
+            #pragma unroll
+            for (int m = 0; m < kPieces; ++m)
+                dma16_nt(dst + 1024 * m, kd[m] + off, k);
+            #pragma unroll
+            for (int m = 0; m < kPieces; ++m)
+                dma16_nt(dst + kHalf + 1024 * m, vd[m] + off, v);
         };
         for (uint32_t s = s0; s < min(s1, s0 + S::kDepth - 1); ++s)
             stage(s);

@@ -2,7 +2,7 @@
 //
 // cache_append: one workgroup a sequence copies its path's rows, 16 bytes a thread at a time, for every kv head. One
 // workgroup reads ctx and seen and writes them after its barrier, so they can be updated in place. Bound by the latency of
-// a launch and a few dependent loads (ctx and the path, then the rows).
+// a launch and a few dependent loads (ctx and the path, then the rows): 2 us for one sequence of 8 kv heads, 3.5 for 32.
 //
 // Eviction, per list (sequence, kv head) of n > budget rows, in two launches:
 // * evict_select, one workgroup a list. A row's key is its weight as an integer in the same order (protected rows the
@@ -21,7 +21,7 @@
 namespace mako {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kThreads = 1024;  // of append_rows
 
 struct AppendParams {
     const void *kd, *vd;
@@ -117,7 +117,8 @@ __device__ __forceinline__ uint32_t scan_threads(uint32_t x, u32x4 (&s)[W / 4], 
 // A workgroup of TH threads; the keys of ROWS rows in LDS (registers would hold them too, but unrolled over them the code
 // outgrows the instruction cache, and each line of it runs once). Thread t has R consecutive rows, its first at t R, in
 // LDS rows of R + 1 words (R even: no bank conflicts). A longer list goes through in blocks of ROWS, read again in each
-// pass. Bound by one CU: about 40 VALU operations a row, and an LDS atomic a row for the first digit.
+// pass. Bound by one CU: about 40 VALU operations a row, and an LDS atomic a row for the first digit. 8 lists of 4096 rows
+// take 7 us, 8 of 32768 23 (clocks: loads 7.5k, first digit 12k, the others 5k each, ranks and lists 9k), 128 of 1024 to 32768 26.
 template <int TH, int ROWS>
 __global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
 {
@@ -318,6 +319,8 @@ __global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
 
 constexpr int kMoveRows = 16;  // rows of K and V a workgroup of evict_move
 
+// Bound by the copy. Streaming loads: a call that moves 4096 rows of 128 lists of 16384 takes 87 us with them, 102 without
+// (93 with streaming stores too); one that moves 152 rows of lists of 2200, 13.8 and 13.5.
 __global__ __launch_bounds__(256) void evict_move(const EvictParams p)
 {
     const uint32_t chunks = (p.most + kMoveRows - 1) / kMoveRows;
@@ -335,7 +338,7 @@ __global__ __launch_bounds__(256) void evict_move(const EvictParams p)
     for (uint32_t x = threadIdx.x; x < (i1 - i0) * cpr; x += 256) {
         const uint32_t i = i0 + x / cpr, c = x % cpr;
         const size_t to = (size_t)hole[i] * cpr + c, from = (size_t)src[count - 1 - i] * cpr + c;
-        const u32x4 kk = k[from], vv = v[from];
+        const u32x4 kk = __builtin_nontemporal_load(k + from), vv = __builtin_nontemporal_load(v + from);
         k[to] = kk;
         v[to] = vv;
     }
@@ -446,6 +449,8 @@ extern "C" int mako_cache_evict(const mako_evict_args* a, mako_dtype in, void* k
                         reinterpret_cast<uint32_t*>(ws + at), reinterpret_cast<uint32_t*>(ws + at + bytes), a->kv_heads,
                         a->dim, a->cap, a->max_ctx, a->budget, a->recent, a->sinks, most};
     hipStream_t s = static_cast<hipStream_t>(stream);
+    // The call's us with 512 threads for blocks of 4096 rows, and with 1024 for 32768: 8 lists of 1024 10.7, 13.0, of 4096
+    // 11.1, 13.4, of 6000 21, 14, of 16384 34, 20; 512 lists of 4096 39, 48, of 8192 87, 89, of 16384 162, 159.
     if (a->max_ctx <= 4096)
         hipLaunchKernelGGL((evict_select<512, 4096>), dim3((uint32_t)lists), dim3(512), 0, s, p);
     else

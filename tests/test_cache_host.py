@@ -1,9 +1,14 @@
-"""The cache operators' host side without a GPU: what they refuse, and with which message, before touching the device."""
+"""The cache operators' host side without a GPU: what they refuse, and with which message, before touching the device; and
+with a HIP runtime that runs nothing, their workspaces and launches."""
 import ctypes
+import re
 
 import pytest
 
-import mako_attn as M
+torch = pytest.importorskip("torch")
+
+import mako_attn as M  # noqa: E402
+from test_host_paths import events, hip, launches, tensor  # noqa: E402, F401
 
 FAKE = ctypes.c_void_p(0x10000)  # aligned, never dereferenced: every call below fails validation first
 ODD = ctypes.c_void_p(0x10008)
@@ -147,3 +152,110 @@ def test_evict_workspace_covers_the_rows_that_can_move():
     assert size() >= 6 * 4 + 2 * 6 * 1000 * 4
     assert size(max_ctx=1300) >= 6 * 4 + 2 * 6 * 300 * 4
     assert size(max_ctx=900) < 6 * 4 * 900
+
+
+# ---- with a HIP runtime that records launches and runs nothing ----
+
+
+def space(nbytes, addr=0x200000):
+    t = tensor(None, addr)
+    t.numel, t.element_size = lambda: nbytes, lambda: 1
+    t.nbytes = nbytes
+    return t
+
+
+X, F, I = tensor(torch.bfloat16), tensor(torch.float32), tensor(torch.int32)
+
+
+def tree_call(a, ws):
+    M.attn_tree(a, X, X, X, X, X, I, X, ws, lse=F, stream=0x71000)
+
+
+def weights_call(a, ws):
+    M.cache_weights(a, X, F, X, I, F, ws, w=F, stream=0x71000)
+
+
+def evict_call(a, ws):
+    M.cache_evict(a, X, X, F, I, F, I, I, ws, stream=0x71000)
+
+
+CALLS = {
+    "tree": (tree_call, M.attn_tree_workspace,
+             M.tree_args(batch=3, n_draft=9, heads=32, kv_heads=8, dim=128, cap=9000, max_ctx=9000),
+             ["tree_split", "tree_merge"]),
+    "weights": (weights_call, M.cache_weights_workspace,
+                M.weights_args(batch=3, n_q=100, heads=32, kv_heads=8, dim=64, cap=9000, max_ctx=9000),
+                ["weights_many", "weights_join"]),
+    "evict": (evict_call, M.cache_evict_workspace,
+              M.evict_args(batch=3, kv_heads=8, dim=128, cap=9000, max_ctx=9000, budget=5000),
+              ["evict_select", "evict_move"]),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_workspaces(hip, name):  # noqa: F811
+    """The bytes that the query names are enough and all are needed; the library allocates nothing of its own."""
+    call, query, a, kernels = CALLS[name]
+    need = query(a)
+    assert need > 0
+    for ws in (None, space(need - 1), space(need, 0x200008), space(0)):
+        with pytest.raises(M.MakoError, match="workspace"):
+            call(a, ws)
+    assert launches(hip) == []
+    call(a, space(need))
+    got = launches(hip)
+    assert len(got) == len(kernels) and all(k in x for k, x in zip(kernels, got)), got
+    assert events(hip, "alloc", "free") == []
+
+
+def test_calls_that_need_no_workspace(hip):  # noqa: F811
+    """Short contexts' trees and few rows' weights take one launch, and null for a workspace."""
+    a = M.tree_args(batch=2, n_draft=8, heads=32, kv_heads=8, dim=128, cap=9000, max_ctx=200)
+    assert M.attn_tree_workspace(a) == 0
+    tree_call(a, None)
+    w = M.weights_args(batch=2, n_q=8, heads=32, kv_heads=8, dim=128, cap=9000, max_ctx=9000)
+    assert M.cache_weights_workspace(w) == 0
+    weights_call(w, None)
+    M.cache_append(M.append_args(batch=2, n_draft=8, kv_heads=8, dim=128, cap=9000), X, X, X, X, I, I, stream=0x71000)
+    got = launches(hip)
+    assert [k in x for k, x in zip(("tree_split", "weights_few", "append_rows"), got)] == [True] * 3 and len(got) == 3
+    assert events(hip, "alloc", "free") == []
+
+
+def test_empty_calls_launch_nothing(hip):  # noqa: F811
+    tree = dict(batch=2, n_draft=8, heads=32, kv_heads=8, dim=128, cap=9000, max_ctx=9000)
+    for kw in (dict(batch=0), dict(n_draft=0)):
+        a = M.tree_args(**dict(tree, **kw))
+        assert M.attn_tree_workspace(a) == 0
+        tree_call(a, None)
+    wts = dict(batch=2, n_q=100, heads=32, kv_heads=8, dim=128, cap=9000, max_ctx=9000)
+    for kw in (dict(batch=0), dict(max_ctx=0)):
+        a = M.weights_args(**dict(wts, **kw))
+        assert M.cache_weights_workspace(a) == 0
+        weights_call(a, None)
+    M.cache_append(M.append_args(batch=0, n_draft=8, kv_heads=8, dim=128, cap=9000), X, X, X, X, I, I, stream=0x71000)
+    a = M.evict_args(batch=0, kv_heads=8, dim=128, cap=9000, max_ctx=9000, budget=5000)
+    evict_call(a, None)
+    assert launches(hip) == []
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n_draft,heads,kv", [(1, 1, 1), (8, 32, 8), (16, 32, 8), (64, 16, 1), (64, 64, 1), (33, 96, 32)])
+def test_tree_split_covers_its_columns(hip, dim, n_draft, heads, kv):  # noqa: F811
+    """Every (range or segment, column block) has a workgroup: blocks of 32, 64 or 128 columns, ranges for at most the CUs."""
+    for batch in (1, 5, 200):
+        for ctx in (0, 1, 100, 5000, 70000):
+            a = M.tree_args(batch=batch, n_draft=n_draft, heads=heads, kv_heads=kv, dim=dim, cap=70000, max_ctx=ctx)
+            hip.fake_clear()
+            tree_call(a, space(M.attn_tree_workspace(a)))
+            ev = events(hip, "launch")
+            nc = n_draft * heads // kv
+            ng = 1 if nc <= 32 else 2 if nc <= 64 else 4
+            ncb = -(-nc // (32 * ng))
+            grid = int(re.match(r"\d+", ev[0][2]).group())
+            if len(ev) == 1:
+                assert grid >= batch * kv * ncb
+            else:
+                assert ncb <= grid <= max(256 + 8 * ncb, 8 * ncb)
+                items = batch * n_draft * heads
+                assert int(re.match(r"\d+", ev[1][2]).group()) in (items, -(-items // 4))
