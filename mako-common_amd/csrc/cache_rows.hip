@@ -6,11 +6,12 @@
 //
 // Eviction, per list (sequence, kv head) of n > budget rows, in two launches:
 // * evict_select, one workgroup a list. A row's key is its weight as an integer in the same order (protected rows the
-//   largest key, NaN that of -inf, -0 that of 0), held in LDS. The budget-th largest key T comes from histograms of
-//   11, 11 and 10 bits, the highest first; rows above T stay, of those at T the first `need` do. A sum over the threads of
-//   their rows' counts gives every row its rank among the kept, and from ranks follow the rows' places: a row j below the
-//   budget that is given up is hole j - (kept before j), a kept row past the budget source (kept before it) - (kept below
-//   the budget). The lists of holes and sources go into the workspace.
+//   largest key, NaN that of -inf, -0 that of 0), held in LDS. The budget-th largest key T comes from histograms of 11 bits
+//   of the unprotected keys' range, the highest first, until the rows of a digit all stay (two digits mostly: weights share
+//   their leading bits, a digit of the range spreads them); rows above T stay, of those at T the first `need` do. A sum
+//   over the threads of their rows' counts gives every row its rank among the kept, and from ranks follow the rows' places:
+//   a row j below the budget that is given up is hole j - (kept before j), a kept row past the budget source (kept before
+//   it) - (kept below the budget). The lists of holes and sources go into the workspace.
 // * evict_move copies source i over hole i, K, V, weight and position. Sources lie past the budget and holes below it,
 //   so no row is read and written.
 #include <algorithm>
@@ -83,14 +84,23 @@ struct EvictParams {
 // for protected rows.
 __device__ __forceinline__ uint32_t order_of(float x)
 {
-    if (x != x)
-        x = -INFINITY;
-    const uint32_t u = as_u32(x + 0.0f);  // -0 + 0 = 0
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = as_u32(fmaxf(x, -INFINITY) + 0.0f);  // (NaN gives the other; -0 + 0 = 0)
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
-constexpr int kDigits = 2048;  // of 11, 11 and 10 bits
-constexpr int kCopies = 2;     // counters a digit, by lane
+constexpr int kDigitBits = 11, kDigits = 1 << kDigitBits;
+
+// The largest x of a wave's lanes, in lane 63.
+__device__ __forceinline__ uint32_t max_lanes(uint32_t x)
+{
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x111, 0xf, 0xf, false));  // row_shr 1
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x112, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x114, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x118, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x142, 0xa, 0xf, false));  // lane 15 of rows 0 and 2 to rows 1 and 3
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x143, 0xc, 0xf, false));  // lane 31 to rows 2 and 3
+    return x;
+}
 
 // The inclusive sum of x over the workgroup's threads up to this one; total: over all of them (s: a word a wave; two barriers).
 template <int W>
@@ -116,17 +126,17 @@ __device__ __forceinline__ uint32_t scan_threads(uint32_t x, u32x4 (&s)[W / 4], 
 
 // A workgroup of TH threads; the keys of ROWS rows in LDS (registers would hold them too, but unrolled over them the code
 // outgrows the instruction cache, and each line of it runs once). Thread t has R consecutive rows, its first at t R, in
-// LDS rows of R + 1 words (R even: no bank conflicts). A longer list goes through in blocks of ROWS, read again in each
-// pass. Bound by one CU: about 40 VALU operations a row, and an LDS atomic a row for the first digit. 8 lists of 4096 rows
-// take 7 us, 8 of 32768 23 (clocks: loads 7.5k, first digit 12k, the others 5k each, ranks and lists 9k), 128 of 1024 to 32768 26.
+// LDS rows of R + 4 words (R a power of two from 8 on: 16-byte reads without bank conflicts). A longer list goes through in
+// blocks of ROWS, read again in each pass. Bound by the passes of one CU: 8 lists of 32768 rows take 20 us, of them loads 5,
+// two digits 6, ranks 1.5, lists 3.5; 128 lists of 2112 rows 9, of them 5 after the launch and the first loads.
 template <int TH, int ROWS>
 __global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
 {
     constexpr int W = TH / 64, kPer = kDigits / TH;  // digits a thread sums
     static_assert(ROWS <= 32768 && ROWS / TH % 8 == 0, "counts of a block fit 16 bits, rows go eight at a time");
-    __shared__ uint32_t keys[ROWS + TH];
-    __shared__ u32x4 hist[kDigits * kCopies / 4], s_scan[W / 4];
-    __shared__ uint32_t s_digit, s_above;
+    __shared__ u32x4 keys[(ROWS + 4 * TH) / 4];
+    __shared__ u32x4 hist[kDigits / 4], s_scan[W / 4], s_lo[W / 4], s_hi[W / 4];
+    __shared__ uint32_t s_digit, s_above, s_count;
     const uint32_t list = blockIdx.x, b = list / p.kv_heads, tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
     const uint32_t n = min(p.ctx[b], p.max_ctx), seen = p.seen ? p.seen[b] : n, budget = p.budget;
     const size_t base = (size_t)list * p.cap;
@@ -146,114 +156,161 @@ __global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
     const uint32_t late = seen > p.recent ? seen - p.recent : 0u;  // positions from here on, and below sinks, are protected
     const uint32_t blocks = (n + ROWS - 1) / ROWS;
     const uint32_t lg = blocks > 1 ? 31 - __builtin_clz(ROWS / TH) : max(3, 32 - __builtin_clz((n - 1) / TH | 1)), R = 1u << lg;
-    // Block blk's keys (rows past the list: key 0, below every row's); `first`: with the copies below the budget (the rows
-    // that are given up get theirs from evict_move).
-    auto load = [&](uint32_t blk, bool first) __attribute__((always_inline)) {
-        #pragma unroll 1
-        for (uint32_t e = 0; e < R; e += 8) {
-            const uint32_t x0 = e * TH + tid, j0 = blk * ROWS + x0;
-            const uint32_t lo = blk * ROWS + e * TH, hi = lo + 8 * TH;  // the rows of all threads
-            float w[8];
-            uint32_t at[8];
-            #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                at[i] = min(j0 + i * TH, n - 1);
-                w[i] = *reinterpret_cast<const float*>(w_in + 4 * at[i]);
-            }
-            if (pos_in)
+    // The unprotected rows' smallest and largest key of what this thread has loaded; and how many rows are protected.
+    uint32_t low = 0xffffffffu, high = 0, safe = 0;
+    const uint32_t lds_step = TH + 4 * (TH >> lg);  // words between a thread's places: rows TH apart
+    // Block blk's keys (rows past the list: key 0, below every row's), eight rows a thread at a time, loaded ahead; `copy`:
+    // with the copies below the budget (the rows that are given up get theirs from evict_move); `count`: with the above.
+    auto load = [&](uint32_t blk, bool copy, bool count) __attribute__((always_inline)) {
+        float next_w[8];
+        uint32_t next_pos[8];
+        auto fetch = [&](uint32_t e) __attribute__((always_inline)) {
+            const uint32_t f = blk * ROWS + e * TH;
+            if (f + 8 * TH <= n) {
                 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i)
-                    at[i] = *reinterpret_cast<const uint32_t*>(pos_in + 4 * at[i]);
-            uint32_t key[8];
+                    next_w[i] = *reinterpret_cast<const float*>(w_in + 4 * (f + i * TH) + 4 * tid);
+                if (pos_in)
+                    #pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        next_pos[i] = *reinterpret_cast<const uint32_t*>(pos_in + 4 * (f + i * TH) + 4 * tid);
+            } else {
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i)
+                    next_w[i] = *reinterpret_cast<const float*>(w_in + 4 * min(f + i * TH + tid, n - 1));
+                if (pos_in)
+                    #pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        next_pos[i] = *reinterpret_cast<const uint32_t*>(pos_in + 4 * min(f + i * TH + tid, n - 1));
+            }
+        };
+        fetch(0);
+        uint32_t* to = reinterpret_cast<uint32_t*>(keys) + tid + 4 * (tid >> lg);
+        #pragma unroll 1
+        for (uint32_t e = 0; e < R; e += 8) {
+            const uint32_t f = blk * ROWS + e * TH, end = f + 8 * TH;  // the rows of all threads
+            float w[8];
+            uint32_t at[8], key[8];
+            #pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                w[i] = next_w[i];
+                at[i] = pos_in ? next_pos[i] : f + i * TH + tid;
+            }
+            if (e + 8 < R)
+                fetch(e + 8);
             #pragma unroll
             for (uint32_t i = 0; i < 8; ++i)
                 key[i] = order_of(w[i]);
-            if (pos_in || lo < p.sinks || hi > late)
+            if (pos_in || f < p.sinks || end > late || end > n) {
+                #pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const bool in = f + i * TH + tid < n, kept = at[i] < p.sinks || at[i] >= late;
+                    if (count) {
+                        low = in && !kept ? min(low, key[i]) : low;
+                        high = in && !kept ? max(high, key[i]) : high;
+                        safe += in && kept;
+                    }
+                    key[i] = !in ? 0u : kept ? 0xffffffffu : key[i];
+                }
+            } else if (count) {
                 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i)
-                    key[i] = at[i] < p.sinks || at[i] >= late ? 0xffffffffu : key[i];
-            if (hi > n)
-                #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    key[i] = j0 + i * TH < n ? key[i] : 0u;
+                    low = min(low, key[i]), high = max(high, key[i]);
+            }
             #pragma unroll
             for (uint32_t i = 0; i < 8; ++i)
-                keys[x0 + i * TH + ((x0 + i * TH) >> lg)] = key[i];
-            if (first && copies && lo < budget)
+                to[(e + i) * lds_step] = key[i];
+            if (copy && copies && f < budget)
                 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    if (j0 + i * TH < budget) {
-                        p.w_out[base + j0 + i * TH] = w[i];
-                        p.pos_out[base + j0 + i * TH] = at[i];
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const uint32_t j = f + i * TH + tid;
+                    if (j < budget) {
+                        p.w_out[base + j] = w[i];
+                        p.pos_out[base + j] = at[i];
                     }
+                }
         }
     };
-    load(0, true);
-    const uint32_t mine = tid * (R + 1);  // this thread's keys
-    // The budget-th largest key, a digit at a time: `need` rows are still to be found among those with the prefix. Protected
-    // rows are counted apart (they would all meet in one counter): where they alone reach the budget, theirs is the key.
-    uint32_t prefix = 0, known = 0, need = budget, total, safe = 0;
-    #pragma unroll 1
-    for (uint32_t shift = 21, d = 0; d < 3; ++d) {
-        const uint32_t mask = d < 2 ? 2047u : 1023u;
-        for (uint32_t i = tid; i < kDigits * kCopies / 4; i += TH)
-            hist[i] = u32x4{};
-        for (uint32_t blk = 0; blk < blocks; ++blk) {
-            if (blocks > 1) {
+    load(0, true, true);
+    for (uint32_t blk = 1; blk < blocks; ++blk)
+        load(blk, true, true);  // (a thread writes the same places of LDS each time)
+    low = max_lanes(~low);
+    high = max_lanes(high);
+    if (lane == 63) {
+        reinterpret_cast<uint32_t*>(s_lo)[wv] = low;
+        reinterpret_cast<uint32_t*>(s_hi)[wv] = high;
+    }
+    uint32_t total;
+    scan_threads<W>(safe, s_scan, lane, wv, total);
+    low = high = 0;
+    #pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+        const u32x4 x = s_lo[i], y = s_hi[i];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j)
+            low = max(low, x[j]), high = max(high, y[j]);
+    }
+    // The budget-th largest key T, a digit of the unprotected keys' range at a time: it is among [lo, lo + span], and `need`
+    // of the rows there stay. Where the protected rows alone reach the budget, theirs is the key.
+    uint32_t lo = ~uniform(low), span = uniform(high) - lo, need = budget;
+    const u32x4* mine = keys + tid * (R / 4 + 1);  // this thread's keys
+    uint32_t T = 0xffffffffu;
+    if (uniform(total) < budget) {
+        need -= uniform(total);
+        #pragma unroll 1
+        for (;;) {
+            T = lo;
+            if (span == 0)
+                break;
+            const uint32_t bits = 32 - __builtin_clz(span), shift = max(bits, (uint32_t)kDigitBits) - kDigitBits;
+            for (uint32_t i = tid; i < kDigits / 4; i += TH)
+                hist[i] = u32x4{};
+            for (uint32_t blk = 0; blk < blocks; ++blk) {
+                if (blocks > 1) {
+                    __syncthreads();
+                    load(blk, false, false);
+                }
                 __syncthreads();
-                load(blk, blk > 0 && d == 0);
+                #pragma unroll 1
+                for (uint32_t e = 0; e < R / 4; e += 2) {
+                    const u32x4 key[2] = {mine[e], mine[e + 1]};
+                    #pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        const uint32_t x = key[i / 4][i % 4] - lo;  // (past the span: key 0 and protected rows too)
+                        if (x <= span)
+                            atomicAdd(reinterpret_cast<uint32_t*>(hist) + (x >> shift), 1u);
+                    }
+                }
             }
             __syncthreads();
-            #pragma unroll 1
-            for (uint32_t e = 0; e < R; e += 8) {
-                uint32_t key[8];
-                #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    key[i] = keys[mine + e + i];
-                if (d == 0)
-                    #pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i)
-                        safe += key[i] == 0xffffffffu;
-                #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    if ((key[i] & known) == prefix && key[i] + 1 > 1)  // (not 0, not a protected row's)
-                        atomicAdd(reinterpret_cast<uint32_t*>(hist) + (key[i] >> shift & mask) * kCopies +
-                                      (lane & (kCopies - 1)), 1u);
+            // Thread t: kPer digits from the largest down.
+            uint32_t c[kPer], sum = 0;
+            #pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                c[i] = reinterpret_cast<const uint32_t*>(hist)[kDigits - 1 - (kPer * tid + i)];
+                sum += c[i];
             }
-        }
-        __syncthreads();
-        if (d == 0) {
-            scan_threads<W>(safe, s_scan, lane, wv, total);
-            if (total >= budget) {
-                prefix = 0xffffffffu;
+            uint32_t above = scan_threads<W>(sum, s_scan, lane, wv, total) - sum;
+            #pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (above < need && above + c[i] >= need) {
+                    s_digit = kDigits - 1 - (kPer * tid + i);
+                    s_above = above;
+                    s_count = c[i];
+                }
+                above += c[i];
+            }
+            __syncthreads();
+            lo += uniform(s_digit) << shift;
+            span = (1u << shift) - 1;
+            need -= uniform(s_above);
+            if (uniform(s_count) == need) {  // all of the digit's rows stay, those below do not
+                T = lo - 1;
+                need = 0;
                 break;
             }
-            need -= total;
         }
-        // Thread t: kPer digits from the largest down.
-        uint32_t c[kPer], sum = 0;
-        #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const u32x2 x = reinterpret_cast<const u32x2*>(hist)[kDigits - 1 - (kPer * tid + i)];
-            c[i] = x[0] + x[1];
-            sum += c[i];
-        }
-        uint32_t above = scan_threads<W>(sum, s_scan, lane, wv, total) - sum;
-        #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (above < need && above + c[i] >= need) {
-                s_digit = kDigits - 1 - (kPer * tid + i);
-                s_above = above;
-            }
-            above += c[i];
-        }
-        __syncthreads();
-        prefix |= uniform(s_digit) << shift;
-        known |= mask << shift;
-        need -= uniform(s_above);
-        shift -= d == 0 ? 11 : 10;
     }
-    const uint32_t T = uniform(prefix);
     // The kept rows before each, in row order: of the blocks before, of the threads before (the counts above T in the low
     // half, at T in the high), and the thread's own.
     uint32_t* hole = p.hole + (size_t)list * p.most;
@@ -262,54 +319,55 @@ __global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
     for (uint32_t blk = 0; blk < blocks; ++blk) {
         if (blocks > 1) {
             __syncthreads();
-            load(blk, false);
+            load(blk, false, false);
             __syncthreads();
         }
         uint32_t c = 0;
         #pragma unroll 1
-        for (uint32_t e = 0; e < R; e += 8)
+        for (uint32_t e = 0; e < R / 4; e += 2) {
+            const u32x4 key[2] = {mine[e], mine[e + 1]};
             #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
-                const uint32_t key = keys[mine + e + i];
-                c += key > T ? 1u : key == T ? 0x10000u : 0u;
+                c += key[i / 4][i % 4] > T;
+                c += key[i / 4][i % 4] == T ? 0x10000u : 0u;
             }
+        }
         const uint32_t before = scan_threads<W>(c, s_scan, lane, wv, total) - c;
-        uint32_t gt = gt0 + (before & 0xffffu), eq = eq0 + (before >> 16);
-        uint32_t x = blk * ROWS + tid * R;
-        if (blk * ROWS + wv * 64 * R > budget && !__any(c >> 16)) {
-            // Sources alone, none of them at T.
-            uint32_t at = budget - 1 - gt - min(eq, need);
+        uint32_t* bases = reinterpret_cast<uint32_t*>(hist);  // the threads' counts, for whoever takes their rows
+        bases[tid] = before;
+        __syncthreads();
+        // Up to the budget, where rows may be holes, and wherever ties at T count, the waves take 64 rows at a time (a lane a
+        // row); behind, a row that stays is a source, and its thread lists it.
+        const uint32_t first = blk * ROWS, per_wave = 64 * R;
+        uint32_t by_lane = first > budget ? 0u : (budget - first) / per_wave * per_wave + per_wave;
+        if (need)
+            by_lane = ROWS;
+        for (uint32_t x0 = 64 * wv; x0 < min(by_lane, n - first); x0 += TH) {
+            const uint32_t x = first + x0 + lane, k = reinterpret_cast<const uint32_t*>(keys)[x0 + lane + 4 * ((x0 + lane) >> lg)];
+            const uint64_t more = __ballot(k > T), tie = __ballot(k == T);
+            const uint32_t counts = bases[x0 >> lg];
+            const uint32_t gt = __builtin_amdgcn_mbcnt_hi((uint32_t)(more >> 32),
+                                                          __builtin_amdgcn_mbcnt_lo((uint32_t)more, gt0 + (counts & 0xffffu)));
+            const uint32_t eq = __builtin_amdgcn_mbcnt_hi((uint32_t)(tie >> 32),
+                                                          __builtin_amdgcn_mbcnt_lo((uint32_t)tie, eq0 + (counts >> 16)));
+            const uint32_t kept_before = gt + min(eq, need);
+            const bool kept = k > T || (k == T && eq < need);
+            if (x == budget)
+                p.count[list] = budget - kept_before;
+            if (x < budget && !kept)
+                hole[x - kept_before] = x;
+            if (x >= budget && kept)
+                src[budget - 1 - kept_before] = x;  // from the end: the first source comes last
+        }
+        if (wv * per_wave >= by_lane) {
+            uint32_t at = budget - 1 - gt0 - (before & 0xffffu);  // (need is 0)
             #pragma unroll 1
-            for (uint32_t e = 0; e < R; e += 8) {
-                uint32_t key[8];
+            for (uint32_t e = 0; e < R / 4; e += 2) {
+                const u32x4 key[2] = {mine[e], mine[e + 1]};
                 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i)
-                    key[i] = keys[mine + e + i];
-                #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    if (key[i] > T)
-                        src[at--] = x + e + i;
-            }
-        } else {
-            #pragma unroll 1
-            for (uint32_t e = 0; e < R; e += 8) {
-                uint32_t key[8];
-                #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    key[i] = keys[mine + e + i];
-                #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i, ++x) {
-                    const uint32_t kept_before = gt + min(eq, need);
-                    const bool kept = key[i] > T || (key[i] == T && eq < need);
-                    if (x == budget)
-                        p.count[list] = budget - kept_before;
-                    if (x < budget && !kept)
-                        hole[x - kept_before] = x;
-                    if (x >= budget && kept)
-                        src[budget - 1 - kept_before] = x;  // from the end: the first source comes last
-                    gt += key[i] > T;
-                    eq += key[i] == T;
-                }
+                    if (key[i / 4][i % 4] > T)
+                        src[at--] = first + tid * R + 4 * e + i;
             }
         }
         gt0 += total & 0xffffu;
