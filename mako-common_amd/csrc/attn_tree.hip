@@ -167,6 +167,8 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
     using S = Shape<D, NG>;
     using E = Elem<T>;
     using V8 = typename E::vec8;
+    // One wave a SIMD: nothing else hides the wave's LDS reads, and its registers hold K's operands beside V's.
+    constexpr bool kAhead = D == 256;
     constexpr bool kSplitP = __is_same(T, __bf16) || __is_same(TO, float);  // P as the sum of two values of T
     constexpr int KW = S::kKW, ND = D / 32, NK = D / 16, W = S::kWaves;
     constexpr int kRow = 2 * D, kHalf = kTK * kRow, kPieces = kHalf / 1024 / NG;  // 1 KiB pieces of K (of V) a wave
@@ -248,21 +250,35 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                              tile_rsrc(static_cast<const T*>(p.v) + cache, ctx * kRow),
                              tile_rsrc(static_cast<const T*>(p.kd) + draft, nodes * kRow),
                              tile_rsrc(static_cast<const T*>(p.vd) + draft, nodes * kRow)};
-        // The tile of way kw in step s into its ring slot (past the segment's tiles: rows past the tree, zeros). Streaming
+        // Piece i of the tile of way kw in step s into its ring slot (past the segment's tiles: rows past the tree, zeros; past
+        // the range's steps: zeros, without a read). Streaming
         // loads: 128 lists of 8192 keys of 128 take 88 us with them, 103 without (with column blocks, which read the keys
         // again from the L2, the same either way).
-        auto stage = [&](uint32_t s) __attribute__((always_inline)) {
-            const uint32_t t = s * KW + kw, dst = lbase + (s % S::kDepth * KW + kw) * S::kSlot + 1024 * cg * kPieces;
-            const uint32_t off = (t < tc ? t : t - tc) * kHalf;
-            const u32x4 k = t < tc ? rs[0] : rs[2], v = t < tc ? rs[1] : rs[3];
-            #pragma unroll
-            for (int m = 0; m < kPieces; ++m)
-                dma16_nt(dst + 1024 * m, kd[m] + off, k);
-            #pragma unroll
-            for (int m = 0; m < kPieces; ++m)
-                dma16_nt(dst + kHalf + 1024 * m, vd[m] + off, v);
+        struct Slot {
+            uint32_t dst, off;
+            u32x4 k, v;
         };
-        for (uint32_t s = s0; s < min(s1, s0 + S::kDepth - 1); ++s)
+        auto slot_for = [&](uint32_t s) __attribute__((always_inline)) {
+            const uint32_t t = s * KW + kw;
+            Slot x{lbase + (s % S::kDepth * KW + kw) * S::kSlot + 1024 * cg * kPieces, (t < tc ? t : t - tc) * kHalf,
+                   t < tc ? rs[0] : rs[2], t < tc ? rs[1] : rs[3]};
+            if (kAhead && s >= s1)
+                x.k[2] = x.v[2] = 0;
+            return x;
+        };
+        auto stage_piece = [&](const Slot& x, int m) __attribute__((always_inline)) {
+            if (m < kPieces)
+                dma16_nt(x.dst + 1024 * m, kd[m] + x.off, x.k);
+            else
+                dma16_nt(x.dst + kHalf + 1024 * (m - kPieces), vd[m - kPieces] + x.off, x.v);
+        };
+        auto stage = [&](uint32_t s) __attribute__((always_inline)) {
+            const Slot x = slot_for(s);
+            #pragma unroll
+            for (int m = 0; m < 2 * kPieces; ++m)
+                stage_piece(x, m);
+        };
+        for (uint32_t s = s0; s < (kAhead ? s0 + S::kDepth - 1 : min(s1, s0 + S::kDepth - 1)); ++s)
             stage(s);
         // The lane's column: row r, head h; its mask, cut to the tree; Q, beside the first tiles' loads.
         const uint32_t col = 32 * (cb * NG + cg) + c32, r = col / p.group, h = kvh * p.group + col % p.group;
@@ -289,37 +305,61 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
         for (int kk = 0; kk < NK; ++kk)
             settle(qreg[kk]);
         // Step s has landed; every wave is done with step s - 1, whose slots take step s + DEPTH - 1.
-        auto arrive = [&](uint32_t s) __attribute__((always_inline)) {
-            if (s + S::kDepth - 1 <= s1)
+        auto landed = [&](uint32_t s) __attribute__((always_inline)) {
+            if (kAhead || s + S::kDepth - 1 <= s1)
                 asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::kDepth - 2) * 2 * kPieces) : "memory");
             else
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             if (NG > 1)
                 asm volatile("s_barrier" ::: "memory");
-            if (s + S::kDepth - 1 < s1)
+        };
+        auto arrive = [&](uint32_t s) __attribute__((always_inline)) {
+            landed(s);
+            if (kAhead || s + S::kDepth - 1 < s1)
                 stage(s + S::kDepth - 1);
+        };
+        // kAhead: K's operands are read a tile ahead, beside the products of the one before.
+        V8 kf[NK];
+        auto read_k = [&](uint32_t s) __attribute__((always_inline)) {
+            const unsigned char* tile = lds + (s % S::kDepth * KW + kw) * S::kSlot;
+            #pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+                kf[kk] = *reinterpret_cast<const V8*>(tile + (ka ^ (32 * kk)));
         };
         // The wave's tile of step s; CUT: one that not every column sees all of.
         auto tile_step = [&](auto cut, uint32_t s) __attribute__((always_inline)) {
             constexpr bool CUT = decltype(cut)::value;
             const uint32_t t = s * KW + kw;
             unsigned char* tile = lds + (s % S::kDepth * KW + kw) * S::kSlot;
+            // V^T's operands come while the scores (kAhead) or the exponentials are made.
+            V8 vf[2][ND];
+            auto read_v = [&]() __attribute__((always_inline)) {
+                if (CUT && t >= tc)
+                    odd |= finite_only<T, kHalf>(tile + kHalf, lane);
+                #pragma unroll
+                for (int a = 0; a < 2; ++a)
+                    #pragma unroll
+                    for (int db = 0; db < ND; ++db) {
+                        const unsigned char* at = tile + va[db % NV] + db / NV * 256 + 16 * a * kRow;
+                        const s16x4 v0 = tr_read(at), v1 = tr_read(at + 4 * kRow);
+                        vf[a][db] = __builtin_bit_cast(V8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    }
+            };
+            if (kAhead) {
+                #pragma unroll
+                for (int kk = 0; kk < NK; ++kk)
+                    settle(kf[kk]);
+                read_v();
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                read_k(s);
+            }
             f32x16 x = f32x16{};
             #pragma unroll
             for (int kk = 0; kk < NK; ++kk)
-                x = E::mfma32(*reinterpret_cast<const V8*>(tile + (ka ^ (32 * kk))), qreg[kk], x);
-            if (CUT && t >= tc)
-                odd |= finite_only<T, kHalf>(tile + kHalf, lane);
-            // V^T's operands come while the exponentials are made.
-            V8 vf[2][ND];
-            #pragma unroll
-            for (int a = 0; a < 2; ++a)
-                #pragma unroll
-                for (int db = 0; db < ND; ++db) {
-                    const unsigned char* at = tile + va[db % NV] + db / NV * 256 + 16 * a * kRow;
-                    const s16x4 v0 = tr_read(at), v1 = tr_read(at + 4 * kRow);
-                    vf[a][db] = __builtin_bit_cast(V8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-                }
+                x = E::mfma32(kf[kk], qreg[kk], x);
+            if (!kAhead)
+                read_v();
             __builtin_amdgcn_sched_barrier(0);
             // Register i holds key 16 (i / 8) + 8 g + i % 8 of the tile.
             #pragma unroll
@@ -371,41 +411,69 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                 l += (x[8 * a] + x[8 * a + 1]) + (x[8 * a + 2] + x[8 * a + 3]) +
                      ((x[8 * a + 4] + x[8 * a + 5]) + (x[8 * a + 6] + x[8 * a + 7]));
             };
-            auto products = [&](int a) __attribute__((always_inline)) {
-                #pragma unroll
-                for (int db = 0; db < ND; ++db)
-                    acc[db] = E::mfma32(vf[a][db], __builtin_bit_cast(V8, hi[a]), acc[db]);
-                if (kSplitP)
-                    #pragma unroll
-                    for (int db = 0; db < ND; ++db)
-                        acc[db] = E::mfma32(vf[a][db], __builtin_bit_cast(V8, lo[a]), acc[db]);
+            auto product = [&](int a, int i) __attribute__((always_inline)) {
+                acc[i % ND] = E::mfma32(vf[a][i % ND], __builtin_bit_cast(V8, i < ND ? hi[a] : lo[a]), acc[i % ND]);
             };
+            constexpr int kMf = ND * (kSplitP ? 2 : 1);  // products of a half
             half(0);
             __builtin_amdgcn_sched_barrier(0);
-            products(0);
+            if (kAhead) {
+                landed(s + 1);
+                read_k(s + 1);
+            }
+            #pragma unroll
+            for (int i = 0; i < kMf; ++i)
+                product(0, i);
             half(1);
-            constexpr int kMf = ND * (kSplitP ? 2 : 1);  // products of a half
             #pragma unroll
             for (int i = 0; i < kMf; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (kAhead)
+                    __builtin_amdgcn_sched_group_barrier(0x100, NK / kMf, 0);
                 __builtin_amdgcn_sched_group_barrier(0x002, (kSplitP ? 40 : 20) / kMf + 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x400, 8 / kMf + 1, 0);
             }
-            products(1);
+            if (kAhead) {
+                // the loads of a step to come between the products: issued together they would hold the wave up
+                const Slot next = slot_for(s + S::kDepth);
+                #pragma unroll
+                for (int i = 0; i < kMf; ++i) {
+                    product(1, i);
+                    __builtin_amdgcn_sched_barrier(0);
+                    #pragma unroll
+                    for (int m = 0; m < 2 * kPieces / kMf; ++m)
+                        stage_piece(next, 2 * kPieces / kMf * i + m);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+                #pragma unroll
+                for (int i = 0; i < kMf; ++i)
+                    product(1, i);
+            }
         };
+        if (kAhead) {
+            arrive(s0);
+            read_k(s0);
+        }
         uint32_t s = s0;
         for (const uint32_t whole = min(s1, ctx / kTK / KW); s < whole; ++s) {
-            arrive(s);
+            if (!kAhead)
+                arrive(s);
             tile_step(std::false_type{}, s);
         }
         for (; s < s1; ++s) {
-            arrive(s);
-            if ((s * KW + kw) * kTK < tc * kTK + nodes)
+            if (!kAhead)
+                arrive(s);
+            if ((s * KW + kw) * kTK < tc * kTK + nodes) {
                 tile_step(std::true_type{}, s);
+            } else if (kAhead) {
+                arrive(s + 1);
+                read_k(s + 1);
+            }
         }
         // The piece's ways join: every wave's columns into LDS (the ring is idle: nothing is in flight), column c32 a row of
         // D floats, its 16-byte chunks XORed by the column.
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __syncthreads();
         {
             f32x4* row = reinterpret_cast<f32x4*>(lds) + (wl * 32 + c32) * (D / 4);
@@ -585,7 +653,7 @@ Plan plan_of(const mako_tree_args* a, uint32_t cus)
     // Column groups: as many as there are columns for. The other side, us at 64 lists (8 lists) of 8192 keys, heads of 128:
     // 64 columns in 2 groups 57 (23), in 1 and two column blocks 61 (20), in 4 68 (26); 96 columns in 4 71 (28), in 2 80
     // (24); 128 columns in 4 77 (30), in 2 81 (25); 32 columns, 32 lists, in 1 group 32, in 2 35, in 4 40.
-    pl.ng = nc <= 32 ? 1 : nc <= 64 ? 2 : 4;
+    pl.ng = nc <= 32 && a->dim != 256 ? 1 : nc <= 64 ? 2 : 4;
     pl.ncb = (nc + 32 * pl.ng - 1) / (32 * pl.ng);
     pl.ways = a->dim == 64 ? ways_of<64>(pl.ng) : a->dim == 128 ? ways_of<128>(pl.ng) : ways_of<256>(pl.ng);
     const uint32_t tiles = (a->max_ctx + kTK - 1) / kTK + (a->n_draft + kTK - 1) / kTK;
@@ -627,8 +695,8 @@ void launch_split(const TreeParams& p, void* o, float* lse, hipStream_t s)
 template <class T, class TO, int D>
 void launch(const TreeParams& p, uint32_t ng, void* o, float* lse, hipStream_t s)
 {
-    if (ng == 1)
-        launch_split<T, TO, D, 1>(p, o, lse, s);
+    if (D < 256 && ng == 1)
+        launch_split<T, TO, D, D < 256 ? 1 : 2>(p, o, lse, s);
     else if (ng == 2)
         launch_split<T, TO, D, 2>(p, o, lse, s);
     else
