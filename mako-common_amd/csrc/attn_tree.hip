@@ -441,8 +441,8 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                     product(1, i);
                     __builtin_amdgcn_sched_barrier(0);
                     #pragma unroll
-                    for (int m = 0; m < 2 * kPieces / kMf; ++m)
-                        stage_piece(next, 2 * kPieces / kMf * i + m);
+                    for (int m = 2 * kPieces * i / kMf; m < 2 * kPieces * (i + 1) / kMf; ++m)
+                        stage_piece(next, m);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             } else {

@@ -124,6 +124,15 @@ def test_tree(case):
     run_tree(dt=dt, out=out, dim=dim, heads=heads, kv=kv, ctx=ctx, n=n, nodes=nodes, seed=len(ctx) + n)
 
 
+@pytest.mark.parametrize("dt,out,dim,heads,n,ctx", [
+    (F16, F16, 64, 2, 4, 300001), (BF16, F32, 64, 2, 32, 150000), (F16, F32, 64, 4, 64, 45001),
+    (BF16, BF16, 128, 2, 4, 150000), (F16, F16, 128, 2, 32, 70001), (BF16, F32, 128, 4, 64, 45000),
+    (F16, F16, 256, 2, 4, 70001), (BF16, BF16, 256, 2, 32, 70000), (F16, F16, 256, 2, 64, 45000), (BF16, F32, 256, 4, 64, 25001)])
+def test_tree_long_ranges(dt, out, dim, heads, n, ctx):
+    """One list so long that each of 256 workgroups goes round its ring several times."""
+    run_tree(dt=dt, out=out, dim=dim, heads=heads, kv=1, ctx=[ctx], n=n, seed=9)
+
+
 def test_tree_chain_padding_and_wide_rows():
     """No mask: node r sees the drafts up to it. Padded heads of q and the draft tiles, o rows wider than the heads, a
     context over max_ctx (cut to it)."""
