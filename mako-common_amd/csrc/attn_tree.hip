@@ -66,16 +66,18 @@ __device__ __forceinline__ uint32_t steps_of(const TreeParams& p, uint32_t ctx, 
     return ((ctx + kTK - 1) / kTK + (nodes + kTK - 1) / kTK + p.ways - 1) / p.ways;
 }
 
-// The units of a segment of sequence i: its steps, and kLead more in front of them for what a piece costs beside its
-// steps, so that ranges that meet two segments get fewer (256 lists of 4096 keys, heads of 128: 94 us with 0 of them, 90
-// with 3, 89.6 with 6, 90 with 10; 40 lists of 5000: 37.1, 34.0, 33.2, 33.8).
-constexpr uint32_t kLead = 6;
+// The units of a segment of sequence i: its steps, and lead_of more in front of them for what a piece costs beside its
+// steps, so that ranges that meet two segments get fewer (heads of 128, 256 lists of 4096 keys: 94 us with 0 of them, 90
+// with 3, 89.6 with 6, 90 with 10; 40 lists of 5000: 37.1, 34.0, 33.2, 33.8. Heads of 256, 4 x 64 drafts, 16 heads over 2,
+// 8700 to 13600 keys: 95 with 10, 90 with 13, as a piece writes 128 columns of 256).
+constexpr uint32_t lead_of(int dim) { return dim == 256 ? 13 : 6; }
+template <int D>
 struct SegUnits {
     const TreeParams& p;
     __device__ __forceinline__ uint32_t operator()(uint32_t i) const
     {
         const uint32_t steps = steps_of(p, ctx_of(p, i), nodes_of(p, i));
-        return steps ? steps + kLead : 0u;
+        return steps ? steps + lead_of(D) : 0u;
     }
 };
 
@@ -167,10 +169,15 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
     using S = Shape<D, NG>;
     using E = Elem<T>;
     using V8 = typename E::vec8;
-    // One wave a SIMD: nothing else hides the wave's LDS reads, and its registers hold K's operands beside V's.
+    // Heads of 256: one wave a SIMD, so nothing else hides the wave's LDS reads. Its registers hold K's operands of the next
+    // tile beside V's of this one and Q (in accumulator registers), reads and loads are issued between products, and the
+    // scores are summed in two chains (a product that waits for its sum takes 72 clocks, others 36). 4 x 64 drafts, 16 heads
+    // over 2: 113 us before, 90-95; clocks a step 2700 (scores and V^T 890, softmax 450, products 1290), 1540 of products.
     constexpr bool kAhead = D == 256;
+    constexpr int kChains = kAhead ? 2 : 1;
     constexpr bool kSplitP = __is_same(T, __bf16) || __is_same(TO, float);  // P as the sum of two values of T
     constexpr int KW = S::kKW, ND = D / 32, NK = D / 16, W = S::kWaves;
+    constexpr uint32_t kLead = lead_of(D);
     constexpr int kRow = 2 * D, kHalf = kTK * kRow, kPieces = kHalf / 1024 / NG;  // 1 KiB pieces of K (of V) a wave
     static_assert(kPieces >= 1, "every wave stages some");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[S::kLds];
@@ -211,7 +218,7 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
     // The first piece of the range (or the segment): steps [s0, s1) of the segment's len; units of the range behind them.
     uint32_t b, kvh, len, s0, s1, left = 0;
     if (p.n_ranges) {
-        const Place at = place_of(p.batch, p.kv_heads, range, p.n_ranges, lane, SegUnits{p});
+        const Place at = place_of(p.batch, p.kv_heads, range, p.n_ranges, lane, SegUnits<D>{p});
         if (at.x0 == at.x1)
             return;
         b = at.b;
@@ -250,10 +257,10 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                              tile_rsrc(static_cast<const T*>(p.v) + cache, ctx * kRow),
                              tile_rsrc(static_cast<const T*>(p.kd) + draft, nodes * kRow),
                              tile_rsrc(static_cast<const T*>(p.vd) + draft, nodes * kRow)};
-        // Piece i of the tile of way kw in step s into its ring slot (past the segment's tiles: rows past the tree, zeros; past
-        // the range's steps: zeros, without a read). Streaming
-        // loads: 128 lists of 8192 keys of 128 take 88 us with them, 103 without (with column blocks, which read the keys
-        // again from the L2, the same either way).
+        // The wave's share of the tile of way kw in step s, into its ring slot, a piece of K or V at a time (past the segment's
+        // tiles: rows past the tree, zeros; kAhead, past the range's steps: zeros too, so that as many are always in flight).
+        // Streaming loads: 128 lists of 8192 keys of 128 take 88 us with them, 103 without (with column blocks, which read the
+        // keys again from the L2, the same either way).
         struct Slot {
             uint32_t dst, off;
             u32x4 k, v;
@@ -292,6 +299,13 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                 qreg[kk] = has ? *reinterpret_cast<const V8*>(src + 16 * kk) : V8{};
         }
         asm volatile("" : "+v"(sees));
+        // Q has come; kAhead: into accumulator registers, which the products read as well as the others.
+        auto operand = [&](V8& x) __attribute__((always_inline)) {
+            if constexpr (kAhead)
+                asm volatile("" : "+a"(x));
+            else
+                settle(x);
+        };
         f32x16 acc[ND];
         #pragma unroll
         for (int db = 0; db < ND; ++db)
@@ -303,7 +317,7 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
             s_odd = 0;
         #pragma unroll
         for (int kk = 0; kk < NK; ++kk)
-            settle(qreg[kk]);
+            operand(qreg[kk]);
         // Step s has landed; every wave is done with step s - 1, whose slots take step s + DEPTH - 1.
         auto landed = [&](uint32_t s) __attribute__((always_inline)) {
             if (kAhead || s + S::kDepth - 1 <= s1)
@@ -350,14 +364,22 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                 for (int kk = 0; kk < NK; ++kk)
                     settle(kf[kk]);
                 read_v();
-                __builtin_amdgcn_sched_barrier(0);
             } else {
                 read_k(s);
             }
-            f32x16 x = f32x16{};
+            f32x16 chain[kChains];
             #pragma unroll
             for (int kk = 0; kk < NK; ++kk)
-                x = E::mfma32(kf[kk], qreg[kk], x);
+                chain[kk % kChains] = E::mfma32(kf[kk], qreg[kk], kk < kChains ? f32x16{} : chain[kk % kChains]);
+            f32x16 x = chain[0];
+            if (kChains > 1)
+                x += chain[kChains - 1];
+            if (kAhead)
+                #pragma unroll
+                for (int kk = 0; kk < NK; ++kk) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 4 * ND / NK, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                }
             if (!kAhead)
                 read_v();
             __builtin_amdgcn_sched_barrier(0);
