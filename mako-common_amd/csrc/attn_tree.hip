@@ -170,9 +170,9 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
     using E = Elem<T>;
     using V8 = typename E::vec8;
     // Heads of 256: one wave a SIMD, so nothing else hides the wave's LDS reads. Its registers hold K's operands of the next
-    // tile beside V's of this one and Q (in accumulator registers), reads and loads are issued between products, and the
-    // scores are summed in two chains (a product that waits for its sum takes 72 clocks, others 36). 4 x 64 drafts, 16 heads
-    // over 2: 113 us before, 90-95; clocks a step 2700 (scores and V^T 890, softmax 450, products 1290), 1540 of products.
+    // tile beside V's of this one and Q (in accumulator registers); K's are read between the products with V, V's between
+    // those of the scores (two chains of these: scores and V^T 860-890 clocks for 1030), loads issued between the last. 4 x
+    // 64 drafts, 16 heads over 2: 113 us before, 96 so; a step 2700 clocks (softmax 450, products with V 1290), 1540 of products.
     constexpr bool kAhead = D == 256;
     constexpr int kChains = kAhead ? 2 : 1;
     constexpr bool kSplitP = __is_same(T, __bf16) || __is_same(TO, float);  // P as the sum of two values of T
@@ -674,7 +674,7 @@ Plan plan_of(const mako_tree_args* a, uint32_t cus)
     Plan pl{};
     // Column groups: as many as there are columns for. The other side, us at 64 lists (8 lists) of 8192 keys, heads of 128:
     // 64 columns in 2 groups 57 (23), in 1 and two column blocks 61 (20), in 4 68 (26); 96 columns in 4 71 (28), in 2 80
-    // (24); 128 columns in 4 77 (30), in 2 81 (25); 32 columns, 32 lists, in 1 group 32, in 2 35, in 4 40.
+    // (24); 128 columns in 4 77 (30), in 2 81 (25); 32 columns, 32 lists, in 1 group 32, in 2 35, in 4 40; heads of 256 61, 58-60, 72.
     pl.ng = nc <= 32 && a->dim != 256 ? 1 : nc <= 64 ? 2 : 4;
     pl.ncb = (nc + 32 * pl.ng - 1) / (32 * pl.ng);
     pl.ways = a->dim == 64 ? ways_of<64>(pl.ng) : a->dim == 128 ? ways_of<128>(pl.ng) : ways_of<256>(pl.ng);
