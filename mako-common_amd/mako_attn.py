@@ -187,10 +187,15 @@ def _stream(stream):
     return _current[1](_current[0]())
 
 
-def dtype_code(t):
-    import torch
+_codes = {}
 
-    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}[t.dtype]
+
+def dtype_code(t):
+    if not _codes:
+        import torch
+
+        _codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    return _codes[t.dtype]
 
 
 LIBRARY = "library"  # workspace= default: the entry point without a workspace argument (the library keeps its own)
