@@ -337,9 +337,9 @@ __global__ __launch_bounds__(TH) void evict_select(const EvictParams p)
         bases[tid] = before;
         __syncthreads();
         // Up to the budget, where rows may be holes, and wherever ties at T count, the waves take 64 rows at a time (a lane a
-        // row); behind, a row that stays is a source, and its thread lists it.
+        // row); behind, a row that stays is a source, and its thread lists it. (Of this block: the budget may lie past it.)
         const uint32_t first = blk * ROWS, per_wave = 64 * R;
-        uint32_t by_lane = first > budget ? 0u : (budget - first) / per_wave * per_wave + per_wave;
+        uint32_t by_lane = first > budget ? 0u : min((uint32_t)ROWS, (budget - first) / per_wave * per_wave + per_wave);
         if (need)
             by_lane = ROWS;
         for (uint32_t x0 = 64 * wv; x0 < min(by_lane, n - first); x0 += TH) {
