@@ -209,9 +209,8 @@ int mako_attn_decode_noalloc(const mako_decode_args* a, mako_dtype in, mako_dtyp
  * from n_nodes[b] on are left as they were. ctx_len, n_nodes and mask are in device memory. A key that a node does
  * not see has no part in its row, whatever its k and v hold (infinities and NaN too), nor has a cache row past ctx_len.
  * dim 64, 128 or 256, n_draft at most 64, width a multiple of 4. o must not overlap the inputs.
- * Precision: scores, sums and lse in f32; the probabilities meet V in V's own type, f16 with 11 bits for f16 tiles and
- * f16 output, else as the sum of two values of the type (bf16: 16 bits; f16: 21), so that the output's rounding is the
- * one that counts. workspace: at least mako_attn_tree_workspace(a) bytes, 16-byte aligned; its contents do not matter,
+ * Precision: scores, sums and lse in f32; the probabilities meet V as the sum of two values of its type (bf16: 16 bits;
+ * f16: 22), so that with f16 or bf16 output the output's rounding is the one that counts. workspace: at least mako_attn_tree_workspace(a) bytes, 16-byte aligned; its contents do not matter,
  * and calls that overlap in time need separate ones.
  */
 typedef struct mako_tree_args {

@@ -175,7 +175,6 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
     // 64 drafts, 16 heads over 2: 113 us before, 96 so; a step 2700 clocks (softmax 450, products with V 1290), 1540 of products.
     constexpr bool kAhead = D == 256;
     constexpr int kChains = kAhead ? 2 : 1;
-    constexpr bool kSplitP = __is_same(T, __bf16) || __is_same(TO, float);  // P as the sum of two values of T
     constexpr int KW = S::kKW, ND = D / 32, NK = D / 16, W = S::kWaves;
     constexpr uint32_t kLead = lead_of(D);
     constexpr int kRow = 2 * D, kHalf = kTK * kRow, kPieces = kHalf / 1024 / NG;  // 1 KiB pieces of K (of V) a wave
@@ -418,7 +417,7 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
             }
             const float mu = m == -INFINITY ? 0.0f : m;
             // 16 keys at a time: the second half's exponentials run beside the first half's products.
-            u32x4 hi[2], lo[2];
+            u32x4 hi[2], lo[2];  // P as the sum of two values of T (bf16: 16 bits, f16: 22; one would show in the output)
             auto half = [&](int a) __attribute__((always_inline)) {
                 #pragma unroll
                 for (int i = 8 * a; i < 8 * a + 8; ++i)
@@ -427,8 +426,7 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                 for (int i = 0; i < 4; ++i) {
                     const float e0 = x[8 * a + 2 * i], e1 = x[8 * a + 2 * i + 1];
                     hi[a][i] = E::pack2(e0, e1);
-                    if (kSplitP)
-                        lo[a][i] = E::pack2(e0 - value_of<T>(hi[a][i], 0), e1 - value_of<T>(hi[a][i], 1));
+                    lo[a][i] = E::pack2(e0 - value_of<T>(hi[a][i], 0), e1 - value_of<T>(hi[a][i], 1));
                 }
                 l += (x[8 * a] + x[8 * a + 1]) + (x[8 * a + 2] + x[8 * a + 3]) +
                      ((x[8 * a + 4] + x[8 * a + 5]) + (x[8 * a + 6] + x[8 * a + 7]));
@@ -436,7 +434,7 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
             auto product = [&](int a, int i) __attribute__((always_inline)) {
                 acc[i % ND] = E::mfma32(vf[a][i % ND], __builtin_bit_cast(V8, i < ND ? hi[a] : lo[a]), acc[i % ND]);
             };
-            constexpr int kMf = ND * (kSplitP ? 2 : 1);  // products of a half
+            constexpr int kMf = 2 * ND;  // products of a half
             half(0);
             __builtin_amdgcn_sched_barrier(0);
             if (kAhead) {
@@ -452,7 +450,7 @@ __global__ __launch_bounds__((Shape<D, NG>::kWaves * 64), ((Shape<D, NG>::kWaves
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 if (kAhead)
                     __builtin_amdgcn_sched_group_barrier(0x100, NK / kMf, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, (kSplitP ? 40 : 20) / kMf + 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 40 / kMf + 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x400, 8 / kMf + 1, 0);
             }
             if (kAhead) {

@@ -1,12 +1,15 @@
-"""The cache operators where their kernels change course: lists of several blocks, budgets at a block's end."""
+"""The cache operators where their kernels change course: lists of several blocks, budgets at a block's end; and the bits that
+f16 output keeps."""
 import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
+import cache_ref as R  # noqa: E402
+import mako_attn as M  # noqa: E402
 import test_gpu_cache as T  # noqa: E402
-from test_gpu_cache import BF16, F16  # noqa: E402
+from test_gpu_cache import BF16, F16, F32, as_i64, gen, i32, randn, random_masks  # noqa: E402
 
 GUARD = 1 << 18  # bytes on either side of a workspace
 
@@ -51,3 +54,24 @@ def test_evict_lists_of_several_blocks(guarded, case, in_place):
     """Distinct weights, so that the selection ends without a tie, and the budget past the first block's rows."""
     T.run_evict(dt=F16 if in_place else BF16, dim=64, kv=2, seed=70, in_place=in_place,
                 **dict(dict(weigh=lambda w, rng: w.__setitem__(..., rng.permutation(w.size).reshape(w.shape))), **case))
+
+
+@pytest.mark.parametrize("dim,heads,kv,ctx,n", [(64, 4, 2, [40, 3], 7), (128, 8, 2, [30, 12], 6), (128, 8, 1, [60, 20], 20),
+                                               (128, 4, 2, [9000, 5000], 16), (256, 8, 2, [33, 31], 9),
+                                               (256, 4, 1, [6000], 40)])
+def test_tree_f16_output_is_rounded_once(dim, heads, kv, ctx, n):
+    """f16 tiles and f16 output: what the output's own rounding (2^-11 of the value, 2^-25 below f16's normal range) does not
+    explain is within the bound of f32 output, that is, the probabilities hold twice f16's bits: where p and v cancel, one
+    f16 value of p would show."""
+    B, cap, g, rng = len(ctx), max(ctx) + 3, gen(80), np.random.default_rng(80)
+    q = randn(g, (heads, B * n, dim), F16, 2.0 ** -4)  # (small scores, so that their own bound is small)
+    k, v = (randn(g, (B, kv, cap, dim), F16) for _ in range(2))
+    kd, vd = (randn(g, (kv, B * n, dim), F16) for _ in range(2))
+    m = random_masks(rng, B, n)
+    a = M.tree_args(batch=B, n_draft=n, heads=heads, kv_heads=kv, dim=dim, cap=cap, max_ctx=cap)
+    o = torch.zeros((B * n, heads * dim), dtype=F16, device="cuda")
+    M.attn_tree(a, q, k, v, kd, vd, i32(ctx), o, T.buffer(M.attn_tree_workspace(a)), mask=as_i64(m))
+    torch.cuda.synchronize()
+    want, _, tol, _ = R.tree(*[R.f64(t) for t in (q, k, v, kd, vd)], ctx, [n] * B, m, n=n, scale=a.scale, out=F32,
+                             in_dtype=F16)
+    T.check(o, want, tol + 2.0 ** -11 * np.abs(want) + 2.0 ** -25, "o")
