@@ -199,10 +199,10 @@ void TransformerRuntime::attention_tree(gpu::Encoder*& enc, gpu::Buffer* q, gpu:
                                         gpu::Buffer* kd, gpu::Buffer* vd, gpu::Buffer* ctx_len, gpu::Buffer* n_nodes,
                                         gpu::Buffer* mask, gpu::Buffer* o, uint32_t batch, uint32_t n_draft,
                                         uint32_t n_heads, uint32_t kv_heads, uint32_t cap, uint32_t max_ctx,
-                                        uint32_t dim, const AttnOptions& opt)
+                                        uint32_t dim, const AttnOptions& opt, uint32_t q_pad, uint32_t d_pad)
 {
-    const mako_tree_args a{batch, n_draft, batch * n_draft, batch * n_draft, n_heads, kv_heads, dim, cap, max_ctx,
-                           n_heads * dim, 1.0f / std::sqrt(float(dim))};
+    const mako_tree_args a{batch, n_draft, q_pad ? q_pad : batch * n_draft, d_pad ? d_pad : batch * n_draft, n_heads,
+                           kv_heads, dim, cap, max_ctx, n_heads * dim, 1.0f / std::sqrt(float(dim))};
     const size_t need = mako_attn_tree_workspace(&a);
     gpu::Buffer* ws = need ? scratch("attn_tree", need) : nullptr;
     before(enc);
@@ -216,9 +216,10 @@ void TransformerRuntime::attention_tree(gpu::Encoder*& enc, gpu::Buffer* q, gpu:
 void TransformerRuntime::cache_append(gpu::Encoder*& enc, gpu::Buffer* kd, gpu::Buffer* vd, gpu::Buffer* path,
                                       gpu::Buffer* n_path, gpu::Buffer* ctx_len, gpu::Buffer* seen, gpu::Buffer* w,
                                       gpu::Buffer* pos, gpu::Buffer* k, gpu::Buffer* v, uint32_t batch,
-                                      uint32_t n_draft, uint32_t kv_heads, uint32_t cap, uint32_t dim, mako_dtype in)
+                                      uint32_t n_draft, uint32_t kv_heads, uint32_t cap, uint32_t dim, mako_dtype in,
+                                      uint32_t d_pad)
 {
-    const mako_append_args a{batch, n_draft, batch * n_draft, kv_heads, dim, cap};
+    const mako_append_args a{batch, n_draft, d_pad ? d_pad : batch * n_draft, kv_heads, dim, cap};
     before(enc);
     // (once: what it appends to has grown by then)
     check(mako_cache_append(&a, in, kd->ptr, vd->ptr, ptr<const uint32_t>(path), ptr<const uint32_t>(n_path),
@@ -230,10 +231,13 @@ void TransformerRuntime::cache_append(gpu::Encoder*& enc, gpu::Buffer* kd, gpu::
 void TransformerRuntime::cache_weights(gpu::Encoder*& enc, gpu::Buffer* q, gpu::Buffer* lse, gpu::Buffer* k,
                                        gpu::Buffer* ctx_len, gpu::Buffer* path, gpu::Buffer* n_path, gpu::Buffer* w,
                                        uint32_t batch, uint32_t n_q, uint32_t n_heads, uint32_t kv_heads, uint32_t cap,
-                                       uint32_t max_ctx, float decay, bool by_sequence, uint32_t dim, mako_dtype in)
+                                       uint32_t max_ctx, float decay, bool by_sequence, uint32_t dim, mako_dtype in,
+                                       uint32_t q_pad)
 {
-    const mako_weights_args a{batch, n_q, by_sequence ? 0u : batch * n_q, n_heads, kv_heads, dim, cap, max_ctx,
-                              1.0f / std::sqrt(float(dim)), decay};
+    if (by_sequence && q_pad)
+        throw std::runtime_error(fmt("cache_weights: queries by sequence in heads of %u rows", q_pad));
+    const mako_weights_args a{batch, n_q, by_sequence ? 0u : q_pad ? q_pad : batch * n_q, n_heads, kv_heads, dim, cap,
+                              max_ctx, 1.0f / std::sqrt(float(dim)), decay};
     const size_t need = mako_cache_weights_workspace(&a);
     gpu::Buffer* ws = need ? scratch("cache_weights", need) : nullptr;
     before(enc);

@@ -96,26 +96,29 @@ protected:
     // The cache of attention_decode with trees of drafted tokens (no counterparts in the reference). attention_tree: node r
     // of sequence b is row b * n_draft + r of q [heads][rows][dim], kd and vd [kv_heads][rows][dim] (the tiles heads() and
     // heads_partial() write for the drafts of all sequences one after another) and of o [rows][heads * dim], opt.lse
-    // [heads][rows]; it sees the cache rows below ctx_len[b] and the drafts of its mask (u64 [batch][n_draft], null: those
-    // up to it), n_nodes u32 [batch] of them (null: all). The split's partials are the Runtime-owned scratch "attn_tree".
+    // [heads][batch * n_draft]; it sees the cache rows below ctx_len[b] and the drafts of its mask (u64 [batch][n_draft],
+    // null: those up to it), n_nodes u32 [batch] of them (null: all). A head of the tiles is q_pad rows in q, d_pad in kd and
+    // vd (here and below 0: the rows that are used, no padding; with attention()'s tiles, its q_pad and k_pad). The split's
+    // partials are the Runtime-owned scratch "attn_tree".
     void attention_tree(gpu::Encoder*& enc, gpu::Buffer* q, gpu::Buffer* k, gpu::Buffer* v, gpu::Buffer* kd,
                         gpu::Buffer* vd, gpu::Buffer* ctx_len, gpu::Buffer* n_nodes, gpu::Buffer* mask, gpu::Buffer* o,
                         uint32_t batch, uint32_t n_draft, uint32_t heads, uint32_t kv_heads, uint32_t cap,
-                        uint32_t max_ctx, uint32_t dim = kHeadDim, const AttnOptions& opt = {});
+                        uint32_t max_ctx, uint32_t dim = kHeadDim, const AttnOptions& opt = {}, uint32_t q_pad = 0,
+                        uint32_t d_pad = 0);
     // Appends each sequence's accepted drafts (path u32 [batch][n_draft] and n_path u32 [batch], null: all in order) to the
     // cache; ctx_len grows by their number, in place, as do seen (tokens so far) and, on the new rows, w (0) and pos (their
-    // tokens), where given.
+    // tokens), where given. A prompt enters so too, with n_draft its rows and d_pad its tiles' k_pad.
     void cache_append(gpu::Encoder*& enc, gpu::Buffer* kd, gpu::Buffer* vd, gpu::Buffer* path, gpu::Buffer* n_path,
                       gpu::Buffer* ctx_len, gpu::Buffer* seen, gpu::Buffer* w, gpu::Buffer* pos, gpu::Buffer* k,
                       gpu::Buffer* v, uint32_t batch, uint32_t n_draft, uint32_t kv_heads, uint32_t cap,
-                      uint32_t dim = kHeadDim, mako_dtype in = MAKO_F16);
+                      uint32_t dim = kHeadDim, mako_dtype in = MAKO_F16, uint32_t d_pad = 0);
     // Adds to w [batch][kv_heads][cap], times decay first, the attention weight that each cache row gets from the last n_q
-    // rows' queries, or those of a path: q [heads][batch * n_q][dim] and lse [heads][batch * n_q] of the attention's call
-    // (by_sequence: attention_decode's [batch][heads][n_q]). Scratch "cache_weights".
+    // rows' queries, or those of a path: q [heads][q_pad][dim] and lse [heads][batch * n_q] of the attention's call
+    // (by_sequence: attention_decode's [batch][heads][n_q], without padding). Scratch "cache_weights".
     void cache_weights(gpu::Encoder*& enc, gpu::Buffer* q, gpu::Buffer* lse, gpu::Buffer* k, gpu::Buffer* ctx_len,
                        gpu::Buffer* path, gpu::Buffer* n_path, gpu::Buffer* w, uint32_t batch, uint32_t n_q,
                        uint32_t heads, uint32_t kv_heads, uint32_t cap, uint32_t max_ctx, float decay = 1.0f,
-                       bool by_sequence = false, uint32_t dim = kHeadDim, mako_dtype in = MAKO_F16);
+                       bool by_sequence = false, uint32_t dim = kHeadDim, mako_dtype in = MAKO_F16, uint32_t q_pad = 0);
     // Evicts rows down to `budget` a (sequence, kv head): tokens below sinks and the last `recent` ones stay, then the rows
     // of the largest w. k, v, w, pos and ctx_len in place. Scratch "cache_evict".
     void cache_evict(gpu::Encoder*& enc, gpu::Buffer* k, gpu::Buffer* v, gpu::Buffer* w, gpu::Buffer* pos,

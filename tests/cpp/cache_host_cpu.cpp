@@ -1,6 +1,6 @@
 // The cache calls of TransformerRuntime without a GPU: the C ABI's entry points and the HIP calls under them are this
 // program's own (they come before the libraries'), record what they are given and run nothing. With MAKO_REPEAT set, the
-// calls that change their own inputs run once.
+// calls that change their own inputs run once; tiles with padded heads are passed on as such.
 //   cache_host_cpu
 #include <hip/hip_runtime_api.h>
 
@@ -112,12 +112,41 @@ void repeated()
     check(evictions.size() == 1, "MAKO_REPEAT: cache_evict once (a second call would find nothing over the budget)");
 }
 
+void padded()
+{
+    Harness h;
+    auto* x = h.scratch("x", 64);
+    auto* enc = h.encoder();
+    trees.clear(), appends.clear(), weighings.clear();
+    h.attention_tree(enc, x, x, x, x, x, x, nullptr, nullptr, x, B, N, H, KV, CAP, CAP, 128, {}, 64, 128);
+    h.attention_tree(enc, x, x, x, x, x, x, nullptr, nullptr, x, B, N, H, KV, CAP, CAP);
+    check(trees[0].q_pad == 64 && trees[0].d_pad == 128 && trees[1].q_pad == B * N && trees[1].d_pad == B * N,
+          "attention_tree: the tiles' padding");
+    h.cache_append(enc, x, x, nullptr, nullptr, x, x, x, x, x, x, 1, 100, KV, CAP, 128, MAKO_BF16, 128);
+    h.cache_append(enc, x, x, nullptr, nullptr, x, x, x, x, x, x, B, N, KV, CAP);
+    check(appends[0].d_pad == 128 && appends[1].d_pad == B * N, "cache_append: the tiles' padding");
+    h.cache_weights(enc, x, x, x, x, nullptr, nullptr, x, 1, 100, H, KV, CAP, CAP, 1.0f, false, 128, MAKO_BF16, 128);
+    h.cache_weights(enc, x, x, x, x, nullptr, nullptr, x, B, N, H, KV, CAP, CAP);
+    h.cache_weights(enc, x, x, x, x, nullptr, nullptr, x, B, 1, H, KV, CAP, CAP, 1.0f, true);
+    check(weighings[0].q_pad == 128 && weighings[1].q_pad == B * N && weighings[2].q_pad == 0,
+          "cache_weights: the tiles' padding");
+    bool refused = false;
+    try {
+        h.cache_weights(enc, x, x, x, x, nullptr, nullptr, x, B, 1, H, KV, CAP, CAP, 1.0f, true, 128, MAKO_F16, 64);
+    } catch (const std::runtime_error&) {
+        refused = true;
+    }
+    check(refused && weighings.size() == 3, "cache_weights refuses padding by sequence");
+    h.finish(enc);
+}
+
 }  // namespace
 
 int main()
 {
     std::setvbuf(stdout, nullptr, _IOLBF, 0);
     repeated();
+    padded();
     std::printf("%s\n", failures ? "FAILED" : "all passed");
     return failures != 0;
 }

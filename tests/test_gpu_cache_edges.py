@@ -1,5 +1,8 @@
-"""The cache operators where their kernels change course: lists of several blocks, budgets at a block's end; and the bits that
-f16 output keeps."""
+"""The cache operators where their kernels change course: lists of several blocks, budgets at a block's end; the bits that
+f16 output keeps; a prompt's padded tiles through the C++ host side (tests/cpp/cache_prompt_test)."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -8,6 +11,7 @@ pytestmark = pytest.mark.gpu
 
 import cache_ref as R  # noqa: E402
 import mako_attn as M  # noqa: E402
+from conftest import ROOT  # noqa: E402
 import test_gpu_cache as T  # noqa: E402
 from test_gpu_cache import BF16, F16, F32, as_i64, gen, i32, randn, random_masks  # noqa: E402
 
@@ -75,3 +79,11 @@ def test_tree_f16_output_is_rounded_once(dim, heads, kv, ctx, n):
     want, _, tol, _ = R.tree(*[R.f64(t) for t in (q, k, v, kd, vd)], ctx, [n] * B, m, n=n, scale=a.scale, out=F32,
                              in_dtype=F16)
     T.check(o, want, tol + 2.0 ** -11 * np.abs(want) + 2.0 ** -25, "o")
+
+
+def test_cpp_prompt_of_padded_tiles():
+    path = os.path.join(ROOT, "tests", "cpp", "bin", "cache_prompt_test")
+    assert os.path.exists(path), f"{path} is not built (build() makes it)"
+    r = subprocess.run([path], capture_output=True, text=True, timeout=120)
+    print(r.stdout)
+    assert r.returncode == 0 and "all passed" in r.stdout, r.stdout + r.stderr
