@@ -704,44 +704,55 @@ size_t workspace_for(const Plan& pl, const mako_tree_args* a)
                      : 0;
 }
 
-template <class T, class TO, int D, int NG>
-void launch_split(const TreeParams& p, void* o, float* lse, hipStream_t s)
+// Workgroups of tree_split, and of tree_merge: a wave an item where segments have few pieces (n_ranges of them over all, and
+// a cut one more each). The call's us with a wave and with four, 16 drafts, heads of 128: 4 pieces 37.9, 43.1; 8 pieces 37.4,
+// 38.9; 32 pieces 41.9, 41.5; 64 drafts, heads of 256, 128 pieces: 60.6, 58.3.
+uint64_t split_groups(const Plan& pl, uint64_t segs)
 {
-    const uint32_t units = p.n_ranges ? p.n_ranges : p.batch * p.kv_heads;
-    const dim3 grid(p.ncb > 1 ? (units + 7) / 8 * 8 * p.ncb : units), block(Shape<D, NG>::kWaves * 64);
+    const uint64_t units = pl.n_ranges ? pl.n_ranges : segs;
+    return pl.ncb > 1 ? (units + 7) / 8 * 8 * pl.ncb : units;
+}
+bool merge_by_wave(uint32_t n_ranges, uint64_t segs) { return n_ranges / segs < 16; }
+uint64_t merge_groups(uint32_t n_ranges, uint64_t segs, uint64_t items)
+{
+    return n_ranges == 0 ? 0 : merge_by_wave(n_ranges, segs) ? (items + 3) / 4 : items;
+}
+
+template <class T, class TO, int D, int NG>
+void launch_split(const TreeParams& p, const Plan& pl, void* o, float* lse, hipStream_t s)
+{
+    const dim3 grid((uint32_t)split_groups(pl, (uint64_t)p.batch * p.kv_heads)), block(Shape<D, NG>::kWaves * 64);
     hipLaunchKernelGGL((tree_split<T, TO, D, NG>), grid, block, 0, s, p, static_cast<TO*>(o), lse);
 }
 
 template <class T, class TO, int D>
-void launch(const TreeParams& p, uint32_t ng, void* o, float* lse, hipStream_t s)
+void launch(const TreeParams& p, const Plan& pl, void* o, float* lse, hipStream_t s)
 {
-    if (D < 256 && ng == 1)
-        launch_split<T, TO, D, D < 256 ? 1 : 2>(p, o, lse, s);
-    else if (ng == 2)
-        launch_split<T, TO, D, 2>(p, o, lse, s);
+    if (D < 256 && pl.ng == 1)
+        launch_split<T, TO, D, D < 256 ? 1 : 2>(p, pl, o, lse, s);
+    else if (pl.ng == 2)
+        launch_split<T, TO, D, 2>(p, pl, o, lse, s);
     else
-        launch_split<T, TO, D, 4>(p, o, lse, s);
-    if (!p.n_ranges)
+        launch_split<T, TO, D, 4>(p, pl, o, lse, s);
+    if (!pl.n_ranges)
         return;
-    // A wave an item where segments have few pieces (n_ranges of them over all, and a cut one more each). The call's us with
-    // a wave and with four, 16 drafts, heads of 128: 4 pieces 37.9, 43.1; 8 pieces 37.4, 38.9; 32 pieces 41.9, 41.5; 64
-    // drafts, heads of 256, 128 pieces: 60.6, 58.3.
-    const uint32_t items = p.batch * p.n_draft * p.heads;
-    if (p.n_ranges / (p.batch * p.kv_heads) < 16)
-        hipLaunchKernelGGL((tree_merge<T, TO, D, 1>), dim3((items + 3) / 4), dim3(256), 0, s, p, static_cast<TO*>(o), lse);
+    const uint64_t segs = (uint64_t)p.batch * p.kv_heads;
+    const dim3 grid((uint32_t)merge_groups(pl.n_ranges, segs, (uint64_t)p.batch * p.n_draft * p.heads));
+    if (merge_by_wave(pl.n_ranges, segs))
+        hipLaunchKernelGGL((tree_merge<T, TO, D, 1>), grid, dim3(256), 0, s, p, static_cast<TO*>(o), lse);
     else
-        hipLaunchKernelGGL((tree_merge<T, TO, D, 4>), dim3(items), dim3(256), 0, s, p, static_cast<TO*>(o), lse);
+        hipLaunchKernelGGL((tree_merge<T, TO, D, 4>), grid, dim3(256), 0, s, p, static_cast<TO*>(o), lse);
 }
 
 template <class T, class TO>
-void launch_dim(const TreeParams& p, uint32_t dim, uint32_t ng, void* o, float* lse, hipStream_t s)
+void launch_dim(const TreeParams& p, uint32_t dim, const Plan& pl, void* o, float* lse, hipStream_t s)
 {
     if (dim == 64)
-        launch<T, TO, 64>(p, ng, o, lse, s);
+        launch<T, TO, 64>(p, pl, o, lse, s);
     else if (dim == 128)
-        launch<T, TO, 128>(p, ng, o, lse, s);
+        launch<T, TO, 128>(p, pl, o, lse, s);
     else
-        launch<T, TO, 256>(p, ng, o, lse, s);
+        launch<T, TO, 256>(p, pl, o, lse, s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -818,6 +829,10 @@ extern "C" int mako_attn_tree(const mako_tree_args* a, mako_dtype in, mako_dtype
     if (workspace_bytes < need || (need && !workspace) || !aligned16(workspace))
         return fail(MAKO_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, workspace_bytes,
                     need);
+    const uint64_t segs = (uint64_t)a->batch * a->kv_heads;
+    if (!grid_fits(split_groups(pl, segs), 64 * pl.ng * pl.ways) ||
+        !grid_fits(merge_groups(pl.n_ranges, segs, (uint64_t)a->batch * a->n_draft * a->heads), 256))
+        return fail(MAKO_EINVAL, "%s: %u x %u rows of %u heads exceed the grid", what, a->batch, a->n_draft, a->heads);
     const uint32_t group = a->heads / a->kv_heads;
     const auto at = [&](size_t off) { return need ? static_cast<char*>(workspace) + off : nullptr; };
     const size_t ob = part_o_bytes(pl, a), mb = part_ml_bytes(pl, a), fb = round256(pl.pieces * sizeof(uint32_t));
@@ -828,12 +843,12 @@ extern "C" int mako_attn_tree(const mako_tree_args* a, mako_dtype in, mako_dtype
                        a->width, a->n_draft * group, pl.ncb, pl.ways, pl.n_ranges, a->scale * kLog2e};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (in == MAKO_BF16 && out == MAKO_F32)
-        launch_dim<__bf16, float>(p, a->dim, pl.ng, o, lse, s);
+        launch_dim<__bf16, float>(p, a->dim, pl, o, lse, s);
     else if (in == MAKO_BF16)
-        launch_dim<__bf16, __bf16>(p, a->dim, pl.ng, o, lse, s);
+        launch_dim<__bf16, __bf16>(p, a->dim, pl, o, lse, s);
     else if (out == MAKO_F32)
-        launch_dim<_Float16, float>(p, a->dim, pl.ng, o, lse, s);
+        launch_dim<_Float16, float>(p, a->dim, pl, o, lse, s);
     else
-        launch_dim<_Float16, _Float16>(p, a->dim, pl.ng, o, lse, s);
+        launch_dim<_Float16, _Float16>(p, a->dim, pl, o, lse, s);
     return check_launch(what);
 }

@@ -446,7 +446,7 @@ extern "C" int mako_cache_append(const mako_append_args* a, mako_dtype in, const
         return fail(MAKO_EINVAL, "%s: %u draft rows of %u kv heads exceed 2^31 chunks", what, a->n_draft, a->kv_heads);
     if ((uint64_t)a->cap * a->dim * 2 > 0x7fffffffu)
         return fail(MAKO_EINVAL, "%s: %u cache rows exceed 2 GiB a head", what, a->cap);
-    if (a->batch > 0x7fffffffu)
+    if (!grid_fits(a->batch, kThreads))
         return fail(MAKO_EINVAL, "%s: %u sequences exceed the grid", what, a->batch);
     if (!aligned16(kd) || !aligned16(vd) || !aligned16(k) || !aligned16(v))
         return fail(MAKO_EINVAL, "%s: kd, vd, k and v must be 16-byte aligned", what);
@@ -491,7 +491,8 @@ extern "C" int mako_cache_evict(const mako_evict_args* a, mako_dtype in, void* k
                     a->budget);
     const uint32_t most = most_of(a), chunks = std::max(1u, (most + kMoveRows - 1) / kMoveRows);
     const uint64_t lists = (uint64_t)a->batch * a->kv_heads;
-    if (lists * chunks > 0x7fffffffu)
+    const uint32_t threads = a->max_ctx <= 4096 ? 512 : 1024;
+    if (!grid_fits(lists, threads) || !grid_fits(lists * chunks, 256))
         return fail(MAKO_EINVAL, "%s: %llu lists of %u rows exceed the grid", what, (unsigned long long)lists, most);
     if (!aligned16(k) || !aligned16(v))
         return fail(MAKO_EINVAL, "%s: k and v must be 16-byte aligned", what);
@@ -509,7 +510,7 @@ extern "C" int mako_cache_evict(const mako_evict_args* a, mako_dtype in, void* k
     hipStream_t s = static_cast<hipStream_t>(stream);
     // The call's us with 512 threads for blocks of 4096 rows, and with 1024 for 32768: 8 lists of 1024 10.7, 13.0, of 4096
     // 11.1, 13.4, of 6000 21, 14, of 16384 34, 20; 512 lists of 4096 39, 48, of 8192 87, 89, of 16384 162, 159.
-    if (a->max_ctx <= 4096)
+    if (threads == 512)
         hipLaunchKernelGGL((evict_select<512, 4096>), dim3((uint32_t)lists), dim3(512), 0, s, p);
     else
         hipLaunchKernelGGL((evict_select<1024, 32768>), dim3((uint32_t)lists), dim3(1024), 0, s, p);

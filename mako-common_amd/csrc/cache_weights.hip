@@ -647,6 +647,8 @@ extern "C" int mako_cache_weights(const mako_weights_args* a, mako_dtype in, con
     if (!pl.few && (uint64_t)a->batch * a->heads * pl.n_blocks * ((a->n_q + kTK - 1) / kTK) >= (1ull << 32))
         return fail(MAKO_EINVAL, "%s: %u x %u heads of %u queries over %u rows exceed 2^32 tiles", what, a->batch, a->heads,
                     a->n_q, a->max_ctx);
+    if (!pl.few && !grid_fits((uint64_t)a->batch * a->kv_heads * ((a->max_ctx + 255) / 256), 256))
+        return fail(MAKO_EINVAL, "%s: %u x %u lists of %u rows exceed the grid", what, a->batch, a->kv_heads, a->max_ctx);
     WeightsParams p{q, k, lse, a->decay == 0.0f ? nullptr : w, w_out, ctx_len, path, n_path,
                     need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + ends_bytes(pl, a)) : nullptr,
                     static_cast<uint32_t*>(workspace), a->batch, a->n_q, a->heads, a->kv_heads, a->heads / a->kv_heads,

@@ -186,6 +186,8 @@ int ok();
 int last_code();
 // MAKO_OK, or MAKO_EHIP with the launch error recorded (hipGetLastError after a launch).
 int check_launch(const char* what);
+// Whether a launch has less than 2^32 threads, as HIP requires: for calls that must not run in part.
+inline bool grid_fits(uint64_t workgroups, uint32_t threads) { return workgroups * threads < (1ull << 32); }
 // Compute units of the current device (cached per device and thread); 0 when there is none.
 uint32_t device_cus();
 
