@@ -207,7 +207,8 @@ int mako_attn_decode_noalloc(const mako_decode_args* a, mako_dtype in, mako_dtyp
  * mask[b * n_draft + r] set (its ancestors and itself, where the caller sets its bit; mask NULL: the drafts j <= r, a
  * chain). A node that sees nothing gives 0 and lse = -inf. n_nodes (u32 [batch], NULL: n_draft each): rows of o and lse
  * from n_nodes[b] on are left as they were. ctx_len, n_nodes and mask are in device memory. A key that a node does
- * not see has no part in its row, whatever its k and v hold (infinities and NaN too), nor has a cache row past ctx_len.
+ * not see has no part in its row, whatever its k and v hold (infinities and NaN too), nor has a cache row past ctx_len;
+ * a v that is not finite in a row that it sees leaves its head dim of the output not finite (an infinity may give NaN).
  * dim 64, 128 or 256, n_draft at most 64, width a multiple of 4. o must not overlap the inputs.
  * Precision: scores, sums and lse in f32; the probabilities meet V as the sum of two values of its type (bf16: 16 bits;
  * f16: 22), so that with f16 or bf16 output the output's rounding is the one that counts. workspace: at least mako_attn_tree_workspace(a) bytes, 16-byte aligned; its contents do not matter,

@@ -1,5 +1,5 @@
 """The cache operators where their kernels change course: lists of several blocks, budgets at a block's end; the bits that
-f16 output keeps; a prompt's padded tiles through the C++ host side (tests/cpp/cache_prompt_test)."""
+f16 output keeps; cached values that are not finite; the append of a prompt; and a prompt's padded tiles through the C++ host side (tests/cpp/cache_prompt_test)."""
 import os
 import subprocess
 
@@ -87,3 +87,35 @@ def test_cpp_prompt_of_padded_tiles():
     r = subprocess.run([path], capture_output=True, text=True, timeout=120)
     print(r.stdout)
     assert r.returncode == 0 and "all passed" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dt,out,dim,ctx", [(F16, F16, 128, 70), (BF16, F32, 64, 5000), (BF16, BF16, 256, 9000)])
+def test_tree_cached_values_that_are_not_finite(dt, out, dim, ctx, bad):
+    """Such a value in a row of the cache: its head dim of the rows that see it is not finite, and no other output changes."""
+    heads, kv, n, g = 4, 2, 6, gen(90)
+    q = randn(g, (heads, 2 * n, dim), dt)
+    k, v = (randn(g, (2, kv, ctx, dim), dt) for _ in range(2))
+    kd, vd = (randn(g, (kv, 2 * n, dim), dt) for _ in range(2))
+    a = M.tree_args(batch=2, n_draft=n, heads=heads, kv_heads=kv, dim=dim, cap=ctx, max_ctx=ctx)
+    ws, outs = T.buffer(M.attn_tree_workspace(a)), []
+    for step in range(2):
+        if step:
+            v[1, 1, [3, ctx // 2, ctx - 1], [5, 7, dim - 1]] = bad
+        o, lse = torch.zeros((2 * n, heads * dim), dtype=out, device="cuda"), torch.zeros((heads, 2 * n), device="cuda")
+        M.attn_tree(a, q, k, v, kd, vd, i32([ctx, ctx]), o, ws, lse=lse)
+        torch.cuda.synchronize()
+        outs.append((o.view(2, n, heads, dim), lse))
+    (o0, l0), (o1, l1) = outs
+    hit = torch.zeros_like(o0, dtype=torch.bool)
+    hit[1, :, heads // kv:, [5, 7, dim - 1]] = True
+    assert not torch.isfinite(o1[hit]).any()
+    assert torch.equal(o1[~hit], o0[~hit]) and torch.equal(l1, l0)
+
+
+@pytest.mark.parametrize("case", [(F16, 128, 8, 4096, [0], [4096], 4100), (BF16, 64, 3, 513, [5, 700, 0], [513, 300, 600], 1000),
+                                  (BF16, 256, 1, 2000, [37], [1999], 1500)], ids=lambda c: f"d{c[1]}kv{c[2]}n{c[3]}")
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append_of_a_prompt(case, in_place):
+    """Thousands of rows a sequence, some lists at their cap, tiles with padded heads."""
+    T.test_append(case, in_place)
