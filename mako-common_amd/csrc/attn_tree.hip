@@ -69,7 +69,8 @@ __device__ __forceinline__ uint32_t steps_of(const TreeParams& p, uint32_t ctx, 
 // The units of a segment of sequence i: its steps, and lead_of more in front of them for what a piece costs beside its
 // steps, so that ranges that meet two segments get fewer (heads of 128, 256 lists of 4096 keys: 94 us with 0 of them, 90
 // with 3, 89.6 with 6, 90 with 10; 40 lists of 5000: 37.1, 34.0, 33.2, 33.8. Heads of 256, 4 x 64 drafts, 16 heads over 2,
-// 8700 to 13600 keys: 95 with 10, 90 with 13, as a piece writes 128 columns of 256).
+// 8700 to 13600 keys: 95 with 10, 90 with 13, as a piece writes 128 columns of 256; trees of fewer columns, whose pieces
+// write less, have the same weight and were not timed with another).
 constexpr uint32_t lead_of(int dim) { return dim == 256 ? 13 : 6; }
 template <int D>
 struct SegUnits {
