@@ -309,6 +309,114 @@ int mako_cache_evict(const mako_evict_args* a, mako_dtype in, void* k, void* v, 
                      void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * A cache kept in pages (no counterpart in the reference). Pages hold `page` rows (a power of two, 64 to 4096) of every kv
+ * head: k and v [pages][kv_heads][page][dim], so a page of a kv head is one run of memory. A sequence's pages are a row of
+ * table u32 [batch][max_pages], in the order of its rows: row j of sequence b is row j % page of page table[b][j / page];
+ * an entry at or past `pages` is no page (the library writes 0xffffffff). Any number of sequences may hold a page: refs u32
+ * [pages] counts the holders, 0 for a free page. ctx_len u32 [batch] are the sequences' rows. The new rows of a step lie one
+ * sequence after another: those of sequence b are rows starts[b] .. starts[b + 1] (starts u32 [batch + 1], not falling; rows
+ * from starts[batch] on are no sequence's; starts past `rows` count as `rows`; starts NULL: one row each, row b). They
+ * become the cache rows ctx_len[b], ctx_len[b] + 1, ... All of these are in device memory, and no call waits for the host. A
+ * step of a batch is mako_pages_reserve, then for each layer mako_pages_write and mako_attn_paged.
+ */
+
+/*
+ * Attention of the sequences' new tokens, one or a chunk of each, over pages that hold them already (mako_pages_write):
+ * new row i of sequence b sees the cache rows up to its own, [0, ctx_len[b] + i]. q [heads][q_pad][dim] and o [rows][width]
+ * by new row, lse [heads][rows] (may be NULL); rows of o and lse that are no sequence's are left as they were, and so are a
+ * sequence's from max_new on. max_new bounds the new rows of a sequence and max_ctx the rows it holds with them
+ * (max_ctx <= max_pages * page): cache rows from max_ctx on are not seen, and a loose bound costs time and workspace only. A
+ * page that the table does not name reads as rows of zeros. What pages hold behind a sequence's last row, and pages that its
+ * table does not name in it, have no part, whatever they hold; a v that is not finite among a sequence's own new rows may
+ * make rows before it in its 64 rows (counted from the sequence's start) not finite.
+ * dim 64, 128 or 256. Precision as mako_attn_fwd: P rounded to the input type for P V, sums and lse of the f32
+ * exponentials; rows that see fewer than 64 keys get bf16 probabilities to ~16 bits. workspace: at least
+ * mako_attn_paged_workspace(a) bytes, 16-byte aligned; its contents do not matter, and calls that overlap in time need
+ * separate ones. width a multiple of 4; o must not overlap the inputs.
+ */
+typedef struct mako_paged_args {
+    uint32_t batch;     /* sequences */
+    uint32_t rows;      /* rows of o, and of a query head that may be used */
+    uint32_t q_pad;     /* rows of a query head in q (>= rows) */
+    uint32_t heads, kv_heads;
+    uint32_t dim;       /* 64, 128 or 256 */
+    uint32_t pages;     /* pages of the pool */
+    uint32_t page;      /* rows a page */
+    uint32_t max_pages; /* entries of a table row */
+    uint32_t max_new;   /* an upper bound on the new rows of a sequence */
+    uint32_t max_ctx;   /* an upper bound on the rows that a sequence holds, the new ones among them */
+    uint32_t width;     /* o row length in elements (>= heads * dim) */
+    float scale;
+} mako_paged_args;
+
+size_t mako_attn_paged_workspace(const mako_paged_args* a);
+int mako_attn_paged(const mako_paged_args* a, mako_dtype in, mako_dtype out, const void* q, const void* k, const void* v,
+                    const uint32_t* table, const uint32_t* starts, const uint32_t* ctx_len, void* o, float* lse,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* What the calls that keep the pages share; values are moved as they are, f16 or bf16. */
+typedef struct mako_pages_args {
+    uint32_t batch;     /* sequences */
+    uint32_t rows;      /* new rows of all sequences together, at most (write, reserve) */
+    uint32_t d_pad;     /* rows of a kv head in kd and vd (>= rows; write) */
+    uint32_t pages, page, max_pages;
+    uint32_t kv_heads, dim; /* dim 64, 128 or 256 (write, and where k and v are given) */
+    uint32_t layers;    /* layers whose pools k and v hold, one after another (reserve, compact) */
+} mako_pages_args;
+
+/*
+ * Writes the new rows into their pages: row starts[b] + i of kd and vd [kv_heads][d_pad][dim] (the tiles mako_heads writes)
+ * becomes row ctx_len[b] + i of sequence b in k and v, for every kv head. Rows that have no page, or that lie at or past
+ * end[b] (end NULL: no such bound; mako_pages_reserve's ctx_out says what has room), are dropped. kd and vd are not in k or v.
+ */
+int mako_pages_write(const mako_pages_args* a, const void* kd, const void* vd, const uint32_t* table,
+                     const uint32_t* starts, const uint32_t* ctx_len, const uint32_t* end, void* k, void* v, void* stream);
+
+/*
+ * Pages for the new rows: each entry of sequence b's table row that rows ctx_len[b] .. ctx_len[b] + n - 1 fall into (n:
+ * starts[b + 1] - starts[b]) gets a free page where it has none, in the order of sequences and rows, the free pages of the
+ * lowest numbers first. A last page that is partly filled and that others hold too is not written to: the sequence gets a
+ * page of its own there with its rows copied, in all layers (of sequences that append to one page which nobody else
+ * holds, the last one keeps it, whether the others get theirs or not). refs_out: 1 for the pages given, one holder fewer for the pages left. When the free pages run out,
+ * the later entries get none; ctx_out[b] is the number of rows that have room (ctx_len[b] + n, or fewer): rows from it on
+ * are not to be written (mako_pages_write's end). k and v [layers][pages][kv_heads][page][dim], or both NULL where no page
+ * can be shared or the caller copies. table_out may be table, refs_out refs and ctx_out ctx_len (where mako_pages_write and
+ * mako_attn_paged still get the rows before); with other arrays the call can be made again. At most 4096 sequences.
+ * workspace: at least mako_pages_reserve_workspace(a) bytes, 16-byte aligned.
+ */
+size_t mako_pages_reserve_workspace(const mako_pages_args* a);
+int mako_pages_reserve(const mako_pages_args* a, const uint32_t* table, const uint32_t* refs, const uint32_t* starts,
+                       const uint32_t* ctx_len, uint32_t* table_out, uint32_t* refs_out, uint32_t* ctx_out, void* k,
+                       void* v, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Sequences go on from others, end, or are cut back: new sequence i holds the first min(keep[i], ctx_len[p]) rows of the old
+ * sequence p = parent[i] (parent NULL: i; at or past batch: no rows; keep NULL: all of them), by sharing its pages; table_out
+ * has no page behind them. ctx_out[i] is their number. refs_out[p] = refs[p] + the holders in table_out - those in table: a
+ * page that nobody holds any more is free, and a caller may count itself a holder of pages that are to stay. No row moves: a
+ * partly filled page that is shared is copied when a sequence appends to it (mako_pages_reserve). refs_out may be refs.
+ * table_out may be table and ctx_out ctx_len (both or neither), with a workspace of mako_pages_fork_workspace(a) bytes,
+ * 16-byte aligned; with other arrays it may be NULL.
+ */
+size_t mako_pages_fork_workspace(const mako_pages_args* a);
+int mako_pages_fork(const mako_pages_args* a, const uint32_t* parent, const uint32_t* keep, const uint32_t* table,
+                    const uint32_t* refs, const uint32_t* ctx_len, uint32_t* table_out, uint32_t* refs_out,
+                    uint32_t* ctx_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Moves the used pages (refs > 0) to the lowest numbers, 0 .. used - 1, so that the rest of the pool is one free run: the
+ * i-th used page from `used` on goes to the i-th free page below it, in all layers of k and v [layers][pages][kv_heads]
+ * [page][dim] (both NULL: the tables alone); the others stay where they are. table_out and refs_out follow; used_out[0] =
+ * used; map_out (u32 [pages], may be NULL): the new number of each used page, 0xffffffff for a free one. Entries of the
+ * table that name a free page become 0xffffffff. table_out may be table and refs_out refs; with other arrays the call can
+ * be made again. workspace: at least mako_pages_compact_workspace(a) bytes, 16-byte aligned.
+ */
+size_t mako_pages_compact_workspace(const mako_pages_args* a);
+int mako_pages_compact(const mako_pages_args* a, const uint32_t* table, const uint32_t* refs, uint32_t* table_out,
+                       uint32_t* refs_out, uint32_t* used_out, uint32_t* map_out, void* k, void* v, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
  * Head tiles from fp32 rows: head h of token t, x[t][col0 + h * stride .. + dim), written as y row
  * [h][row0 + t][dim] in f16 (the reference's half tiles) or bf16, optionally RMS-normed (times w) and then rotated by
  * the angle table cs. One call stands for each of the reference's tile producers (src/kernels/ops.metal:11-52,

@@ -22,7 +22,10 @@ EXPORTS = ("mako_attn_abi_version", "mako_last_error", "mako_attn_fwd", "mako_cu
            "mako_kda_scan_ws", "mako_attn_fwd_workspace", "mako_attn_fwd_ws", "mako_attn_sparse_workspace",
            "mako_attn_sparse_ws", "mako_attn_fwd_rows_workspace", "mako_attn_fwd_rows_ws", "mako_attn_release",
            "mako_attn_held_bytes", "mako_attn_tree_workspace", "mako_attn_tree", "mako_cache_append",
-           "mako_cache_weights_workspace", "mako_cache_weights", "mako_cache_evict_workspace", "mako_cache_evict")
+           "mako_cache_weights_workspace", "mako_cache_weights", "mako_cache_evict_workspace", "mako_cache_evict",
+           "mako_attn_paged_workspace", "mako_attn_paged", "mako_pages_write", "mako_pages_reserve_workspace",
+           "mako_pages_reserve", "mako_pages_fork_workspace", "mako_pages_fork", "mako_pages_compact_workspace",
+           "mako_pages_compact")
 
 
 class AttnArgs(ctypes.Structure):
@@ -58,6 +61,17 @@ class WeightsArgs(ctypes.Structure):
 class EvictArgs(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint32) for n in ("batch", "kv_heads", "dim", "cap", "max_ctx", "budget", "recent",
                                                "sinks")]
+
+
+class PagedArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("batch", "rows", "q_pad", "heads", "kv_heads", "dim", "pages", "page",
+                                               "max_pages", "max_new", "max_ctx", "width")] + \
+        [("scale", ctypes.c_float)]
+
+
+class PagesArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("batch", "rows", "d_pad", "pages", "page", "max_pages", "kv_heads", "dim",
+                                               "layers")]
 
 
 class HeadsArgs(ctypes.Structure):
@@ -151,7 +165,21 @@ def lib():
         L.mako_cache_evict_workspace.argtypes = [ctypes.POINTER(EvictArgs)]
         L.mako_cache_evict_workspace.restype = SZ
         L.mako_cache_evict.argtypes = [ctypes.POINTER(EvictArgs), I] + [P] * 10 + [SZ, P]
-        for name in ("mako_attn_tree", "mako_cache_append", "mako_cache_weights", "mako_cache_evict",
+        L.mako_attn_paged_workspace.argtypes = [ctypes.POINTER(PagedArgs)]
+        L.mako_attn_paged_workspace.restype = SZ
+        L.mako_attn_paged.argtypes = [ctypes.POINTER(PagedArgs), I, I] + [P] * 9 + [SZ, P]
+        L.mako_pages_write.argtypes = [ctypes.POINTER(PagesArgs)] + [P] * 9
+        L.mako_pages_reserve_workspace.argtypes = [ctypes.POINTER(PagesArgs)]
+        L.mako_pages_reserve_workspace.restype = SZ
+        L.mako_pages_reserve.argtypes = [ctypes.POINTER(PagesArgs)] + [P] * 10 + [SZ, P]
+        L.mako_pages_fork_workspace.argtypes = [ctypes.POINTER(PagesArgs)]
+        L.mako_pages_fork_workspace.restype = SZ
+        L.mako_pages_fork.argtypes = [ctypes.POINTER(PagesArgs)] + [P] * 9 + [SZ, P]
+        L.mako_pages_compact_workspace.argtypes = [ctypes.POINTER(PagesArgs)]
+        L.mako_pages_compact_workspace.restype = SZ
+        L.mako_pages_compact.argtypes = [ctypes.POINTER(PagesArgs)] + [P] * 9 + [SZ, P]
+        for name in ("mako_attn_paged", "mako_pages_write", "mako_pages_reserve", "mako_pages_fork",
+                     "mako_pages_compact", "mako_attn_tree", "mako_cache_append", "mako_cache_weights", "mako_cache_evict",
                      "mako_attn_fwd", "mako_cube_select", "mako_attn_sparse", "mako_attn_decode",
                      "mako_attn_decode_noalloc", "mako_heads", "mako_attn_fwd_rows", "mako_attn_fwd_ws",
                      "mako_attn_sparse_ws", "mako_attn_fwd_rows_ws", "mako_attn_release",
@@ -368,6 +396,74 @@ def cache_evict(a, k, v, w, ctx_len, w_out, pos_out, ctx_out, workspace, *, pos=
     _check(lib().mako_cache_evict(ctypes.byref(a), dtype_code(k), _ptr(k), _ptr(v), _ptr(w), _ptr(pos), _ptr(seen),
                                   _ptr(ctx_len), _ptr(w_out), _ptr(pos_out), _ptr(ctx_out), _ptr(workspace),
                                   _nbytes(workspace), _stream(stream)))
+
+
+def paged_args(*, batch, rows, heads, kv_heads, dim, pages, page, max_pages, max_new, max_ctx, q_pad=None, width=None,
+               scale=None):
+    return PagedArgs(batch, rows, rows if q_pad is None else q_pad, heads, kv_heads, dim, pages, page, max_pages,
+                     max_new, max_ctx, heads * dim if width is None else width,
+                     1.0 / dim ** 0.5 if scale is None else scale)
+
+
+def attn_paged_workspace(a):
+    return lib().mako_attn_paged_workspace(ctypes.byref(a))
+
+
+def attn_paged(a, q, k, v, table, ctx_len, o, workspace, *, starts=None, lse=None, stream=None):
+    """mako_attn_paged on torch tensors: q [heads][q_pad][dim], k, v [pages][kv_heads][page][dim], table int32
+    [batch][max_pages], ctx_len int32 [batch], starts int32 [batch + 1] (all read as u32), o [rows][width], lse float32
+    [heads][rows]."""
+    _check(lib().mako_attn_paged(ctypes.byref(a), dtype_code(q), dtype_code(o), _ptr(q), _ptr(k), _ptr(v), _ptr(table),
+                                 _ptr(starts), _ptr(ctx_len), _ptr(o), _ptr(lse), _ptr(workspace), _nbytes(workspace),
+                                 _stream(stream)))
+
+
+def pages_args(*, batch, pages, page, max_pages, rows=0, kv_heads=0, dim=0, layers=1, d_pad=None):
+    return PagesArgs(batch, rows, rows if d_pad is None else d_pad, pages, page, max_pages, kv_heads, dim, layers)
+
+
+def pages_write(a, kd, vd, k, v, table, ctx_len, *, starts=None, end=None, stream=None):
+    """mako_pages_write on torch tensors: kd, vd [kv_heads][d_pad][dim], k, v [pages][kv_heads][page][dim], table int32
+    [batch][max_pages], ctx_len and end int32 [batch], starts int32 [batch + 1]."""
+    _check(lib().mako_pages_write(ctypes.byref(a), _ptr(kd), _ptr(vd), _ptr(table), _ptr(starts), _ptr(ctx_len),
+                                  _ptr(end), _ptr(k), _ptr(v), _stream(stream)))
+
+
+def pages_reserve_workspace(a):
+    return lib().mako_pages_reserve_workspace(ctypes.byref(a))
+
+
+def pages_reserve(a, k, v, table, refs, ctx_len, table_out, refs_out, ctx_out, workspace, *, starts=None, stream=None):
+    """mako_pages_reserve on torch tensors: k, v [layers][pages][kv_heads][page][dim] or None, table and table_out int32
+    [batch][max_pages], refs and refs_out int32 [pages], ctx_len and ctx_out int32 [batch], starts int32 [batch + 1]."""
+    _check(lib().mako_pages_reserve(ctypes.byref(a), _ptr(table), _ptr(refs), _ptr(starts), _ptr(ctx_len),
+                                    _ptr(table_out), _ptr(refs_out), _ptr(ctx_out), _ptr(k), _ptr(v), _ptr(workspace),
+                                    _nbytes(workspace), _stream(stream)))
+
+
+def pages_fork_workspace(a):
+    return lib().mako_pages_fork_workspace(ctypes.byref(a))
+
+
+def pages_fork(a, table, refs, ctx_len, table_out, refs_out, ctx_out, workspace=None, *, parent=None, keep=None,
+               stream=None):
+    """mako_pages_fork on torch tensors: table and table_out int32 [batch][max_pages], refs and refs_out int32 [pages],
+    ctx_len, ctx_out, parent and keep int32 [batch]."""
+    _check(lib().mako_pages_fork(ctypes.byref(a), _ptr(parent), _ptr(keep), _ptr(table), _ptr(refs), _ptr(ctx_len),
+                                 _ptr(table_out), _ptr(refs_out), _ptr(ctx_out), _ptr(workspace), _nbytes(workspace),
+                                 _stream(stream)))
+
+
+def pages_compact_workspace(a):
+    return lib().mako_pages_compact_workspace(ctypes.byref(a))
+
+
+def pages_compact(a, k, v, table, refs, table_out, refs_out, used_out, workspace, *, map_out=None, stream=None):
+    """mako_pages_compact on torch tensors: k, v [layers][pages][kv_heads][page][dim] or None, table and table_out int32
+    [batch][max_pages], refs, refs_out and map_out int32 [pages], used_out int32 [1]."""
+    _check(lib().mako_pages_compact(ctypes.byref(a), _ptr(table), _ptr(refs), _ptr(table_out), _ptr(refs_out),
+                                    _ptr(used_out), _ptr(map_out), _ptr(k), _ptr(v), _ptr(workspace),
+                                    _nbytes(workspace), _stream(stream)))
 
 
 def window_random_blocks(n_blocks, lists, window=8, n_random=8, seed=0):
