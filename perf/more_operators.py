@@ -391,7 +391,7 @@ def _own(s):
     if not p:
         table = s["table"]
         rows = c["steps"] + c["chunks"] * c["new"] if "steps" in c else 0
-        a = M.pages_args(batch=table.shape[0], rows=rows, pages=c.get("pages", s["k"].shape[0] if "k" in s else 0),
+        a = M.pages_args(batch=table.shape[0], rows=rows, pages=c["pages"] if "pages" in c else s["k"].shape[0],
                          page=c["page"], max_pages=table.shape[1], kv_heads=c.get("kv", 0), dim=c.get("dim", 0),
                          layers=c.get("layers", 1))
         p.update(a=a)
