@@ -2,116 +2,345 @@
 //
 // Mathematics: new row i of sequence b sits at position c + i, c = ctx_len[b], and sees the cache rows j <= c + i:
 //   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  s_j = scale q.k_j,  lse = m + ln(sum),  m any bound
-// Row j is row j % page of page table[b][j / page].
+// Row j is row j % page of page table[b][j / page]. Sums over parts of the keys join by their log-sums.
 //
-// paged_simple: a workgroup a (row, head), 256 keys a round: a thread a key's score, the round's maximum and sum through
-// LDS, then a thread a head dim (and part of the keys) for the outputs. Every row reads all of its keys.
+// Bound: the matrix unit for chunks, the read of K and V for single tokens (64 keys of a kv head are 32 KiB at heads of 128,
+// 1.2 us of a CU's products for 64 rows of four heads: 7 TB/s over the chip, so the same stream serves both).
+//
+// * paged_rows runs the streams of flash_fwd_r64 (heads of 64 and 128) and flash_fwd_r32 (256) over pages
+//   (gen_attn_paged.py): a tile is 64 keys, a run of memory within a page; its page's number is read by a scalar load an
+//   iteration before the tile is staged.
+// * An item is a block of R rows of a sequence and `hq` heads of a kv head (4, 2 or 1, as they divide the group), R = 4 RW /
+//   hq: one workgroup's four waves. A group of more heads takes further workgroups (column blocks) on the same keys beside
+//   each other on an XCD, so that the second read hits its L2.
+// * Lengths are known on the device only, so every workgroup works out its share of the work (paged_split.hpp): ranges of
+//   equal cost over the items of all sequences, one a workgroup.
+// * A piece of an item leaves normalised f32 rows and their log-sums at slot 2 range (+ 1 if the item starts in it): a range
+//   has at most one of each kind. The range with an item's last piece names its first one, and paged_merge joins them.
+//   Contexts that are too short for a second launch (max_ctx) take whole items and none.
 #include <algorithm>
 
-#include "pages_common.hpp"
-#include "split_ranges.hpp"
+#include "attn_paged_asm.inc"
+#include "fwd64_common.hpp"
+#include "paged_split.hpp"
 
 namespace mako {
 namespace {
 
-struct PagedParams {
+constexpr uint32_t kNone = 0xffffffffu;
+
+struct PagedParams : PagedSplit {
     const void *q, *k, *v;
-    const uint32_t *table, *starts, *ctx;
+    const uint32_t* table;
     void* o;
     float* lse;
-    uint32_t batch, rows, q_pad, heads, kv_heads, group, pages, shift, max_pages, max_new, max_ctx, width;
+    float* part_o;    // [ranges][ncb][2][slot_rows][hq][D]: pieces' normalised rows
+    float* part_l;    // [ranges][ncb][2][hq][slot_rows]: their log-sums
+    uint32_t* whole;  // [ranges][2]: which of a range's pieces there are
+    u32x4* last;      // [ranges]: the item whose last piece a range has: first range, first row of o, rows, kv head (first kNone: none)
+    uint32_t q_pad, group, pages, page_bytes, shift, max_pages, width, hq, ncb, slot_rows;
     float scale_log2;
 };
 
-template <class T, class TO, int D>
-__global__ __launch_bounds__(256) void paged_simple(const PagedParams p)
+__device__ __forceinline__ uint64_t uniform64(uint64_t x)
 {
-    __shared__ float s_q[D], s_p[256], s_red[4], s_o[256];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, w = tid >> 6;
-    const uint32_t r = blockIdx.x / p.heads, h = blockIdx.x % p.heads, kvh = h / p.group;
-    uint32_t seq = r;
-    if (p.starts) {
-        seq = 0;
-        for (uint32_t i = 0; i < p.batch; i += 64)
-            seq += __popcll(__ballot(i + lane < p.batch && p.starts[i + lane + 1] <= r));
-    }
-    if (seq >= p.batch)
-        return;
-    const NewRows nr = new_rows(p.starts, p.rows, seq);
-    if (r < nr.s0 || r - nr.s0 >= min(nr.n, p.max_new))
-        return;
-    const uint32_t n_k = min(min(p.ctx[seq], p.max_ctx) + (r - nr.s0) + 1, p.max_ctx);
-    const uint32_t* table = p.table + (size_t)seq * p.max_pages;
-    const auto row_of = [&](uint32_t j, bool& has) {
-        const uint32_t page = table[j >> p.shift];
-        has = page < p.pages;
-        return ((((size_t)page * p.kv_heads + kvh) << p.shift) + (j & ((1u << p.shift) - 1))) * D;
+    return (uint64_t)uniform((uint32_t)(x >> 32)) << 32 | uniform((uint32_t)x);
+}
+
+// What a piece is to the streams: tiles [ta, tb) of a sequence, rows `rows` of its block from position p0 on.
+struct Piece {
+    const void *q, *k, *v;  // of the block's first row and this wave's head; of the kv head in page 0
+    void* o;                // of the block's first row and the wave's first head column
+    float* l;               // of the block's first row and the wave's head
+    uint64_t table;         // the sequence's row
+    uint32_t ta, tb, rows, p0, keys;  // keys: those of the block's last row
+    uint32_t seen;                    // keys of the sequence: no row sees more
+    uint32_t o_row, l_bytes;          // bytes of a row of o; of l that may be written
+};
+
+template <class T, class TO, int D>
+__device__ __forceinline__ void run_piece(const PagedParams& p, unsigned char* lds, const Piece& x)
+{
+    constexpr bool kWide = D == 256;
+    constexpr uint32_t RW = kWide ? 32 : 64, NBUF = kWide ? 2 : kNBuf;
+    constexpr uint32_t kKRowB = 2 * D + 16, kKTileB = 64 * kKRowB, kVRowB = 2 * D, kVTileB = 64 * kVRowB;
+    constexpr uint32_t NKP = (kKTileB / 1024 - 1) / 4;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, g = lane >> 5, c32 = lane & 31u, w = uniform(tid >> 6);
+    const uint32_t q0 = w / p.hq * RW;  // this wave's first row in the block
+    const uint32_t ks = 64 * x.ta, n_keys = min(64 * x.tb, x.keys) - ks;
+    const uint32_t lim_w = x.p0 + min(q0 + RW, x.rows);  // (position of the wave's last row) + 1
+    const uint32_t w_keys = q0 < x.rows ? min(n_keys, min(lim_w, x.seen) - ks) : 0u;
+    const uint32_t nt = x.tb - x.ta, ntw = (w_keys + 63) / 64;
+    // keys that a row sees, counted from the piece's first one: lmin the wave's first row, lim0 and lim1 the lane's
+    const uint32_t r0 = x.p0 + q0;
+    const uint32_t lmin = min(r0 + 1, x.seen) - ks;
+    const uint32_t lim0 = min(r0 + c32 + 1, x.seen) - ks - 8 * g;
+
+    // LDS addresses, staging and epilogue: as flash_fwd_r64 and flash_fwd_r32 have them.
+    const uint32_t lbase = (uint32_t)reinterpret_cast<uintptr_t>(lds), vbase = lbase + NBUF * kKTileB;
+    uint32_t kr = lbase + c32 * kKRowB + 16 * g;
+    const uint32_t th = (lane >> 4) & 1u, ti = lane & 15u;
+    const uint32_t vrow = vbase + (8 * g + ti / 4) * kVRowB + 8 * (ti % 4);
+    auto kd_of = [&](uint32_t i) {
+        const uint32_t by = 1024 * i + 16 * lane, row = by / kKRowB, ch = by % kKRowB / 16;
+        return slot_of(row) * (2 * D) + 16 * (ch < D / 8 ? ch : 0);
     };
-    if (tid < D)
-        s_q[tid] = (float)static_cast<const T*>(p.q)[((size_t)h * p.q_pad + r) * D + tid];
-    constexpr uint32_t kParts = 256 / D;
-    const uint32_t d = tid % D, part = tid / D;
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    for (uint32_t j0 = 0; j0 < n_k; j0 += 256) {
-        __syncthreads();
-        float x = -INFINITY;
-        if (j0 + tid < n_k) {
-            bool has;
-            const size_t at = row_of(j0 + tid, has);
-            x = 0.0f;
-            if (has)
-                for (int i = 0; i < D; ++i)
-                    x += s_q[i] * (float)static_cast<const T*>(p.k)[at + i];
-            x *= p.scale_log2;
-        }
-        float mx = x;
-        for (int i = 32; i; i >>= 1)
-            mx = fmaxf(mx, __shfl_xor(mx, i));
-        if (lane == 0)
-            s_red[w] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-        const float nm = fmaxf(m, mx), mu = nm == -INFINITY ? 0.0f : nm, f = m == -INFINITY ? 0.0f : exp2_fast(m - mu);
-        m = nm;
-        const float e = exp2_fast(x - mu);
-        s_p[tid] = e;
-        float sum = e;
-        for (int i = 32; i; i >>= 1)
-            sum += __shfl_xor(sum, i);
-        __syncthreads();
-        if (lane == 0)
-            s_red[w] = sum;
-        __syncthreads();
-        l = l * f + ((s_red[0] + s_red[1]) + (s_red[2] + s_red[3]));
-        acc *= f;
-        for (uint32_t j = part; j < 256 && j0 + j < n_k; j += kParts) {
-            bool has;
-            const size_t at = row_of(j0 + j, has);
-            if (has)
-                acc += s_p[j] * (float)static_cast<const T*>(p.v)[at + d];
-        }
+    const uint32_t skw = uniform(lbase), skww = uniform(lbase + 1024 * w), svww = uniform(vbase + (kVTileB / 4) * w);
+    const uint32_t qo = ((q0 + c32) * D + 8 * g) * 2;
+    constexpr uint32_t so = sizeof(TO), orow = D * so, lpr = orow / 16;
+    const uint32_t obase = lbase + w * RW * orow;
+    const uint32_t ew = so == 4 ? obase + c32 * orow + 16 * ((c32 & 7u) ^ g)
+                                : obase + c32 * orow + 8 * g + 16 * (c32 & 7u);
+    const uint32_t er = obase + (lane / lpr) * orow + 16 * ((lane % lpr) ^ (lane / lpr));
+    const uint32_t og = (q0 + lane / lpr) * x.o_row + 16 * (lane % lpr);
+    const uint32_t ogs = uniform((64 / lpr) * x.o_row);
+    const uint32_t lo0 = q0 + c32 < x.rows ? (q0 + c32) * 4 : kNone;
+    const uint32_t swp = (lane ^ 32) * 4;
+    const u32x4 qrs = rsrc_of(x.q, x.rows * 2 * D), ors = rsrc_of(x.o, (x.rows - 1) * x.o_row + orow);
+    const u32x4 lrs = rsrc_of(x.l, x.l ? x.l_bytes : 0);
+    const uint32_t has_lse = uniform(x.l ? 1u : 0u);
+    const float c = __builtin_bit_cast(float, uniform(__builtin_bit_cast(uint32_t, p.scale_log2)));
+    const uint32_t s_nt = uniform(nt), s_ntw = uniform(ntw), s_lmin = uniform(lmin), kn = uniform(n_keys * 2 * D);
+    const uint64_t kb = reinterpret_cast<uint64_t>(x.k), vb = reinterpret_cast<uint64_t>(x.v);
+    const uint32_t kb0 = uniform((uint32_t)kb), kb1 = uniform((uint32_t)(kb >> 32) & 0xffffu);
+    const uint32_t vb0 = uniform((uint32_t)vb), vb1 = uniform((uint32_t)(vb >> 32) & 0xffffu);
+    const uint32_t pshift = p.shift - 6;
+    const uint32_t* row = reinterpret_cast<const uint32_t*>(x.table);
+    const auto page_of = [&](uint32_t t) { return uniform(row[min(t, x.tb - 1) >> pshift]); };
+    const uint32_t pg0 = page_of(x.ta), pg1 = page_of(x.ta + 1), pg2 = page_of(x.ta + 2), pg3 = page_of(x.ta + 3);
+    const uint64_t ent = uniform64(x.table);
+    const uint32_t t0 = uniform(x.ta), tlast = uniform(x.tb - 1), npages = uniform(p.pages);
+    const uint32_t pstride = uniform(p.page_bytes), pmask = uniform((1u << pshift) - 1), s_pshift = uniform(pshift);
+
+#define MAKO_PAGED_SCALARS                                                                                        \
+    [qrs] "s"(qrs), [ors] "s"(ors), [lrs] "s"(lrs), [c] "s"(c), [nt] "s"(s_nt), [ntw] "s"(s_ntw), [lmin] "s"(s_lmin),  \
+        [has_lse] "s"(has_lse), [ogs] "s"(ogs), [kb0] "s"(kb0), [kb1] "s"(kb1), [kn] "s"(kn), [vb0] "s"(vb0),     \
+        [vb1] "s"(vb1), [skw] "s"(skw), [skww] "s"(skww), [svww] "s"(svww), [ent] "s"(ent), [t0] "s"(t0),          \
+        [tlast] "s"(tlast), [npages] "s"(npages), [pstride] "s"(pstride), [pmask] "s"(pmask), [pshift] "s"(s_pshift), \
+        [pg0] "s"(pg0), [pg1] "s"(pg1), [pg2] "s"(pg2)
+#define MAKO_PAGED_STREAM(NAME, OPERANDS)                                                                         \
+    do {                                                                                                          \
+        if constexpr (__is_same(T, __bf16)) {                                                                     \
+            if constexpr (__is_same(TO, float))                                                                   \
+                asm volatile(NAME##_BF16_F32 OPERANDS);                                                           \
+            else                                                                                                  \
+                asm volatile(NAME##_BF16_BF16 OPERANDS);                                                          \
+        } else {                                                                                                  \
+            if constexpr (__is_same(TO, float))                                                                   \
+                asm volatile(NAME##_F16_F32 OPERANDS);                                                            \
+            else                                                                                                  \
+                asm volatile(NAME##_F16_F16 OPERANDS);                                                            \
+        }                                                                                                         \
+    } while (0)
+
+    if constexpr (kWide) {
+        // r32's V image: the bytes a lane's slot holds, for pieces that start on a multiple of 4 rows and the others
+        const auto vunit = [](uint32_t u, uint32_t k) { return u ^ (k & 3u) ^ (4u * (u & 1u)); };
+        const auto vd_at = [&](uint32_t row0) {
+            const uint32_t by = 16 * lane, r = by / kVRowB, pos = by % kVRowB;
+            const uint32_t y = (pos / 32) ^ ((row0 + r) & 3u), u = y ^ (4u * (y & 1u));
+            return r * kVRowB + 32 * u + 16 * ((pos / 16) & 1u);
+        };
+        uint32_t vr0 = vrow + 32 * vunit(th, ti / 4), vr1 = vrow + 32 * vunit(2 + th, ti / 4);
+        uint32_t vr2 = vrow + 32 * vunit(4 + th, ti / 4), vr3 = vrow + 32 * vunit(6 + th, ti / 4);
+        const uint32_t kd0 = kd_of(w), kd1 = kd_of(w + 4), kd2 = kd_of(w + 8), kd3 = kd_of(w + 12);
+        const uint32_t kd4 = kd_of(w + 16), kd5 = kd_of(w + 20), kd6 = kd_of(w + 24), kd7 = kd_of(w + 28);
+        const uint32_t kd8 = kd_of(4 * NKP);
+        const uint32_t vd = (kVTileB / 4) * w + vd_at(0), vdo = (kVTileB / 4) * w + vd_at(2);
+        const uint32_t vd2 = vd + 4096, vdo2 = vdo + 4096;
+#define MAKO_PAGED_R32                                                                                            \
+    : [kr] "+v"(kr), [vr0] "+v"(vr0), [vr1] "+v"(vr1), [vr2] "+v"(vr2), [vr3] "+v"(vr3)                           \
+    : [kd0] "v"(kd0), [kd1] "v"(kd1), [kd2] "v"(kd2), [kd3] "v"(kd3), [kd4] "v"(kd4), [kd5] "v"(kd5),              \
+      [kd6] "v"(kd6), [kd7] "v"(kd7), [kd8] "v"(kd8), [vd] "v"(vd), [vdo] "v"(vdo), [vd2] "v"(vd2),                  \
+      [vdo2] "v"(vdo2), [lim0] "v"(lim0), [qo] "v"(qo), [lo0] "v"(lo0), [swp] "v"(swp), [ew] "v"(ew), [er] "v"(er),   \
+      [og] "v"(og), MAKO_PAGED_SCALARS                                                                            \
+    : MAKO_PAGED_D256_CLOBBERS, "vcc", "scc", "memory"
+        MAKO_PAGED_STREAM(MAKO_PAGED_D256, MAKO_PAGED_R32);
+    } else {
+        uint32_t vr0 = vrow + 32 * v_unit(th, ti / 4), vr1 = vrow + 32 * v_unit(2 + th, ti / 4);
+        const uint32_t kr0 = kr, lim1 = min(r0 + c32 + 33, x.seen) - ks - 8 * g;
+        const uint32_t lo1 = q0 + 32 + c32 < x.rows ? (q0 + 32 + c32) * 4 : kNone;
+        const uint32_t kd0 = kd_of(w), kd1 = kd_of(w + 4);
+        const uint32_t kd2 = NKP > 2 ? kd_of(w + 8) : 0u, kd3 = NKP > 3 ? kd_of(w + 12) : 0u, kd4 = kd_of(4 * NKP);
+        const uint32_t vd = (kVTileB / 4) * w + vd_of<D == 256 ? 128 : D>(lane);
+#define MAKO_PAGED_R64                                                                                            \
+    : [kr] "+v"(kr), [vr0] "+v"(vr0), [vr1] "+v"(vr1)                                                             \
+    : [kd0] "v"(kd0), [kd1] "v"(kd1), [kd2] "v"(kd2), [kd3] "v"(kd3), [kd4] "v"(kd4), [vd] "v"(vd),                \
+      [lim0] "v"(lim0), [lim1] "v"(lim1), [kr0] "v"(kr0), [qo] "v"(qo), [lo0] "v"(lo0), [lo1] "v"(lo1),            \
+      [swp] "v"(swp), [ew] "v"(ew), [er] "v"(er), [og] "v"(og), [pg3] "s"(pg3), MAKO_PAGED_SCALARS                 \
+    : MAKO_PAGED_CLOBBERS, "vcc", "scc", "memory"
+        if constexpr (D == 64)
+            MAKO_PAGED_STREAM(MAKO_PAGED_D64, MAKO_PAGED_R64);
+        else
+            MAKO_PAGED_STREAM(MAKO_PAGED_D128, MAKO_PAGED_R64);
     }
-    s_o[tid] = acc;
-    __syncthreads();
-    if (tid < D) {
-        for (uint32_t i = 1; i < kParts; ++i)
-            acc += s_o[i * D + tid];
-        static_cast<TO*>(p.o)[(size_t)r * p.width + (size_t)h * D + tid] = (TO)(l == 0.0f ? 0.0f : acc / l);
-        if (p.lse && tid == 0)
-            p.lse[(size_t)h * p.rows + r] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
+#undef MAKO_PAGED_R64
+#undef MAKO_PAGED_R32
+#undef MAKO_PAGED_STREAM
+#undef MAKO_PAGED_SCALARS
+    // every wave's stream has ended (its LDS reads landed) before the next piece's staging overwrites LDS
+    asm volatile("s_barrier" ::: "memory");
+}
+
+template <int D>
+constexpr uint32_t lds_bytes()
+{
+    return (D == 256 ? 2 : kNBuf) * (64 * (2 * D + 16) + 128 * D);
+}
+
+template <class T, class TO, int D>
+__global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams p)
+{
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[lds_bytes<D>()];
+    const uint32_t lane = threadIdx.x & 63u, w = uniform(threadIdx.x >> 6);
+    const uint32_t xcds = p.n_ranges % 8 == 0 ? 8 : 1;  // ranges side by side on an XCD, a range's column blocks too
+    const uint32_t at_xcd = blockIdx.x / xcds;
+    const uint32_t range = blockIdx.x % xcds * (p.n_ranges / xcds) + at_xcd / p.ncb, cb = at_xcd % p.ncb;
+
+    uint32_t here[2] = {0, 0};
+    u32x4 done = u32x4{kNone, 0, 0, 0};
+    walk_range(p, range, lane, [&](const PagedPiece& at) __attribute__((always_inline)) {
+        const uint32_t hl = w % p.hq, h = at.kvh * p.group + cb * p.hq + hl;
+        Piece x;
+        x.q = static_cast<const T*>(p.q) + ((size_t)h * p.q_pad + at.row0) * D;
+        x.k = static_cast<const T*>(p.k) + ((size_t)at.kvh << p.shift) * D;
+        x.v = static_cast<const T*>(p.v) + ((size_t)at.kvh << p.shift) * D;
+        x.table = reinterpret_cast<uint64_t>(p.table + (size_t)at.b * p.max_pages);
+        x.ta = at.ta, x.tb = at.tb, x.rows = at.rows, x.p0 = at.p0, x.keys = at.keys, x.seen = at.seen;
+        x.o = static_cast<TO*>(p.o) + (size_t)at.row0 * p.width + (size_t)h * D;
+        x.o_row = p.width * sizeof(TO);
+        x.l = p.lse ? p.lse + (size_t)h * p.rows + at.row0 : nullptr;
+        x.l_bytes = at.rows * 4;
+        if (at.part) {
+            const size_t slot = ((size_t)range * p.ncb + cb) * 2 + at.kind;
+            x.o = p.part_o + (slot * p.slot_rows * p.hq + hl) * D;
+            x.o_row = p.hq * D * 4;
+            x.l = p.part_l + (slot * p.hq + hl) * p.slot_rows;
+            here[at.kind] = 1;
+            if (at.first != kNone)
+                done = u32x4{at.first, at.row0, at.rows, at.kvh};
+        }
+        if (at.part || __is_same(TO, float))
+            run_piece<T, float, D>(p, lds, x);
+        else
+            run_piece<T, TO, D>(p, lds, x);
+    });
+    if (!p.direct && cb == 0 && threadIdx.x == 0) {
+        p.whole[2 * range] = here[0];
+        p.whole[2 * range + 1] = here[1];
+        p.last[range] = done;
     }
 }
 
-template <class T, class TO>
-void launch_dim(const PagedParams& p, uint32_t dim, uint32_t groups, hipStream_t s)
+// The pieces of the item whose last one range r has: their normalised rows weighted by exp(their log-sum - the largest), D / 4
+// lanes a (row, head), four head dims each. As merge_pieces (attn_fwd64.hip), a piece with a log-sum of -inf is added with
+// weight 0, so that NaN reaches the result whichever piece it is in; a row of NaN throughout gives -inf.
+template <class TO, int D>
+__global__ __launch_bounds__(256) void paged_merge(const PagedParams p, uint32_t per)
 {
-    const dim3 grid(groups), block(256);
+    const uint32_t r = blockIdx.x / per, sub = blockIdx.x % per;
+    const u32x4 item = p.last[r];
+    if (item[0] == kNone)
+        return;
+    const uint32_t t = sub * (1024 / D) + threadIdx.x / (D / 4), d = 4 * (threadIdx.x % (D / 4));
+    const uint32_t hl = t % p.hq, cb = t / p.hq % p.ncb, row = t / p.hq / p.ncb;
+    if (row >= item[2])
+        return;
+    constexpr uint32_t U = 4;  // pieces whose loads are in flight together
+    float mx = -INFINITY, sum = 0.0f;
+    f32x4 acc = f32x4{};
+    for (uint32_t i0 = item[0]; i0 <= r; i0 += U) {
+        float l[U];
+        f32x4 v[U];
+        #pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t i = i0 + u, kind = i == item[0] ? 1 : 0;
+            const bool has = i <= r && p.whole[2 * min(i, r) + kind];
+            const size_t slot = ((size_t)min(i, r) * p.ncb + cb) * 2 + kind;
+            l[u] = has ? p.part_l[(slot * p.hq + hl) * p.slot_rows + row] : -INFINITY;
+            v[u] = has ? *reinterpret_cast<const f32x4*>(p.part_o + ((slot * p.slot_rows + row) * p.hq + hl) * D + d) : f32x4{};
+        }
+        #pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            if (l[u] == -INFINITY) {  // (the same in a row's lanes)
+                const uint64_t nan = __ballot(v[u][0] != v[u][0] && v[u][1] != v[u][1] && v[u][2] != v[u][2] && v[u][3] != v[u][3]);
+                const uint64_t lanes = D == 256 ? ~0ull : ((1ull << (D / 4 % 64)) - 1) << (threadIdx.x & 63u & ~(D / 4 - 1));
+                acc += v[u] * 0.0f;
+                if ((nan & lanes) == lanes)
+                    sum = NAN;
+                continue;
+            }
+            const float m = fmaxf(mx, l[u]);
+            const float a = exp2_fast((mx - m) * kLog2e), b = exp2_fast((l[u] - m) * kLog2e);
+            sum = sum * a + b;
+            acc = acc * a + v[u] * b;
+            mx = m;
+        }
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const uint32_t h = item[3] * p.group + cb * p.hq + hl, at = item[1] + row;
+    store4<TO>(static_cast<TO*>(p.o) + (size_t)at * p.width + (size_t)h * D + d, acc[0] * inv, acc[1] * inv, acc[2] * inv,
+               acc[3] * inv);
+    if (p.lse && d == 0)
+        p.lse[(size_t)h * p.rows + at] = sum > 0.0f ? mx + __log2f(sum) * kLn2 : -INFINITY;
+}
+
+// A call's split, from its sizes alone (lengths are known on the device only).
+struct Plan {
+    uint32_t hq, rshift, ncb, n_ranges, slot_rows, direct;
+};
+constexpr uint32_t kDirectTiles = 8;
+
+Plan plan_of(const mako_paged_args* a, uint32_t cus)
+{
+    const uint32_t group = a->heads / a->kv_heads;
+    Plan pl{};
+    pl.hq = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+    pl.rshift = log2_of((a->dim == 256 ? 128 : 256) / pl.hq);
+    pl.ncb = group / pl.hq;
+    pl.n_ranges = std::max(1u, cus / pl.ncb);
+    if (pl.n_ranges > 8)
+        pl.n_ranges &= ~7u;
+    pl.slot_rows = std::min(1u << pl.rshift, a->max_new);
+    pl.direct = (a->max_ctx + 63) / 64 <= kDirectTiles;
+    return pl;
+}
+size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+size_t part_o_bytes(const Plan& pl, uint32_t dim)
+{
+    return round256((size_t)pl.n_ranges * pl.ncb * 2 * pl.slot_rows * pl.hq * dim * 4);
+}
+size_t part_l_bytes(const Plan& pl) { return round256((size_t)pl.n_ranges * pl.ncb * 2 * pl.slot_rows * pl.hq * 4); }
+size_t workspace_for(const Plan& pl, uint32_t dim)
+{
+    return pl.direct ? 0 : part_o_bytes(pl, dim) + part_l_bytes(pl) + (size_t)pl.n_ranges * 24;
+}
+
+template <class T, class TO, int D>
+void launch(const PagedParams& p, hipStream_t s)
+{
+    hipLaunchKernelGGL((paged_rows<T, TO, D>), dim3(p.n_ranges * p.ncb), dim3(256), 0, s, p);
+    if (p.direct)
+        return;
+    const uint32_t per = (p.slot_rows * p.group * D + 1023) / 1024;
+    hipLaunchKernelGGL((paged_merge<TO, D>), dim3(p.n_ranges * per), dim3(256), 0, s, p, per);
+}
+
+template <class T, class TO>
+void launch_dim(const PagedParams& p, uint32_t dim, hipStream_t s)
+{
     if (dim == 64)
-        hipLaunchKernelGGL((paged_simple<T, TO, 64>), grid, block, 0, s, p);
+        launch<T, TO, 64>(p, s);
     else if (dim == 128)
-        hipLaunchKernelGGL((paged_simple<T, TO, 128>), grid, block, 0, s, p);
+        launch<T, TO, 128>(p, s);
     else
-        hipLaunchKernelGGL((paged_simple<T, TO, 256>), grid, block, 0, s, p);
+        launch<T, TO, 256>(p, s);
+}
+
+bool valid(const mako_paged_args* a)
+{
+    return a && a->heads && a->kv_heads && a->heads % a->kv_heads == 0 && a->batch && a->max_new &&
+           (a->dim == 64 || a->dim == 128 || a->dim == 256);
 }
 
 int check_args(const mako_paged_args* a, mako_dtype in, mako_dtype out, const void* q, const void* k, const void* v,
@@ -158,32 +387,46 @@ int check_args(const mako_paged_args* a, mako_dtype in, mako_dtype out, const vo
 
 using namespace mako;
 
-extern "C" size_t mako_attn_paged_workspace(const mako_paged_args*) { return 0; }
+extern "C" size_t mako_attn_paged_workspace(const mako_paged_args* a)
+{
+    const uint32_t cus = device_cus();
+    return valid(a) && cus ? workspace_for(plan_of(a, cus), a->dim) : 0;
+}
 
 extern "C" int mako_attn_paged(const mako_paged_args* a, mako_dtype in, mako_dtype out, const void* q, const void* k,
                                const void* v, const uint32_t* table, const uint32_t* starts, const uint32_t* ctx_len,
-                               void* o, float* lse, void*, size_t, void* stream)
+                               void* o, float* lse, void* workspace, size_t workspace_bytes, void* stream)
 {
     const char* what = "attention_paged";
     if (const int rc = check_args(a, in, out, q, k, v, table, starts, ctx_len, o))
         return rc;
-    if (!a->batch || !a->max_new)
+    if (!a->batch || !a->max_new || !a->max_ctx)
         return ok();
-    const uint32_t rows = starts ? a->rows : a->batch;
-    if (!grid_fits((uint64_t)rows * a->heads, 256))
-        return fail(MAKO_EINVAL, "%s: %u rows of %u heads exceed the grid", what, rows, a->heads);
-    const PagedParams p{q, k, v, table, starts, ctx_len, o, lse, a->batch, a->rows, a->q_pad, a->heads, a->kv_heads,
-                        a->heads / a->kv_heads, a->pages, log2_of(a->page), a->max_pages, a->max_new, a->max_ctx,
-                        a->width, a->scale * kLog2e};
+    const uint32_t cus = device_cus();
+    if (!cus)
+        return fail(MAKO_EHIP, "%s: no device to size the split for", what);
+    const Plan pl = plan_of(a, cus);
+    const size_t need = workspace_for(pl, a->dim);
+    if (workspace_bytes < need || (need && !workspace) || !aligned16(workspace))
+        return fail(MAKO_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, workspace_bytes,
+                    need);
+    char* ws = need ? static_cast<char*>(workspace) : nullptr;
+    const size_t ob = part_o_bytes(pl, a->dim), lb = part_l_bytes(pl), wb = (size_t)pl.n_ranges * 8;
+    const auto at = [&](size_t off) { return ws ? ws + off : nullptr; };
+    const PagedParams p{{starts, ctx_len, a->batch, a->rows, a->kv_heads, a->max_new, a->max_ctx, pl.rshift, pl.n_ranges,
+                         pl.direct},
+                        q, k, v, table, o, lse, reinterpret_cast<float*>(at(0)), reinterpret_cast<float*>(at(ob)),
+                        reinterpret_cast<uint32_t*>(at(ob + lb + 2 * wb)), reinterpret_cast<u32x4*>(at(ob + lb)), a->q_pad,
+                        a->heads / a->kv_heads, a->pages, a->kv_heads * a->page * a->dim * 2, log2_of(a->page),
+                        a->max_pages, a->width, pl.hq, pl.ncb, pl.slot_rows, a->scale * kLog2e};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const uint32_t groups = rows * a->heads;
     if (in == MAKO_BF16 && out == MAKO_F32)
-        launch_dim<__bf16, float>(p, a->dim, groups, s);
+        launch_dim<__bf16, float>(p, a->dim, s);
     else if (in == MAKO_BF16)
-        launch_dim<__bf16, __bf16>(p, a->dim, groups, s);
+        launch_dim<__bf16, __bf16>(p, a->dim, s);
     else if (out == MAKO_F32)
-        launch_dim<_Float16, float>(p, a->dim, groups, s);
+        launch_dim<_Float16, float>(p, a->dim, s);
     else
-        launch_dim<_Float16, _Float16>(p, a->dim, groups, s);
+        launch_dim<_Float16, _Float16>(p, a->dim, s);
     return check_launch(what);
 }

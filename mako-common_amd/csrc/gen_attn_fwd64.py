@@ -157,6 +157,16 @@ SEW = "s[94:95]"        # that tile's validity words (the exact path's are s[78:
 SEW_LO, SEW_HI = "s94", "s95"   # which the sparse stream's masks leave alone
 MAPV = "v184"           # the output row map[q0 + lane] (-1: dropped)
 
+# The stream over a cache in pages (body(..., paged=True)): the dense stream, whose tiles come from the pages that the
+# sequence's table row names (%[ent]: its words; %[pshift] and %[pmask]: tiles a page, as a shift and a mask; %[pstride]:
+# bytes from a page to the next; a number at or past %[npages]: no page, whose tile loads zeros). A tile's page is read with
+# a scalar load an iteration ahead of its staging; %[pg0] .. %[pg3] are those of the first four tiles, %[t0] the first
+# tile's number in the sequence and %[tlast] the last one's (no entry past its page is read).
+PAGED = False
+SPG = "s65"             # page of the tile the next staging loads
+SREM = "s58"           # bytes of K (of V) from that tile to the end of the keys
+STN = "s59"            # that tile's number in the sequence
+
 
 def quad(r):
     return f"s[{r[0][1:]}:{r[3][1:]}]"
@@ -167,6 +177,7 @@ CLOBBER_A = 224
 CLOBBER_S = (60, 100)
 CLOBBER_V_SPARSE = 185     # + MAPV
 CLOBBER_S_SPARSE = (60, 100)
+CLOBBER_S_PAGED = (58, 100)
 
 
 class Emit:
@@ -220,7 +231,8 @@ def dma_groups():
     instructions behind it (a timing probe of the plain iteration on one CU: 2654 cycles a tile with the loads at
     the phase's start, 2536 spread one every few MFMAs)."""
     groups = []
-    pre = []
+    pre = page_source(SPG, SREM, STN, SROT["k"], SROT["wk"], SROT["wv"]) + \
+        value_source(SROT["wk"], SROT["wv"]) if PAGED else []
     if SPARSE:
         t = SROT["k"]
         pre = [f"s_lshl_b32 {t}, {SD}, 8",
@@ -238,7 +250,9 @@ def dma_groups():
     groups[0] = pre + groups[0]
     ops = []
     step = 128 * D   # K and V rows: 2 d bytes a key, 64 keys a tile
-    for r in (KRS, VRS) if not SPARSE else ():
+    if PAGED:
+        ops += page_advance(SREM, STN)
+    for r in (KRS, VRS) if not (SPARSE or PAGED) else ():
         ops += [f"s_add_u32 {r[0]}, {r[0]}, {step:#x}", f"s_addc_u32 {r[1]}, {r[1]}, 0",
                 f"s_sub_u32 {r[2]}, {r[2]}, {step:#x}", f"s_cselect_b32 {r[2]}, 0, {r[2]}"]
     wk, wv = SROT["wk"], SROT["wv"]
@@ -249,6 +263,31 @@ def dma_groups():
             f"s_add_u32 {SKW}, {SKW}, {wk}", f"s_add_u32 {SKWW}, {SKWW}, {wk}", f"s_add_u32 {SVWW}, {SVWW}, {wv}",
             f"s_add_u32 {SBW}, {SBW}, 1", f"s_cmp_eq_u32 {SBW}, {NBUF}", f"s_cselect_b32 {SBW}, 0, {SBW}"]
     return groups, ops
+
+
+def page_source(page, rem, tile, t, lo, hi):
+    """Paged: K's descriptor at the tile `tile` of page `page`, `rem` bytes long (none where there is no page); (lo, hi) keep
+    the tile's offset in the pool."""
+    return [f"s_and_b32 {t}, {tile}, %[pmask]", f"s_lshl_b32 {t}, {t}, {(128 * D).bit_length() - 1}",
+            f"s_mul_i32 {lo}, {page}, %[pstride]", f"s_mul_hi_u32 {hi}, {page}, %[pstride]",
+            f"s_add_u32 {lo}, {lo}, {t}", f"s_addc_u32 {hi}, {hi}, 0",
+            f"s_add_u32 {KRS[0]}, %[kb0], {lo}", f"s_addc_u32 {KRS[1]}, %[kb1], {hi}",
+            f"s_cmp_lt_u32 {page}, %[npages]", f"s_cselect_b32 {KRS[2]}, {rem}, 0"]
+
+
+def value_source(lo, hi):
+    """Paged: V's descriptor at the offset (lo, hi) that K's was set to, as long."""
+    return [f"s_add_u32 {VRS[0]}, %[vb0], {lo}", f"s_addc_u32 {VRS[1]}, %[vb1], {hi}", f"s_mov_b32 {VRS[2]}, {KRS[2]}"]
+
+
+def page_advance(rem, tile):
+    return [f"s_sub_u32 {rem}, {rem}, {128 * D:#x}", f"s_cselect_b32 {rem}, 0, {rem}", f"s_add_u32 {tile}, {tile}, 1"]
+
+
+def page_load(page, tile, t):
+    """Paged: the scalar load of the page of tile `tile`, the next to be staged (past the last tile: the last one's)."""
+    return [f"s_min_u32 {t}, {tile}, %[tlast]", f"s_lshr_b32 {t}, {t}, %[pshift]", f"s_lshl_b32 {t}, {t}, 2",
+            f"s_load_dword {page}, %[ent], {t}"]
 
 
 def staging():
@@ -512,6 +551,10 @@ def early_dma():
         g1 = [["s_mov_b32 %s, s89" % SD] + g1[0]] + g1[1:]
         g2 = [["s_mov_b32 %s, s90" % SD] + g2[0]] + g2[1:]
         t2 = t2 + ["s_mov_b32 %s, s91" % SD]
+    if PAGED:
+        g1 = [[f"s_mov_b32 {SPG}, %[pg1]"] + g1[0]] + g1[1:]
+        g2 = [[f"s_mov_b32 {SPG}, %[pg2]"] + g2[0]] + g2[1:]
+        t2 = t2 + [f"s_mov_b32 {SPG}, %[pg3]"]
     return g1 + [t1 + g2[0]] + g2[1:], t2
 
 
@@ -723,17 +766,17 @@ def epilogue(e, out_dtype):
 
 # ---- the kernel body ----------------------------------------------------------------------------------------------
 
-def body(in_dtype, out_dtype, sparse=False, d=128):
+def body(in_dtype, out_dtype, sparse=False, d=128, paged=False):
     """The stream for one item (a workgroup's rows) at head width d; sparse: the block-sparse one (tiles from the
-    pass table, heads of 128)."""
-    global SPARSE
-    assert d == 128 or not sparse
-    SPARSE = sparse
+    pass table, heads of 128); paged: over a cache in pages."""
+    global SPARSE, PAGED
+    assert not sparse or (d == 128 and not paged)
+    SPARSE, PAGED = sparse, paged
     set_dim(d)
     try:
         return body_of(in_dtype, out_dtype)
     finally:
-        SPARSE = False
+        SPARSE = PAGED = False
         set_dim(128)
 
 
@@ -759,10 +802,15 @@ def body_of(in_dtype, out_dtype):
         e(f"v_mov_b32 {MAXV[rb]}, {NINF}")
     # load sources of tile 0
     for r, pre in ((KRS, "k"), (VRS, "v")):
-        e(f"s_mov_b32 {r[0]}, %[{pre}b0]")
-        e(f"s_mov_b32 {r[1]}, %[{pre}b1]")
-        e(f"s_mov_b32 {r[2]}, %[{pre}n]")
+        if not PAGED:
+            e(f"s_mov_b32 {r[0]}, %[{pre}b0]")
+            e(f"s_mov_b32 {r[1]}, %[{pre}b1]")
+            e(f"s_mov_b32 {r[2]}, %[{pre}n]")
         e(f"s_mov_b32 {r[3]}, 0x20000")
+    if PAGED:
+        e(f"s_mov_b32 {SREM}, %[kn]")
+        e(f"s_mov_b32 {STN}, %[t0]")
+        e(f"s_mov_b32 {SPG}, %[pg0]")
     e(f"s_mov_b32 {SBW}, 0")
     # M0 is the compiler's: kept in SM0 while the stream uses it, restored at the end
     e(f"s_mov_b32 {SM0}, m0")
@@ -864,7 +912,7 @@ def body_rest(e, in_dtype, out_dtype):
             kind = masked_next or variant
             m = mask(nxt, SJ0) if kind == "masked" else mask_general(nxt, SJ0, SEW) if kind == "general" else []
             # sparse: the next entries load once this phase has read SEW (the general mask's third instruction)
-            loads = entry_loads() if SPARSE else []
+            loads = entry_loads() if SPARSE else page_load(SPG, STN, ST[0]) if PAGED else []
             valu = ["s_nop 7", "s_nop 7"] + m[:3] + loads + m[3:] + exps(nxt)
         elif SPARSE:
             valu = entry_loads()
@@ -968,6 +1016,9 @@ def body_rest(e, in_dtype, out_dtype):
         e(f"s_add_u32 {ST[0]}, {ST[0]}, 48")
         e(f"s_load_dword {SD}, %[ent], {ST[0]}")
         e("s_waitcnt lgkmcnt(0)")
+    if PAGED:
+        for op in page_load(SPG, STN, ST[0]) + ["s_waitcnt lgkmcnt(0)"]:
+            e(op)
     for op in staging() + barrier():
         e(op)
     e(f"s_add_u32 {SJ}, {SJ}, 1")
@@ -977,14 +1028,14 @@ def body_rest(e, in_dtype, out_dtype):
     e(f"s_mov_b32 m0, {SM0}")
 
 
-def clobbers(sparse=False):
+def clobbers(sparse=False, paged=False):
     regs = [f'"v{i}"' for i in range(CLOBBER_V_SPARSE if sparse else CLOBBER_V)]
     regs += [f'"a{i}"' for i in range(CLOBBER_A)]
-    regs += [f'"s{i}"' for i in range(*(CLOBBER_S_SPARSE if sparse else CLOBBER_S))]
+    regs += [f'"s{i}"' for i in range(*(CLOBBER_S_SPARSE if sparse else CLOBBER_S_PAGED if paged else CLOBBER_S))]
     return ", ".join(regs)
 
 
-def check_registers(lines, sparse=False):
+def check_registers(lines, sparse=False, paged=False):
     """Every register the stream names must be one the clobber list reserves (the wave is only given those)."""
     import re
     for ln in lines:
@@ -992,7 +1043,7 @@ def check_registers(lines, sparse=False):
             top = int(one) if one else int(hi)
             bot = int(one) if one else int(lo)
             limit = {"v": (0, CLOBBER_V_SPARSE if sparse else CLOBBER_V), "a": (0, CLOBBER_A),
-                     "s": CLOBBER_S_SPARSE if sparse else CLOBBER_S}[kind]
+                     "s": CLOBBER_S_SPARSE if sparse else CLOBBER_S_PAGED if paged else CLOBBER_S}[kind]
             assert limit[0] <= bot and top < limit[1], f"{kind}{bot}..{top} outside the reserved registers: {ln}"
             assert one or bot % 2 == 0, f"{kind}[{bot}:{top}]: a register tuple must start on an even register: {ln}"
 

@@ -72,6 +72,15 @@ KRS, VRS, ST, SCMP, SJ0, SM0, SMASK = G.KRS, G.VRS, G.ST, G.SCMP, G.SJ0, G.SM0, 
 CLOBBER_V = 184
 CLOBBER_A = 192 + 4 * RING
 CLOBBER_S = (60, 100)
+CLOBBER_S_PAGED = (58, 100)
+
+# The stream over a cache in pages (body(..., paged=True)), as gen_attn_fwd64's: K(j + 2)'s page is read an iteration ahead,
+# and V(j + 1) takes the offset that K(j + 1) was loaded from.
+PAGED = False
+SPG = "s86"        # page of the K tile the next staging loads
+SREM = "s96"       # bytes of K from that tile to the end of the keys
+STN = "s97"        # that tile's number in the sequence
+SLO, SHI = "s58", "s59"   # offset in the pool of the K tile staged last
 
 
 @contextlib.contextmanager
@@ -147,9 +156,12 @@ def dma_k():
     groups.append([f"s_add_u32 m0, {SKW}, {4 * NKP * 1024}", "s_nop 0",
                    f"buffer_load_dwordx4 %[kd{NKP}], {G.quad(KRS)}, 0 offen lds"])
     step = 128 * D
-    tail = [f"s_add_u32 {KRS[0]}, {KRS[0]}, {step:#x}", f"s_addc_u32 {KRS[1]}, {KRS[1]}, 0",
-            f"s_sub_u32 {KRS[2]}, {KRS[2]}, {step:#x}", f"s_cselect_b32 {KRS[2]}, 0, {KRS[2]}",
-            f"s_add_u32 {SKW}, {SKW}, {SKT}", f"s_add_u32 {SKWW}, {SKWW}, {SKT}", f"s_sub_u32 {SKT}, 0, {SKT}"]
+    move = [f"s_add_u32 {KRS[0]}, {KRS[0]}, {step:#x}", f"s_addc_u32 {KRS[1]}, {KRS[1]}, 0",
+            f"s_sub_u32 {KRS[2]}, {KRS[2]}, {step:#x}", f"s_cselect_b32 {KRS[2]}, 0, {KRS[2]}"]
+    if PAGED:
+        groups[0] = G.page_source(SPG, SREM, STN, "s98", SLO, SHI) + groups[0]
+        move = G.page_advance(SREM, STN)
+    tail = [*move, f"s_add_u32 {SKW}, {SKW}, {SKT}", f"s_add_u32 {SKWW}, {SKWW}, {SKT}", f"s_sub_u32 {SKT}, 0, {SKT}"]
     return groups, tail
 
 
@@ -167,9 +179,12 @@ def dma_v():
         pre = [f"s_mov_b32 m0, {SVWW}" if half == 0 else f"s_add_u32 m0, {SVWW}, 4096", "s_nop 0"]
         groups.append(pre + [f"buffer_load_dwordx4 %[{reg}], {G.quad(VRS)}, 0 offen offset:{1024 * (k % 4)} lds"])
     step = 128 * D
-    tail = [f"s_add_u32 {VRS[0]}, {VRS[0]}, {step:#x}", f"s_addc_u32 {VRS[1]}, {VRS[1]}, 0",
-            f"s_sub_u32 {VRS[2]}, {VRS[2]}, {step:#x}", f"s_cselect_b32 {VRS[2]}, 0, {VRS[2]}",
-            f"s_add_u32 {SVWW}, {SVWW}, {SVT}", f"s_sub_u32 {SVT}, 0, {SVT}"]
+    move = [f"s_add_u32 {VRS[0]}, {VRS[0]}, {step:#x}", f"s_addc_u32 {VRS[1]}, {VRS[1]}, 0",
+            f"s_sub_u32 {VRS[2]}, {VRS[2]}, {step:#x}", f"s_cselect_b32 {VRS[2]}, 0, {VRS[2]}"]
+    if PAGED:
+        groups[0] = G.value_source(SLO, SHI) + groups[0]
+        move = []
+    tail = [*move, f"s_add_u32 {SVWW}, {SVWW}, {SVT}", f"s_sub_u32 {SVT}, 0, {SVT}"]
     return groups, tail
 
 
@@ -177,8 +192,12 @@ def unit_groups():
     """The staging of an iteration (K(j + 2) and V(j + 1)) as one (groups, tail)."""
     gk, tk = dma_k()
     gv, tv = dma_v()
-    # interleave K and V loads so both streams start early; each group keeps its own M0 write
+    # interleave K and V loads so both streams start early; each group keeps its own M0 write (paged: V's source is set
+    # first, from what K's is set anew by)
     groups = []
+    if PAGED:
+        n = len(G.value_source(SLO, SHI))
+        gk[0], gv[0] = gv[0][:n] + gk[0], gv[0][n:]
     for i in range(max(len(gk), len(gv))):
         if i < len(gk):
             groups.append(gk[i])
@@ -434,9 +453,14 @@ def epilogue(e, out_dtype):
 
 # ---- the kernel body ----------------------------------------------------------------------------------------------
 
-def body(in_dtype, out_dtype):
-    with shapes():
-        return body_of(in_dtype, out_dtype)
+def body(in_dtype, out_dtype, paged=False):
+    global PAGED
+    PAGED = paged
+    try:
+        with shapes():
+            return body_of(in_dtype, out_dtype)
+    finally:
+        PAGED = False
 
 
 def body_of(in_dtype, out_dtype):
@@ -450,10 +474,15 @@ def body_of(in_dtype, out_dtype):
     e(f"v_mov_b32 {LSUM}, 0")
     e(f"v_mov_b32 {MAXV}, {NINF}")
     for r, pre in ((KRS, "k"), (VRS, "v")):
-        e(f"s_mov_b32 {r[0]}, %[{pre}b0]")
-        e(f"s_mov_b32 {r[1]}, %[{pre}b1]")
-        e(f"s_mov_b32 {r[2]}, %[{pre}n]")
+        if not PAGED:
+            e(f"s_mov_b32 {r[0]}, %[{pre}b0]")
+            e(f"s_mov_b32 {r[1]}, %[{pre}b1]")
+            e(f"s_mov_b32 {r[2]}, %[{pre}n]")
         e(f"s_mov_b32 {r[3]}, 0x20000")
+    if PAGED:
+        e(f"s_mov_b32 {SREM}, %[kn]")
+        e(f"s_mov_b32 {STN}, %[t0]")
+        e(f"s_mov_b32 {SPG}, %[pg0]")
     for r, v in ((SKRT, K_TILE), (SVRT, V_TILE), (SKT, K_TILE), (SVT, V_TILE)):
         e(f"s_mov_b32 {r}, {v:#x}")
     # M0 is the compiler's: kept in SM0 while the stream uses it, restored at the end
@@ -467,6 +496,8 @@ def body_of(in_dtype, out_dtype):
     # barrier after tile 0 for K(1).
     for op in flat(dma_k()) + flat(dma_v()):
         e(op)
+    if PAGED:
+        e(f"s_mov_b32 {SPG}, %[pg1]")
     for kk in range(NKK):
         e(f"buffer_load_dwordx4 {G.Q(0, kk)}, %[qo], %[qrs], 0 offen offset:{32 * kk}")
     z = f"v[{TMP[8][1:]}:{TMP[11][1:]}]"
@@ -490,6 +521,8 @@ def body_rest(e, in_dtype, out_dtype):
     # tile 0: scores into raw set 0 (K(1) staged between the MFMAs), masked, then the exact path
     mfmas = qk_mfmas(in_dtype, 0)
     early = dma_k()
+    if PAGED:
+        early = (early[0], early[1] + [f"s_mov_b32 {SPG}, %[pg2]"])
     G.phase(e, "X", G.k_reads("%[kr]"), mfmas, [], fwait=q_waits(mfmas, len(early[0])), dma=early)
     for op in G.wait_mfma() + mask(0, 0):
         e(op)
@@ -532,7 +565,8 @@ def body_rest(e, in_dtype, out_dtype):
         if variant != "last":
             kind = masked_next or variant
             m = mask(nxt, SJ0) if kind == "masked" else []
-            valu = ["s_nop 7", "s_nop 7"] + m + exps(nxt)
+            loads = G.page_load(SPG, STN, ST[0]) if PAGED else []
+            valu = ["s_nop 7", "s_nop 7"] + loads + m + exps(nxt)
         n_k = G.phase(e, "V", v_reads(), pv_mfmas(in_dtype), valu, pre=n_v,
                       nxt=None if variant == "last" else ("K", G.k_reads("%[kr]")), gate_at=BAR_AT, gate=barrier())
         assert variant == "last" or n_k == G.N_K_AHEAD
@@ -594,6 +628,9 @@ def body_rest(e, in_dtype, out_dtype):
     e.label("L_tail")
     e(f"s_cmp_ge_u32 {SJ}, %[nt]")
     e(f"s_cbranch_scc1 {G.lbl('L_epi')}")
+    if PAGED:
+        for op in G.page_load(SPG, STN, ST[0]) + ["s_waitcnt lgkmcnt(0)"]:
+            e(op)
     for op in staging() + barrier():
         e(op)
     e(f"s_add_u32 {SJ}, {SJ}, 1")
@@ -603,21 +640,21 @@ def body_rest(e, in_dtype, out_dtype):
     e(f"s_mov_b32 m0, {SM0}")
 
 
-def clobbers():
+def clobbers(paged=False):
     regs = [f'"v{i}"' for i in range(CLOBBER_V)]
     regs += [f'"a{i}"' for i in range(CLOBBER_A)]
-    regs += [f'"s{i}"' for i in range(*CLOBBER_S)]
+    regs += [f'"s{i}"' for i in range(*(CLOBBER_S_PAGED if paged else CLOBBER_S))]
     return ", ".join(regs)
 
 
-def check_registers(lines):
+def check_registers(lines, paged=False):
     """Every register the stream names must be one the clobber list reserves."""
     import re
     for ln in lines:
         for kind, one, lo, hi in re.findall(r"\b([vas])(?:(\d+)|\[(\d+):(\d+)\])", ln.split(";")[0]):
             top = int(one) if one else int(hi)
             bot = int(one) if one else int(lo)
-            limit = {"v": (0, CLOBBER_V), "a": (0, CLOBBER_A), "s": CLOBBER_S}[kind]
+            limit = {"v": (0, CLOBBER_V), "a": (0, CLOBBER_A), "s": CLOBBER_S_PAGED if paged else CLOBBER_S}[kind]
             assert limit[0] <= bot and top < limit[1], f"{kind}{bot}..{top} outside the reserved registers: {ln}"
             assert one or bot % 2 == 0, f"{kind}[{bot}:{top}]: a register tuple must start on an even register: {ln}"
 

@@ -1,0 +1,165 @@
+// The split of attention over a cache in pages: which tiles of which items a workgroup takes. Lengths are known on the device
+// only, so every workgroup works it out.
+//
+// An item is a block of R = 1 << rshift rows of a sequence and a kv head; its tiles are the 64 keys each up to its last row's.
+// Its cost is its keys, in units of 32, and kLead for what it costs beside them. The items of all (sequence, kv head)
+// segments lie end to end and are cut into equal ranges, one a workgroup. Within a segment the row blocks go heavy and light
+// in turn (the last, the first, the last but one, the second, ...), so two neighbours cost the same everywhere, and the ranges of a whole
+// prompt fall on items' ends. A cut inside an item leaves kLeast tiles on either side, and no row without keys in a piece's
+// first tile, which the attention's streams rely on; with `direct`, items are not cut: the range of an item's middle has it.
+#pragma once
+
+#include "pages_common.hpp"
+#include "split_ranges.hpp"
+
+namespace mako {
+
+constexpr uint32_t kLead = 8;
+constexpr uint32_t kLeast = 3;
+
+struct PagedSplit {
+    const uint32_t *starts, *ctx;
+    uint32_t batch, rows, kv_heads, max_new, max_ctx, rshift, n_ranges, direct;
+};
+
+// A piece of an item: tiles [ta, tb) of sequence b for its rows row0 .. of o, the first at position p0.
+struct PagedPiece {
+    uint32_t b, kvh, row0, rows, p0;
+    uint32_t keys, seen;  // of the item's last row; of the sequence's
+    uint32_t ta, tb;
+    uint32_t part, kind;  // part: not the whole item; kind: 1 if the item starts in this range
+    uint32_t first;       // where it is an item's last piece of several: the range that the item starts in (else kNoPage)
+};
+
+// A sequence's new rows n, from row s0, behind c cache rows, keys with them, in nqb blocks; lead: units of an item whatever
+// its block.
+struct PagedSeq {
+    uint32_t c, n, s0, keys, nqb, lead;
+};
+__device__ __forceinline__ PagedSeq seq_of(const PagedSplit& p, uint32_t b)
+{
+    const NewRows nr = new_rows(p.starts, p.rows, b);
+    PagedSeq s;
+    s.n = min(nr.n, p.max_new);
+    s.s0 = nr.s0;
+    s.c = min(p.ctx[b], p.max_ctx);
+    s.keys = s.c + min(s.n, p.max_ctx - s.c);
+    s.nqb = (s.n + (1u << p.rshift) - 1) >> p.rshift;
+    s.lead = kLead + (s.c + 31) / 32;
+    return s;
+}
+__device__ __forceinline__ PagedSeq uniform_seq(const PagedSeq& s)
+{
+    return {uniform(s.c), uniform(s.n), uniform(s.s0), uniform(s.keys), uniform(s.nqb), uniform(s.lead)};
+}
+__device__ __forceinline__ uint32_t item_units(const PagedSplit& p, const PagedSeq& s, uint32_t qb)
+{
+    return s.lead + ((qb + 1) << (p.rshift - 5));
+}
+__device__ __forceinline__ uint32_t segment_units(const PagedSplit& p, const PagedSeq& s)
+{
+    return s.nqb * s.lead + ((s.nqb * (s.nqb + 1) / 2) << (p.rshift - 5));
+}
+
+// The tile that unit u of an item of nt tiles falls to (those from tmax on stay together).
+__device__ __forceinline__ uint32_t cut_of(const PagedSplit& p, uint32_t u, uint32_t nt, uint32_t tmax)
+{
+    const uint32_t t = (max(u, kLead) - kLead) / 2;
+    if (p.direct)
+        return 2 * t < nt ? 0u : nt;
+    return t < kLeast ? 0u : t + kLeast > nt ? nt : min(t, tmax);
+}
+
+// Calls piece(PagedPiece) for the pieces of a range, in order; all lanes of a wave do so together.
+template <class F>
+__device__ __forceinline__ void walk_range(const PagedSplit& p, uint32_t range, uint32_t lane, F piece)
+{
+    // The units of all segments; up to 64 sequences are looked up once, a lane each.
+    uint32_t total = 0, units = 0, inc = 0;
+    for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
+        units = i0 + lane < p.batch ? segment_units(p, seq_of(p, i0 + lane)) : 0u;
+        inc = scan_lanes(units * p.kv_heads);
+        total += (uint32_t)__builtin_amdgcn_readlane(inc, 63);
+    }
+    const uint32_t n = min(p.n_ranges, total);
+    if (range >= n)
+        return;
+    const Ranges rg(total, n);
+    const uint32_t x0 = rg.start(range);
+    uint32_t left = rg.start(range + 1) - x0;
+    // The sequence b whose segments (from unit `at` on, len units each) hold x0.
+    uint32_t b = 0, at = 0, len = 1;
+    for (uint32_t i0 = 0, base = 0; i0 < p.batch; i0 += 64) {
+        if (p.batch > 64) {
+            units = i0 + lane < p.batch ? segment_units(p, seq_of(p, i0 + lane)) : 0u;
+            inc = scan_lanes(units * p.kv_heads);
+        }
+        if (const uint64_t hit = __ballot(x0 < base + inc)) {
+            const uint32_t l = (uint32_t)__builtin_ctzll(hit);
+            b = i0 + l;
+            len = (uint32_t)__builtin_amdgcn_readlane(units, l);
+            at = base + (uint32_t)__builtin_amdgcn_readlane(inc, l) - len * p.kv_heads;
+            break;
+        }
+        base += (uint32_t)__builtin_amdgcn_readlane(inc, 63);
+    }
+    PagedSeq s = uniform_seq(seq_of(p, b));
+    uint32_t kvh = (x0 - at) / len, u0 = (x0 - at) % len, item;
+    {
+        // item 2 i is block nqb - 1 - i, item 2 i + 1 block i: a pair's units do not depend on i
+        const uint32_t pair = 2 * s.lead + ((s.nqb + 1) << (p.rshift - 5)), i = u0 / pair;
+        u0 -= i * pair;
+        item = 2 * i;
+        const uint32_t heavy = item_units(p, s, s.nqb - 1 - i);
+        if (u0 >= heavy) {
+            u0 -= heavy;
+            ++item;
+        }
+    }
+    uint32_t start = x0 - u0;  // the item's first unit
+    for (;;) {
+        const uint32_t qb = item & 1 ? item / 2 : s.nqb - 1 - item / 2;
+        const uint32_t cost = item_units(p, s, qb), u1 = min(cost, u0 + left), i0 = qb << p.rshift;
+        PagedPiece x;
+        x.b = b, x.kvh = kvh, x.row0 = s.s0 + i0, x.rows = min(1u << p.rshift, s.n - i0), x.p0 = s.c + i0;
+        x.seen = s.keys, x.keys = min(x.p0 + x.rows, s.keys);
+        const uint32_t nt = (x.keys + 63) / 64, tmax = (min(x.p0 + 1, s.keys) - 1) / 64;
+        x.ta = cut_of(p, u0, nt, tmax);
+        x.tb = u1 == cost ? nt : cut_of(p, u1, nt, tmax);
+        if (x.ta < x.tb) {
+            x.part = x.ta != 0 || x.tb != nt;
+            x.kind = u0 == 0 ? 1 : 0;
+            x.first = kNoPage;
+            if (x.part && x.tb == nt) {
+                uint32_t lo = 0, hi = range;  // the last range that starts at or before the item
+                while (lo < hi) {
+                    const uint32_t mid = (lo + hi + 1) / 2;
+                    if (rg.start(mid) <= start)
+                        lo = mid;
+                    else
+                        hi = mid - 1;
+                }
+                x.first = lo;
+            }
+            piece(x);
+        }
+        left -= u1 - u0;
+        if (left == 0)
+            return;
+        start += cost;
+        u0 = 0;
+        if (++item == s.nqb) {
+            item = 0;
+            if (++kvh == p.kv_heads) {
+                kvh = 0;
+                do {
+                    if (++b >= p.batch)
+                        return;  // (not where the lengths are as they were when the units were summed)
+                    s = uniform_seq(seq_of(p, b));
+                } while (s.nqb == 0);
+            }
+        }
+    }
+}
+
+}  // namespace mako

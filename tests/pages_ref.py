@@ -1,7 +1,10 @@
 """Plain forms of the operators of a cache kept in pages, in 64 bits, and the error their kernels may make.
 
-The attention's kernels round the probabilities to the input type for the product with V (rows that see fewer than 64 keys
-get them to twice as many bits), so an output is off by at most `half a step of the type` * sum_j w_j |v_j|, by what the
+The attention's kernels round the probabilities to the input type for the product with V: p (1 + e), |e| <= h, half a step of
+the type (bf16 2^-8, f16 2^-11). Rows that see fewer than 64 keys get bf16 probabilities as a sum of two bf16 values: the
+second is off by h of what the first left, h p, so |e| <= h^2. Below f16's smallest normal value, 2^-14, f16 probabilities
+are off by up to half a step there, 2^-25, against a sum of at least 1 (the running maximum
+is a score that was met). So an output is off by at most |e| sum_j w_j |v_j| + 2^-25 sum_j |v_j| (f16), by what the
 scores' errors make of the weights (a score off by ds moves each weight by at most a factor exp(2 ds)), and by its own
 rounding. A score is a sum of dim products in 32 bits: ds <= 2^-24 ((dim + 2) scale sum |q k| + |score| + 8)."""
 import math
@@ -39,7 +42,9 @@ def attention(q, k, v, table, ctx, new, starts, *, scale, max_ctx, max_new, out_
         ltol = torch.zeros_like(lse)
         seen = torch.clamp(torch.arange(n, device=q.device) + c + 1, max=max_ctx)
         hidden = torch.arange(keys, device=q.device) >= seen[:, None]
-        p_err = torch.where(seen < 64, half_step(q.dtype) ** 2 * 4, half_step(q.dtype))[:, None]
+        e = half_step(q.dtype)
+        f16 = q.dtype == torch.float16
+        p_err = torch.where(seen < 64, e if f16 else e * e, e)[:, None]
         for h in range(H):
             kk, vv = rows_of(k, table[b], keys, h * KV // H), rows_of(v, table[b], keys, h * KV // H)
             qq = q[h, s0:s0 + n].double()
@@ -50,6 +55,8 @@ def attention(q, k, v, table, ctx, new, starts, *, scale, max_ctx, max_new, out_
             ds = 2.0 ** -24 * ((D + 2) * size.amax(1, keepdim=True) + sc.masked_fill(hidden, 0).abs().amax(1, keepdim=True) + 8)
             o[:, h] = torch.matmul(w, vv)
             tol[:, h] = torch.matmul(w, vv.abs()) * (p_err + 2.5 * ds + keys * 2.0 ** -24)
+            if f16:
+                tol[:, h] += 2.0 ** -25 * torch.matmul((~hidden).double(), vv.abs())
             lse[:, h] = torch.logsumexp(sc, 1)
             # the sums: at most a chain of a tile's 32 terms a lane and the tiles, then the logarithm
             ltol[:, h] = ds[:, 0] + (64 + keys / 64) * 2.0 ** -24 + 2.0 ** -22 * (lse[:, h].abs() + 4)

@@ -1,5 +1,5 @@
 """The operators of a cache kept in pages without a GPU: csrc/pages.hip's kernels run on the CPU (tests/cpp/pages_cpu.cpp),
-also over malformed tables; what the entry points refuse, and with which message, before touching the device."""
+also over malformed tables, and so does the attention's split (tests/cpp/paged_split_cpu.cpp); what the entry points refuse, and with which message, before touching the device."""
 import ctypes
 import os
 import subprocess
@@ -17,9 +17,10 @@ ODD = ctypes.c_void_p(0x10008)
 BIG = ctypes.c_size_t(1 << 40)
 
 
-def test_pages_on_the_cpu():
-    subprocess.run(["make", "-s", "-C", CPP, "bin/pages_cpu"], check=True)
-    r = subprocess.run([os.path.join(CPP, "bin", "pages_cpu")], capture_output=True, text=True, timeout=600)
+@pytest.mark.parametrize("name", ["pages_cpu", "paged_split_cpu"])
+def test_on_the_cpu(name):
+    subprocess.run(["make", "-s", "-C", CPP, f"bin/{name}"], check=True)
+    r = subprocess.run([os.path.join(CPP, "bin", name)], capture_output=True, text=True, timeout=600)
     assert r.returncode == 0 and "all passed" in r.stdout, r.stdout + r.stderr
 
 
