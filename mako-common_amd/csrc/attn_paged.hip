@@ -10,8 +10,9 @@
 // * paged_rows runs the streams of flash_fwd_r64 (heads of 64 and 128) and flash_fwd_r32 (256) over pages
 //   (gen_attn_paged.py): a tile is 64 keys, a run of memory within a page; its page's number is read by a scalar load an
 //   iteration before the tile is staged.
-// * An item is a block of R rows of a sequence and `hq` heads of a kv head (4, 2 or 1, as they divide the group), R = 4 RW /
-//   hq: one workgroup's four waves. A group of more heads takes further workgroups (column blocks) on the same keys beside
+// * An item is a block of R rows of a sequence and `hq` heads of a kv head (4, 2 or 1, as they divide the group), R = 256 / hq
+//   (heads of 256: 128 / hq): one workgroup's four waves, 64 (32) rows each. Items of half the rows or fewer take the stream of
+//   32 rows a wave. A group of more heads takes further workgroups (column blocks) on the same keys beside
 //   each other on an XCD, so that the second read hits its L2.
 // * Lengths are known on the device only, so every workgroup works out its share of the work (paged_split.hpp): ranges of
 //   equal cost over the items of all sequences, one a workgroup.
@@ -58,17 +59,18 @@ struct Piece {
     uint32_t o_row, l_bytes;          // bytes of a row of o; of l that may be written
 };
 
-template <class T, class TO, int D>
+// RW: rows a wave, 64 or 32 (heads of 256: 32).
+template <class T, class TO, int D, int RW>
 __device__ __forceinline__ void run_piece(const PagedParams& p, unsigned char* lds, const Piece& x)
 {
     constexpr bool kWide = D == 256;
-    constexpr uint32_t RW = kWide ? 32 : 64, NBUF = kWide ? 2 : kNBuf;
+    constexpr uint32_t NBUF = kWide ? 2 : kNBuf;
     constexpr uint32_t kKRowB = 2 * D + 16, kKTileB = 64 * kKRowB, kVRowB = 2 * D, kVTileB = 64 * kVRowB;
     constexpr uint32_t NKP = (kKTileB / 1024 - 1) / 4;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, g = lane >> 5, c32 = lane & 31u, w = uniform(tid >> 6);
     const uint32_t q0 = w / p.hq * RW;  // this wave's first row in the block
     const uint32_t ks = 64 * x.ta, n_keys = min(64 * x.tb, x.keys) - ks;
-    const uint32_t lim_w = x.p0 + min(q0 + RW, x.rows);  // (position of the wave's last row) + 1
+    const uint32_t lim_w = x.p0 + min(q0 + (uint32_t)RW, x.rows);  // (position of the wave's last row) + 1
     const uint32_t w_keys = q0 < x.rows ? min(n_keys, min(lim_w, x.seen) - ks) : 0u;
     const uint32_t nt = x.tb - x.ta, ntw = (w_keys + 63) / 64;
     // keys that a row sees, counted from the piece's first one: lmin the wave's first row, lim0 and lim1 the lane's
@@ -155,7 +157,7 @@ __device__ __forceinline__ void run_piece(const PagedParams& p, unsigned char* l
       [vdo2] "v"(vdo2), [lim0] "v"(lim0), [qo] "v"(qo), [lo0] "v"(lo0), [swp] "v"(swp), [ew] "v"(ew), [er] "v"(er),   \
       [og] "v"(og), MAKO_PAGED_SCALARS                                                                            \
     : MAKO_PAGED_D256_CLOBBERS, "vcc", "scc", "memory"
-        MAKO_PAGED_STREAM(MAKO_PAGED_D256, MAKO_PAGED_R32);
+        MAKO_PAGED_STREAM(MAKO_PAGED_D256_R32, MAKO_PAGED_R32);
     } else {
         uint32_t vr0 = vrow + 32 * v_unit(th, ti / 4), vr1 = vrow + 32 * v_unit(2 + th, ti / 4);
         const uint32_t kr0 = kr, lim1 = min(r0 + c32 + 33, x.seen) - ks - 8 * g;
@@ -169,10 +171,14 @@ __device__ __forceinline__ void run_piece(const PagedParams& p, unsigned char* l
       [lim0] "v"(lim0), [lim1] "v"(lim1), [kr0] "v"(kr0), [qo] "v"(qo), [lo0] "v"(lo0), [lo1] "v"(lo1),            \
       [swp] "v"(swp), [ew] "v"(ew), [er] "v"(er), [og] "v"(og), [pg3] "s"(pg3), MAKO_PAGED_SCALARS                 \
     : MAKO_PAGED_CLOBBERS, "vcc", "scc", "memory"
-        if constexpr (D == 64)
-            MAKO_PAGED_STREAM(MAKO_PAGED_D64, MAKO_PAGED_R64);
+        if constexpr (D == 64 && RW == 64)
+            MAKO_PAGED_STREAM(MAKO_PAGED_D64_R64, MAKO_PAGED_R64);
+        else if constexpr (D == 64)
+            MAKO_PAGED_STREAM(MAKO_PAGED_D64_R32, MAKO_PAGED_R64);
+        else if constexpr (RW == 64)
+            MAKO_PAGED_STREAM(MAKO_PAGED_D128_R64, MAKO_PAGED_R64);
         else
-            MAKO_PAGED_STREAM(MAKO_PAGED_D128, MAKO_PAGED_R64);
+            MAKO_PAGED_STREAM(MAKO_PAGED_D128_R32, MAKO_PAGED_R64);
     }
 #undef MAKO_PAGED_R64
 #undef MAKO_PAGED_R32
@@ -220,10 +226,16 @@ __global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams p)
             if (at.first != kNone)
                 done = u32x4{at.first, at.row0, at.rows, at.kvh};
         }
-        if (at.part || __is_same(TO, float))
-            run_piece<T, float, D>(p, lds, x);
+        const bool f32 = at.part || __is_same(TO, float), few = D == 256 || 2 * at.rows <= 1u << p.rshift;
+        constexpr int kMany = D == 256 ? 32 : 64;
+        if (f32 && few)
+            run_piece<T, float, D, 32>(p, lds, x);
+        else if (f32)
+            run_piece<T, float, D, kMany>(p, lds, x);
+        else if (few)
+            run_piece<T, TO, D, 32>(p, lds, x);
         else
-            run_piece<T, TO, D>(p, lds, x);
+            run_piece<T, TO, D, kMany>(p, lds, x);
     });
     if (!p.direct && cb == 0 && threadIdx.x == 0) {
         p.whole[2 * range] = here[0];

@@ -166,6 +166,10 @@ PAGED = False
 SPG = "s65"             # page of the tile the next staging loads
 SREM = "s58"           # bytes of K (of V) from that tile to the end of the keys
 STN = "s59"            # that tile's number in the sequence
+# Its form for few rows (body(..., rows=32)): a wave owns 32 rows, one row block, so a tile is half the products and half the
+# softmax against the same staging; tiles come by streaming loads, as few workgroups read them again.
+NRB = 2                 # row blocks a wave
+STREAMING = False
 
 
 def quad(r):
@@ -231,6 +235,7 @@ def dma_groups():
     instructions behind it (a timing probe of the plain iteration on one CU: 2654 cycles a tile with the loads at
     the phase's start, 2536 spread one every few MFMAs)."""
     groups = []
+    nt = " nt" if STREAMING else ""
     pre = page_source(SPG, SREM, STN, SROT["k"], SROT["wk"], SROT["wv"]) + \
         value_source(SROT["wk"], SROT["wv"]) if PAGED else []
     if SPARSE:
@@ -241,12 +246,12 @@ def dma_groups():
                f"s_cmp_eq_u32 {SD}, -1", f"s_cselect_b32 {KRS[2]}, 0, 0x4000", f"s_mov_b32 {VRS[2]}, {KRS[2]}"]
     for m in range(NKP):
         groups.append([f"s_add_u32 m0, {SKWW}, {4096 * m}" if m else f"s_mov_b32 m0, {SKWW}", "s_nop 0",
-                       f"buffer_load_dwordx4 %[kd{m}], {quad(KRS)}, 0 offen lds"])
+                       f"buffer_load_dwordx4 %[kd{m}], {quad(KRS)}, 0 offen{nt} lds"])
     groups.append([f"s_add_u32 m0, {SKW}, {4 * NKP * 1024}", "s_nop 0",
-                   f"buffer_load_dwordx4 %[kd4], {quad(KRS)}, 0 offen lds"])
+                   f"buffer_load_dwordx4 %[kd4], {quad(KRS)}, 0 offen{nt} lds"])
     for i in range(NVP):
         groups.append(([f"s_mov_b32 m0, {SVWW}", "s_nop 0"] if i == 0 else []) +
-                      [f"buffer_load_dwordx4 %[vd], {quad(VRS)}, 0 offen offset:{1024 * i} lds"])
+                      [f"buffer_load_dwordx4 %[vd], {quad(VRS)}, 0 offen offset:{1024 * i}{nt} lds"])
     groups[0] = pre + groups[0]
     ops = []
     step = 128 * D   # K and V rows: 2 d bytes a key, 64 keys a tile
@@ -318,7 +323,7 @@ def qk_mfmas(dtype, sbuf):
     out = []
     for f in range(2 * NKK):
         kk, t = f // 2, f % 2
-        for rb in range(2):
+        for rb in range(NRB):
             src_c = "0" if kk == 0 else S(sbuf, rb, t)
             out.append((f, f"{mf} {S(sbuf, rb, t)}, {{ring}}, {Q(rb, kk)}, {src_c}"))
     return out
@@ -351,7 +356,7 @@ def pv_mfmas(dtype):
     out = []
     for f in range(4 * NDB):
         cc, db = f // NDB, f % NDB
-        for rb in range(2):
+        for rb in range(NRB):
             out.append((f, f"v_mfma_f32_32x32x16_{dtype} {O(rb, db)}, {{ring}}, {P(rb, cc)}, {O(rb, db)}"))
     return out
 
@@ -437,8 +442,8 @@ def interleave(e, reads, mfmas, valu):
 def mask(sbuf, j0):
     """Keys a row does not see become -inf: key (tile first key) + C is seen by a lane when C < its limit - 8 g - j0
     (the limit: the reference's visibility rule collapsed to `key < lim` for the lane's row)."""
-    ops = [f"v_sub_u32 {TMP[rb]}, %[lim{rb}], {j0}" for rb in range(2)]
-    elems = [(rb, t, r) for rb in range(2) for t in range(2) for r in range(16)]
+    ops = [f"v_sub_u32 {TMP[rb]}, %[lim{rb}], {j0}" for rb in range(NRB)]
+    elems = [(rb, t, r) for rb in range(NRB) for t in range(2) for r in range(16)]
     nm = 3 if SPARSE else 4   # the sparse stream keeps the fourth pair for SEW
     cmp = [f"v_cmp_lt_i32 {SMASK[i % nm]}, {32 * t + 16 * (r >> 3) + (r & 7)}, {TMP[rb]}"
            for i, (rb, t, r) in enumerate(elems)]
@@ -456,7 +461,7 @@ def mask(sbuf, j0):
 def mask_general(sbuf, j0, w):
     """Sparse masking of a tile (first key in scalar j0, validity words in the SGPR pair w): the row limit as mask(),
     then the keys whose validity bit is clear. The lane's word W_g is w shifted right by 32 g (%[g32])."""
-    ops = [f"v_sub_u32 {TMP[rb]}, %[lim{rb}], {j0}" for rb in range(2)]
+    ops = [f"v_sub_u32 {TMP[rb]}, %[lim{rb}], {j0}" for rb in range(NRB)]
     wlo = int(TMP[2][1:])
     ops.append(f"v_lshrrev_b64 v[{wlo}:{wlo + 1}], %[g32], {w}")
     for t in range(2):
@@ -486,7 +491,7 @@ def entry_loads():
 def exps(sbuf):
     """Exponentials in place: exp2(s c - m)."""
     ops = []
-    for rb in range(2):
+    for rb in range(NRB):
         for t in range(2):
             for r in range(16):
                 ops.append(f"v_fma_f32 {S(sbuf, rb, t, r)}, {S(sbuf, rb, t, r)}, %[c], {NEGMU[rb]}")
@@ -501,20 +506,20 @@ def pack_and_sum(sbuf, dtype):
     before it."""
     cvt = f"v_cvt_pk_{dtype}_f32"
     ops = []
-    for rb in range(2):
+    for rb in range(NRB):
         for cc in range(4):
             t, r0 = cc // 2, 8 * (cc % 2)
             for i in range(4):
                 ops.append(f"{cvt} {P(rb, cc, i)}, {S(sbuf, rb, t, r0 + 2 * i)}, "
                            f"{S(sbuf, rb, t, r0 + 2 * i + 1)}")
-    vals = {rb: [S(sbuf, rb, t, r) for t in range(2) for r in range(16)] for rb in range(2)}
+    vals = {rb: [S(sbuf, rb, t, r) for t in range(2) for r in range(16)] for rb in range(NRB)}
     for k in range(1, 8):       # chain c of row block rb sums values c, c + 4, c + 8, ...
-        for rb in range(2):
+        for rb in range(NRB):
             for c in range(4):
                 acc = TMP[4 * rb + c]
                 first = vals[rb][c] if k == 1 else acc
                 ops.append(f"v_add_f32 {acc}, {first}, {vals[rb][4 * k + c]}")
-    for rb in range(2):
+    for rb in range(NRB):
         a = TMP[4 * rb: 4 * rb + 4]
         ops += [f"v_add_f32 {a[0]}, {a[0]}, {a[1]}", f"v_add_f32 {a[2]}, {a[2]}, {a[3]}",
                 f"v_add_f32 {a[0]}, {a[0]}, {a[2]}"]
@@ -536,7 +541,7 @@ def q_waits(mfmas, n_groups):
     for kk in range(NKK):
         first = next(i for i, (f, _) in enumerate(mfmas) if f == 2 * kk)
         issued = sum(1 for g in range(n_groups) if g * n // n_groups < first)
-        out[2 * kk] = [f"s_waitcnt vmcnt({2 * (NKK - 1 - kk) + issued})"]
+        out[2 * kk] = [f"s_waitcnt vmcnt({NRB * (NKK - 1 - kk) + issued})"]
     return out
 
 
@@ -569,7 +574,7 @@ def exact_tile(e, dtype, sbuf, kaddr, j0, first=False, w=None):
     phase(e, "X", k_reads(kaddr), mfmas, [], fwait=q_waits(mfmas, len(dma[0])) if first else None, dma=dma)
     for op in wait_mfma() + (mask_general(sbuf, j0, w) if SPARSE else mask(sbuf, j0)):
         e(op)
-    for rb in range(2):
+    for rb in range(NRB):
         mx = TMP[2 + rb]
         vals = [S(sbuf, rb, t, r) for t in range(2) for r in range(16)]
         e(f"v_max3_f32 {mx}, {vals[0]}, {vals[1]}, {vals[2]}")
@@ -581,10 +586,10 @@ def exact_tile(e, dtype, sbuf, kaddr, j0, first=False, w=None):
             e(f"v_max_f32 {mx}, {mx}, {rest[0]}")
     # the row's maximum over both halves of the wave (lane l ^ 32), to base 2 (c > 0)
     e("s_waitcnt lgkmcnt(0)")
-    for rb in range(2):
+    for rb in range(NRB):
         e(f"ds_bpermute_b32 {TMP[4 + rb]}, %[swp], {TMP[2 + rb]}")
     e("s_waitcnt lgkmcnt(0)")
-    for rb in range(2):
+    for rb in range(NRB):
         mx, other, f = TMP[2 + rb], TMP[4 + rb], TMP[8 + rb]
         e(f"v_max_f32 {mx}, {mx}, {other}")
         e(f"v_mul_f32 {mx}, %[c], {mx}")
@@ -601,7 +606,7 @@ def exact_tile(e, dtype, sbuf, kaddr, j0, first=False, w=None):
         if not first:
             e(f"v_mul_f32 {LSUM[rb]}, {LSUM[rb]}, {f}")
     # rescale the outputs (the MFMAs that wrote them were issued before the last barrier)
-    for rb in range(2 if not first else 0):
+    for rb in range(NRB if not first else 0):
         f = TMP[8 + rb]
         for i in range(16 * NDB):
             a, tv = f"a{16 * NDB * rb + i}", TMP[10 + (i % 4)]
@@ -638,7 +643,7 @@ def low_part_pass(e):
     lo = {}
     ops_a, ops_b, ops_c = [], [], []
     k = 0
-    for rb in range(2):
+    for rb in range(NRB):
         for cc in range(4):
             t, r0 = cc // 2, 8 * (cc % 2)
             for i in range(4):
@@ -653,7 +658,7 @@ def low_part_pass(e):
     mfmas = []
     for f in range(4 * NDB):
         cc, db = f // NDB, f % NDB
-        for rb in range(2):
+        for rb in range(NRB):
             plo = f"v[{64 + 16 * rb + 4 * cc}:{64 + 16 * rb + 4 * cc + 3}]"
             mfmas.append((f, f"v_mfma_f32_32x32x16_bf16 {O(rb, db)}, {{ring}}, {plo}, {O(rb, db)}"))
     interleave(e, v_reads(), mfmas, [])
@@ -680,7 +685,7 @@ def epilogue(e, out_dtype):
     sz = {"f32": 4, "bf16": 2, "f16": 2}[out_dtype]
     row = D * sz
     inv = (TMP[1], TMP[2])
-    for rb in range(2):
+    for rb in range(NRB):
         lt = TMP[0]
         e(f"ds_bpermute_b32 {lt}, %[swp], {LSUM[rb]}")
         e("s_waitcnt lgkmcnt(0)")
@@ -702,7 +707,7 @@ def epilogue(e, out_dtype):
     # writes: piece (rb, db, r4) is head dims 32 db + 8 r4 + 4 g .. + 3 of row 32 rb + c32; its address is
     # %[ew] ^ (16 x its chunk without the lane's part), %[ew] holding the row, the lane's part and the swizzle
     n = 0
-    for rb in range(2):
+    for rb in range(NRB):
         for db in range(NDB):
             for r4 in range(4):
                 vals = [f"v{4 * n + i}" for i in range(4)]
@@ -725,7 +730,7 @@ def epilogue(e, out_dtype):
     # reads: load i covers rows (rows_i) i .. of the wave's 64 (16 lanes a row for 2-byte outputs, 32 for f32); the
     # lane's chunk swizzle depends on the row through i, folded in by an xor of %[er]
     rows_i = 1024 // row
-    n_ld = 64 // rows_i
+    n_ld = 32 * NRB // rows_i
     for i in range(n_ld):
         swz = ((rows_i * i) & 7) * 16
         addr = f"v{128 + i}"
@@ -766,17 +771,18 @@ def epilogue(e, out_dtype):
 
 # ---- the kernel body ----------------------------------------------------------------------------------------------
 
-def body(in_dtype, out_dtype, sparse=False, d=128, paged=False):
+def body(in_dtype, out_dtype, sparse=False, d=128, paged=False, rows=64):
     """The stream for one item (a workgroup's rows) at head width d; sparse: the block-sparse one (tiles from the
-    pass table, heads of 128); paged: over a cache in pages."""
-    global SPARSE, PAGED
+    pass table, heads of 128); paged: over a cache in pages, rows a wave 64 or 32."""
+    global SPARSE, PAGED, NRB, STREAMING
     assert not sparse or (d == 128 and not paged)
-    SPARSE, PAGED = sparse, paged
+    assert rows == 64 or (rows == 32 and paged)
+    SPARSE, PAGED, NRB, STREAMING = sparse, paged, rows // 32, rows == 32
     set_dim(d)
     try:
         return body_of(in_dtype, out_dtype)
     finally:
-        SPARSE = PAGED = False
+        SPARSE, PAGED, NRB, STREAMING = False, False, 2, False
         set_dim(128)
 
 
@@ -796,7 +802,7 @@ def body_of(in_dtype, out_dtype):
         e(f"v_mov_b32 {r}, 0")
     e(f"v_mov_b32 {NINF}, 0xff800000")
     e(f"v_mov_b32 {ZERO}, 0")
-    for rb in range(2):
+    for rb in range(NRB):
         e(f"v_mov_b32 {NEGMU[rb]}, 0")
         e(f"v_mov_b32 {LSUM[rb]}, 0")
         e(f"v_mov_b32 {MAXV[rb]}, {NINF}")
@@ -827,15 +833,16 @@ def body_of(in_dtype, out_dtype):
         e(f"s_mov_b32 {SD}, s88")
     for op in dma_issue():
         e(op)
-    e(f"v_add_u32 {TMP[0]}, {64 * D:#x}, %[qo]")   # row block 1: 32 rows of 2 d bytes on
+    if NRB == 2:
+        e(f"v_add_u32 {TMP[0]}, {64 * D:#x}, %[qo]")   # row block 1: 32 rows of 2 d bytes on
     for kk in range(NKK):
-        for rb in range(2):
+        for rb in range(NRB):
             e(f"buffer_load_dwordx4 {Q(rb, kk)}, {'%[qo]' if rb == 0 else TMP[0]}, %[qrs], 0 offen "
               f"offset:{32 * kk}")
     # the outputs cleared by MFMAs of zero operands: a few issue slots, the matrix unit does the rest (128
     # v_accvgpr_write took ~700 cycles of the prologue)
     z = f"v[{TMP[8][1:]}:{TMP[11][1:]}]"
-    for i in range(2 * NDB):
+    for i in range(NRB * NDB):
         e(f"v_mfma_f32_32x32x16_{in_dtype} a[{16 * i}:{16 * i + 15}], {z}, {z}, 0")
     body_rest(e, in_dtype, out_dtype)
     return e.out
@@ -846,7 +853,7 @@ def body_rest(e, in_dtype, out_dtype):
     e(f"s_mov_b32 {SBK}, 0")
     e(f"s_mov_b32 {SBV}, 0")
     # the first barrier: every wave's loads of tile 0 have landed (Q may still be in flight)
-    e(f"s_waitcnt vmcnt({2 * NKK}) lgkmcnt(0)")
+    e(f"s_waitcnt vmcnt({NRB * NKK}) lgkmcnt(0)")
     e("s_barrier")
     e("s_cmp_eq_u32 %[ntw], 0")
     e(f"s_cbranch_scc0 {lbl('L_live')}")
@@ -862,8 +869,8 @@ def body_rest(e, in_dtype, out_dtype):
     else:
         e(f"s_mov_b32 {SJX}, 0")
         exact_tile(e, in_dtype, 0, "%[kr]", SJX, first=True)
-    e(f"v_add_f32 {LSUM[0]}, {LSUM[0]}, {TMP[0]}")
-    e(f"v_add_f32 {LSUM[1]}, {LSUM[1]}, {TMP[4]}")
+    for rb in range(NRB):
+        e(f"v_add_f32 {LSUM[rb]}, {LSUM[rb]}, {TMP[4 * rb]}")
     if in_dtype == "bf16":
         low_part_pass(e)
     for op in barrier():   # every wave's loads of tile 1 have landed
@@ -894,13 +901,13 @@ def body_rest(e, in_dtype, out_dtype):
             for op in valu + iteration_last_staging():
                 e(op)
         if variant != "first":
-            e(f"v_cmp_nle_f32 {SCMP[0]}, {TMP[0]}, {S256}")
-            e(f"v_cmp_nle_f32 {SCMP[1]}, {TMP[4]}, {S256}")
+            for rb in range(NRB):
+                e(f"v_cmp_nle_f32 {SCMP[rb]}, {TMP[4 * rb]}, {S256}")
             e("s_nop 1")
-            e(f"s_or_b64 vcc, {SCMP[0]}, {SCMP[1]}")
+            e(f"s_or_b64 vcc, {SCMP[0]}, {SCMP[NRB - 1]}")
             e(f"s_cbranch_vccnz {lbl('L_exact_' + tag)}")
-            e(f"v_add_f32 {LSUM[0]}, {LSUM[0]}, {TMP[0]}")
-            e(f"v_add_f32 {LSUM[1]}, {LSUM[1]}, {TMP[4]}")
+            for rb in range(NRB):
+                e(f"v_add_f32 {LSUM[rb]}, {LSUM[rb]}, {TMP[4 * rb]}")
             e.label(f"L_back_{tag}")
             exact_v[tag] = n_v
         if variant != "last":
@@ -939,8 +946,8 @@ def body_rest(e, in_dtype, out_dtype):
         else:
             e(f"s_lshl_b32 {SJX}, {SJ}, 6")
             exact_tile(e, in_dtype, par, TMP[15], SJX)
-        e(f"v_add_f32 {LSUM[0]}, {LSUM[0]}, {TMP[0]}")
-        e(f"v_add_f32 {LSUM[1]}, {LSUM[1]}, {TMP[4]}")
+        for rb in range(NRB):
+            e(f"v_add_f32 {LSUM[rb]}, {LSUM[rb]}, {TMP[4 * rb]}")
         # the V^T reads phase QK sent ahead (their ring slots were reused here), again, as the last LDS instructions
         reads = v_reads()
         for f in range(exact_v[tag]):

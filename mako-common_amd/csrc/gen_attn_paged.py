@@ -13,12 +13,12 @@ import gen_attn_fwd_r32 as R
 
 def streams():
     """(macro name, lines) of every stream."""
-    for d in (128, 64, 256):
+    for d, rows in ((128, 64), (128, 32), (64, 64), (64, 32), (256, 32)):
         for ind in ("bf16", "f16"):
             for outd in ("f32", ind):
-                lines = R.body(ind, outd, paged=True) if d == 256 else G.body(ind, outd, d=d, paged=True)
+                lines = R.body(ind, outd, paged=True) if d == 256 else G.body(ind, outd, d=d, paged=True, rows=rows)
                 (R if d == 256 else G).check_registers(lines, paged=True)
-                yield f"MAKO_PAGED_D{d}_{ind.upper()}_{outd.upper()}", lines
+                yield f"MAKO_PAGED_D{d}_R{rows}_{ind.upper()}_{outd.upper()}", lines
 
 
 def main(path):

@@ -51,9 +51,9 @@ class Emu(E.Emu):
         return None
 
 
-def program(ind, outd, d, lines=None):
+def program(ind, outd, d, lines=None, wave_rows=64):
     r32 = d == 256
-    lines = lines or (G32.body(ind, outd, paged=True) if r32 else G.body(ind, outd, d=d, paged=True))
+    lines = lines or (G32.body(ind, outd, paged=True) if r32 else G.body(ind, outd, d=d, paged=True, rows=wave_rows))
     vreg = (R32 if r32 else R64).VREG
     out = []
     for ln in lines:
@@ -65,8 +65,8 @@ def program(ind, outd, d, lines=None):
     return E.parse(out)
 
 
-def run(heads, kv, n, ctx, page, d, ind='bf16', outd='f32', cut=None, seed=0, kgrow=0.0, missing=(), lines=None):
-    """n new rows behind ctx; cut = (ta, tb): the piece of tiles [ta, tb) (one item only). Returns the worst errors."""
+def run(heads, kv, n, ctx, page, d, ind='bf16', outd='f32', cut=None, seed=0, kgrow=0.0, missing=(), lines=None, wave_rows=64):
+    """n new rows behind ctx; cut = (ta, tb): the piece of tiles [ta, tb) (one item only); wave_rows: 64 or 32 (heads of 64 and 128). Returns the worst errors."""
     rng = np.random.default_rng(seed)
     conv = O.to_bf16_bits if ind == 'bf16' else O.to_f16_bits
     dt = O.BF16 if ind == 'bf16' else O.F16
@@ -100,9 +100,9 @@ def run(heads, kv, n, ctx, page, d, ind='bf16', outd='f32', cut=None, seed=0, kg
     for at, a in zip((Q0, K0, V0, T0), arrays):
         mem.b[at:at + a.nbytes] = np.ascontiguousarray(a).view(np.uint8).ravel()
     mem.b[O0:O0 + n * width * so] = 0xAB
-    prog, labels = program(ind, outd, d, lines)
+    prog, labels = program(ind, outd, d, lines, wave_rows)
     r32 = d == 256
-    RW = 32 if r32 else 64
+    RW = 32 if r32 else wave_rows
     K_ROW = 2 * d + 16
     K_TILE, V_TILE = 64 * K_ROW, 128 * d
     NKP = (K_TILE // 1024 - 1) // 4
