@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams p)
             if (at.first != kNone)
                 done = u32x4{at.first, at.row0, at.rows, at.kvh};
         }
-        const bool f32 = at.part || __is_same(TO, float), few = D == 256 || 2 * at.rows <= 1u << p.rshift;
+        const bool f32 = at.part || __is_same(TO, float), few = D == 256 || at.rows <= p.few;
         constexpr int kMany = D == 256 ? 32 : 64;
         if (f32 && few)
             run_piece<T, float, D, 32>(p, lds, x);
@@ -244,64 +244,89 @@ __global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams p)
     }
 }
 
-// The pieces of the item whose last one range r has: their normalised rows weighted by exp(their log-sum - the largest), D / 4
-// lanes a (row, head), four head dims each. As merge_pieces (attn_fwd64.hip), a piece with a log-sum of -inf is added with
-// weight 0, so that NaN reaches the result whichever piece it is in; a row of NaN throughout gives -inf.
-template <class TO, int D>
+// The pieces of the item whose last one range r has: their normalised rows weighted by exp(their log-sum - the largest). D / 4
+// lanes a (row, head), four head dims each; where rows are few, NW such sets take every NW-th piece and meet in LDS. A piece
+// with a log-sum of -inf is added with weight 0, so that NaN reaches the result whichever piece it is in; a row that is NaN
+// throughout in such a piece gives -inf, as in a call without pieces.
+template <class TO, int D, int NW>
 __global__ __launch_bounds__(256) void paged_merge(const PagedParams p, uint32_t per)
 {
+    constexpr uint32_t L = D / 4, U = 8 / (NW == 1 ? 2 : 1);  // U pieces' loads in flight together
+    __shared__ float s_m[NW][256 / L], s_l[NW][256 / L];
+    __shared__ f32x4 s_o[NW][256];
     const uint32_t r = blockIdx.x / per, sub = blockIdx.x % per;
     const u32x4 item = p.last[r];
-    if (item[0] == kNone)
+    const uint32_t first = item[0];
+    if (first == kNone)
         return;
-    const uint32_t t = sub * (1024 / D) + threadIdx.x / (D / 4), d = 4 * (threadIdx.x % (D / 4));
+    const uint32_t set = threadIdx.x / L, w = set % NW, t = (sub * (256 / L) + set) / NW, d = 4 * (threadIdx.x % L);
     const uint32_t hl = t % p.hq, cb = t / p.hq % p.ncb, row = t / p.hq / p.ncb;
-    if (row >= item[2])
-        return;
-    constexpr uint32_t U = 4;  // pieces whose loads are in flight together
+    const bool live = row < item[2];
     float mx = -INFINITY, sum = 0.0f;
     f32x4 acc = f32x4{};
-    for (uint32_t i0 = item[0]; i0 <= r; i0 += U) {
+    for (uint32_t i0 = first + w; live && i0 <= r; i0 += U * NW) {
         float l[U];
         f32x4 v[U];
         #pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t i = i0 + u, kind = i == item[0] ? 1 : 0;
-            const bool has = i <= r && p.whole[2 * min(i, r) + kind];
-            const size_t slot = ((size_t)min(i, r) * p.ncb + cb) * 2 + kind;
-            l[u] = has ? p.part_l[(slot * p.hq + hl) * p.slot_rows + row] : -INFINITY;
-            v[u] = has ? *reinterpret_cast<const f32x4*>(p.part_o + ((slot * p.slot_rows + row) * p.hq + hl) * D + d) : f32x4{};
+        for (uint32_t u = 0; u < U; ++u) {  // (slots that no piece is in are read too, and left out)
+            const uint32_t i = min(i0 + u * NW, r), kind = i == first ? 1 : 0;
+            const size_t slot = ((size_t)i * p.ncb + cb) * 2 + kind;
+            const bool has = i0 + u * NW <= r && p.whole[2 * i + kind];
+            const float y = p.part_l[(slot * p.hq + hl) * p.slot_rows + row];
+            const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + ((slot * p.slot_rows + row) * p.hq + hl) * D + d);
+            l[u] = has ? y * kLog2e : -INFINITY;
+            v[u] = has ? x : f32x4{};
         }
         #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
             if (l[u] == -INFINITY) {  // (the same in a row's lanes)
                 const uint64_t nan = __ballot(v[u][0] != v[u][0] && v[u][1] != v[u][1] && v[u][2] != v[u][2] && v[u][3] != v[u][3]);
-                const uint64_t lanes = D == 256 ? ~0ull : ((1ull << (D / 4 % 64)) - 1) << (threadIdx.x & 63u & ~(D / 4 - 1));
+                const uint64_t lanes = L == 64 ? ~0ull : ((1ull << (L % 64)) - 1) << (threadIdx.x & 63u & ~(L - 1));
                 acc += v[u] * 0.0f;
                 if ((nan & lanes) == lanes)
                     sum = NAN;
                 continue;
             }
-            const float m = fmaxf(mx, l[u]);
-            const float a = exp2_fast((mx - m) * kLog2e), b = exp2_fast((l[u] - m) * kLog2e);
+            const float m = fmaxf(mx, l[u]), a = exp2_fast(mx - m), b = exp2_fast(l[u] - m);
             sum = sum * a + b;
             acc = acc * a + v[u] * b;
             mx = m;
         }
     }
+    if (NW > 1) {
+        if (threadIdx.x % L == 0) {
+            s_m[w][set / NW] = mx;
+            s_l[w][set / NW] = sum;
+        }
+        s_o[w][set / NW * L + threadIdx.x % L] = acc;
+        __syncthreads();
+        if (w != 0)
+            return;
+        #pragma unroll
+        for (uint32_t i = 1; i < NW; ++i) {
+            const float mi = s_m[i][set / NW], m = fmaxf(mx, mi);
+            const float a = mx == -INFINITY ? 1.0f : exp2_fast(mx - m), b = mi == -INFINITY ? 1.0f : exp2_fast(mi - m);
+            sum = sum * a + s_l[i][set / NW] * b;  // (without a piece: zeros, or NaN)
+            acc = acc * a + s_o[i][set / NW * L + threadIdx.x % L] * b;
+            mx = m;
+        }
+    }
+    if (!live)
+        return;
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
     const uint32_t h = item[3] * p.group + cb * p.hq + hl, at = item[1] + row;
     store4<TO>(static_cast<TO*>(p.o) + (size_t)at * p.width + (size_t)h * D + d, acc[0] * inv, acc[1] * inv, acc[2] * inv,
                acc[3] * inv);
     if (p.lse && d == 0)
-        p.lse[(size_t)h * p.rows + at] = sum > 0.0f ? mx + __log2f(sum) * kLn2 : -INFINITY;
+        p.lse[(size_t)h * p.rows + at] = sum > 0.0f ? (mx + __log2f(sum)) * kLn2 : -INFINITY;
 }
 
 // A call's split, from its sizes alone (lengths are known on the device only).
 struct Plan {
-    uint32_t hq, rshift, ncb, n_ranges, slot_rows, direct;
+    uint32_t hq, rshift, ncb, n_ranges, slot_rows, direct, few;
 };
 constexpr uint32_t kDirectTiles = 8;
+constexpr uint32_t kFewMerged = 16;  // (row, head) pairs a range up to which paged_merge parts an item's pieces
 
 Plan plan_of(const mako_paged_args* a, uint32_t cus)
 {
@@ -309,6 +334,7 @@ Plan plan_of(const mako_paged_args* a, uint32_t cus)
     Plan pl{};
     pl.hq = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
     pl.rshift = log2_of((a->dim == 256 ? 128 : 256) / pl.hq);
+    pl.few = a->dim == 256 ? 0 : 128 / pl.hq;
     pl.ncb = group / pl.hq;
     pl.n_ranges = std::max(1u, cus / pl.ncb);
     if (pl.n_ranges > 8)
@@ -334,8 +360,11 @@ void launch(const PagedParams& p, hipStream_t s)
     hipLaunchKernelGGL((paged_rows<T, TO, D>), dim3(p.n_ranges * p.ncb), dim3(256), 0, s, p);
     if (p.direct)
         return;
-    const uint32_t per = (p.slot_rows * p.group * D + 1023) / 1024;
-    hipLaunchKernelGGL((paged_merge<TO, D>), dim3(p.n_ranges * per), dim3(256), 0, s, p, per);
+    const uint32_t nw = p.slot_rows * p.group <= kFewMerged ? 4 : 1, per = (p.slot_rows * p.group * nw * D + 1023) / 1024;
+    if (nw == 4)
+        hipLaunchKernelGGL((paged_merge<TO, D, 4>), dim3(p.n_ranges * per), dim3(256), 0, s, p, per);
+    else
+        hipLaunchKernelGGL((paged_merge<TO, D, 1>), dim3(p.n_ranges * per), dim3(256), 0, s, p, per);
 }
 
 template <class T, class TO>
@@ -383,8 +412,8 @@ int check_args(const mako_paged_args* a, mako_dtype in, mako_dtype out, const vo
     if ((uint64_t)a->heads * a->dim > a->width || a->width % 4 || a->width >= (1u << 20))
         return fail(MAKO_EINVAL, "%s: o rows of %u for %u heads of %u (a multiple of 4, at least their width, below 2^20)",
                     what, a->width, a->heads, a->dim);
-    // what the split counts: 32 keys a unit, for every 32 rows of a sequence at least
-    const uint64_t units = ((uint64_t)a->rows / 32 + a->batch) * ((uint64_t)a->max_ctx / 32 + 512) * a->kv_heads;
+    // what the split counts: at most kTile units a tile, for every 32 rows of a sequence at least
+    const uint64_t units = ((uint64_t)a->rows / 32 + a->batch) * ((uint64_t)a->max_ctx / 10 + 512) * a->kv_heads;
     if (units >= (1ull << 32) || (uint64_t)a->rows * a->heads >= (1u << 30))
         return fail(MAKO_EINVAL, "%s: %u rows of %u heads over %u keys are too many", what, a->rows, a->heads, a->max_ctx);
     if (!(a->scale > 0.0f) || a->scale == INFINITY)
@@ -426,7 +455,7 @@ extern "C" int mako_attn_paged(const mako_paged_args* a, mako_dtype in, mako_dty
     const size_t ob = part_o_bytes(pl, a->dim), lb = part_l_bytes(pl), wb = (size_t)pl.n_ranges * 8;
     const auto at = [&](size_t off) { return ws ? ws + off : nullptr; };
     const PagedParams p{{starts, ctx_len, a->batch, a->rows, a->kv_heads, a->max_new, a->max_ctx, pl.rshift, pl.n_ranges,
-                         pl.direct},
+                         pl.direct, pl.few},
                         q, k, v, table, o, lse, reinterpret_cast<float*>(at(0)), reinterpret_cast<float*>(at(ob)),
                         reinterpret_cast<uint32_t*>(at(ob + lb + 2 * wb)), reinterpret_cast<u32x4*>(at(ob + lb)), a->q_pad,
                         a->heads / a->kv_heads, a->pages, a->kv_heads * a->page * a->dim * 2, log2_of(a->page),

@@ -2,8 +2,11 @@
 // only, so every workgroup works it out.
 //
 // An item is a block of R = 1 << rshift rows of a sequence and a kv head; its tiles are the 64 keys each up to its last row's.
-// Its cost is its keys, in units of 32, and kLead for what it costs beside them. The items of all (sequence, kv head)
-// segments lie end to end and are cut into equal ranges, one a workgroup. Within a segment the row blocks go heavy and light
+// Its cost is kTile units a tile (kTileFew in a sequence of at most `few` rows) and kLead (kLeadFew) for what it costs beside
+// them. The items of all (kv head, sequence)
+// segments lie end to end, a kv head's sequences together, and are cut into equal ranges, one a workgroup: ranges side by side
+// on an XCD share keys, and every XCD has its part of each sequence (with a sequence's kv heads together, a batch's single
+// tokens met on one XCD, whose reads bound the call: 16 MB of a mixed batch of 224 us took it 207 of 180). Within a segment the row blocks go heavy and light
 // in turn (the last, the first, the last but one, the second, ...), so two neighbours cost the same everywhere, and the ranges of a whole
 // prompt fall on items' ends. A cut inside an item leaves kLeast tiles on either side, and no row without keys in a piece's
 // first tile, which the attention's streams rely on; with `direct`, items are not cut: the range of an item's middle has it.
@@ -14,12 +17,15 @@
 
 namespace mako {
 
-constexpr uint32_t kLead = 8;
-constexpr uint32_t kLeast = 3;
+// The streams' tiles and pieces side by side in a mixed batch, in units of 0.28 us: 64 rows a wave 1.7 us a tile and 8 a piece,
+// 32 rows 1.1 and 5 (a tile of these alone on a full chip: 1.6 and 0.9). With a tile of 32 rows at half of one of 64 the
+// workgroups that met single tokens ended at 220 us, the others at 175.
+constexpr uint32_t kTile = 6, kTileFew = 4, kLead = 30, kLeadFew = 18;
+constexpr uint32_t kLeast = 3;  // tiles of a piece
 
 struct PagedSplit {
     const uint32_t *starts, *ctx;
-    uint32_t batch, rows, kv_heads, max_new, max_ctx, rshift, n_ranges, direct;
+    uint32_t batch, rows, kv_heads, max_new, max_ctx, rshift, n_ranges, direct, few;
 };
 
 // A piece of an item: tiles [ta, tb) of sequence b for its rows row0 .. of o, the first at position p0.
@@ -31,10 +37,10 @@ struct PagedPiece {
     uint32_t first;       // where it is an item's last piece of several: the range that the item starts in (else kNoPage)
 };
 
-// A sequence's new rows n, from row s0, behind c cache rows, keys with them, in nqb blocks; lead: units of an item whatever
-// its block.
+// A sequence's new rows n, from row s0, behind c cache rows, keys with them, in nqb blocks. Block qb's item is lead + (qb + 1)
+// step units.
 struct PagedSeq {
-    uint32_t c, n, s0, keys, nqb, lead;
+    uint32_t c, n, s0, keys, nqb, lead, step, few;
 };
 __device__ __forceinline__ PagedSeq seq_of(const PagedSplit& p, uint32_t b)
 {
@@ -45,26 +51,29 @@ __device__ __forceinline__ PagedSeq seq_of(const PagedSplit& p, uint32_t b)
     s.c = min(p.ctx[b], p.max_ctx);
     s.keys = s.c + min(s.n, p.max_ctx - s.c);
     s.nqb = (s.n + (1u << p.rshift) - 1) >> p.rshift;
-    s.lead = kLead + (s.c + 31) / 32;
+    s.few = s.n <= p.few ? 1 : 0;
+    const uint32_t tiles = (s.c + 63) / 64;
+    s.lead = s.few ? kLeadFew + tiles * kTileFew : kLead + tiles * kTile;
+    s.step = ((1u << p.rshift) * (s.few ? kTileFew : kTile)) / 64;
     return s;
 }
-__device__ __forceinline__ PagedSeq uniform_seq(const PagedSeq& s)
+// Sequence b, from the lane that holds it (lane b % 64).
+__device__ __forceinline__ PagedSeq of_lane(const PagedSeq& s, uint32_t b)
 {
-    return {uniform(s.c), uniform(s.n), uniform(s.s0), uniform(s.keys), uniform(s.nqb), uniform(s.lead)};
+    const uint32_t l = b % 64;
+    const auto at = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane(x, l); };
+    return {at(s.c), at(s.n), at(s.s0), at(s.keys), at(s.nqb), at(s.lead), at(s.step), at(s.few)};
 }
-__device__ __forceinline__ uint32_t item_units(const PagedSplit& p, const PagedSeq& s, uint32_t qb)
+__device__ __forceinline__ uint32_t item_units(const PagedSeq& s, uint32_t qb) { return s.lead + (qb + 1) * s.step; }
+__device__ __forceinline__ uint32_t segment_units(const PagedSeq& s)
 {
-    return s.lead + ((qb + 1) << (p.rshift - 5));
-}
-__device__ __forceinline__ uint32_t segment_units(const PagedSplit& p, const PagedSeq& s)
-{
-    return s.nqb * s.lead + ((s.nqb * (s.nqb + 1) / 2) << (p.rshift - 5));
+    return s.nqb * s.lead + s.nqb * (s.nqb + 1) / 2 * s.step;
 }
 
 // The tile that unit u of an item of nt tiles falls to (those from tmax on stay together).
-__device__ __forceinline__ uint32_t cut_of(const PagedSplit& p, uint32_t u, uint32_t nt, uint32_t tmax)
+__device__ __forceinline__ uint32_t cut_of(const PagedSplit& p, uint32_t u, uint32_t few, uint32_t nt, uint32_t tmax)
 {
-    const uint32_t t = (max(u, kLead) - kLead) / 2;
+    const uint32_t t = few ? (max(u, kLeadFew) - kLeadFew) / kTileFew : (max(u, kLead) - kLead) / kTile;
     if (p.direct)
         return 2 * t < nt ? 0u : nt;
     return t < kLeast ? 0u : t + kLeast > nt ? nt : min(t, tmax);
@@ -74,43 +83,44 @@ __device__ __forceinline__ uint32_t cut_of(const PagedSplit& p, uint32_t u, uint
 template <class F>
 __device__ __forceinline__ void walk_range(const PagedSplit& p, uint32_t range, uint32_t lane, F piece)
 {
-    // The units of all segments; up to 64 sequences are looked up once, a lane each.
+    // The units of all segments; a lane holds a sequence, so up to 64 are looked up once.
+    PagedSeq mine{};
     uint32_t total = 0, units = 0, inc = 0;
+    const auto look_up = [&](uint32_t i0) __attribute__((always_inline)) {
+        mine = seq_of(p, min(i0 + lane, p.batch - 1));
+        units = i0 + lane < p.batch ? segment_units(mine) : 0u;
+        inc = scan_lanes(units);
+    };
     for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
-        units = i0 + lane < p.batch ? segment_units(p, seq_of(p, i0 + lane)) : 0u;
-        inc = scan_lanes(units * p.kv_heads);
+        look_up(i0);
         total += (uint32_t)__builtin_amdgcn_readlane(inc, 63);
     }
-    const uint32_t n = min(p.n_ranges, total);
+    const uint32_t n = min(p.n_ranges, total * p.kv_heads);
     if (range >= n)
         return;
-    const Ranges rg(total, n);
+    const Ranges rg(total * p.kv_heads, n);
     const uint32_t x0 = rg.start(range);
     uint32_t left = rg.start(range + 1) - x0;
-    // The sequence b whose segments (from unit `at` on, len units each) hold x0.
-    uint32_t b = 0, at = 0, len = 1;
-    for (uint32_t i0 = 0, base = 0; i0 < p.batch; i0 += 64) {
-        if (p.batch > 64) {
-            units = i0 + lane < p.batch ? segment_units(p, seq_of(p, i0 + lane)) : 0u;
-            inc = scan_lanes(units * p.kv_heads);
-        }
-        if (const uint64_t hit = __ballot(x0 < base + inc)) {
+    // Of kv head kvh, the sequence b whose segment holds x0, u0 units into it.
+    uint32_t b = 0, kvh = x0 / total, u0 = x0 % total, item;
+    for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
+        if (p.batch > 64)
+            look_up(i0);
+        if (const uint64_t hit = __ballot(u0 < inc)) {
             const uint32_t l = (uint32_t)__builtin_ctzll(hit);
             b = i0 + l;
-            len = (uint32_t)__builtin_amdgcn_readlane(units, l);
-            at = base + (uint32_t)__builtin_amdgcn_readlane(inc, l) - len * p.kv_heads;
+            u0 -= (uint32_t)__builtin_amdgcn_readlane(inc - units, l);
             break;
         }
-        base += (uint32_t)__builtin_amdgcn_readlane(inc, 63);
+        u0 -= (uint32_t)__builtin_amdgcn_readlane(inc, 63);
     }
-    PagedSeq s = uniform_seq(seq_of(p, b));
-    uint32_t kvh = (x0 - at) / len, u0 = (x0 - at) % len, item;
+    PagedSeq s = of_lane(mine, b);
     {
         // item 2 i is block nqb - 1 - i, item 2 i + 1 block i: a pair's units do not depend on i
-        const uint32_t pair = 2 * s.lead + ((s.nqb + 1) << (p.rshift - 5)), i = u0 / pair;
+        const uint32_t pair = 2 * s.lead + (s.nqb + 1) * s.step, i = u0 / pair;
         u0 -= i * pair;
         item = 2 * i;
-        const uint32_t heavy = item_units(p, s, s.nqb - 1 - i);
+        const uint32_t heavy = item_units(s, s.nqb - 1 - i);
         if (u0 >= heavy) {
             u0 -= heavy;
             ++item;
@@ -119,13 +129,13 @@ __device__ __forceinline__ void walk_range(const PagedSplit& p, uint32_t range, 
     uint32_t start = x0 - u0;  // the item's first unit
     for (;;) {
         const uint32_t qb = item & 1 ? item / 2 : s.nqb - 1 - item / 2;
-        const uint32_t cost = item_units(p, s, qb), u1 = min(cost, u0 + left), i0 = qb << p.rshift;
+        const uint32_t cost = item_units(s, qb), u1 = min(cost, u0 + left), i0 = qb << p.rshift;
         PagedPiece x;
         x.b = b, x.kvh = kvh, x.row0 = s.s0 + i0, x.rows = min(1u << p.rshift, s.n - i0), x.p0 = s.c + i0;
         x.seen = s.keys, x.keys = min(x.p0 + x.rows, s.keys);
         const uint32_t nt = (x.keys + 63) / 64, tmax = (min(x.p0 + 1, s.keys) - 1) / 64;
-        x.ta = cut_of(p, u0, nt, tmax);
-        x.tb = u1 == cost ? nt : cut_of(p, u1, nt, tmax);
+        x.ta = cut_of(p, u0, s.few, nt, tmax);
+        x.tb = u1 == cost ? nt : cut_of(p, u1, s.few, nt, tmax);
         if (x.ta < x.tb) {
             x.part = x.ta != 0 || x.tb != nt;
             x.kind = u0 == 0 ? 1 : 0;
@@ -150,14 +160,16 @@ __device__ __forceinline__ void walk_range(const PagedSplit& p, uint32_t range, 
         u0 = 0;
         if (++item == s.nqb) {
             item = 0;
-            if (++kvh == p.kv_heads) {
-                kvh = 0;
-                do {
-                    if (++b >= p.batch)
+            do {
+                if (++b == p.batch) {
+                    b = 0;
+                    if (++kvh == p.kv_heads)
                         return;  // (not where the lengths are as they were when the units were summed)
-                    s = uniform_seq(seq_of(p, b));
-                } while (s.nqb == 0);
-            }
+                }
+                if (b % 64 == 0 && p.batch > 64)
+                    look_up(b);
+                s = of_lane(mine, b);
+            } while (s.nqb == 0);
         }
     }
 }

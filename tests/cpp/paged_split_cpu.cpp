@@ -60,8 +60,9 @@ bool run(mako::PagedSplit p, bool good)
         CHECK(x.ta < x.tb && x.keys <= p.max_ctx && x.seen <= p.max_ctx && 64 * (x.tb - 1) < x.keys);
         CHECK(64 * x.ta < std::min(x.p0 + 1, x.seen));  // the first row sees a key of the piece's first tile
         CHECK(x.ta == 0 || !p.direct);
-        cost[g.range] += x.tb - x.ta + 4;
-        all += x.tb - x.ta + 4;
+        const double few = x.rows <= p.few && x.seen - x.p0 <= p.few ? mako::kTileFew : mako::kTile;
+        cost[g.range] += (x.tb - x.ta) * few + mako::kLead;
+        all += (x.tb - x.ta) * few + mako::kLead;
         if (x.part)
             CHECK(slots[{g.range, x.kind}]++ == 0);
         if (!good)
@@ -93,7 +94,7 @@ bool run(mako::PagedSplit p, bool good)
     for (const auto& c : cost)
         most = std::max(most, c.second);
     // no range has more than its share and a little
-    CHECK(p.direct || most <= all / p.n_ranges + 3 * R / 64 + 4 * (items / p.n_ranges + 2) + 16);
+    CHECK(p.direct || most <= all / p.n_ranges + mako::kTile * (3 * R / 64 + 8) + mako::kLead * (items / p.n_ranges + 3));
     return true;
 }
 
@@ -113,7 +114,8 @@ int main()
             top = std::max(top, ctx[b] + starts[b + 1] - starts[b]);
         }
         mako::PagedSplit p{most == 1 ? nullptr : starts.data(), ctx.data(), batch, starts[batch] + upto(3), 1 + upto(8), most,
-                           top + upto(1) * upto(500), 5 + upto(3), round % 2 ? 256 : 1 + upto(100), upto(5) == 0};
+                           top + upto(1) * upto(500), 5 + upto(3), round % 2 ? 256 : 1 + upto(100), upto(5) == 0, 0};
+        p.few = upto(2) ? 1u << p.rshift >> 1 : 0;
         if (p.starts == nullptr)
             p.rows = batch;
         good &= run(p, true);
