@@ -325,8 +325,20 @@ __global__ __launch_bounds__(256) void paged_merge(const PagedParams p, uint32_t
 struct Plan {
     uint32_t hq, rshift, ncb, n_ranges, slot_rows, direct, few;
 };
-constexpr uint32_t kDirectTiles = 8;
+
 constexpr uint32_t kFewMerged = 16;  // (row, head) pairs a range up to which paged_merge parts an item's pieces
+
+// Whole items and no second launch up to this many tiles a sequence: 11, where a merge joins more rows 17, and more the
+// nearer the items come to one a workgroup. us split / direct, single tokens, 32 heads of 128 over 8: 8 items of 8 tiles 15.6 /
+// 12.7, of 12 16.2 / 15.9, of 16 16.3 / 18.9; 64 of 12 15.9 / 16.4; 128 of 16 21.6 / 20.4, of 26 27.2 / 28.8; 256 of 33 48 / 46.
+// 16 heads of 256 over 2: 8 items of 8 17.8 / 16.4, of 12 18.0 / 20.5; 128 of 33 63 / 62. 256 rows of 32 heads: 32 items of 16
+// 28.8 / 27.7, of 24 31.5 / 36.8; 128 of 24 41 / 37. A workgroup takes its item's tiles one after the other whatever the
+// others' lengths, so the limit also bounds what one long sequence among short ones costs.
+uint32_t direct_tiles(uint64_t items, uint32_t ranges, bool many)
+{
+    const uint64_t x = std::min<uint64_t>(items * 30 / ranges, 30);
+    return (many ? 17 : 11) + (x > 7 ? (uint32_t)x - 7 : 0);
+}
 
 Plan plan_of(const mako_paged_args* a, uint32_t cus)
 {
@@ -340,7 +352,8 @@ Plan plan_of(const mako_paged_args* a, uint32_t cus)
     if (pl.n_ranges > 8)
         pl.n_ranges &= ~7u;
     pl.slot_rows = std::min(1u << pl.rshift, a->max_new);
-    pl.direct = (a->max_ctx + 63) / 64 <= kDirectTiles;
+    const uint64_t items = ((uint64_t)(a->rows >> pl.rshift) + a->batch) * a->kv_heads;
+    pl.direct = (a->max_ctx + 63) / 64 <= direct_tiles(items, pl.n_ranges, pl.slot_rows * group > kFewMerged);
     return pl;
 }
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }

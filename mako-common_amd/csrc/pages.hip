@@ -24,6 +24,7 @@ constexpr int kPlan = 1024;           // threads of the planning workgroups
 constexpr uint32_t kMaxSeqs = 4096;   // sequences that reserve_plan takes
 constexpr uint32_t kSlots = 2 * kMaxSeqs;
 constexpr uint32_t kLook = 8;         // refs a thread looks at a round
+constexpr uint64_t kForkSmall = 4096; // table entries that one workgroup forks alone
 constexpr uint32_t kFew = 2;          // entries of a sequence that one thread goes through alone
 
 // ---- write ---------------------------------------------------------------------------------------------------------
@@ -128,18 +129,26 @@ __device__ __forceinline__ void load_refs(const uint32_t* refs, uint32_t p, uint
     }
 }
 
+// Arrays that a call copies before it changes the copies: by the planning workgroup itself where they are short
+// (kCopyInPlan words; a launch of its own takes longer), else by copy_words before it.
 struct CopyWords {
     const uint32_t* from[3];
     uint32_t* to[3];
     uint64_t n[3];
     uint32_t groups;
 };
-__global__ __launch_bounds__(256) void copy_words(const CopyWords p)
+constexpr uint64_t kCopyInPlan = 16384;
+__device__ __forceinline__ void copy_share(const CopyWords& p, uint64_t thread, uint64_t all)
 {
     #pragma unroll
     for (int a = 0; a < 3; ++a)
-        for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < p.n[a]; i += (uint64_t)p.groups * 256)
+        #pragma unroll 4
+        for (uint64_t i = thread; i < p.n[a]; i += all)
             p.to[a][i] = p.from[a][i];
+}
+__global__ __launch_bounds__(256) void copy_words(const CopyWords p)
+{
+    copy_share(p, (uint64_t)blockIdx.x * 256 + threadIdx.x, (uint64_t)p.groups * 256);
 }
 
 // Rows [0, rows) of page src over page dst, in every layer and kv head.
@@ -194,6 +203,7 @@ struct ReserveParams {
     Move* moves;      // [batch]
     uint32_t* list;   // free pages, in order
     uint32_t batch, rows, pages, shift, max_pages, list_max;
+    CopyWords copy;   // (done before any entry is given)
 };
 
 __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
@@ -205,6 +215,7 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
     const uint32_t tid = threadIdx.x, lane = tid & 63u, cap = p.max_pages << p.shift, in_page = (1u << p.shift) - 1;
     if (tid == 0)
         s_any = s_moves = 0;
+    copy_share(p.copy, tid, kPlan);
     __syncthreads();
 
     // The entries [first, last) that the new rows [c, end) of sequence b fall into.
@@ -383,21 +394,23 @@ struct ForkParams {
     const uint32_t *parent, *keep, *table, *ctx;
     uint32_t *table_out, *refs_out, *ctx_out;
     uint32_t batch, pages, shift, max_pages;
+    CopyWords copy;
 };
 
-__global__ __launch_bounds__(256) void fork_rows(const ForkParams p)
+// New sequence i, by `threads` threads.
+__device__ __forceinline__ void fork_row(const ForkParams& p, uint32_t i, uint32_t thread, uint32_t threads)
 {
-    const uint32_t i = blockIdx.x, cap = p.max_pages << p.shift;
+    const uint32_t cap = p.max_pages << p.shift;
     const uint32_t src = p.parent ? p.parent[i] : i;
     uint32_t c = 0;
     if (src < p.batch)
         c = min(min(p.keep ? p.keep[i] : ~0u, p.ctx[src]), cap);
     const uint32_t kept = (c + (1u << p.shift) - 1) >> p.shift;
-    if (threadIdx.x == 0)
+    if (thread == 0)
         p.ctx_out[i] = c;
     const uint32_t* from = p.table + (size_t)(src < p.batch ? src : i) * p.max_pages;
     const uint32_t* old = p.table + (size_t)i * p.max_pages;
-    for (uint32_t j = threadIdx.x; j < p.max_pages; j += 256) {
+    for (uint32_t j = thread; j < p.max_pages; j += threads) {
         const uint32_t was = old[j];
         uint32_t e = j < kept ? from[j] : kNoPage;
         if (e >= p.pages)
@@ -410,6 +423,16 @@ __global__ __launch_bounds__(256) void fork_rows(const ForkParams p)
         if (was < p.pages)
             atomicSub(&p.refs_out[was], 1u);
     }
+}
+__global__ __launch_bounds__(256) void fork_rows(const ForkParams p) { fork_row(p, blockIdx.x, threadIdx.x, 256); }
+
+// A small call whole, by one workgroup: the copies, then a wave a sequence.
+__global__ __launch_bounds__(kPlan) void fork_small(const ForkParams p)
+{
+    copy_share(p.copy, threadIdx.x, kPlan);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x >> 6; i < p.batch; i += kPlan / 64)
+        fork_row(p, i, threadIdx.x & 63u, 64);
 }
 
 // ---- compact -------------------------------------------------------------------------------------------------------
@@ -424,9 +447,10 @@ struct CompactParams {
     uint32_t batch, pages, shift, max_pages, most;
 };
 
+constexpr uint32_t kHolesHere = 16384;  // holes that are listed in LDS
 __global__ __launch_bounds__(kPlan) void compact_plan(const CompactParams p)
 {
-    __shared__ uint32_t s_wave[kPlan / 64];
+    __shared__ uint32_t s_wave[kPlan / 64], s_hole[kHolesHere];
     const uint32_t tid = threadIdx.x;
     uint32_t mine = 0, used;
     for (uint32_t at = tid * kLook; at < p.pages; at += kPlan * kLook) {
@@ -457,10 +481,15 @@ __global__ __launch_bounds__(kPlan) void compact_plan(const CompactParams p)
             const uint32_t page = at + i;
             if (page >= used)
                 continue;
-            if (x[i] == 0)
-                p.hole[h++] = page;
-            else
+            if (x[i] == 0) {
+                if (h < kHolesHere)
+                    s_hole[h] = page;
+                else
+                    p.hole[h] = page;
+                ++h;
+            } else {
                 p.refs_out[page] = x[i];
+            }
             p.map[page] = x[i] ? page : kNoPage;
         }
         __syncthreads();
@@ -471,7 +500,7 @@ __global__ __launch_bounds__(kPlan) void compact_plan(const CompactParams p)
                 continue;
             uint32_t to = kNoPage;
             if (x[i] != 0) {
-                to = p.hole[s];
+                to = s < kHolesHere ? s_hole[s] : p.hole[s];
                 p.moves[s++] = Move{page, to, 1u << p.shift, 0u};
                 p.refs_out[to] = x[i];
             }
@@ -550,19 +579,22 @@ uint64_t compact_most(const mako_pages_args* a) { return a->pages / 2; }
 
 uint32_t groups_for(uint64_t items) { return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(items, 2048)); }
 
-void launch_copy(const uint32_t* const (&from)[3], uint32_t* const (&to)[3], const uint64_t (&n)[3], hipStream_t s)
+CopyWords copies_of(const uint32_t* const (&from)[3], uint32_t* const (&to)[3], const uint64_t (&n)[3])
 {
     CopyWords c{};
-    uint64_t most = 0;
     for (int i = 0; i < 3; ++i)
-        if (to[i] && from[i] != to[i]) {
+        if (to[i] && from[i] != to[i])
             c.from[i] = from[i], c.to[i] = to[i], c.n[i] = n[i];
-            most = std::max(most, n[i]);
-        }
-    if (!most)
+    return c;
+}
+// Copies more than `most` words by a launch, and leaves c empty then.
+void launch_long(CopyWords& c, uint64_t most, hipStream_t s)
+{
+    if (c.n[0] + c.n[1] + c.n[2] <= most)
         return;
-    c.groups = groups_for((most + 1023) / 1024);
+    c.groups = groups_for((std::max({c.n[0], c.n[1], c.n[2]}) + 1023) / 1024);
     hipLaunchKernelGGL(copy_words, dim3(c.groups), dim3(256), 0, s, c);
+    c = CopyWords{};
 }
 
 }  // namespace
@@ -621,15 +653,15 @@ extern "C" int mako_pages_reserve(const mako_pages_args* a, const uint32_t* tabl
     if (const int rc = check_workspace(what, workspace, workspace_bytes, mako_pages_reserve_workspace(a)))
         return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    launch_copy({table, refs, nullptr}, {table_out, refs_out, nullptr}, {(uint64_t)a->batch * a->max_pages, a->pages, 0}, s);
-    if (!a->batch)
-        return check_launch(what);
+    CopyWords copy = copies_of({table, refs, nullptr}, {table_out, refs_out, nullptr},
+                               {(uint64_t)a->batch * a->max_pages, a->pages, 0});
+    launch_long(copy, kCopyInPlan, s);
     char* ws = static_cast<char*>(workspace);
     uint32_t* count = reinterpret_cast<uint32_t*>(ws);
     Move* moves = reinterpret_cast<Move*>(ws + 16);
     const ReserveParams p{table, refs, starts, ctx_len, table_out, refs_out, ctx_out, count, moves,
                           reinterpret_cast<uint32_t*>(ws + 16 + (size_t)a->batch * sizeof(Move)), a->batch, a->rows,
-                          a->pages, log2_of(a->page), a->max_pages, (uint32_t)reserve_most(a)};
+                          a->pages, log2_of(a->page), a->max_pages, (uint32_t)reserve_most(a), copy};
     hipLaunchKernelGGL(reserve_plan, dim3(1), dim3(kPlan), 0, s, p);
     if (k) {
         const uint32_t groups = groups_for((uint64_t)a->batch * a->layers * a->kv_heads);
@@ -667,13 +699,16 @@ extern "C" int mako_pages_fork(const mako_pages_args* a, const uint32_t* parent,
     const uint64_t entries = (uint64_t)a->batch * a->max_pages;
     uint32_t* table_ws = static_cast<uint32_t*>(workspace);
     uint32_t* ctx_ws = in_place ? table_ws + round16(entries * 4) / 4 : nullptr;
-    launch_copy({in_place ? table : nullptr, refs, in_place ? ctx_len : nullptr},
-                {in_place ? table_ws : nullptr, refs_out, ctx_ws}, {entries, a->pages, a->batch}, s);
-    if (!a->batch)
-        return check_launch(what);
+    CopyWords copy = copies_of({in_place ? table : nullptr, refs, in_place ? ctx_len : nullptr},
+                               {in_place ? table_ws : nullptr, refs_out, ctx_ws}, {entries, a->pages, a->batch});
+    const bool small = entries <= kForkSmall;
+    launch_long(copy, small ? kCopyInPlan : 0, s);
     const ForkParams p{parent, keep, in_place ? table_ws : table, in_place ? ctx_ws : ctx_len, table_out, refs_out,
-                       ctx_out, a->batch, a->pages, log2_of(a->page), a->max_pages};
-    hipLaunchKernelGGL(fork_rows, dim3(a->batch), dim3(256), 0, s, p);
+                       ctx_out, a->batch, a->pages, log2_of(a->page), a->max_pages, copy};
+    if (small)
+        hipLaunchKernelGGL(fork_small, dim3(1), dim3(kPlan), 0, s, p);
+    else
+        hipLaunchKernelGGL(fork_rows, dim3(a->batch), dim3(256), 0, s, p);
     return check_launch(what);
 }
 
