@@ -170,7 +170,7 @@ __device__ __forceinline__ void move_rows(const MoveParams& p, uint64_t item)
     const uint32_t n = m.rows * p.cpr;
     const size_t src = (((layer * p.pages + m.src) * p.kv_heads + h) << p.shift) * p.cpr;
     const size_t dst = (((layer * p.pages + m.dst) * p.kv_heads + h) << p.shift) * p.cpr;
-    constexpr int U = 4;
+    constexpr int U = 8;
     for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 256 * U) {
         u32x4 a[U], b[U];
         #pragma unroll
@@ -182,8 +182,8 @@ __device__ __forceinline__ void move_rows(const MoveParams& p, uint64_t item)
         #pragma unroll
         for (int u = 0; u < U; ++u)
             if (i0 + 256 * u < n) {
-                p.k[dst + i0 + 256 * u] = a[u];
-                p.v[dst + i0 + 256 * u] = b[u];
+                __builtin_nontemporal_store(a[u], p.k + dst + i0 + 256 * u);
+                __builtin_nontemporal_store(b[u], p.v + dst + i0 + 256 * u);
             }
     }
 }
