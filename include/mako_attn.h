@@ -330,9 +330,9 @@ int mako_cache_evict(const mako_evict_args* a, mako_dtype in, void* k, void* v, 
  * table does not name in it, have no part, whatever they hold; a v that is not finite among a sequence's own new rows may
  * make rows before it in its 64 rows (counted from the sequence's start) not finite.
  * dim 64, 128 or 256. Precision as mako_attn_fwd: P rounded to the input type for P V, sums and lse of the f32
- * exponentials; rows that see fewer than 64 keys get bf16 probabilities to ~16 bits. workspace: at least
- * mako_attn_paged_workspace(a) bytes, 16-byte aligned; its contents do not matter, and calls that overlap in time need
- * separate ones. width a multiple of 4; o must not overlap the inputs.
+ * exponentials; rows that see fewer than 64 keys (heads of 256: fewer than 32) get bf16 probabilities to ~16 bits.
+ * workspace: at least mako_attn_paged_workspace(a) bytes, 16-byte aligned; its contents do not matter, and calls that
+ * overlap in time need separate ones. width a multiple of 4; o must not overlap the inputs.
  */
 typedef struct mako_paged_args {
     uint32_t batch;     /* sequences */

@@ -10,10 +10,13 @@
 // * paged_rows runs the streams of flash_fwd_r64 (heads of 64 and 128) and flash_fwd_r32 (256) over pages
 //   (gen_attn_paged.py): a tile is 64 keys, a run of memory within a page; its page's number is read by a scalar load an
 //   iteration before the tile is staged.
-// * An item is a block of R rows of a sequence and `hq` heads of a kv head (4, 2 or 1, as they divide the group), R = 256 / hq
-//   (heads of 256: 128 / hq): one workgroup's four waves, 64 (32) rows each. Items of half the rows or fewer take the stream of
-//   32 rows a wave. A group of more heads takes further workgroups (column blocks) on the same keys beside
-//   each other on an XCD, so that the second read hits its L2.
+// * An item is a block of R rows of a sequence and `hq` heads of a kv head (8, 4, 2 or 1, as they divide the group), R = 256 / hq
+//   (heads of 256: 128 / hq): one workgroup's four waves, 64 (32) columns each. A wave has one head; of eight, two side by
+//   side, since a second workgroup on the same keys costs their read again (16 heads of 256 over 2, a step of 16 sequences,
+//   605 MB: 143 us with two workgroups of four heads, 103 us with one of eight; 32 heads of 128 over 4 149 and 103 us).
+//   Larger groups take further workgroups (column blocks), beside each other on an XCD, whose L2 the second read hits.
+// * Items of half the rows or fewer take a stream of 32 columns a wave with streaming loads (heads of 256, in calls of such
+//   items alone: tiles of 32 keys, three of them in flight).
 // * Lengths are known on the device only, so every workgroup works out its share of the work (paged_split.hpp): ranges of
 //   equal cost over the items of all sequences, one a workgroup.
 // * A piece of an item leaves normalised f32 rows and their log-sums at slot 2 range (+ 1 if the item starts in it): a range
@@ -35,11 +38,12 @@ struct PagedParams : PagedSplit {
     const uint32_t* table;
     void* o;
     float* lse;
-    float* part_o;    // [ranges][ncb][2][slot_rows][hq][D]: pieces' normalised rows
+    float* part_o;    // [ranges][ncb][2][hq / hpw][slot_rows][hpw][D]: pieces' normalised rows
     float* part_l;    // [ranges][ncb][2][hq][slot_rows]: their log-sums
     uint32_t* whole;  // [ranges][2]: which of a range's pieces there are
-    u32x4* last;      // [ranges]: the item whose last piece a range has: first range, first row of o, rows, kv head (first kNone: none)
+    u32x4* last;      // [ranges]: the item whose last piece a range has: first range (kNone: no item), row of o, rows, kv head
     uint32_t q_pad, group, pages, page_bytes, shift, max_pages, width, hq, ncb, slot_rows;
+    uint32_t hs, ws;  // log2 of hpw (heads a wave) and of hq / hpw
     float scale_log2;
 };
 
@@ -48,35 +52,60 @@ __device__ __forceinline__ uint64_t uniform64(uint64_t x)
     return (uint64_t)uniform((uint32_t)(x >> 32)) << 32 | uniform((uint32_t)x);
 }
 
+// uniform(x), kept in a scalar register: the compiler takes a uniform value's readfirstlane away, and where it has the value in a
+// vector register gives a stream that for a scalar operand. It adds wait states around its own instructions only, so these are
+// here: between the write of x and its read by readfirstlane, and before a vector instruction reads the scalar.
+__device__ __forceinline__ uint32_t scalar(uint32_t x)
+{
+    uint32_t y;
+    asm("s_nop 1\n\tv_readfirstlane_b32 %0, %1\n\ts_nop 4" : "=s"(y) : "v"(x));
+    return y;
+}
+
+// The kernel's parameters, read where they are named: held in scalar registers through the streams, which take most of those,
+// they would be spilled and restored around each.
+typedef const __attribute__((address_space(4))) PagedParams* ParamsAt;
+__device__ __forceinline__ ParamsAt params_here(ParamsAt p)
+{
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
 // What a piece is to the streams: tiles [ta, tb) of a sequence, rows `rows` of its block from position p0 on.
 struct Piece {
-    const void *q, *k, *v;  // of the block's first row and this wave's head; of the kv head in page 0
-    void* o;                // of the block's first row and the wave's first head column
-    float* l;               // of the block's first row and the wave's head
+    const void *q, *k, *v;  // of the block's first row and the wave's first head; of the kv head in page 0
+    void* o;                // of the block's first row and the wave's first head
+    float* l;               // of the block's first row and the wave's first head
     uint64_t table;         // the sequence's row
     uint32_t ta, tb, rows, p0, keys;  // keys: those of the block's last row
     uint32_t seen;                    // keys of the sequence: no row sees more
-    uint32_t o_row, l_bytes;          // bytes of a row of o; of l that may be written
+    uint32_t o_row, o_head;           // bytes between rows of o and between the wave's heads
+    uint32_t l_head;                  // floats between the wave's heads in l
 };
 
-// RW: rows a wave, 64 or 32 (heads of 256: 32).
-template <class T, class TO, int D, int RW>
-__device__ __forceinline__ void run_piece(const PagedParams& p, unsigned char* lds, const Piece& x)
+// FEW: the stream of 32 rows a wave and streaming loads, at heads of 256 by tiles of 32 keys; else 64 rows a wave, at heads of
+// 256 flash_fwd_r32's 32.
+template <class T, class TO, int D, bool FEW>
+__device__ __forceinline__ void run_piece(ParamsAt at_p, unsigned char* lds, const Piece& x)
 {
-    constexpr bool kWide = D == 256;
-    constexpr uint32_t NBUF = kWide ? 2 : kNBuf;
-    constexpr uint32_t kKRowB = 2 * D + 16, kKTileB = 64 * kKRowB, kVRowB = 2 * D, kVTileB = 64 * kVRowB;
+    const auto& p = *params_here(at_p);
+    constexpr bool kR32 = D == 256 && !FEW;
+    constexpr uint32_t RW = FEW || kR32 ? 32 : 64, KT = D == 256 && FEW ? 32 : 64, NBUF = kR32 ? 2 : kNBuf;
+    constexpr uint32_t kKRowB = 2 * D + 16, kKTileB = (KT * kKRowB + 1023) / 1024 * 1024, kVRowB = 2 * D, kVTileB = KT * kVRowB;
     constexpr uint32_t NKP = (kKTileB / 1024 - 1) / 4;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, g = lane >> 5, c32 = lane & 31u, w = uniform(tid >> 6);
-    const uint32_t q0 = w / p.hq * RW;  // this wave's first row in the block
+    // A wave's RW columns are RW / hpw rows of hpw heads, a row's heads side by side: lane column c32 (block 1: c32 + 32) is row
+    // q0 + cr (+ 32 / hpw), head ch.
+    const uint32_t hs = p.hs, RR = RW >> hs;  // (0 or 1)
+    const uint32_t q0 = (w >> p.ws) * RR, cr = c32 >> hs, ch = c32 & hs;
     const uint32_t ks = 64 * x.ta, n_keys = min(64 * x.tb, x.keys) - ks;
-    const uint32_t lim_w = x.p0 + min(q0 + (uint32_t)RW, x.rows);  // (position of the wave's last row) + 1
+    const uint32_t lim_w = x.p0 + min(q0 + RR, x.rows);  // (position of the wave's last row) + 1
     const uint32_t w_keys = q0 < x.rows ? min(n_keys, min(lim_w, x.seen) - ks) : 0u;
-    const uint32_t nt = x.tb - x.ta, ntw = (w_keys + 63) / 64;
+    const uint32_t nt = (n_keys + KT - 1) / KT, ntw = (w_keys + KT - 1) / KT;
     // keys that a row sees, counted from the piece's first one: lmin the wave's first row, lim0 and lim1 the lane's
     const uint32_t r0 = x.p0 + q0;
     const uint32_t lmin = min(r0 + 1, x.seen) - ks;
-    const uint32_t lim0 = min(r0 + c32 + 1, x.seen) - ks - 8 * g;
+    const uint32_t lim0 = min(r0 + cr + 1, x.seen) - ks - 8 * g;
 
     // LDS addresses, staging and epilogue: as flash_fwd_r64 and flash_fwd_r32 have them.
     const uint32_t lbase = (uint32_t)reinterpret_cast<uintptr_t>(lds), vbase = lbase + NBUF * kKTileB;
@@ -85,39 +114,43 @@ __device__ __forceinline__ void run_piece(const PagedParams& p, unsigned char* l
     const uint32_t vrow = vbase + (8 * g + ti / 4) * kVRowB + 8 * (ti % 4);
     auto kd_of = [&](uint32_t i) {
         const uint32_t by = 1024 * i + 16 * lane, row = by / kKRowB, ch = by % kKRowB / 16;
-        return slot_of(row) * (2 * D) + 16 * (ch < D / 8 ? ch : 0);
+        return row < KT ? slot_of(row) * (2 * D) + 16 * (ch < D / 8 ? ch : 0) : 0u;
     };
     const uint32_t skw = uniform(lbase), skww = uniform(lbase + 1024 * w), svww = uniform(vbase + (kVTileB / 4) * w);
-    const uint32_t qo = ((q0 + c32) * D + 8 * g) * 2;
+    const uint32_t qo = ((ch * p.q_pad + q0 + cr) * D + 8 * g) * 2, qo1 = uniform((64u >> hs) * D);
     constexpr uint32_t so = sizeof(TO), orow = D * so, lpr = orow / 16;
     const uint32_t obase = lbase + w * RW * orow;
     const uint32_t ew = so == 4 ? obase + c32 * orow + 16 * ((c32 & 7u) ^ g)
                                 : obase + c32 * orow + 8 * g + 16 * (c32 & 7u);
     const uint32_t er = obase + (lane / lpr) * orow + 16 * ((lane % lpr) ^ (lane / lpr));
-    const uint32_t og = (q0 + lane / lpr) * x.o_row + 16 * (lane % lpr);
-    const uint32_t ogs = uniform((64 / lpr) * x.o_row);
-    const uint32_t lo0 = q0 + c32 < x.rows ? (q0 + c32) * 4 : kNone;
+    // stores of 64 / lpr columns each: one of both heads steps by rows, one of a single column by head and row in turn
+    constexpr uint32_t cols = 64 / lpr;
+    const uint32_t oc = lane / lpr, og = (q0 + (oc >> hs)) * x.o_row + (oc & hs) * x.o_head + 16 * (lane % lpr);
+    const uint32_t ogs = uniform(cols > hs ? (cols >> hs) * x.o_row : x.o_head);
+    const uint32_t ogs2 = uniform(cols > hs ? 2 * ogs : x.o_row);
+    const uint32_t lo0 = q0 + cr < x.rows ? (ch * x.l_head + q0 + cr) * 4 : kNone;
     const uint32_t swp = (lane ^ 32) * 4;
-    const u32x4 qrs = rsrc_of(x.q, x.rows * 2 * D), ors = rsrc_of(x.o, (x.rows - 1) * x.o_row + orow);
-    const u32x4 lrs = rsrc_of(x.l, x.l ? x.l_bytes : 0);
-    const uint32_t has_lse = uniform(x.l ? 1u : 0u);
+    const u32x4 qrs = rsrc_of(x.q, (hs * p.q_pad + x.rows) * 2 * D);
+    const u32x4 ors = rsrc_of(x.o, (x.rows - 1) * x.o_row + hs * x.o_head + orow);
+    const u32x4 lrs = rsrc_of(x.l, x.l ? (hs * x.l_head + x.rows) * 4 : 0);
+    const uint32_t has_lse = scalar(x.l ? 1u : 0u);
     const float c = __builtin_bit_cast(float, uniform(__builtin_bit_cast(uint32_t, p.scale_log2)));
     const uint32_t s_nt = uniform(nt), s_ntw = uniform(ntw), s_lmin = uniform(lmin), kn = uniform(n_keys * 2 * D);
     const uint64_t kb = reinterpret_cast<uint64_t>(x.k), vb = reinterpret_cast<uint64_t>(x.v);
     const uint32_t kb0 = uniform((uint32_t)kb), kb1 = uniform((uint32_t)(kb >> 32) & 0xffffu);
     const uint32_t vb0 = uniform((uint32_t)vb), vb1 = uniform((uint32_t)(vb >> 32) & 0xffffu);
-    const uint32_t pshift = p.shift - 6;
+    const uint32_t pshift = p.shift - (KT == 64 ? 6 : 5);
     const uint32_t* row = reinterpret_cast<const uint32_t*>(x.table);
-    const auto page_of = [&](uint32_t t) { return uniform(row[min(t, x.tb - 1) >> pshift]); };
-    const uint32_t pg0 = page_of(x.ta), pg1 = page_of(x.ta + 1), pg2 = page_of(x.ta + 2), pg3 = page_of(x.ta + 3);
+    const uint32_t t0 = uniform(ks / KT), tlast = uniform(t0 + nt - 1), npages = uniform(p.pages);
+    const auto page_of = [&](uint32_t t) { return uniform(row[min(t, tlast) >> pshift]); };
+    const uint32_t pg0 = page_of(t0), pg1 = page_of(t0 + 1), pg2 = page_of(t0 + 2), pg3 = page_of(t0 + 3);
     const uint64_t ent = uniform64(x.table);
-    const uint32_t t0 = uniform(x.ta), tlast = uniform(x.tb - 1), npages = uniform(p.pages);
     const uint32_t pstride = uniform(p.page_bytes), pmask = uniform((1u << pshift) - 1), s_pshift = uniform(pshift);
 
 #define MAKO_PAGED_SCALARS                                                                                        \
     [qrs] "s"(qrs), [ors] "s"(ors), [lrs] "s"(lrs), [c] "s"(c), [nt] "s"(s_nt), [ntw] "s"(s_ntw), [lmin] "s"(s_lmin),  \
-        [has_lse] "s"(has_lse), [ogs] "s"(ogs), [kb0] "s"(kb0), [kb1] "s"(kb1), [kn] "s"(kn), [vb0] "s"(vb0),     \
-        [vb1] "s"(vb1), [skw] "s"(skw), [skww] "s"(skww), [svww] "s"(svww), [ent] "s"(ent), [t0] "s"(t0),          \
+        [has_lse] "s"(has_lse), [ogs] "s"(ogs), [ogs2] "s"(ogs2), [kb0] "s"(kb0), [kb1] "s"(kb1), [kn] "s"(kn),    \
+        [vb0] "s"(vb0), [vb1] "s"(vb1), [skw] "s"(skw), [skww] "s"(skww), [svww] "s"(svww), [ent] "s"(ent), [t0] "s"(t0), \
         [tlast] "s"(tlast), [npages] "s"(npages), [pstride] "s"(pstride), [pmask] "s"(pmask), [pshift] "s"(s_pshift), \
         [pg0] "s"(pg0), [pg1] "s"(pg1), [pg2] "s"(pg2)
 #define MAKO_PAGED_STREAM(NAME, OPERANDS)                                                                         \
@@ -135,7 +168,7 @@ __device__ __forceinline__ void run_piece(const PagedParams& p, unsigned char* l
         }                                                                                                         \
     } while (0)
 
-    if constexpr (kWide) {
+    if constexpr (kR32) {
         // r32's V image: the bytes a lane's slot holds, for pieces that start on a multiple of 4 rows and the others
         const auto vunit = [](uint32_t u, uint32_t k) { return u ^ (k & 3u) ^ (4u * (u & 1u)); };
         const auto vd_at = [&](uint32_t row0) {
@@ -156,29 +189,38 @@ __device__ __forceinline__ void run_piece(const PagedParams& p, unsigned char* l
       [kd6] "v"(kd6), [kd7] "v"(kd7), [kd8] "v"(kd8), [vd] "v"(vd), [vdo] "v"(vdo), [vd2] "v"(vd2),                  \
       [vdo2] "v"(vdo2), [lim0] "v"(lim0), [qo] "v"(qo), [lo0] "v"(lo0), [swp] "v"(swp), [ew] "v"(ew), [er] "v"(er),   \
       [og] "v"(og), MAKO_PAGED_SCALARS                                                                            \
-    : MAKO_PAGED_D256_CLOBBERS, "vcc", "scc", "memory"
-        MAKO_PAGED_STREAM(MAKO_PAGED_D256_R32, MAKO_PAGED_R32);
+    : MAKO_PAGED_R32_CLOBBERS, "vcc", "scc", "memory"
+        MAKO_PAGED_STREAM(MAKO_PAGED_D256_MANY, MAKO_PAGED_R32);
     } else {
         uint32_t vr0 = vrow + 32 * v_unit(th, ti / 4), vr1 = vrow + 32 * v_unit(2 + th, ti / 4);
-        const uint32_t kr0 = kr, lim1 = min(r0 + c32 + 33, x.seen) - ks - 8 * g;
-        const uint32_t lo1 = q0 + 32 + c32 < x.rows ? (q0 + 32 + c32) * 4 : kNone;
+        const uint32_t kr0 = kr, lim1 = min(r0 + (32u >> hs) + cr + 1, x.seen) - ks - 8 * g;
+        const uint32_t r1 = q0 + (32u >> hs) + cr, lo1 = r1 < x.rows ? (ch * x.l_head + r1) * 4 : kNone;
         const uint32_t kd0 = kd_of(w), kd1 = kd_of(w + 4);
         const uint32_t kd2 = NKP > 2 ? kd_of(w + 8) : 0u, kd3 = NKP > 3 ? kd_of(w + 12) : 0u, kd4 = kd_of(4 * NKP);
-        const uint32_t vd = (kVTileB / 4) * w + vd_of<D == 256 ? 128 : D>(lane);
+        // the bytes a lane's slot of a V piece holds (vd_of); a piece of heads of 256 is two rows, so every other one starts
+        // two rows on
+        const auto vd_at = [&](uint32_t row0) {
+            const uint32_t by = 16 * lane, r = by / kVRowB, pos = by % kVRowB;
+            return (kVTileB / 4) * w + r * kVRowB + 32 * v_unit(pos / 32, r + row0) + 16 * ((pos / 16) & 1u);
+        };
+        const uint32_t vd = vd_at(0), vdo = vd_at(2);
 #define MAKO_PAGED_R64                                                                                            \
     : [kr] "+v"(kr), [vr0] "+v"(vr0), [vr1] "+v"(vr1)                                                             \
     : [kd0] "v"(kd0), [kd1] "v"(kd1), [kd2] "v"(kd2), [kd3] "v"(kd3), [kd4] "v"(kd4), [vd] "v"(vd),                \
-      [lim0] "v"(lim0), [lim1] "v"(lim1), [kr0] "v"(kr0), [qo] "v"(qo), [lo0] "v"(lo0), [lo1] "v"(lo1),            \
-      [swp] "v"(swp), [ew] "v"(ew), [er] "v"(er), [og] "v"(og), [pg3] "s"(pg3), MAKO_PAGED_SCALARS                 \
+      [vdo] "v"(vdo), [lim0] "v"(lim0), [lim1] "v"(lim1), [kr0] "v"(kr0), [qo] "v"(qo), [lo0] "v"(lo0),             \
+      [lo1] "v"(lo1), [swp] "v"(swp), [ew] "v"(ew), [er] "v"(er), [og] "v"(og), [pg3] "s"(pg3), [qo1] "s"(qo1),   \
+      MAKO_PAGED_SCALARS                                                                                          \
     : MAKO_PAGED_CLOBBERS, "vcc", "scc", "memory"
-        if constexpr (D == 64 && RW == 64)
-            MAKO_PAGED_STREAM(MAKO_PAGED_D64_R64, MAKO_PAGED_R64);
+        if constexpr (D == 64 && FEW)
+            MAKO_PAGED_STREAM(MAKO_PAGED_D64_FEW, MAKO_PAGED_R64);
         else if constexpr (D == 64)
-            MAKO_PAGED_STREAM(MAKO_PAGED_D64_R32, MAKO_PAGED_R64);
-        else if constexpr (RW == 64)
-            MAKO_PAGED_STREAM(MAKO_PAGED_D128_R64, MAKO_PAGED_R64);
+            MAKO_PAGED_STREAM(MAKO_PAGED_D64_MANY, MAKO_PAGED_R64);
+        else if constexpr (D == 128 && FEW)
+            MAKO_PAGED_STREAM(MAKO_PAGED_D128_FEW, MAKO_PAGED_R64);
+        else if constexpr (D == 128)
+            MAKO_PAGED_STREAM(MAKO_PAGED_D128_MANY, MAKO_PAGED_R64);
         else
-            MAKO_PAGED_STREAM(MAKO_PAGED_D128_R32, MAKO_PAGED_R64);
+            MAKO_PAGED_STREAM(MAKO_PAGED_D256_FEW, MAKO_PAGED_R64);
     }
 #undef MAKO_PAGED_R64
 #undef MAKO_PAGED_R32
@@ -191,22 +233,24 @@ __device__ __forceinline__ void run_piece(const PagedParams& p, unsigned char* l
 template <int D>
 constexpr uint32_t lds_bytes()
 {
-    return (D == 256 ? 2 : kNBuf) * (64 * (2 * D + 16) + 128 * D);
+    return kNBuf * (D == 64 ? 9 + 8 : 17 + 16) * 1024;  // (heads of 256: four tiles of 32 keys; two of 64 take less)
 }
 
-template <class T, class TO, int D>
-__global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams p)
+// FEW: every piece takes the stream of 32 rows a wave; else pieces of few rows do (heads of 256: none).
+template <class T, class TO, int D, bool FEW>
+__global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams q)
 {
     __shared__ __attribute__((aligned(1024))) unsigned char lds[lds_bytes<D>()];
     const uint32_t lane = threadIdx.x & 63u, w = uniform(threadIdx.x >> 6);
-    const uint32_t xcds = p.n_ranges % 8 == 0 ? 8 : 1;  // ranges side by side on an XCD, a range's column blocks too
-    const uint32_t at_xcd = blockIdx.x / xcds;
-    const uint32_t range = blockIdx.x % xcds * (p.n_ranges / xcds) + at_xcd / p.ncb, cb = at_xcd % p.ncb;
+    // blockIdx.x is the XCD: ranges side by side on one, a range's column blocks too
+    const uint32_t range = blockIdx.x * gridDim.z + blockIdx.z, cb = blockIdx.y;
 
     uint32_t here[2] = {0, 0};
     u32x4 done = u32x4{kNone, 0, 0, 0};
-    walk_range(p, range, lane, [&](const PagedPiece& at) __attribute__((always_inline)) {
-        const uint32_t hl = w % p.hq, h = at.kvh * p.group + cb * p.hq + hl;
+    const ParamsAt at_p = (ParamsAt)__builtin_amdgcn_kernarg_segment_ptr();
+    walk_range(q, range, lane, [&](const PagedPiece& at) __attribute__((always_inline)) {
+        const auto& p = *params_here(at_p);
+        const uint32_t hl = (w & ((1u << p.ws) - 1)) << p.hs, h = at.kvh * p.group + cb * p.hq + hl;
         Piece x;
         x.q = static_cast<const T*>(p.q) + ((size_t)h * p.q_pad + at.row0) * D;
         x.k = static_cast<const T*>(p.k) + ((size_t)at.kvh << p.shift) * D;
@@ -214,29 +258,30 @@ __global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams p)
         x.table = reinterpret_cast<uint64_t>(p.table + (size_t)at.b * p.max_pages);
         x.ta = at.ta, x.tb = at.tb, x.rows = at.rows, x.p0 = at.p0, x.keys = at.keys, x.seen = at.seen;
         x.o = static_cast<TO*>(p.o) + (size_t)at.row0 * p.width + (size_t)h * D;
-        x.o_row = p.width * sizeof(TO);
+        x.o_row = p.width * sizeof(TO), x.o_head = D * sizeof(TO), x.l_head = p.rows;
         x.l = p.lse ? p.lse + (size_t)h * p.rows + at.row0 : nullptr;
-        x.l_bytes = at.rows * 4;
         if (at.part) {
             const size_t slot = ((size_t)range * p.ncb + cb) * 2 + at.kind;
-            x.o = p.part_o + (slot * p.slot_rows * p.hq + hl) * D;
-            x.o_row = p.hq * D * 4;
+            x.o = p.part_o + (slot * p.hq + hl) * p.slot_rows * D;
+            x.o_row = (D * 4) << p.hs, x.o_head = D * 4, x.l_head = p.slot_rows;
             x.l = p.part_l + (slot * p.hq + hl) * p.slot_rows;
             here[at.kind] = 1;
             if (at.first != kNone)
                 done = u32x4{at.first, at.row0, at.rows, at.kvh};
         }
-        const bool f32 = at.part || __is_same(TO, float), few = D == 256 || at.rows <= p.few;
-        constexpr int kMany = D == 256 ? 32 : 64;
-        if (f32 && few)
-            run_piece<T, float, D, 32>(p, lds, x);
-        else if (f32)
-            run_piece<T, float, D, kMany>(p, lds, x);
-        else if (few)
-            run_piece<T, TO, D, 32>(p, lds, x);
-        else
-            run_piece<T, TO, D, kMany>(p, lds, x);
+        const bool few = FEW || (D != 256 && at.rows <= p.few);
+        if (at.part || __is_same(TO, float)) {
+            if (few)
+                run_piece<T, float, D, D != 256 || FEW>(at_p, lds, x);
+            else
+                run_piece<T, float, D, FEW>(at_p, lds, x);
+        } else if (few) {
+            run_piece<T, TO, D, D != 256 || FEW>(at_p, lds, x);
+        } else {
+            run_piece<T, TO, D, FEW>(at_p, lds, x);
+        }
     });
+    const auto& p = *params_here(at_p);
     if (!p.direct && cb == 0 && threadIdx.x == 0) {
         p.whole[2 * range] = here[0];
         p.whole[2 * range + 1] = here[1];
@@ -260,7 +305,7 @@ __global__ __launch_bounds__(256) void paged_merge(const PagedParams p, uint32_t
     if (first == kNone)
         return;
     const uint32_t set = threadIdx.x / L, w = set % NW, t = (sub * (256 / L) + set) / NW, d = 4 * (threadIdx.x % L);
-    const uint32_t hl = t % p.hq, cb = t / p.hq % p.ncb, row = t / p.hq / p.ncb;
+    const uint32_t hl = t & (p.hq - 1), at_cb = t >> (p.hs + p.ws), cb = at_cb % p.ncb, row = at_cb / p.ncb;
     const bool live = row < item[2];
     float mx = -INFINITY, sum = 0.0f;
     f32x4 acc = f32x4{};
@@ -273,7 +318,8 @@ __global__ __launch_bounds__(256) void paged_merge(const PagedParams p, uint32_t
             const size_t slot = ((size_t)i * p.ncb + cb) * 2 + kind;
             const bool has = i0 + u * NW <= r && p.whole[2 * i + kind];
             const float y = p.part_l[(slot * p.hq + hl) * p.slot_rows + row];
-            const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + ((slot * p.slot_rows + row) * p.hq + hl) * D + d);
+            const size_t at = ((slot * p.hq + (hl >> p.hs << p.hs)) * p.slot_rows + (row << p.hs) + (hl & p.hs)) * D + d;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(p.part_o + at);
             l[u] = has ? y * kLog2e : -INFINITY;
             v[u] = has ? x : f32x4{};
         }
@@ -323,7 +369,7 @@ __global__ __launch_bounds__(256) void paged_merge(const PagedParams p, uint32_t
 
 // A call's split, from its sizes alone (lengths are known on the device only).
 struct Plan {
-    uint32_t hq, rshift, ncb, n_ranges, slot_rows, direct, few;
+    uint32_t hq, hpw, rshift, ncb, n_ranges, slot_rows, direct, few;
 };
 
 constexpr uint32_t kFewMerged = 16;  // (row, head) pairs a range up to which paged_merge parts an item's pieces
@@ -344,9 +390,10 @@ Plan plan_of(const mako_paged_args* a, uint32_t cus)
 {
     const uint32_t group = a->heads / a->kv_heads;
     Plan pl{};
-    pl.hq = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+    const bool both = group % 8 == 0 && 4ull * a->dim * a->q_pad < (1ull << 32);  // (a wave's q: 32-bit offsets)
+    pl.hpw = both ? 2 : 1;
+    pl.hq = both ? 8 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
     pl.rshift = log2_of((a->dim == 256 ? 128 : 256) / pl.hq);
-    pl.few = a->dim == 256 ? 0 : 128 / pl.hq;
     pl.ncb = group / pl.hq;
     pl.n_ranges = std::max(1u, cus / pl.ncb);
     if (pl.n_ranges > 8)
@@ -354,6 +401,11 @@ Plan plan_of(const mako_paged_args* a, uint32_t cus)
     pl.slot_rows = std::min(1u << pl.rshift, a->max_new);
     const uint64_t items = ((uint64_t)(a->rows >> pl.rshift) + a->batch) * a->kv_heads;
     pl.direct = (a->max_ctx + 63) / 64 <= direct_tiles(items, pl.n_ranges, pl.slot_rows * group > kFewMerged);
+    // Heads of 256, tiles of 32 keys / of 64: a step of 16 sequences over up to 32767 rows 103 us / 116, 8 tokens each 110 / 121,
+    // 16 tokens each 136 / 129; steps among chunks 267 / 225; one token over 391 rows in one launch 16.1 / 15.5.
+    pl.few = (1u << pl.rshift) / 2;
+    if (a->dim == 256 && (pl.direct || a->max_new > pl.few))
+        pl.few = 0;
     return pl;
 }
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
@@ -370,7 +422,12 @@ size_t workspace_for(const Plan& pl, uint32_t dim)
 template <class T, class TO, int D>
 void launch(const PagedParams& p, hipStream_t s)
 {
-    hipLaunchKernelGGL((paged_rows<T, TO, D>), dim3(p.n_ranges * p.ncb), dim3(256), 0, s, p);
+    const uint32_t xcds = p.n_ranges % 8 == 0 ? 8 : 1;
+    const dim3 grid(xcds, p.ncb, p.n_ranges / xcds);
+    if (p.max_new <= p.few)
+        hipLaunchKernelGGL((paged_rows<T, TO, D, true>), grid, dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((paged_rows<T, TO, D, false>), grid, dim3(256), 0, s, p);
     if (p.direct)
         return;
     const uint32_t nw = p.slot_rows * p.group <= kFewMerged ? 4 : 1, per = (p.slot_rows * p.group * nw * D + 1023) / 1024;
@@ -425,8 +482,8 @@ int check_args(const mako_paged_args* a, mako_dtype in, mako_dtype out, const vo
     if ((uint64_t)a->heads * a->dim > a->width || a->width % 4 || a->width >= (1u << 20))
         return fail(MAKO_EINVAL, "%s: o rows of %u for %u heads of %u (a multiple of 4, at least their width, below 2^20)",
                     what, a->width, a->heads, a->dim);
-    // what the split counts: at most kTile units a tile, for every 32 rows of a sequence at least
-    const uint64_t units = ((uint64_t)a->rows / 32 + a->batch) * ((uint64_t)a->max_ctx / 10 + 512) * a->kv_heads;
+    // what the split counts: at most kTile units a tile, for every 16 rows of a sequence at least
+    const uint64_t units = ((uint64_t)a->rows / 16 + a->batch) * ((uint64_t)a->max_ctx / 5 + 1024) * a->kv_heads;
     if (units >= (1ull << 32) || (uint64_t)a->rows * a->heads >= (1u << 30))
         return fail(MAKO_EINVAL, "%s: %u rows of %u heads over %u keys are too many", what, a->rows, a->heads, a->max_ctx);
     if (!(a->scale > 0.0f) || a->scale == INFINITY)
@@ -472,7 +529,8 @@ extern "C" int mako_attn_paged(const mako_paged_args* a, mako_dtype in, mako_dty
                         q, k, v, table, o, lse, reinterpret_cast<float*>(at(0)), reinterpret_cast<float*>(at(ob)),
                         reinterpret_cast<uint32_t*>(at(ob + lb + 2 * wb)), reinterpret_cast<u32x4*>(at(ob + lb)), a->q_pad,
                         a->heads / a->kv_heads, a->pages, a->kv_heads * a->page * a->dim * 2, log2_of(a->page),
-                        a->max_pages, a->width, pl.hq, pl.ncb, pl.slot_rows, a->scale * kLog2e};
+                        a->max_pages, a->width, pl.hq, pl.ncb, pl.slot_rows, pl.hpw - 1,
+                        log2_of(pl.hq / pl.hpw), a->scale * kLog2e};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (in == MAKO_BF16 && out == MAKO_F32)
         launch_dim<__bf16, float>(p, a->dim, s);

@@ -60,28 +60,30 @@ AHEAD = 6               # operand reads in flight ahead of their MFMAs (a slot i
 N_K_AHEAD = 6           # K reads of the next phase QK that go out in phase PV's tail, after the barrier
 
 
-def set_dim(d):
-    """The head width's constants (128, or 64: the same stream with half the head dimensions):
+def set_dim(d, keys=64):
+    """The head width's constants (128, or 64: the same stream with half the head dimensions; paged with 32 rows a wave also
+    256, by tiles of 32 keys):
+    KT, NT  keys of a tile, 32-key halves of it;
     K_ROW   LDS bytes of a K row: 2 d + 16 of padding (an odd number of 16-byte chunks, so 16-byte reads down a column
             are conflict-free);
-    K_TILE  the padded K image of a 64-key tile (17 or 9 pieces of 1 KiB: a wave DMAs pieces w + 4 m, m < NKP, and
-            every wave the last, piece 4 NKP);
+    K_TILE  the padded K image of a tile (17 or 9 pieces of 1 KiB, the last one in part at 256: a wave DMAs pieces w + 4 m,
+            m < NKP, and every wave the last, piece 4 NKP);
     V_ROW   LDS bytes of a V row: 2 d, its 32-byte units permuted by row (v_unit);
-    V_TILE  the V image of a tile, 64 rows (a wave DMAs NVP KiB of it);
+    V_TILE  the V image of a tile (a wave DMAs NVP KiB of it);
     NKK, NDB  16-wide head-dimension steps of Q K^T, 32-wide output blocks;
-    BAR_AT  phase PV's fragment (of 4 NDB) after whose MFMAs the tile's barrier sits."""
-    global D, K_ROW, V_ROW, K_TILE, V_TILE, NKK, NDB, NKP, NVP, DMA_PER_TILE, BAR_AT
-    assert d in (64, 128)
-    D = d
+    BAR_AT  phase PV's fragment (of 2 NT NDB) after whose MFMAs the tile's barrier sits."""
+    global D, KT, NT, K_ROW, V_ROW, K_TILE, V_TILE, NKK, NDB, NKP, NVP, DMA_PER_TILE, BAR_AT
+    assert (d in (64, 128) and keys == 64) or (d == 256 and keys == 32)
+    D, KT, NT = d, keys, keys // 32
     K_ROW = 2 * d + 16
     V_ROW = 2 * d
-    K_TILE = 64 * K_ROW
-    V_TILE = d * 64 * 2
+    K_TILE = -(-keys * K_ROW // 1024) * 1024
+    V_TILE = d * keys * 2
     NKK, NDB = d // 16, d // 32
     NKP = (K_TILE // 1024 - 1) // 4
     NVP = V_TILE // 4096
-    DMA_PER_TILE = NKP + 1 + NVP   # LDS DMA loads a wave issues a tile (9 at d 128, 5 at 64)
-    BAR_AT = 12 if d == 128 else 6
+    DMA_PER_TILE = NKP + 1 + NVP   # LDS DMA loads a wave issues a tile (9 at d 128 and 256, 5 at 64)
+    BAR_AT = 6 if d == 64 else 12
 
 
 set_dim(128)
@@ -251,7 +253,8 @@ def dma_groups():
                    f"buffer_load_dwordx4 %[kd4], {quad(KRS)}, 0 offen{nt} lds"])
     for i in range(NVP):
         groups.append(([f"s_mov_b32 m0, {SVWW}", "s_nop 0"] if i == 0 else []) +
-                      [f"buffer_load_dwordx4 %[vd], {quad(VRS)}, 0 offen offset:{1024 * i}{nt} lds"])
+                      [f"buffer_load_dwordx4 %[{'vdo' if D == 256 and i % 2 else 'vd'}], {quad(VRS)}, 0 offen "
+                       f"offset:{1024 * i}{nt} lds"])
     groups[0] = pre + groups[0]
     ops = []
     step = 128 * D   # K and V rows: 2 d bytes a key, 64 keys a tile
@@ -273,7 +276,7 @@ def dma_groups():
 def page_source(page, rem, tile, t, lo, hi):
     """Paged: K's descriptor at the tile `tile` of page `page`, `rem` bytes long (none where there is no page); (lo, hi) keep
     the tile's offset in the pool."""
-    return [f"s_and_b32 {t}, {tile}, %[pmask]", f"s_lshl_b32 {t}, {t}, {(128 * D).bit_length() - 1}",
+    return [f"s_and_b32 {t}, {tile}, %[pmask]", f"s_lshl_b32 {t}, {t}, {(2 * D * KT).bit_length() - 1}",
             f"s_mul_i32 {lo}, {page}, %[pstride]", f"s_mul_hi_u32 {hi}, {page}, %[pstride]",
             f"s_add_u32 {lo}, {lo}, {t}", f"s_addc_u32 {hi}, {hi}, 0",
             f"s_add_u32 {KRS[0]}, %[kb0], {lo}", f"s_addc_u32 {KRS[1]}, %[kb1], {hi}",
@@ -286,7 +289,7 @@ def value_source(lo, hi):
 
 
 def page_advance(rem, tile):
-    return [f"s_sub_u32 {rem}, {rem}, {128 * D:#x}", f"s_cselect_b32 {rem}, 0, {rem}", f"s_add_u32 {tile}, {tile}, 1"]
+    return [f"s_sub_u32 {rem}, {rem}, {2 * D * KT:#x}", f"s_cselect_b32 {rem}, 0, {rem}", f"s_add_u32 {tile}, {tile}, 1"]
 
 
 def page_load(page, tile, t):
@@ -313,16 +316,16 @@ def barrier():
 
 
 def k_reads(addr):
-    """LDS reads of K fragment f = (kk, t) = (f // 2, f % 2): rows 32 t + c32 (slot order), head dims 16 kk + 8 g.
+    """LDS reads of K fragment f = (kk, t) = (f // NT, f % NT): rows 32 t + c32 (slot order), head dims 16 kk + 8 g.
     Each fragment's reads are a list of instruction texts ({ring} the ring slot, {lo} / {hi} its halves)."""
-    return [[f"ds_read_b128 {{ring}}, {addr} offset:{32 * K_ROW * (f % 2) + 32 * (f // 2)}"] for f in range(2 * NKK)]
+    return [[f"ds_read_b128 {{ring}}, {addr} offset:{32 * K_ROW * (f % NT) + 32 * (f // NT)}"] for f in range(NT * NKK)]
 
 
 def qk_mfmas(dtype, sbuf):
     mf = f"v_mfma_f32_32x32x16_{dtype}"
     out = []
-    for f in range(2 * NKK):
-        kk, t = f // 2, f % 2
+    for f in range(NT * NKK):
+        kk, t = f // NT, f % NT
         for rb in range(NRB):
             src_c = "0" if kk == 0 else S(sbuf, rb, t)
             out.append((f, f"{mf} {S(sbuf, rb, t)}, {{ring}}, {Q(rb, kk)}, {src_c}"))
@@ -344,7 +347,7 @@ def v_reads():
     lane's address for even db (unit h ^ (i / 4)), %[vr1] for odd db (unit (2 + h) ^ (i / 4)); db / 2 adds 128
     bytes, cc and r add whole rows."""
     out = []
-    for f in range(4 * NDB):
+    for f in range(2 * NT * NDB):
         cc, db = f // NDB, f % NDB
         base = 16 * cc * V_ROW + 128 * (db >> 1)
         out.append([f"ds_read_b64_tr_b16 {{{half}}}, %[vr{db & 1}] offset:{base + 4 * r * V_ROW}"
@@ -354,7 +357,7 @@ def v_reads():
 
 def pv_mfmas(dtype):
     out = []
-    for f in range(4 * NDB):
+    for f in range(2 * NT * NDB):
         cc, db = f // NDB, f % NDB
         for rb in range(NRB):
             out.append((f, f"v_mfma_f32_32x32x16_{dtype} {O(rb, db)}, {{ring}}, {P(rb, cc)}, {O(rb, db)}"))
@@ -443,7 +446,7 @@ def mask(sbuf, j0):
     """Keys a row does not see become -inf: key (tile first key) + C is seen by a lane when C < its limit - 8 g - j0
     (the limit: the reference's visibility rule collapsed to `key < lim` for the lane's row)."""
     ops = [f"v_sub_u32 {TMP[rb]}, %[lim{rb}], {j0}" for rb in range(NRB)]
-    elems = [(rb, t, r) for rb in range(NRB) for t in range(2) for r in range(16)]
+    elems = [(rb, t, r) for rb in range(NRB) for t in range(NT) for r in range(16)]
     nm = 3 if SPARSE else 4   # the sparse stream keeps the fourth pair for SEW
     cmp = [f"v_cmp_lt_i32 {SMASK[i % nm]}, {32 * t + 16 * (r >> 3) + (r & 7)}, {TMP[rb]}"
            for i, (rb, t, r) in enumerate(elems)]
@@ -492,7 +495,7 @@ def exps(sbuf):
     """Exponentials in place: exp2(s c - m)."""
     ops = []
     for rb in range(NRB):
-        for t in range(2):
+        for t in range(NT):
             for r in range(16):
                 ops.append(f"v_fma_f32 {S(sbuf, rb, t, r)}, {S(sbuf, rb, t, r)}, %[c], {NEGMU[rb]}")
                 ops.append(f"v_exp_f32 {S(sbuf, rb, t, r)}, {S(sbuf, rb, t, r)}")
@@ -507,13 +510,13 @@ def pack_and_sum(sbuf, dtype):
     cvt = f"v_cvt_pk_{dtype}_f32"
     ops = []
     for rb in range(NRB):
-        for cc in range(4):
+        for cc in range(2 * NT):
             t, r0 = cc // 2, 8 * (cc % 2)
             for i in range(4):
                 ops.append(f"{cvt} {P(rb, cc, i)}, {S(sbuf, rb, t, r0 + 2 * i)}, "
                            f"{S(sbuf, rb, t, r0 + 2 * i + 1)}")
-    vals = {rb: [S(sbuf, rb, t, r) for t in range(2) for r in range(16)] for rb in range(NRB)}
-    for k in range(1, 8):       # chain c of row block rb sums values c, c + 4, c + 8, ...
+    vals = {rb: [S(sbuf, rb, t, r) for t in range(NT) for r in range(16)] for rb in range(NRB)}
+    for k in range(1, 4 * NT):   # chain c of row block rb sums values c, c + 4, c + 8, ...
         for rb in range(NRB):
             for c in range(4):
                 acc = TMP[4 * rb + c]
@@ -539,9 +542,9 @@ def q_waits(mfmas, n_groups):
     n = len(mfmas)
     out = {}
     for kk in range(NKK):
-        first = next(i for i, (f, _) in enumerate(mfmas) if f == 2 * kk)
+        first = next(i for i, (f, _) in enumerate(mfmas) if f == NT * kk)
         issued = sum(1 for g in range(n_groups) if g * n // n_groups < first)
-        out[2 * kk] = [f"s_waitcnt vmcnt({NRB * (NKK - 1 - kk) + issued})"]
+        out[NT * kk] = [f"s_waitcnt vmcnt({NRB * (NKK - 1 - kk) + issued})"]
     return out
 
 
@@ -576,7 +579,7 @@ def exact_tile(e, dtype, sbuf, kaddr, j0, first=False, w=None):
         e(op)
     for rb in range(NRB):
         mx = TMP[2 + rb]
-        vals = [S(sbuf, rb, t, r) for t in range(2) for r in range(16)]
+        vals = [S(sbuf, rb, t, r) for t in range(NT) for r in range(16)]
         e(f"v_max3_f32 {mx}, {vals[0]}, {vals[1]}, {vals[2]}")
         rest = vals[3:]
         while len(rest) >= 2:
@@ -638,13 +641,13 @@ def low_part_pass(e):
         e(f"s_cbranch_scc1 {skip}")
         e.label("L_lo")
     else:
-        e("s_cmp_ge_u32 %[lmin], 64")
+        e(f"s_cmp_ge_u32 %[lmin], {KT}")
         e(f"s_cbranch_scc1 {skip}")
     lo = {}
     ops_a, ops_b, ops_c = [], [], []
     k = 0
     for rb in range(NRB):
-        for cc in range(4):
+        for cc in range(2 * NT):
             t, r0 = cc // 2, 8 * (cc % 2)
             for i in range(4):
                 hi, lr, tr = P(rb, cc, i), f"v{64 + 16 * rb + 4 * cc + i}", f"v{96 + k}"
@@ -656,7 +659,7 @@ def low_part_pass(e):
     for op in ops_a + ops_b + ops_c:
         e(op)
     mfmas = []
-    for f in range(4 * NDB):
+    for f in range(2 * NT * NDB):
         cc, db = f // NDB, f % NDB
         for rb in range(NRB):
             plo = f"v[{64 + 16 * rb + 4 * cc}:{64 + 16 * rb + 4 * cc + 3}]"
@@ -759,7 +762,7 @@ def epilogue(e, out_dtype):
     ga = (TMP[4], TMP[5])
     e(f"v_mov_b32 {ga[0]}, %[og]")
     e(f"v_add_u32 {ga[1]}, %[ogs], %[og]")
-    e(f"s_lshl_b32 {ST[0]}, %[ogs], 1")
+    e(f"s_mov_b32 {ST[0]}, %[ogs2]" if PAGED else f"s_lshl_b32 {ST[0]}, %[ogs], 1")
     e("s_waitcnt lgkmcnt(0)")
     for i in range(n_ld):
         a = ga[i % 2]
@@ -777,8 +780,9 @@ def body(in_dtype, out_dtype, sparse=False, d=128, paged=False, rows=64):
     global SPARSE, PAGED, NRB, STREAMING
     assert not sparse or (d == 128 and not paged)
     assert rows == 64 or (rows == 32 and paged)
+    assert d != 256 or rows == 32
     SPARSE, PAGED, NRB, STREAMING = sparse, paged, rows // 32, rows == 32
-    set_dim(d)
+    set_dim(d, 32 if d == 256 else 64)
     try:
         return body_of(in_dtype, out_dtype)
     finally:
@@ -834,7 +838,7 @@ def body_of(in_dtype, out_dtype):
     for op in dma_issue():
         e(op)
     if NRB == 2:
-        e(f"v_add_u32 {TMP[0]}, {64 * D:#x}, %[qo]")   # row block 1: 32 rows of 2 d bytes on
+        e(f"v_add_u32 {TMP[0]}, {'%[qo1]' if PAGED else f'{64 * D:#x}'}, %[qo]")   # row block 1: 32 rows of 2 d bytes on
     for kk in range(NKK):
         for rb in range(NRB):
             e(f"buffer_load_dwordx4 {Q(rb, kk)}, {'%[qo]' if rb == 0 else TMP[0]}, %[qrs], 0 offen "
@@ -944,7 +948,7 @@ def body_rest(e, in_dtype, out_dtype):
             e("s_waitcnt lgkmcnt(0)")
             exact_tile(e, in_dtype, par, TMP[15], ST[0], w="s[78:79]")
         else:
-            e(f"s_lshl_b32 {SJX}, {SJ}, 6")
+            e(f"s_lshl_b32 {SJX}, {SJ}, {KT.bit_length() - 1}")
             exact_tile(e, in_dtype, par, TMP[15], SJX)
         for rb in range(NRB):
             e(f"v_add_f32 {LSUM[rb]}, {LSUM[rb]}, {TMP[4 * rb]}")
@@ -969,8 +973,8 @@ def body_rest(e, in_dtype, out_dtype):
             e(f"s_cmp_eq_u32 {ST[2]}, -1")
             e(f"s_cbranch_scc0 {lbl(f'L_general_{name}')}")
         else:
-            e(f"s_lshl_b32 {SJ0}, {ST[1]}, 6")
-        e(f"s_add_u32 {ST[2]}, {SJ0}, 64")
+            e(f"s_lshl_b32 {SJ0}, {ST[1]}, {KT.bit_length() - 1}")
+        e(f"s_add_u32 {ST[2]}, {SJ0}, {KT}")
         e(f"s_cmp_le_u32 {ST[2]}, %[lmin]")
         e(f"s_cbranch_scc0 {lbl(f'L_masked_{name}')}")
         iteration(par, "first" if first else "plain")

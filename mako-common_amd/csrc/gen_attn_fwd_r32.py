@@ -441,7 +441,7 @@ def epilogue(e, out_dtype):
     ga = (TMP[4], TMP[5])
     e(f"v_mov_b32 {ga[0]}, %[og]")
     e(f"v_add_u32 {ga[1]}, %[ogs], %[og]")
-    e(f"s_lshl_b32 {ST[0]}, %[ogs], 1")
+    e(f"s_mov_b32 {ST[0]}, %[ogs2]" if PAGED else f"s_lshl_b32 {ST[0]}, %[ogs], 1")
     e("s_waitcnt lgkmcnt(0)")
     for i in range(n_ld):
         a = ga[i % 2]

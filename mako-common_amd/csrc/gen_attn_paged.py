@@ -13,12 +13,15 @@ import gen_attn_fwd_r32 as R
 
 def streams():
     """(macro name, lines) of every stream."""
-    for d, rows in ((128, 64), (128, 32), (64, 64), (64, 32), (256, 32)):
-        for ind in ("bf16", "f16"):
-            for outd in ("f32", ind):
-                lines = R.body(ind, outd, paged=True) if d == 256 else G.body(ind, outd, d=d, paged=True, rows=rows)
-                (R if d == 256 else G).check_registers(lines, paged=True)
-                yield f"MAKO_PAGED_D{d}_R{rows}_{ind.upper()}_{outd.upper()}", lines
+    for d in (128, 64, 256):
+        for form in ("MANY", "FEW"):  # rows a wave: 64 (heads of 256: 32, by flash_fwd_r32's stream), 32
+            for ind in ("bf16", "f16"):
+                for outd in ("f32", ind):
+                    r32 = d == 256 and form == "MANY"
+                    lines = R.body(ind, outd, paged=True) if r32 else \
+                        G.body(ind, outd, d=d, paged=True, rows=64 if form == "MANY" else 32)
+                    (R if r32 else G).check_registers(lines, paged=True)
+                    yield f"MAKO_PAGED_D{d}_{form}_{ind.upper()}_{outd.upper()}", lines
 
 
 def main(path):
@@ -26,7 +29,7 @@ def main(path):
     for name, lines in streams():
         out += [f"#define {name} \\"] + [f'    "{ln}\\n" \\' for ln in lines] + ['    ""', ""]
     out += [f"#define MAKO_PAGED_CLOBBERS {G.clobbers(paged=True)}",
-            f"#define MAKO_PAGED_D256_CLOBBERS {R.clobbers(paged=True)}", ""]
+            f"#define MAKO_PAGED_R32_CLOBBERS {R.clobbers(paged=True)}", ""]
     with open(path, "w") as f:
         f.write("\n".join(out))
 

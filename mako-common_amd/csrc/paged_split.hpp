@@ -3,13 +3,13 @@
 //
 // An item is a block of R = 1 << rshift rows of a sequence and a kv head; its tiles are the 64 keys each up to its last row's.
 // Its cost is kTile units a tile (kTileFew in a sequence of at most `few` rows) and kLead (kLeadFew) for what it costs beside
-// them. The items of all (kv head, sequence)
-// segments lie end to end, a kv head's sequences together, and are cut into equal ranges, one a workgroup: ranges side by side
-// on an XCD share keys, and every XCD has its part of each sequence (with a sequence's kv heads together, a batch's single
-// tokens met on one XCD, whose reads bound the call: 16 MB of a mixed batch of 224 us took it 207 of 180). Within a segment the row blocks go heavy and light
-// in turn (the last, the first, the last but one, the second, ...), so two neighbours cost the same everywhere, and the ranges of a whole
-// prompt fall on items' ends. A cut inside an item leaves kLeast tiles on either side, and no row without keys in a piece's
-// first tile, which the attention's streams rely on; with `direct`, items are not cut: the range of an item's middle has it.
+// them. The items of all (kv head, sequence) segments lie end to end, a kv head's sequences together, and are cut into
+// equal ranges, one a workgroup: ranges side by side on an XCD share keys, and every XCD has its part of each sequence. (With
+// a sequence's kv heads together a batch's single tokens met on one XCD, whose reads then bound the call: a mixed batch took
+// 225 us, 208 so.) Within a segment the row blocks go heavy and light in turn (the last, the first, the last but one, the
+// second, ...), so two neighbours cost the same everywhere, and the ranges of a whole prompt fall on items' ends.
+// A cut inside an item leaves kLeast tiles on either side, and no row without keys in a piece's first tile, which the
+// attention's streams rely on; with `direct`, items are not cut: the range of an item's middle has it.
 #pragma once
 
 #include "pages_common.hpp"
@@ -17,10 +17,10 @@
 
 namespace mako {
 
-// The streams' tiles and pieces side by side in a mixed batch, in units of 0.28 us: 64 rows a wave 1.7 us a tile and 8 a piece,
+// The streams' tiles and pieces side by side in a mixed batch, in units of 0.14 us: 64 rows a wave 1.7 us a tile and 8 a piece,
 // 32 rows 1.1 and 5 (a tile of these alone on a full chip: 1.6 and 0.9). With a tile of 32 rows at half of one of 64 the
 // workgroups that met single tokens ended at 220 us, the others at 175.
-constexpr uint32_t kTile = 6, kTileFew = 4, kLead = 30, kLeadFew = 18;
+constexpr uint32_t kTile = 12, kTileFew = 8, kLead = 60, kLeadFew = 36;
 constexpr uint32_t kLeast = 3;  // tiles of a piece
 
 struct PagedSplit {

@@ -18,8 +18,11 @@ import oracle as O  # noqa: E402
 SOPS = {'qrs': 's[0:3]', 'ors': 's[4:7]', 'lrs': 's[8:11]', 'ent': 's[12:13]'}
 SOPS.update({n: f's{14 + i}' for i, n in enumerate(
     ['c', 'ntw', 'nt', 'lmin', 'has_lse', 'ogs', 'kb0', 'kb1', 'kn', 'vb0', 'vb1', 'skww', 'skw', 'svww', 't0', 'tlast',
-     'npages', 'pstride', 'pmask', 'pshift', 'pg0', 'pg1', 'pg2', 'pg3'])})
+     'npages', 'pstride', 'pmask', 'pshift', 'pg0', 'pg1', 'pg2', 'pg3', 'ogs2', 'qo1'])})
 SREG = {n: int(r[2:].split(':')[0]) if r[1] == '[' else int(r[1:]) for n, r in SOPS.items()}
+
+
+VREG64 = {**R64.VREG, 'vdo': f'v{G.CLOBBER_V + len(R64.VREG)}'}
 
 
 class Emu(E.Emu):
@@ -52,9 +55,9 @@ class Emu(E.Emu):
 
 
 def program(ind, outd, d, lines=None, wave_rows=64):
-    r32 = d == 256
+    r32 = d == 256 and wave_rows != 32
     lines = lines or (G32.body(ind, outd, paged=True) if r32 else G.body(ind, outd, d=d, paged=True, rows=wave_rows))
-    vreg = (R32 if r32 else R64).VREG
+    vreg = R32.VREG if r32 else VREG64
     out = []
     for ln in lines:
         ln = ln.replace('%=', '0')
@@ -66,7 +69,8 @@ def program(ind, outd, d, lines=None, wave_rows=64):
 
 
 def run(heads, kv, n, ctx, page, d, ind='bf16', outd='f32', cut=None, seed=0, kgrow=0.0, missing=(), lines=None, wave_rows=64):
-    """n new rows behind ctx; cut = (ta, tb): the piece of tiles [ta, tb) (one item only); wave_rows: 64 or 32 (heads of 64 and 128). Returns the worst errors."""
+    """n new rows behind ctx; cut = (ta, tb): the piece of tiles [ta, tb) (one item only); wave_rows: 64 or 32 (heads of 256: the stream of
+    32-key tiles). Returns the worst errors."""
     rng = np.random.default_rng(seed)
     conv = O.to_bf16_bits if ind == 'bf16' else O.to_f16_bits
     dt = O.BF16 if ind == 'bf16' else O.F16
@@ -101,14 +105,15 @@ def run(heads, kv, n, ctx, page, d, ind='bf16', outd='f32', cut=None, seed=0, kg
         mem.b[at:at + a.nbytes] = np.ascontiguousarray(a).view(np.uint8).ravel()
     mem.b[O0:O0 + n * width * so] = 0xAB
     prog, labels = program(ind, outd, d, lines, wave_rows)
-    r32 = d == 256
+    r32 = d == 256 and wave_rows != 32
     RW = 32 if r32 else wave_rows
-    K_ROW = 2 * d + 16
-    K_TILE, V_TILE = 64 * K_ROW, 128 * d
+    K_ROW, KT = 2 * d + 16, 32 if d == 256 and not r32 else 64
+    K_TILE, V_TILE = -(-KT * K_ROW // 1024) * 1024, 2 * KT * d
     NKP = (K_TILE // 1024 - 1) // 4
     nbuf = 2 if r32 else G.NBUF
     group = heads // kv
-    hq = 4 if group % 4 == 0 else 2 if group % 2 == 0 else 1
+    hq = 8 if group % 8 == 0 else 4 if group % 4 == 0 else 2 if group % 2 == 0 else 1
+    hpw = 2 if hq == 8 else 1  # heads a wave
     R = RW * 4 // hq
     c = np.float32(1.0 / np.sqrt(float(d))) * np.float32(1.4426950408889634)
     lane = np.arange(64)
@@ -128,28 +133,32 @@ def run(heads, kv, n, ctx, page, d, ind='bf16', outd='f32', cut=None, seed=0, kg
             waves = []
             for w in range(4):
                 W = E.Wave(w)
-                h = hg * hq + w % hq
+                h = hg * hq + w % (hq // hpw) * hpw
                 kvh = hg * hq // group
-                q0 = (w // hq) * RW
+                q0 = (w // (hq // hpw)) * (RW // hpw)
+                row, hh = q0 + c32 // hpw, c32 % hpw
+                row1 = row + 32 // hpw
                 live = q0 < rows
-                w_lim = ctx + qb_i * R + min(q0 + RW, rows)
-                ntw = -(-min(n_keys, w_lim - ks) // 64) if live else 0
+                w_lim = ctx + qb_i * R + min(q0 + RW // hpw, rows)
+                ntw = -(-min(n_keys, w_lim - ks) // KT) if live else 0
                 p0 = ctx + qb_i * R + q0
-                lim = [np.minimum(p0 + 32 * i + c32 + 1, keys) - ks - 8 * g for i in range(2)]
+                lim = [np.minimum(p0 + 32 // hpw * i + c32 // hpw + 1, keys) - ks - 8 * g for i in range(2)]
                 kr = c32 * K_ROW + 16 * g
 
                 def kd_of(i):
                     b = 1024 * i + 16 * lane
                     rr, ch = b // K_ROW, (b % K_ROW) // 16
-                    return np.array([R64.slot_of(int(r)) for r in rr]) * row_b + 16 * np.where(ch < d // 8, ch, 0)
+                    at = np.array([R64.slot_of(int(r)) for r in rr]) * row_b + 16 * np.where(ch < d // 8, ch, 0)
+                    return np.where(rr < KT, at, 0)
                 orow = d * so
                 lpr = orow // 16
                 obase = w * RW * orow
                 ew = obase + c32 * orow + (16 * ((c32 & 7) ^ g) if so == 4 else 8 * g + 16 * (c32 & 7))
-                vals = dict(kr=kr, qo=((q0 + c32) * d + 8 * g) * 2, swp=(lane ^ 32) * 4, ew=ew, lim0=lim[0],
+                oc = lane // lpr
+                vals = dict(kr=kr, qo=((hh * n + row) * d + 8 * g) * 2, swp=(lane ^ 32) * 4, ew=ew, lim0=lim[0],
                             er=obase + (lane // lpr) * orow + 16 * ((lane % lpr) ^ (lane // lpr)),
-                            og=(q0 + lane // lpr) * width * so + h * orow + 16 * (lane % lpr),
-                            lo0=np.where(q0 + c32 < rows, (h * n + qb_i * R + q0 + c32) * 4, 0xffffffff))
+                            og=(q0 + oc // hpw) * width * so + (h + oc % hpw) * orow + 16 * (lane % lpr),
+                            lo0=np.where(row < rows, ((h + hh) * n + qb_i * R + row) * 4, 0xffffffff))
                 if r32:
                     hh, ii = (lane >> 4) & 1, lane & 15
                     vals.update({f'vr{x}': vbase + (8 * g + ii // 4) * 2 * d + 8 * (ii % 4) +
@@ -161,24 +170,28 @@ def run(heads, kv, n, ctx, page, d, ind='bf16', outd='f32', cut=None, seed=0, kg
                     vreg = R32.VREG
                 else:
                     vr = R64.v_read_regs(vbase, d, lane)
-                    vals.update(vr0=vr[0], vr1=vr[1], kr0=kr, lim1=lim[1], vd=(V_TILE // 4) * w + R64.vd_lane(d, lane),
-                                lo1=np.where(q0 + 32 + c32 < rows, (h * n + qb_i * R + q0 + 32 + c32) * 4, 0xffffffff))
+                    rr, pos = 16 * lane // (2 * d), 16 * lane % (2 * d)
+                    vd, vdo = ((V_TILE // 4) * w + rr * 2 * d + 16 * ((pos // 16) & 1) +
+                               32 * np.array([G.v_unit(int(u), int(r) + r0) for u, r in zip(pos // 32, rr)]) for r0 in (0, 2))
+                    vals.update(vr0=vr[0], vr1=vr[1], kr0=kr, lim1=lim[1], vd=vd, vdo=vdo,
+                                lo1=np.where(row1 < rows, ((h + hh) * n + qb_i * R + row1) * 4, 0xffffffff))
                     vals.update({f'kd{m}': kd_of(w + 4 * m) if m < NKP else 0 for m in range(4)}, kd4=kd_of(4 * NKP))
-                    vreg = R64.VREG
+                    vreg = VREG64
                 for name, x in vals.items():
                     W.v[int(vreg[name][1:])] = np.broadcast_to(np.asarray(x, np.int64), 64).astype(np.uint32)
-                for name, base, nbytes in (('qrs', Q0 + (h * n + qb_i * R) * row_b, rows * row_b),
+                for name, base, nbytes in (('qrs', Q0 + (h * n + qb_i * R) * row_b, ((hpw - 1) * n + rows) * row_b),
                                            ('ors', O0 + qb_i * R * width * so, rows * width * so),
                                            ('lrs', L0, heads * n * 4)):
                     W.s[SREG[name]:SREG[name] + 4] = [base & 0xFFFFFFFF, base >> 32, nbytes, 0x20000]
                 W.s[SREG['ent']:SREG['ent'] + 2] = [T0 & 0xFFFFFFFF, T0 >> 32]
                 kbase, vb0 = (x + kvh * page * row_b for x in (K0, V0))
-                per = page // 64
-                pg = [int(table[min(ta + i, tb - 1) // per]) for i in range(4)]
-                sv = dict(c=int(c.view(np.uint32)), nt=-(-n_keys // 64), ntw=ntw, lmin=min(p0 + 1, keys) - ks, has_lse=1,
-                          ogs=(64 // lpr) * width * so, kb0=kbase & 0xFFFFFFFF, kb1=kbase >> 32, kn=n_keys * row_b,
-                          vb0=vb0 & 0xFFFFFFFF, vb1=vb0 >> 32, skw=0, skww=1024 * w, svww=vbase + (V_TILE // 4) * w, t0=ta,
-                          tlast=tb - 1, npages=pages, pstride=kv * page * row_b, pmask=per - 1,
+                per, t0, last = page // KT, ks // KT, ks // KT + -(-n_keys // KT) - 1
+                pg = [int(table[min(t0 + i, last) // per]) for i in range(4)]
+                step = 64 // lpr // hpw * width * so if 64 // lpr >= hpw else orow
+                sv = dict(c=int(c.view(np.uint32)), nt=-(-n_keys // KT), ntw=ntw, lmin=min(p0 + 1, keys) - ks, has_lse=1,
+                          ogs=step, ogs2=2 * step if step != orow or hpw == 1 else width * so, qo1=64 // hpw * d, kb0=kbase & 0xFFFFFFFF, kb1=kbase >> 32, kn=n_keys * row_b,
+                          vb0=vb0 & 0xFFFFFFFF, vb1=vb0 >> 32, skw=0, skww=1024 * w, svww=vbase + (V_TILE // 4) * w, t0=t0,
+                          tlast=last, npages=pages, pstride=kv * page * row_b, pmask=per - 1,
                           pshift=per.bit_length() - 1, pg0=pg[0], pg1=pg[1], pg2=pg[2], pg3=pg[3])
                 for name, x in sv.items():
                     W.s[SREG[name]] = x & 0xFFFFFFFF

@@ -1,8 +1,8 @@
 """Plain forms of the operators of a cache kept in pages, in 64 bits, and the error their kernels may make.
 
 The attention's kernels round the probabilities to the input type for the product with V: p (1 + e), |e| <= h, half a step of
-the type (bf16 2^-8, f16 2^-11). Rows that see fewer than 64 keys get bf16 probabilities as a sum of two bf16 values: the
-second is off by h of what the first left, h p, so |e| <= h^2. Below f16's smallest normal value, 2^-14, f16 probabilities
+the type (bf16 2^-8, f16 2^-11). Rows that see fewer than 64 keys (heads of 256: 32) get bf16 probabilities as a sum of two
+bf16 values: the second is off by h of what the first left, h p, so |e| <= h^2. Below f16's smallest normal value, 2^-14, f16 probabilities
 are off by up to half a step there, 2^-25, against a sum of at least 1 (the running maximum
 is a score that was met). So an output is off by at most |e| sum_j w_j |v_j| + 2^-25 sum_j |v_j| (f16), by what the
 scores' errors make of the weights (a score off by ds moves each weight by at most a factor exp(2 ds)), and by its own
@@ -44,7 +44,7 @@ def attention(q, k, v, table, ctx, new, starts, *, scale, max_ctx, max_new, out_
         hidden = torch.arange(keys, device=q.device) >= seen[:, None]
         e = half_step(q.dtype)
         f16 = q.dtype == torch.float16
-        p_err = torch.where(seen < 64, e if f16 else e * e, e)[:, None]
+        p_err = torch.where(seen < (32 if D == 256 else 64), e if f16 else e * e, e)[:, None]
         for h in range(H):
             kk, vv = rows_of(k, table[b], keys, h * KV // H), rows_of(v, table[b], keys, h * KV // H)
             qq = q[h, s0:s0 + n].double()

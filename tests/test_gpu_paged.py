@@ -116,6 +116,15 @@ def test_single_tokens(dim, heads, kv, ctx):
     run_attention("bf16", heads, kv, dim, 64, [ctx, max(0, ctx - 1), ctx + 3], [1, 1, 1], decode=True, seed=ctx)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(8, 1, 64), (16, 2, 128), (24, 1, 128), (16, 1, 256), (32, 4, 128)])
+@pytest.mark.parametrize("out", [None, "f32"])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 16, 8], [31, 1, 64], [100, 33, 1]], ids=str)
+def test_groups_of_eight(heads, kv, dim, out, new):
+    """Two heads a wave: steps and chunks over short and long contexts, whole items and pieces, every kind of output."""
+    for ctx in ([0, 65, 300], [3000, 17, 900]):
+        run_attention("bf16", heads, kv, dim, 64, ctx, new, out=out, behind=2, q_pad=5, width=8, seed=heads + new[0])
+
+
 @pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 191, 255, 256, 257, 300])
 @pytest.mark.parametrize("dim,heads,kv", [(64, 2, 2), (128, 4, 1), (256, 4, 1)])
 def test_chunk_lengths(n, dim, heads, kv):

@@ -23,7 +23,7 @@ def test_registers_and_hazards():
     for name, lines in P.streams():
         names.append(name)
         assert Hz.check(lines, name) == 0
-    assert len(set(names)) == 20
+    assert len(set(names)) == 24
 
 
 def test_other_streams_are_as_before():
@@ -64,6 +64,27 @@ CASES = [
     dict(heads=2, kv=1, n=5, ctx=500, page=64, d=256, cut=(2, 8)),
     dict(heads=4, kv=1, n=5, ctx=500, page=64, d=256, cut=(7, 8)),
     dict(heads=4, kv=1, n=10, ctx=350, page=64, d=256, ind="f16", kgrow=1.5),
+    # tiles of 32 keys
+    dict(heads=4, kv=1, n=1, ctx=0, page=64, d=256, wave_rows=32),
+    dict(heads=4, kv=1, n=1, ctx=31, page=64, d=256, wave_rows=32, outd="bf16"),
+    dict(heads=4, kv=1, n=33, ctx=300, page=128, d=256, wave_rows=32, outd="bf16", missing=(1,)),
+    dict(heads=1, kv=1, n=128, ctx=64, page=64, d=256, wave_rows=32, ind="f16", outd="f16"),
+    dict(heads=2, kv=1, n=5, ctx=500, page=64, d=256, wave_rows=32, cut=(2, 8)),
+    dict(heads=4, kv=1, n=5, ctx=500, page=64, d=256, wave_rows=32, cut=(7, 8)),
+    dict(heads=4, kv=1, n=10, ctx=350, page=64, d=256, wave_rows=32, ind="f16", kgrow=1.5),
+    # two heads a wave
+    dict(heads=8, kv=1, n=1, ctx=300, page=64, d=128),
+    dict(heads=8, kv=1, n=40, ctx=130, page=64, d=128, outd="bf16"),
+    dict(heads=16, kv=2, n=33, ctx=70, page=64, d=64, ind="f16", outd="f16"),
+    dict(heads=8, kv=1, n=1, ctx=700, page=128, d=128, wave_rows=32, outd="bf16"),
+    dict(heads=8, kv=1, n=15, ctx=300, page=64, d=128, wave_rows=32, missing=(2,)),
+    dict(heads=8, kv=1, n=3, ctx=300, page=64, d=64, wave_rows=32),
+    dict(heads=8, kv=1, n=16, ctx=100, page=64, d=64, wave_rows=32, ind="f16", outd="f16"),
+    dict(heads=8, kv=1, n=17, ctx=100, page=64, d=256),
+    dict(heads=8, kv=1, n=1, ctx=200, page=64, d=256, outd="bf16"),
+    dict(heads=8, kv=1, n=1, ctx=500, page=64, d=256, cut=(2, 6)),
+    dict(heads=8, kv=1, n=9, ctx=200, page=64, d=256, wave_rows=32),
+    dict(heads=8, kv=1, n=16, ctx=200, page=64, d=256, wave_rows=32, ind="f16", outd="f16"),
 ]
 
 
@@ -77,12 +98,12 @@ def test_stream(case, monkeypatch):
         assert E.EXACT_COUNT[0] > taken  # the exact path ran
 
 
-@pytest.mark.parametrize("d", [128, 256])
-def test_planted_page_of_another_tile_is_found(d, monkeypatch):
+@pytest.mark.parametrize("d,rows", [(128, 64), (128, 32), (256, 64), (256, 32)])
+def test_planted_page_of_another_tile_is_found(d, rows, monkeypatch):
     """Every tile from the page read before: the outputs are off."""
     of = G.page_load
     monkeypatch.setattr(G, "page_load", lambda page, tile, t: of(page, tile, t)[:3] + ["s_nop 0"])
-    assert R.run(heads=4, kv=1, n=3, ctx=600, page=64, d=d)["out_bad"] > 0
+    assert R.run(heads=4, kv=1, n=3, ctx=600, page=64, d=d, wave_rows=rows)["out_bad"] > 0
 
 
 def test_planted_look_past_the_table_is_found(monkeypatch):
