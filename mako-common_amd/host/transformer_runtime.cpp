@@ -264,4 +264,96 @@ void TransformerRuntime::cache_evict(gpu::Encoder*& enc, gpu::Buffer* k, gpu::Bu
     after(enc, "cache_evict");
 }
 
+namespace {
+
+mako_pages_args pages_args(const PagedCache& c, uint32_t rows = 0, uint32_t d_pad = 0)
+{
+    return {c.batch, rows, d_pad ? d_pad : rows, c.pages, c.page, c.max_pages, c.kv_heads, c.dim, c.layers};
+}
+
+void* of_layer(gpu::Buffer* pool, const PagedCache& c, uint32_t layer)
+{
+    const uint64_t bytes = 2ull * c.pages * c.kv_heads * c.page * c.dim;
+    if (layer >= c.layers || (layer + 1) * bytes > pool->bytes)
+        throw std::runtime_error(fmt("paged cache: layer %u of %u in a pool of %llu bytes", layer, c.layers,
+                                     (unsigned long long)pool->bytes));
+    return static_cast<char*>(pool->ptr) + layer * bytes;
+}
+
+}  // namespace
+
+void TransformerRuntime::attention_paged(gpu::Encoder*& enc, gpu::Buffer* q, const PagedCache& c, uint32_t layer,
+                                         gpu::Buffer* starts, gpu::Buffer* o, uint32_t rows, uint32_t n_heads,
+                                         uint32_t max_new, uint32_t max_ctx, const AttnOptions& opt, uint32_t q_pad)
+{
+    const mako_paged_args a{c.batch, rows, q_pad ? q_pad : rows, n_heads, c.kv_heads, c.dim, c.pages, c.page, c.max_pages,
+                            max_new, max_ctx, n_heads * c.dim, 1.0f / std::sqrt(float(c.dim))};
+    const void *k = of_layer(c.k, c, layer), *v = of_layer(c.v, c, layer);
+    const size_t need = mako_attn_paged_workspace(&a);
+    gpu::Buffer* ws = need ? scratch("attn_paged", need) : nullptr;
+    before(enc);
+    for (int r = repeats("attn_paged"); r > 0; --r)
+        check(mako_attn_paged(&a, opt.in, opt.out, q->ptr, k, v, ptr<const uint32_t>(c.table),
+                              ptr<const uint32_t>(starts), ptr<const uint32_t>(c.ctx_len), o->ptr, ptr<float>(opt.lse),
+                              ptr<void>(ws), ws ? ws->bytes : 0, enc->stream));
+    after(enc, "attn_paged");
+}
+
+void TransformerRuntime::pages_write(gpu::Encoder*& enc, gpu::Buffer* kd, gpu::Buffer* vd, const PagedCache& c,
+                                     uint32_t layer, gpu::Buffer* starts, gpu::Buffer* end, uint32_t rows, uint32_t d_pad)
+{
+    const mako_pages_args a = pages_args(c, rows, d_pad);
+    void *k = of_layer(c.k, c, layer), *v = of_layer(c.v, c, layer);
+    before(enc);
+    for (int r = repeats("pages_write"); r > 0; --r)
+        check(mako_pages_write(&a, kd->ptr, vd->ptr, ptr<const uint32_t>(c.table), ptr<const uint32_t>(starts),
+                               ptr<const uint32_t>(c.ctx_len), ptr<const uint32_t>(end), k, v, enc->stream));
+    after(enc, "pages_write");
+}
+
+void TransformerRuntime::pages_reserve(gpu::Encoder*& enc, const PagedCache& c, gpu::Buffer* starts, gpu::Buffer* end,
+                                       uint32_t rows)
+{
+    if (end == c.ctx_len)
+        throw std::runtime_error("pages_reserve: end is ctx_len, which the step's writes and attention still read");
+    const mako_pages_args a = pages_args(c, rows);
+    of_layer(c.k, c, c.layers - 1), of_layer(c.v, c, c.layers - 1);
+    const size_t need = mako_pages_reserve_workspace(&a);
+    gpu::Buffer* ws = need ? scratch("pages_reserve", need) : nullptr;
+    before(enc);
+    // (once: the pages are there by then)
+    check(mako_pages_reserve(&a, ptr<const uint32_t>(c.table), ptr<const uint32_t>(c.refs), ptr<const uint32_t>(starts),
+                             ptr<const uint32_t>(c.ctx_len), ptr<uint32_t>(c.table), ptr<uint32_t>(c.refs),
+                             ptr<uint32_t>(end), c.k->ptr, c.v->ptr, ptr<void>(ws), ws ? ws->bytes : 0, enc->stream));
+    after(enc, "pages_reserve");
+}
+
+void TransformerRuntime::pages_fork(gpu::Encoder*& enc, const PagedCache& c, gpu::Buffer* parent, gpu::Buffer* keep)
+{
+    const mako_pages_args a = pages_args(c);
+    const size_t need = mako_pages_fork_workspace(&a);
+    gpu::Buffer* ws = need ? scratch("pages_fork", need) : nullptr;
+    before(enc);
+    // (once: a second call would fork the new sequences)
+    check(mako_pages_fork(&a, ptr<const uint32_t>(parent), ptr<const uint32_t>(keep), ptr<const uint32_t>(c.table),
+                          ptr<const uint32_t>(c.refs), ptr<const uint32_t>(c.ctx_len), ptr<uint32_t>(c.table),
+                          ptr<uint32_t>(c.refs), ptr<uint32_t>(c.ctx_len), ptr<void>(ws), ws ? ws->bytes : 0,
+                          enc->stream));
+    after(enc, "pages_fork");
+}
+
+void TransformerRuntime::pages_compact(gpu::Encoder*& enc, const PagedCache& c, gpu::Buffer* used, gpu::Buffer* map)
+{
+    const mako_pages_args a = pages_args(c);
+    of_layer(c.k, c, c.layers - 1), of_layer(c.v, c, c.layers - 1);
+    const size_t need = mako_pages_compact_workspace(&a);
+    gpu::Buffer* ws = need ? scratch("pages_compact", need) : nullptr;
+    before(enc);
+    // (once: nothing is left to move, and map would say so)
+    check(mako_pages_compact(&a, ptr<const uint32_t>(c.table), ptr<const uint32_t>(c.refs), ptr<uint32_t>(c.table),
+                             ptr<uint32_t>(c.refs), ptr<uint32_t>(used), ptr<uint32_t>(map), c.k->ptr, c.v->ptr,
+                             ptr<void>(ws), ws ? ws->bytes : 0, enc->stream));
+    after(enc, "pages_compact");
+}
+
 }  // namespace mako::models

@@ -24,6 +24,17 @@ struct AttnOptions {
     bool sel_per_kv_head = false;  // attention_sparse: sel / nsel hold one list per kv head
 };
 
+// A cache kept in pages for `batch` sequences (include/mako_attn.h): all layers' pools of f16 or bf16 rows, and what says who
+// holds which page.
+struct PagedCache {
+    gpu::Buffer *k, *v;    // [layers][pages][kv_heads][page][dim]
+    gpu::Buffer* table;    // u32 [batch][max_pages]
+    gpu::Buffer* refs;     // u32 [pages]
+    gpu::Buffer* ctx_len;  // u32 [batch]
+    uint32_t batch, pages, page, max_pages, kv_heads;
+    uint32_t dim = 128, layers = 1;
+};
+
 class TransformerRuntime : public gpu::Runtime {
 public:
     virtual const char* name() const { return "model"; }
@@ -125,6 +136,29 @@ protected:
                      gpu::Buffer* seen, gpu::Buffer* ctx_len, uint32_t batch, uint32_t kv_heads, uint32_t cap,
                      uint32_t max_ctx, uint32_t budget, uint32_t recent, uint32_t sinks, uint32_t dim = kHeadDim,
                      mako_dtype in = MAKO_F16);
+    // A cache kept in pages (no counterparts in the reference). A step of a batch, one token or a chunk of each sequence, is
+    // pages_reserve, then for each layer pages_write and attention_paged, then c.ctx_len and `end` change places. The new
+    // rows of all sequences lie one after another, sequence b's at starts[b] .. starts[b + 1] (u32 [batch + 1]; null: one row
+    // each), in `rows` rows; q_pad and d_pad as in attention_tree.
+    //
+    // attention_paged: q [heads][q_pad][dim], o [rows][heads * dim], opt.lse [heads][rows]; row i of sequence b sees the
+    // cache rows up to ctx_len[b] + i, its own. max_new bounds a sequence's new rows, max_ctx its rows with them. Scratch
+    // "attn_paged".
+    void attention_paged(gpu::Encoder*& enc, gpu::Buffer* q, const PagedCache& c, uint32_t layer, gpu::Buffer* starts,
+                         gpu::Buffer* o, uint32_t rows, uint32_t heads, uint32_t max_new, uint32_t max_ctx,
+                         const AttnOptions& opt = {}, uint32_t q_pad = 0);
+    // kd and vd [kv_heads][d_pad][dim] into the pages of a layer; rows from end[b] on (null: none) are dropped.
+    void pages_write(gpu::Encoder*& enc, gpu::Buffer* kd, gpu::Buffer* vd, const PagedCache& c, uint32_t layer,
+                     gpu::Buffer* starts, gpu::Buffer* end, uint32_t rows, uint32_t d_pad = 0);
+    // Pages for the new rows, table and refs in place; end u32 [batch]: the rows of a sequence that have room, the new ones
+    // among them (not c.ctx_len, which the step's other calls still read). Scratch "pages_reserve".
+    void pages_reserve(gpu::Encoder*& enc, const PagedCache& c, gpu::Buffer* starts, gpu::Buffer* end, uint32_t rows);
+    // Sequence i goes on from parent[i]'s first keep[i] rows (null: its own; all), table, refs and ctx_len in place. Scratch
+    // "pages_fork".
+    void pages_fork(gpu::Encoder*& enc, const PagedCache& c, gpu::Buffer* parent, gpu::Buffer* keep);
+    // Moves the used pages of all layers to the pool's start, table and refs in place; used u32 [1]: their number; map u32
+    // [pages] (null: not wanted): where each went. Scratch "pages_compact".
+    void pages_compact(gpu::Encoder*& enc, const PagedCache& c, gpu::Buffer* used, gpu::Buffer* map = nullptr);
 };
 
 }  // namespace mako::models
