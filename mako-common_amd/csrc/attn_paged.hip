@@ -386,14 +386,22 @@ uint32_t direct_tiles(uint64_t items, uint32_t ranges, bool many)
     return (many ? 17 : 11) + (x > 7 ? (uint32_t)x - 7 : 0);
 }
 
+uint32_t item_heads(const mako_paged_args* a)
+{
+    const uint32_t group = a->heads / a->kv_heads;
+    if (group % 8 == 0 && 4ull * a->dim * a->q_pad < (1ull << 32))  // (two heads' queries have 32-bit offsets)
+        return 8;
+    return group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+}
+uint32_t item_rows(const mako_paged_args* a) { return (a->dim == 256 ? 128 : 256) / item_heads(a); }
+
 Plan plan_of(const mako_paged_args* a, uint32_t cus)
 {
     const uint32_t group = a->heads / a->kv_heads;
     Plan pl{};
-    const bool both = group % 8 == 0 && 4ull * a->dim * a->q_pad < (1ull << 32);  // (a wave's q: 32-bit offsets)
-    pl.hpw = both ? 2 : 1;
-    pl.hq = both ? 8 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
-    pl.rshift = log2_of((a->dim == 256 ? 128 : 256) / pl.hq);
+    pl.hq = item_heads(a);
+    pl.hpw = pl.hq == 8 ? 2 : 1;
+    pl.rshift = log2_of(item_rows(a));
     pl.ncb = group / pl.hq;
     pl.n_ranges = std::max(1u, cus / pl.ncb);
     if (pl.n_ranges > 8)
@@ -482,8 +490,10 @@ int check_args(const mako_paged_args* a, mako_dtype in, mako_dtype out, const vo
     if ((uint64_t)a->heads * a->dim > a->width || a->width % 4 || a->width >= (1u << 20))
         return fail(MAKO_EINVAL, "%s: o rows of %u for %u heads of %u (a multiple of 4, at least their width, below 2^20)",
                     what, a->width, a->heads, a->dim);
-    // what the split counts: at most kTile units a tile, for every 16 rows of a sequence at least
-    const uint64_t units = ((uint64_t)a->rows / 16 + a->batch) * ((uint64_t)a->max_ctx / 5 + 1024) * a->kv_heads;
+    // What the split counts: the items, kLead and kTile a tile each (tiles of new rows past max_ctx too).
+    const uint32_t R = item_rows(a);
+    const uint64_t units = ((uint64_t)a->rows / R + a->batch) * a->kv_heads *
+                           (kLead + kTile * (((uint64_t)a->max_ctx + a->max_new + R) / 64 + 2));
     if (units >= (1ull << 32) || (uint64_t)a->rows * a->heads >= (1u << 30))
         return fail(MAKO_EINVAL, "%s: %u rows of %u heads over %u keys are too many", what, a->rows, a->heads, a->max_ctx);
     if (!(a->scale > 0.0f) || a->scale == INFINITY)

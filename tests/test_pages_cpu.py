@@ -69,6 +69,7 @@ def paged_rc(**kw):
     (dict(o=ODD), M.EINVAL, "aligned"),
     (dict(rows=1 << 26, q_pad=1 << 26, heads=64, width=8192), M.EINVAL, "too many"),
     (dict(rows=1 << 22, q_pad=1 << 22, max_ctx=1 << 30, max_pages=1 << 24), M.EINVAL, "too many"),
+    (dict(rows=1 << 21, q_pad=1 << 21, max_new=1 << 21), M.EINVAL, "too many"),  # (new rows far past max_ctx)
 ])
 def test_attention_refuses(kw, code, msg):
     rc, err = paged_rc(**kw)
