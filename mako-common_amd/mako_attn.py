@@ -413,9 +413,10 @@ def attn_paged(a, q, k, v, table, ctx_len, o, workspace, *, starts=None, lse=Non
     """mako_attn_paged on torch tensors: q [heads][q_pad][dim], k, v [pages][kv_heads][page][dim], table int32
     [batch][max_pages], ctx_len int32 [batch], starts int32 [batch + 1] (all read as u32), o [rows][width], lse float32
     [heads][rows]."""
-    _check(lib().mako_attn_paged(ctypes.byref(a), dtype_code(q), dtype_code(o), _ptr(q), _ptr(k), _ptr(v), _ptr(table),
-                                 _ptr(starts), _ptr(ctx_len), _ptr(o), _ptr(lse), _ptr(workspace), _nbytes(workspace),
-                                 _stream(stream)))
+    # (data_ptr() where there has to be a tensor, here and below: the small calls' time is the host's, 6.4 us with _ptr, 5.7)
+    _check(lib().mako_attn_paged(a, dtype_code(q), dtype_code(o), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                 table.data_ptr(), _ptr(starts), ctx_len.data_ptr(), o.data_ptr(), _ptr(lse),
+                                 _ptr(workspace), _nbytes(workspace), _stream(stream)))
 
 
 def pages_args(*, batch, pages, page, max_pages, rows=0, kv_heads=0, dim=0, layers=1, d_pad=None):
@@ -425,8 +426,8 @@ def pages_args(*, batch, pages, page, max_pages, rows=0, kv_heads=0, dim=0, laye
 def pages_write(a, kd, vd, k, v, table, ctx_len, *, starts=None, end=None, stream=None):
     """mako_pages_write on torch tensors: kd, vd [kv_heads][d_pad][dim], k, v [pages][kv_heads][page][dim], table int32
     [batch][max_pages], ctx_len and end int32 [batch], starts int32 [batch + 1]."""
-    _check(lib().mako_pages_write(ctypes.byref(a), _ptr(kd), _ptr(vd), _ptr(table), _ptr(starts), _ptr(ctx_len),
-                                  _ptr(end), _ptr(k), _ptr(v), _stream(stream)))
+    _check(lib().mako_pages_write(a, kd.data_ptr(), vd.data_ptr(), table.data_ptr(), _ptr(starts), ctx_len.data_ptr(),
+                                  _ptr(end), k.data_ptr(), v.data_ptr(), _stream(stream)))
 
 
 def pages_reserve_workspace(a):
@@ -436,9 +437,9 @@ def pages_reserve_workspace(a):
 def pages_reserve(a, k, v, table, refs, ctx_len, table_out, refs_out, ctx_out, workspace, *, starts=None, stream=None):
     """mako_pages_reserve on torch tensors: k, v [layers][pages][kv_heads][page][dim] or None, table and table_out int32
     [batch][max_pages], refs and refs_out int32 [pages], ctx_len and ctx_out int32 [batch], starts int32 [batch + 1]."""
-    _check(lib().mako_pages_reserve(ctypes.byref(a), _ptr(table), _ptr(refs), _ptr(starts), _ptr(ctx_len),
-                                    _ptr(table_out), _ptr(refs_out), _ptr(ctx_out), _ptr(k), _ptr(v), _ptr(workspace),
-                                    _nbytes(workspace), _stream(stream)))
+    _check(lib().mako_pages_reserve(a, table.data_ptr(), refs.data_ptr(), _ptr(starts), ctx_len.data_ptr(),
+                                    table_out.data_ptr(), refs_out.data_ptr(), ctx_out.data_ptr(), _ptr(k), _ptr(v),
+                                    _ptr(workspace), _nbytes(workspace), _stream(stream)))
 
 
 def pages_fork_workspace(a):
@@ -449,9 +450,9 @@ def pages_fork(a, table, refs, ctx_len, table_out, refs_out, ctx_out, workspace=
                stream=None):
     """mako_pages_fork on torch tensors: table and table_out int32 [batch][max_pages], refs and refs_out int32 [pages],
     ctx_len, ctx_out, parent and keep int32 [batch]."""
-    _check(lib().mako_pages_fork(ctypes.byref(a), _ptr(parent), _ptr(keep), _ptr(table), _ptr(refs), _ptr(ctx_len),
-                                 _ptr(table_out), _ptr(refs_out), _ptr(ctx_out), _ptr(workspace), _nbytes(workspace),
-                                 _stream(stream)))
+    _check(lib().mako_pages_fork(a, _ptr(parent), _ptr(keep), table.data_ptr(), refs.data_ptr(), ctx_len.data_ptr(),
+                                 table_out.data_ptr(), refs_out.data_ptr(), ctx_out.data_ptr(), _ptr(workspace),
+                                 _nbytes(workspace), _stream(stream)))
 
 
 def pages_compact_workspace(a):
@@ -461,8 +462,8 @@ def pages_compact_workspace(a):
 def pages_compact(a, k, v, table, refs, table_out, refs_out, used_out, workspace, *, map_out=None, stream=None):
     """mako_pages_compact on torch tensors: k, v [layers][pages][kv_heads][page][dim] or None, table and table_out int32
     [batch][max_pages], refs, refs_out and map_out int32 [pages], used_out int32 [1]."""
-    _check(lib().mako_pages_compact(ctypes.byref(a), _ptr(table), _ptr(refs), _ptr(table_out), _ptr(refs_out),
-                                    _ptr(used_out), _ptr(map_out), _ptr(k), _ptr(v), _ptr(workspace),
+    _check(lib().mako_pages_compact(a, table.data_ptr(), refs.data_ptr(), table_out.data_ptr(), refs_out.data_ptr(),
+                                    used_out.data_ptr(), _ptr(map_out), _ptr(k), _ptr(v), _ptr(workspace),
                                     _nbytes(workspace), _stream(stream)))
 
 
