@@ -242,13 +242,13 @@ __global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams q)
 {
     __shared__ __attribute__((aligned(1024))) unsigned char lds[lds_bytes<D>()];
     const uint32_t lane = threadIdx.x & 63u, w = uniform(threadIdx.x >> 6);
-    // blockIdx.x is the XCD: ranges side by side on one, a range's column blocks too
-    const uint32_t range = blockIdx.x * gridDim.z + blockIdx.z, cb = blockIdx.y;
+    // blockIdx.x is the XCD: ranges side by side on one, a range's column blocks too (kItems: the kv head)
+    const uint32_t range = q.how == kItems ? blockIdx.z : blockIdx.x * gridDim.z + blockIdx.z, cb = blockIdx.y;
 
     uint32_t here[2] = {0, 0};
     u32x4 done = u32x4{kNone, 0, 0, 0};
     const ParamsAt at_p = (ParamsAt)__builtin_amdgcn_kernarg_segment_ptr();
-    walk_range(q, range, lane, [&](const PagedPiece& at) __attribute__((always_inline)) {
+    walk_range(q, range, blockIdx.x, lane, [&](const PagedPiece& at) __attribute__((always_inline)) {
         const auto& p = *params_here(at_p);
         const uint32_t hl = (w & ((1u << p.ws) - 1)) << p.hs, h = at.kvh * p.group + cb * p.hq + hl;
         Piece x;
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams q)
         }
     });
     const auto& p = *params_here(at_p);
-    if (!p.direct && cb == 0 && threadIdx.x == 0) {
+    if (p.how == kRanges && cb == 0 && threadIdx.x == 0) {
         p.whole[2 * range] = here[0];
         p.whole[2 * range + 1] = here[1];
         p.last[range] = done;
@@ -369,13 +369,14 @@ __global__ __launch_bounds__(256) void paged_merge(const PagedParams p, uint32_t
 
 // A call's split, from its sizes alone (lengths are known on the device only).
 struct Plan {
-    uint32_t hq, hpw, rshift, ncb, n_ranges, slot_rows, direct, few;
+    uint32_t hq, hpw, rshift, ncb, n_ranges, slot_rows, how, few;
 };
 
 constexpr uint32_t kFewMerged = 16;  // (row, head) pairs a range up to which paged_merge parts an item's pieces
 
 // Whole items and no second launch up to this many tiles a sequence: 11, where a merge joins more rows 17, and more the
-// nearer the items come to one a workgroup. us split / direct, single tokens, 32 heads of 128 over 8: 8 items of 8 tiles 15.6 /
+// nearer the items come to one a workgroup. (With a workgroup an item of sequences that are one item each: 0.4 to 0.6 us less a
+// call than by looking for its range; more items than workgroups are better spread by ranges.) us split / direct, single tokens, 32 heads of 128 over 8: 8 items of 8 tiles 15.6 /
 // 12.7, of 12 16.2 / 15.9, of 16 16.3 / 18.9; 64 of 12 15.9 / 16.4; 128 of 16 21.6 / 20.4, of 26 27.2 / 28.8; 256 of 33 48 / 46.
 // 16 heads of 256 over 2: 8 items of 8 17.8 / 16.4, of 12 18.0 / 20.5; 128 of 33 63 / 62. 256 rows of 32 heads: 32 items of 16
 // 28.8 / 27.7, of 24 31.5 / 36.8; 128 of 24 41 / 37. A workgroup takes its item's tiles one after the other whatever the
@@ -408,11 +409,12 @@ Plan plan_of(const mako_paged_args* a, uint32_t cus)
         pl.n_ranges &= ~7u;
     pl.slot_rows = std::min(1u << pl.rshift, a->max_new);
     const uint64_t items = ((uint64_t)(a->rows >> pl.rshift) + a->batch) * a->kv_heads;
-    pl.direct = (a->max_ctx + 63) / 64 <= direct_tiles(items, pl.n_ranges, pl.slot_rows * group > kFewMerged);
+    if ((a->max_ctx + 63) / 64 <= direct_tiles(items, pl.n_ranges, pl.slot_rows * group > kFewMerged))
+        pl.how = a->max_new <= item_rows(a) && (uint64_t)a->batch * a->kv_heads <= pl.n_ranges ? kItems : kWhole;
     // Heads of 256, tiles of 32 keys / of 64: a step of 16 sequences over up to 32767 rows 103 us / 116, 8 tokens each 110 / 121,
     // 16 tokens each 136 / 129; steps among chunks 267 / 225; one token over 391 rows in one launch 16.1 / 15.5.
     pl.few = (1u << pl.rshift) / 2;
-    if (a->dim == 256 && (pl.direct || a->max_new > pl.few))
+    if (a->dim == 256 && (pl.how != kRanges || a->max_new > pl.few))
         pl.few = 0;
     return pl;
 }
@@ -424,19 +426,19 @@ size_t part_o_bytes(const Plan& pl, uint32_t dim)
 size_t part_l_bytes(const Plan& pl) { return round256((size_t)pl.n_ranges * pl.ncb * 2 * pl.slot_rows * pl.hq * 4); }
 size_t workspace_for(const Plan& pl, uint32_t dim)
 {
-    return pl.direct ? 0 : part_o_bytes(pl, dim) + part_l_bytes(pl) + (size_t)pl.n_ranges * 24;
+    return pl.how != kRanges ? 0 : part_o_bytes(pl, dim) + part_l_bytes(pl) + (size_t)pl.n_ranges * 24;
 }
 
 template <class T, class TO, int D>
 void launch(const PagedParams& p, hipStream_t s)
 {
     const uint32_t xcds = p.n_ranges % 8 == 0 ? 8 : 1;
-    const dim3 grid(xcds, p.ncb, p.n_ranges / xcds);
+    const dim3 grid = p.how == kItems ? dim3(p.kv_heads, p.ncb, p.batch) : dim3(xcds, p.ncb, p.n_ranges / xcds);
     if (p.max_new <= p.few)
         hipLaunchKernelGGL((paged_rows<T, TO, D, true>), grid, dim3(256), 0, s, p);
     else
         hipLaunchKernelGGL((paged_rows<T, TO, D, false>), grid, dim3(256), 0, s, p);
-    if (p.direct)
+    if (p.how != kRanges)
         return;
     const uint32_t nw = p.slot_rows * p.group <= kFewMerged ? 4 : 1, per = (p.slot_rows * p.group * nw * D + 1023) / 1024;
     if (nw == 4)
@@ -535,7 +537,7 @@ extern "C" int mako_attn_paged(const mako_paged_args* a, mako_dtype in, mako_dty
     const size_t ob = part_o_bytes(pl, a->dim), lb = part_l_bytes(pl), wb = (size_t)pl.n_ranges * 8;
     const auto at = [&](size_t off) { return ws ? ws + off : nullptr; };
     const PagedParams p{{starts, ctx_len, a->batch, a->rows, a->kv_heads, a->max_new, a->max_ctx, pl.rshift, pl.n_ranges,
-                         pl.direct, pl.few},
+                         pl.how, pl.few},
                         q, k, v, table, o, lse, reinterpret_cast<float*>(at(0)), reinterpret_cast<float*>(at(ob)),
                         reinterpret_cast<uint32_t*>(at(ob + lb + 2 * wb)), reinterpret_cast<u32x4*>(at(ob + lb)), a->q_pad,
                         a->heads / a->kv_heads, a->pages, a->kv_heads * a->page * a->dim * 2, log2_of(a->page),

@@ -9,7 +9,7 @@
 // 225 us, 208 so.) Within a segment the row blocks go heavy and light in turn (the last, the first, the last but one, the
 // second, ...), so two neighbours cost the same everywhere, and the ranges of a whole prompt fall on items' ends.
 // A cut inside an item leaves kLeast tiles on either side, and no row without keys in a piece's first tile, which the
-// attention's streams rely on; with `direct`, items are not cut: the range of an item's middle has it.
+// attention's streams rely on; with kWhole, items are not cut: the range of an item's middle has it.
 #pragma once
 
 #include "pages_common.hpp"
@@ -23,9 +23,13 @@ namespace mako {
 constexpr uint32_t kTile = 12, kTileFew = 8, kLead = 60, kLeadFew = 36;
 constexpr uint32_t kLeast = 3;  // tiles of a piece
 
+// How a call is split: by equal ranges; by equal ranges that whole items fall to; or, where no sequence has more rows than an
+// item, by sequence and kv head.
+enum : uint32_t { kRanges, kWhole, kItems };
+
 struct PagedSplit {
     const uint32_t *starts, *ctx;
-    uint32_t batch, rows, kv_heads, max_new, max_ctx, rshift, n_ranges, direct, few;
+    uint32_t batch, rows, kv_heads, max_new, max_ctx, rshift, n_ranges, how, few;
 };
 
 // A piece of an item: tiles [ta, tb) of sequence b for its rows row0 .. of o, the first at position p0.
@@ -74,48 +78,56 @@ __device__ __forceinline__ uint32_t segment_units(const PagedSeq& s)
 __device__ __forceinline__ uint32_t cut_of(const PagedSplit& p, uint32_t u, uint32_t few, uint32_t nt, uint32_t tmax)
 {
     const uint32_t t = few ? (max(u, kLeadFew) - kLeadFew) / kTileFew : (max(u, kLead) - kLead) / kTile;
-    if (p.direct)
+    if (p.how == kWhole)
         return 2 * t < nt ? 0u : nt;
     return t < kLeast ? 0u : t + kLeast > nt ? nt : min(t, tmax);
 }
 
-// Calls piece(PagedPiece) for the pieces of a range, in order; all lanes of a wave do so together.
+// Calls piece(PagedPiece) for the pieces of a range, in order (kItems: for the item of sequence `range` and kv head kvh); all
+// lanes of a wave do so together.
 template <class F>
-__device__ __forceinline__ void walk_range(const PagedSplit& p, uint32_t range, uint32_t lane, F piece)
+__device__ __forceinline__ void walk_range(const PagedSplit& p, uint32_t range, uint32_t kvh, uint32_t lane, F piece)
 {
+    uint32_t b = range, u0 = 0, item = 0, start = 0, left = 1;
+    Ranges rg{};
+    PagedSeq mine{}, s{};
     // The units of all segments; a lane holds a sequence, so up to 64 are looked up once.
-    PagedSeq mine{};
-    uint32_t total = 0, units = 0, inc = 0;
+    uint32_t units = 0, inc = 0;
     const auto look_up = [&](uint32_t i0) __attribute__((always_inline)) {
         mine = seq_of(p, min(i0 + lane, p.batch - 1));
         units = i0 + lane < p.batch ? segment_units(mine) : 0u;
         inc = scan_lanes(units);
     };
-    for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
-        look_up(i0);
-        total += (uint32_t)__builtin_amdgcn_readlane(inc, 63);
-    }
-    const uint32_t n = min(p.n_ranges, total * p.kv_heads);
-    if (range >= n)
-        return;
-    const Ranges rg(total * p.kv_heads, n);
-    const uint32_t x0 = rg.start(range);
-    uint32_t left = rg.start(range + 1) - x0;
-    // Of kv head kvh, the sequence b whose segment holds x0, u0 units into it.
-    uint32_t b = 0, kvh = x0 / total, u0 = x0 % total, item;
-    for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
-        if (p.batch > 64)
+    if (p.how == kItems) {
+        s = of_lane(seq_of(p, b), 0);
+        if (s.n == 0)
+            return;
+    } else {
+        uint32_t total = 0;
+        for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
             look_up(i0);
-        if (const uint64_t hit = __ballot(u0 < inc)) {
-            const uint32_t l = (uint32_t)__builtin_ctzll(hit);
-            b = i0 + l;
-            u0 -= (uint32_t)__builtin_amdgcn_readlane(inc - units, l);
-            break;
+            total += (uint32_t)__builtin_amdgcn_readlane(inc, 63);
         }
-        u0 -= (uint32_t)__builtin_amdgcn_readlane(inc, 63);
-    }
-    PagedSeq s = of_lane(mine, b);
-    {
+        const uint32_t n = min(p.n_ranges, total * p.kv_heads);
+        if (range >= n)
+            return;
+        rg = Ranges(total * p.kv_heads, n);
+        const uint32_t x0 = rg.start(range);
+        left = rg.start(range + 1) - x0;
+        // Of kv head kvh, the sequence b whose segment holds x0, u0 units into it.
+        kvh = x0 / total, u0 = x0 % total, b = 0;
+        for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
+            if (p.batch > 64)
+                look_up(i0);
+            if (const uint64_t hit = __ballot(u0 < inc)) {
+                const uint32_t l = (uint32_t)__builtin_ctzll(hit);
+                b = i0 + l;
+                u0 -= (uint32_t)__builtin_amdgcn_readlane(inc - units, l);
+                break;
+            }
+            u0 -= (uint32_t)__builtin_amdgcn_readlane(inc, 63);
+        }
+        s = of_lane(mine, b);
         // item 2 i is block nqb - 1 - i, item 2 i + 1 block i: a pair's units do not depend on i
         const uint32_t pair = 2 * s.lead + (s.nqb + 1) * s.step, i = u0 / pair;
         u0 -= i * pair;
@@ -125,16 +137,16 @@ __device__ __forceinline__ void walk_range(const PagedSplit& p, uint32_t range, 
             u0 -= heavy;
             ++item;
         }
+        start = x0 - u0;  // the item's first unit
     }
-    uint32_t start = x0 - u0;  // the item's first unit
     for (;;) {
-        const uint32_t qb = item & 1 ? item / 2 : s.nqb - 1 - item / 2;
-        const uint32_t cost = item_units(s, qb), u1 = min(cost, u0 + left), i0 = qb << p.rshift;
+        const uint32_t qb = item & 1 ? item / 2 : s.nqb - 1 - item / 2, i0 = qb << p.rshift;
+        const uint32_t cost = p.how == kItems ? 1 : item_units(s, qb), u1 = min(cost, u0 + left);
         PagedPiece x;
         x.b = b, x.kvh = kvh, x.row0 = s.s0 + i0, x.rows = min(1u << p.rshift, s.n - i0), x.p0 = s.c + i0;
         x.seen = s.keys, x.keys = min(x.p0 + x.rows, s.keys);
         const uint32_t nt = (x.keys + 63) / 64, tmax = (min(x.p0 + 1, s.keys) - 1) / 64;
-        x.ta = cut_of(p, u0, s.few, nt, tmax);
+        x.ta = u0 == 0 ? 0 : cut_of(p, u0, s.few, nt, tmax);
         x.tb = u1 == cost ? nt : cut_of(p, u1, s.few, nt, tmax);
         if (x.ta < x.tb) {
             x.part = x.ta != 0 || x.tb != nt;

@@ -24,6 +24,7 @@ __device__ __forceinline__ uint32_t scan_lanes(uint32_t x)
 // T units cut into n equal ranges: range w starts at floor(w T / n), without a 64-bit division (w r < n^2 fits 32 bits).
 struct Ranges {
     uint32_t q, r, n;
+    Ranges() = default;
     __device__ Ranges(uint32_t T, uint32_t ranges) : q(T / ranges), r(T % ranges), n(ranges) {}
     __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * q + (w * r) / n; }
 };

@@ -29,7 +29,8 @@ std::vector<Got> got;
 void record(const mako::PagedSplit& p)
 {
     const uint32_t range = blockIdx.x;
-    mako::walk_range(p, range, threadIdx.x, [&](const mako::PagedPiece& x) {
+    const bool items = p.how == mako::kItems;
+    mako::walk_range(p, items ? range % p.batch : range, items ? range / p.batch : 0, threadIdx.x, [&](const mako::PagedPiece& x) {
         if (threadIdx.x == 0)
             got.push_back({range, x});
     });
@@ -38,8 +39,8 @@ void record(const mako::PagedSplit& p)
 #define CHECK(...)                                                                                            \
     do {                                                                                                     \
         if (!(__VA_ARGS__)) {                                                                                       \
-            std::printf("FAILED %s: batch %u kv %u rshift %u ranges %u direct %u max_ctx %u\n", #__VA_ARGS__, p.batch, p.kv_heads, \
-                        p.rshift, p.n_ranges, p.direct, p.max_ctx);                                           \
+            std::printf("FAILED %s: batch %u kv %u rshift %u ranges %u how %u max_ctx %u\n", #__VA_ARGS__, p.batch, p.kv_heads, \
+                        p.rshift, p.n_ranges, p.how, p.max_ctx);                                           \
             return false;                                                                                    \
         }                                                                                                    \
     } while (0)
@@ -47,7 +48,7 @@ void record(const mako::PagedSplit& p)
 bool run(mako::PagedSplit p, bool good)
 {
     got.clear();
-    cpu_hip::launch(dim3(p.n_ranges), dim3(64), [&] { record(p); });
+    cpu_hip::launch(dim3(p.how == mako::kItems ? p.batch * p.kv_heads : p.n_ranges), dim3(64), [&] { record(p); });
     std::map<std::tuple<uint32_t, uint32_t, uint32_t>, uint32_t> next;  // the tile that an item's next piece starts with
     std::map<std::tuple<uint32_t, uint32_t, uint32_t>, std::vector<Got>> parts;
     std::map<std::pair<uint32_t, uint32_t>, int> slots;
@@ -59,7 +60,7 @@ bool run(mako::PagedSplit p, bool good)
         CHECK(x.b < p.batch && x.kvh < p.kv_heads && x.rows >= 1 && x.rows <= R && x.row0 + x.rows <= p.rows);
         CHECK(x.ta < x.tb && x.keys <= p.max_ctx && x.seen <= p.max_ctx && 64 * (x.tb - 1) < x.keys);
         CHECK(64 * x.ta < std::min(x.p0 + 1, x.seen));  // the first row sees a key of the piece's first tile
-        CHECK(x.ta == 0 || !p.direct);
+        CHECK(p.how == mako::kRanges || !x.part);
         const double few = x.rows <= p.few && x.seen - x.p0 <= p.few ? mako::kTileFew : mako::kTile;
         cost[g.range] += (x.tb - x.ta) * few + mako::kLead;
         all += (x.tb - x.ta) * few + mako::kLead;
@@ -94,7 +95,7 @@ bool run(mako::PagedSplit p, bool good)
     for (const auto& c : cost)
         most = std::max(most, c.second);
     // no range has more than its share and a little
-    CHECK(p.direct || most <= all / p.n_ranges + mako::kTile * (3 * R / 64 + 8) + mako::kLead * (items / p.n_ranges + 3));
+    CHECK(p.how != mako::kRanges || most <= all / p.n_ranges + mako::kTile * (3 * R / 64 + 8) + mako::kLead * (items / p.n_ranges + 3));
     return true;
 }
 
@@ -114,7 +115,9 @@ int main()
             top = std::max(top, ctx[b] + starts[b + 1] - starts[b]);
         }
         mako::PagedSplit p{most == 1 ? nullptr : starts.data(), ctx.data(), batch, starts[batch] + upto(3), 1 + upto(8), most,
-                           top + upto(1) * upto(500), 5 + upto(3), round % 2 ? 256 : 1 + upto(100), upto(5) == 0, 0};
+                           top + upto(1) * upto(500), 5 + upto(3), round % 2 ? 256 : 1 + upto(100), mako::kRanges, 0};
+        if (upto(4) == 0)
+            p.how = most <= 1u << p.rshift ? mako::kItems : mako::kWhole;
         p.few = upto(2) ? 1u << p.rshift >> 1 : 0;
         if (p.starts == nullptr)
             p.rows = batch;
