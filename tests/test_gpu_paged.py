@@ -185,6 +185,32 @@ def test_growing_scores(dim, growth):
     run_attention("f16", 4, 2, dim, 64, [900, 5000], [70, 1], edit=edit, seed=11)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [2, 16, 33, 100])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf, "low"])
+def test_a_later_rows_k_is_not_seen(dim, n, value):
+    """Whatever the k of a sequence's last new row holds, the rows before it are as with any other."""
+    def run(x):
+        g = gen(17)
+        pool = Pool(g, [900, 70], [n, n], 2, dim, 64, torch.bfloat16, fill=0.0)
+        at = [(900 + n - 1) // 64, (70 + n - 1) // 64]
+        if x is not None:
+            for b, c in ((0, 900), (1, 70)):
+                pool.k[pool.table[b, at[b]].item(), :, (c + n - 1) % 64] = torch.finfo(torch.bfloat16).min if x == "low" else x
+        a = M.paged_args(batch=2, rows=2 * n, heads=8, kv_heads=2, dim=dim, pages=pool.pages, page=64,
+                         max_pages=pool.max_pages, max_new=n, max_ctx=900 + n)
+        q = torch.randn((8, 2 * n, dim), generator=g, device="cuda").bfloat16()
+        o = torch.zeros((2 * n, 8 * dim), dtype=torch.bfloat16, device="cuda")
+        lse = torch.zeros((8, 2 * n), device="cuda")
+        M.attn_paged(a, q, pool.k, pool.v, pool.table, ints([900, 70]), o, space(M.attn_paged_workspace(a)),
+                     starts=ints([0, n, 2 * n]), lse=lse)
+        torch.cuda.synchronize()
+        before = [i for i in range(2 * n) if i % n != n - 1]
+        return o[before], lse[:, before]
+    (o, lse), (want, want_l) = run(value), run(None)
+    assert torch.equal(o, want) and torch.equal(lse, want_l)
+
+
 def test_scale_and_no_lse():
     run_attention("bf16", 4, 2, 128, 64, [200, 0], [33, 1], scale=0.5, want_lse=False, seed=12)
 
