@@ -11,7 +11,7 @@
 //   brings many), summed over the sequences, and the free pages looked for from the lowest number on until there are enough,
 //   so the look ends early in a pool that is kept compact. Sequences that append to one shared page meet in a hash table in
 //   LDS, by counts and maxima, which the order of the threads does not change. copy_pages then copies the shared pages' rows.
-//   64 sequences' step 5.4 us; 64 beams of 16 prompts 7.0, and 5.0 for the copies.
+//   64 sequences' step 4.8 us; 64 beams of 16 prompts 6.0, and 5.0 for the copies.
 // * fork_rows: a workgroup a new sequence; the holders' counts change by integer atomics, only where old and new entry differ.
 //   1024 sequences of up to 129 pages 3.8 us after the copies' 2.6; fork_small 3.9-4.2 for 64 beams.
 // * compact_plan, one workgroup: used pages counted, then holes and sources ranked by one pass of sums over the threads; a
@@ -30,6 +30,7 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kPlan = 1024;           // threads of the planning workgroups
 constexpr uint32_t kMaxSeqs = 4096;   // sequences that reserve_plan takes
 constexpr uint32_t kSlots = 2 * kMaxSeqs;
+constexpr uint32_t kListHere = 2048;  // free pages that reserve_plan lists in LDS
 constexpr uint32_t kLook = 8;         // refs a thread looks at a round
 constexpr uint64_t kForkSmall = 4096; // table entries that one workgroup forks alone (64 x 32: 6.7 us a pass, by rows 9.3)
 constexpr uint32_t kFew = 2;          // entries of a sequence that one thread goes through alone
@@ -137,7 +138,7 @@ __device__ __forceinline__ void load_refs(const uint32_t* refs, uint32_t p, uint
 }
 
 // Arrays that a call copies before it changes the copies: by the planning workgroup itself where they are short
-// (kCopyInPlan words; 64 sequences' reservation among 4096 pages 6.7 us a pass, 8.8 with a launch), else by copy_words.
+// (kCopyInPlan words; with a launch 64 sequences' reservation among 4096 pages takes 2.1 us more), else by copy_words.
 struct CopyWords {
     const uint32_t* from[3];
     uint32_t* to[3];
@@ -217,13 +218,12 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
 {
     __shared__ uint32_t s_key[kSlots], s_cnt[kSlots], s_last[kSlots];  // pages that are appended to and shared
     __shared__ uint32_t s_need[kMaxSeqs];  // a sequence's entries, then the sum before it; bit 31: it copies its last page
+    __shared__ uint32_t s_list[kListHere];  // the list's first entries
     __shared__ uint32_t s_wave[kPlan / 64];
     __shared__ uint32_t s_any, s_moves;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, cap = p.max_pages << p.shift, in_page = (1u << p.shift) - 1;
     if (tid == 0)
         s_any = s_moves = 0;
-    copy_share(p.copy, tid, kPlan);
-    __syncthreads();
 
     // The entries [first, last) that the new rows [c, end) of sequence b fall into.
     struct Window {
@@ -240,18 +240,38 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
         return w;
     };
     const auto entry = [&](uint32_t b, uint32_t j) { return p.table[(size_t)b * p.max_pages + j]; };
-    // The partly filled page that sequence b appends to and others hold (kNoPage: none).
-    const auto shared_page = [&](uint32_t b, const Window& w) __attribute__((always_inline)) {
-        if (w.end == w.c || !(w.c & in_page))
-            return kNoPage;
-        const uint32_t e = entry(b, w.first);
-        return e < p.pages && p.refs[e] > 1 ? e : kNoPage;
+    // Sequence b: its window, the first kFew entries of it, and the partly filled page that it appends to and others hold
+    // (kNoPage: none) with its holders.
+    struct Seq {
+        Window w;
+        uint32_t e[kFew], page, held;
     };
+    const auto look = [&](uint32_t b, const Window& w) __attribute__((always_inline)) {
+        Seq s{w, {}, kNoPage, 0};
+        #pragma unroll
+        for (uint32_t i = 0; i < kFew; ++i)
+            s.e[i] = w.first + i < w.last ? entry(b, w.first + i) : 0u;
+        if (w.end != w.c && (w.c & in_page) && s.e[0] < p.pages) {
+            s.held = p.refs[s.e[0]];
+            s.page = s.held > 1 ? s.e[0] : kNoPage;
+        }
+        return s;
+    };
+    // Most calls have a sequence a thread at most and few pages to look through: what those need is loaded once, all of it before
+    // the first use (64 sequences' step 4.8 us of kernel, 5.5 with a load in front of each use).
+    const Window mine_w = window(tid);
+    uint32_t refs0[kLook];
+    load_refs(p.refs, tid * kLook, p.pages, refs0);
+    copy_share(p.copy, tid, kPlan);
+    const Seq mine = look(tid, mine_w);
+    const auto seq = [&](uint32_t b) __attribute__((always_inline)) { return b == tid ? mine : look(b, window(b)); };
+    __syncthreads();
+
     const auto slot_of = [](uint32_t e) { return (e * 2654435761u) >> (32 - 13); };
     static_assert(kSlots == 1u << 13, "slot_of takes 13 bits");
 
     for (uint32_t b = tid; b < p.batch; b += kPlan)
-        if (shared_page(b, window(b)) != kNoPage)
+        if (seq(b).page != kNoPage)
             s_any = 1;
     __syncthreads();
     const bool any = s_any != 0;
@@ -262,7 +282,7 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
         }
         __syncthreads();
         for (uint32_t b = tid; b < p.batch; b += kPlan) {
-            const uint32_t e = shared_page(b, window(b));
+            const uint32_t e = seq(b).page;
             if (e == kNoPage)
                 continue;
             uint32_t i = slot_of(e);
@@ -278,26 +298,26 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
         __syncthreads();
     }
     // Whether sequence b copies its last page: unless all of its holders append to it and b is the last of them.
-    const auto copies = [&](uint32_t b, const Window& w) __attribute__((always_inline)) {
-        const uint32_t e = any ? shared_page(b, w) : kNoPage;
-        if (e == kNoPage)
+    const auto copies = [&](uint32_t b, const Seq& s) __attribute__((always_inline)) {
+        if (s.page == kNoPage)
             return false;
-        uint32_t i = slot_of(e);
-        while (s_key[i] != e)
+        uint32_t i = slot_of(s.page);
+        while (s_key[i] != s.page)
             i = (i + 1) % kSlots;
-        return p.refs[e] > s_cnt[i] || s_last[i] != b;
+        return s.held > s_cnt[i] || s_last[i] != b;
     };
 
     // A sequence's entries without a page, in the order of their rows: few by its thread, many by its wave.
     uint32_t carry = 0;
     for (uint32_t b0 = 0; b0 < p.batch; b0 += kPlan) {
         const uint32_t b = b0 + tid;
-        const Window w = window(b);
-        const bool copy = copies(b, w), few = w.last - w.first <= kFew;
+        const Seq s = seq(b);
+        const Window& w = s.w;
+        const bool copy = copies(b, s), few = w.last - w.first <= kFew;
         uint32_t need = copy ? 1u : 0u;
-        if (few)
-            for (uint32_t j = w.first; j < w.last; ++j)
-                need += entry(b, j) >= p.pages ? 1u : 0u;
+        #pragma unroll
+        for (uint32_t i = 0; i < kFew; ++i)
+            need += few && w.first + i < w.last && s.e[i] >= p.pages ? 1u : 0u;
         for (uint64_t m = __ballot(!few); m; m &= m - 1) {
             const uint32_t l = (uint32_t)__builtin_ctzll(m), bl = b - lane + l;
             const uint32_t first = (uint32_t)__builtin_amdgcn_readlane(w.first, l);
@@ -320,15 +340,20 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
     for (uint32_t p0 = 0; p0 < p.pages && found < want; p0 += kPlan * kLook) {
         uint32_t x[kLook], n = 0, total;
         const uint32_t at = p0 + tid * kLook;
-        load_refs(p.refs, at, p.pages, x);
+        if (p0 != 0)
+            load_refs(p.refs, at, p.pages, x);
         #pragma unroll
-        for (uint32_t i = 0; i < kLook; ++i)
+        for (uint32_t i = 0; i < kLook; ++i) {
+            x[i] = p0 == 0 ? refs0[i] : x[i];
             n += x[i] == 0 ? 1u : 0u;
+        }
         uint32_t to = found + scan_threads(n, s_wave, total);
         #pragma unroll
         for (uint32_t i = 0; i < kLook; ++i)
-            if (x[i] == 0 && to < want)
-                p.list[to++] = at + i;
+            if (x[i] == 0 && to < want) {
+                (to < kListHere ? s_list[to] : p.list[to]) = at + i;
+                ++to;
+            }
         found += total;
     }
     found = min(found, want);
@@ -336,16 +361,17 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
 
     for (uint32_t b0 = 0; b0 < p.batch; b0 += kPlan) {
         const uint32_t b = b0 + tid;
-        const Window w = window(b);
+        // (refs, and so what `look` says of shared pages, may have changed by now: the sequence copies if s_need says so)
+        const Seq s = seq(b);
+        const Window& w = s.w;
         const bool few = w.last - w.first <= kFew;
         const uint32_t prefix = b < p.batch ? s_need[b] & 0x7fffffffu : 0u;
         const bool copy = b < p.batch && s_need[b] >> 31;
         uint32_t fail = kNoPage;  // the first entry that gets none
-        // entry j of sequence x takes the idx-th page; cp: in place of its shared page of rows [0, part)
-        const auto give = [&](uint32_t x, uint32_t j, uint32_t idx, bool cp, uint32_t part) __attribute__((always_inline)) {
-            const uint32_t page = p.list[idx];
+        // entry j of sequence x, now old, takes the idx-th page; cp: in place of its shared page of rows [0, part)
+        const auto give = [&](uint32_t x, uint32_t j, uint32_t idx, uint32_t old, bool cp, uint32_t part) __attribute__((always_inline)) {
+            const uint32_t page = idx < kListHere ? s_list[idx] : p.list[idx];
             if (cp) {
-                const uint32_t old = entry(x, j);
                 atomicSub(&p.refs_out[old], 1u);
                 p.moves[atomicAdd(&s_moves, 1u)] = Move{old, page, part, 0u};
             }
@@ -354,12 +380,14 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
         };
         if (few) {
             uint32_t idx = prefix;
-            for (uint32_t j = w.first; j < w.last; ++j) {
-                const bool cp = copy && j == w.first;
-                if (!cp && entry(b, j) < p.pages)
+            #pragma unroll
+            for (uint32_t i = 0; i < kFew; ++i) {
+                const uint32_t j = w.first + i;
+                const bool cp = copy && i == 0;
+                if (j >= w.last || (!cp && s.e[i] < p.pages))
                     continue;
                 if (idx < found)
-                    give(b, j, idx, cp, w.c & in_page);
+                    give(b, j, idx, s.e[i], cp, w.c & in_page);
                 else
                     fail = min(fail, j);
                 ++idx;
@@ -375,12 +403,13 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
             for (uint32_t j0 = first; j0 < last; j0 += 64) {
                 const uint32_t j = j0 + lane;
                 const bool cp = cpl && j == first;
-                const bool needs = j < last && (cp || entry(bl, j) >= p.pages);
+                const uint32_t old = j < last ? entry(bl, j) : 0u;
+                const bool needs = j < last && (cp || old >= p.pages);
                 const uint64_t all = __ballot(needs);
-                const uint32_t mine = idx + (uint32_t)__popcll(all & ((1ull << lane) - 1));
-                if (needs && mine < found)
-                    give(bl, j, mine, cp, c & in_page);
-                const uint64_t lack = __ballot(needs && mine >= found);
+                const uint32_t rank = idx + (uint32_t)__popcll(all & ((1ull << lane) - 1));
+                if (needs && rank < found)
+                    give(bl, j, rank, old, cp, c & in_page);
+                const uint64_t lack = __ballot(needs && rank >= found);
                 if (lack && none == kNoPage)
                     none = j0 + (uint32_t)__builtin_ctzll(lack);
                 idx += (uint32_t)__popcll(all);
