@@ -327,8 +327,8 @@ int mako_cache_evict(const mako_evict_args* a, mako_dtype in, void* k, void* v, 
  * sequence's from max_new on. max_new bounds the new rows of a sequence and max_ctx the rows it holds with them
  * (max_ctx <= max_pages * page): cache rows from max_ctx on are not seen, and a loose bound costs time and workspace only. A
  * page that the table does not name reads as rows of zeros. What pages hold behind a sequence's last row, and pages that its
- * table does not name in it, have no part, whatever they hold; a v that is not finite among a sequence's own new rows may
- * make rows before it in its 64 rows (counted from the sequence's start) not finite.
+ * table does not name in it, have no part, whatever they hold, nor has a new row in the rows before it (infinities and NaN
+ * too; blocks of up to 256 rows that meet a v of their own that is not finite are computed a second time, row by row).
  * dim 64, 128 or 256. Precision as mako_attn_fwd: P rounded to the input type for P V, sums and lse of the f32
  * exponentials; rows that see fewer than 64 keys (heads of 256: fewer than 32) get bf16 probabilities to ~16 bits.
  * workspace: at least mako_attn_paged_workspace(a) bytes, 16-byte aligned; its contents do not matter, and calls that

@@ -22,6 +22,7 @@
 // * A piece of an item leaves normalised f32 rows and their log-sums at slot 2 range (+ 1 if the item starts in it): a range
 //   has at most one of each kind. The range with an item's last piece names its first one, and paged_merge joins them.
 //   Contexts that are too short for a second launch (max_ctx) take whole items and none.
+// * A piece of several rows ends with a look at the v that some of its rows do not see (hidden_not_finite).
 #include <algorithm>
 
 #include "attn_paged_asm.inc"
@@ -236,6 +237,37 @@ constexpr uint32_t lds_bytes()
     return kNBuf * (D == 64 ? 9 + 8 : 17 + 16) * 1024;  // (heads of 256: four tiles of 32 keys; two of 64 take less)
 }
 
+// Whether some v that a piece's tiles hold and some of its rows do not see (positions past the first row's) is not finite. All
+// threads of the workgroup; lds is between two streams.
+template <class T, int D>
+__device__ __forceinline__ bool hidden_not_finite(ParamsAt at_p, unsigned char* lds, const PagedPiece& at)
+{
+    const auto& p = *params_here(at_p);
+    constexpr uint32_t kExp = __is_same(T, __bf16) ? 0x7f807f80u : 0x7c007c00u;
+    const uint32_t lo = max(at.p0 + 1, 64 * at.ta), hi = min(at.keys, 64 * at.tb), n = hi > lo ? (hi - lo) * (D / 8) : 0u;
+    const uint32_t* row = p.table + (size_t)at.b * p.max_pages;
+    uint32_t finite = 0x80008000u;  // the upper bits of (the exponent's complement + 0x7fff) are 0 where that is 0
+    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+        const uint32_t j = lo + i / (D / 8), page = row[j >> p.shift];
+        if (page >= p.pages)
+            continue;
+        const size_t base = ((size_t)page * p.kv_heads + at.kvh) << p.shift;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(static_cast<const T*>(p.v) +
+                                                        (base + (j & ((1u << p.shift) - 1))) * D + i % (D / 8) * 8);
+        #pragma unroll
+        for (int u = 0; u < 4; ++u)
+            finite &= (~v[u] & kExp) + 0x7fff7fffu;
+    }
+    uint32_t* flags = reinterpret_cast<uint32_t*>(lds);
+    const bool bad = __ballot((finite & 0x80008000u) != 0x80008000u) != 0;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the piece's stores are done, where another wave is to write there again
+    flags[threadIdx.x >> 6] = bad ? 1 : 0;
+    __syncthreads();
+    const uint32_t any = flags[0] | flags[1] | flags[2] | flags[3];
+    __syncthreads();
+    return uniform(any) != 0;
+}
+
 // FEW: every piece takes the stream of 32 rows a wave; else pieces of few rows do (heads of 256: none).
 template <class T, class TO, int D, bool FEW>
 __global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams q)
@@ -269,16 +301,32 @@ __global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams q)
             if (at.first != kNone)
                 done = u32x4{at.first, at.row0, at.rows, at.kvh};
         }
-        const bool few = FEW || (D != 256 && at.rows <= p.few);
-        if (at.part || __is_same(TO, float)) {
-            if (few)
-                run_piece<T, float, D, D != 256 || FEW>(at_p, lds, x);
-            else
-                run_piece<T, float, D, FEW>(at_p, lds, x);
-        } else if (few) {
-            run_piece<T, TO, D, D != 256 || FEW>(at_p, lds, x);
-        } else {
-            run_piece<T, TO, D, FEW>(at_p, lds, x);
+        // A row's probability of 0 for a key that it does not see, times a v that is not finite, is NaN: where there is such a v
+        // the piece is done again row by row, so that no row meets keys past its own.
+        for (uint32_t n = at.rows, r = 0;;) {
+            const uint32_t few_rows = params_here(at_p)->few;
+            const bool few = FEW || (D != 256 && n <= few_rows);
+            if (at.part || __is_same(TO, float)) {
+                if (few)
+                    run_piece<T, float, D, D != 256 || FEW>(at_p, lds, x);
+                else
+                    run_piece<T, float, D, FEW>(at_p, lds, x);
+            } else if (few) {
+                run_piece<T, TO, D, D != 256 || FEW>(at_p, lds, x);
+            } else {
+                run_piece<T, TO, D, FEW>(at_p, lds, x);
+            }
+            r += n;
+            if (r == at.rows) {
+                if (n == 1 || !hidden_not_finite<T, D>(at_p, lds, at))
+                    break;
+                n = 1, r = 0;
+            } else {
+                x.q = static_cast<const T*>(x.q) + D;
+                x.o = static_cast<char*>(x.o) + x.o_row;
+                x.l = x.l ? x.l + 1 : x.l;
+            }
+            x.rows = 1, x.p0 = at.p0 + r, x.keys = min(x.p0 + 1, at.seen), x.tb = min(at.tb, (x.keys + 63) / 64);
         }
     });
     const auto& p = *params_here(at_p);

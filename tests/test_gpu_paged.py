@@ -211,6 +211,40 @@ def test_a_later_rows_k_is_not_seen(dim, n, value):
     assert torch.equal(o, want) and torch.equal(lse, want_l)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (8, 2, 128), (8, 1, 128), (4, 2, 256), (8, 1, 256)])
+@pytest.mark.parametrize("n", [2, 16, 33, 100])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype,out", [("bf16", None), ("f16", "f32")])
+def test_a_later_rows_v_is_not_seen(heads, kv, dim, n, value, dtype, out):
+    """A v that is not finite in one of a sequence's new rows reaches the rows from there on, in its head dim, and none before."""
+    ctx, dt, rows = [5000, 70], DT[dtype], 2 * n
+    odt = torch.float32 if out else dt
+    g = gen(19)
+    pool = Pool(g, ctx, [n, n], kv, dim, 64, dt, fill=math.nan)
+    first = n // 2  # the first row that sees it
+    for b in range(2):
+        j = ctx[b] + first
+        pool.v[pool.table[b, j // 64].item(), kv - 1, j % 64, 5] = value
+    a = M.paged_args(batch=2, rows=rows, heads=heads, kv_heads=kv, dim=dim, pages=pool.pages, page=64, max_pages=pool.max_pages,
+                     max_new=n, max_ctx=5000 + n)
+    q = torch.randn((heads, rows, dim), generator=g, device="cuda").to(dt)
+    o, lse = torch.zeros((rows, heads * dim), dtype=odt, device="cuda"), torch.zeros((heads, rows), device="cuda")
+    M.attn_paged(a, q, pool.k, pool.v, pool.table, ints(ctx), o, space(M.attn_paged_workspace(a)), starts=ints([0, n, rows]),
+                 lse=lse)
+    torch.cuda.synchronize()
+    pool.v.nan_to_num_(nan=0.0, posinf=0.0)
+    res = R.attention(q, pool.k.nan_to_num(0.0), pool.v, pool.table.tolist(), ctx, [n, n], [0, n], scale=a.scale,
+                      max_ctx=a.max_ctx, max_new=n, out_dtype=odt)
+    mine = torch.arange(heads, device="cuda") * kv // heads == kv - 1
+    for b, s0, m, want, want_l, tol, ltol in res:
+        got = o[s0:s0 + m].double().view(m, heads, dim)
+        off = ~((got - want).abs() <= tol)
+        assert not off[:first].any() and not off[:, :, :5].any() and not off[:, :, 6:].any() and not off[:, ~mine].any()
+        hit = got[first:, mine, 5]
+        assert (hit.isnan() | hit.isinf()).all()
+        assert ((lse[:, s0:s0 + m].t().double() - want_l).abs() <= ltol).all()
+
+
 def test_scale_and_no_lse():
     run_attention("bf16", 4, 2, 128, 64, [200, 0], [33, 1], scale=0.5, want_lse=False, seed=12)
 
