@@ -47,7 +47,7 @@ class Pool:
 
 
 def run_attention(dtype, heads, kv, dim, page, ctx, new, *, out=None, seed=0, decode=False, max_new=None, max_ctx=None,
-                  behind=0, q_pad=0, width=0, scale=None, pool=None, want_lse=True, edit=None, ws_fill=0xA5, repeat=1):
+                  behind=0, q_pad=0, width=0, scale=None, pool=None, want_lse=True, edit=None, ws_fill=0xA5, repeat=1, q_fill=None):
     g = gen(seed)
     dt = DT[dtype]
     odt = {None: dt, "f32": torch.float32}[out]
@@ -58,6 +58,8 @@ def run_attention(dtype, heads, kv, dim, page, ctx, new, *, out=None, seed=0, de
     starts = [sum(new[:b]) for b in range(B + 1)]
     rows = starts[-1] + behind
     q = torch.randn((heads, rows + q_pad, dim), generator=g, device="cuda").to(dt)
+    if q_fill is not None:
+        q[:, starts[-1]:] = q_fill
     w = heads * dim + width
     a = M.paged_args(batch=B, rows=rows, heads=heads, kv_heads=kv, dim=dim, pages=pool.pages, page=page,
                      max_pages=pool.max_pages, max_new=max(new) if max_new is None else max_new,
@@ -243,6 +245,14 @@ def test_a_later_rows_v_is_not_seen(heads, kv, dim, n, value, dtype, out):
         hit = got[first:, mine, 5]
         assert (hit.isnan() | hit.isinf()).all()
         assert ((lse[:, s0:s0 + m].t().double() - want_l).abs() <= ltol).all()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (8, 2, 128), (8, 1, 128), (4, 2, 256), (8, 1, 256)])
+@pytest.mark.parametrize("fill", [math.nan, math.inf])
+def test_queries_of_no_sequence(heads, kv, dim, fill):
+    """What q holds behind the last sequence's rows, and in its padding, has no part."""
+    for new in ([1, 1], [3, 17], [40, 70]):
+        run_attention("bf16", heads, kv, dim, 64, [700, 90], new, behind=3, q_pad=70, q_fill=fill, seed=20)
 
 
 def test_scale_and_no_lse():
