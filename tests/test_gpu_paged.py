@@ -1,6 +1,7 @@
 """The operators of a cache kept in pages on the GPU, against plain forms in 64 bits (tests/pages_ref.py): attention of one
 token or a chunk of each sequence over its pages, the write of rows, reservation, fork and compaction."""
 import math
+import random
 
 import pytest
 import torch
@@ -253,6 +254,26 @@ def test_queries_of_no_sequence(heads, kv, dim, fill):
     """What q holds behind the last sequence's rows, and in its padding, has no part."""
     for new in ([1, 1], [3, 17], [40, 70]):
         run_attention("bf16", heads, kv, dim, 64, [700, 90], new, behind=3, q_pad=70, q_fill=fill, seed=20)
+
+
+@pytest.mark.parametrize("seed", range(32))
+def test_calls_of_any_kind(seed):
+    """Batches, groups, lengths, pages, types, paddings and bounds drawn together."""
+    r = random.Random(seed)
+    dim, kv, group = r.choice([64, 128, 256]), r.choice([1, 2, 3, 8]), r.choice([1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24])
+    kv = kv if kv * group <= 48 else 1
+    batch = r.choice([1, 2, 3, 5, 9, 40, 70])
+    high, most = (6000, 700) if batch <= 5 else (400, 40)
+    ctx = [r.choice([0, 1, 63, 64, r.randint(0, 200), r.randint(0, high)]) for _ in range(batch)]
+    kind = r.choice(["step", "few", "chunk", "mixed"])
+    new = [1 if kind == "step" or (kind == "mixed" and r.random() < 0.7) else r.randint(0, 20 if kind == "few" else most)
+           for _ in range(batch)]
+    new[0] = max(new[0], 1)
+    page, dtype, step = r.choice([64, 128, 512]), r.choice(["f16", "bf16"]), kind == "step"
+    pool = Pool(gen(seed), ctx, new, kv, dim, page, DT[dtype], extra=r.choice([0, 512 // page]))
+    run_attention(dtype, kv * group, kv, dim, page, ctx, new, out=r.choice([None, "f32"]), behind=0 if step else r.choice([0, 3]),
+                  q_pad=r.choice([0, 7, 64]), width=r.choice([0, 8]), decode=step, seed=seed, pool=pool,
+                  max_new=r.choice([None, sum(new)]), max_ctx=r.choice([None, pool.max_pages * page]))
 
 
 def test_scale_and_no_lse():
