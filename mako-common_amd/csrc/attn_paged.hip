@@ -82,6 +82,7 @@ struct Piece {
     uint32_t seen;                    // keys of the sequence: no row sees more
     uint32_t o_row, o_head;           // bytes between rows of o and between the wave's heads
     uint32_t l_head;                  // floats between the wave's heads in l
+    uint32_t items, first_pages;      // items: lane i of first_pages has the table row's entry i
 };
 
 // FEW: the stream of 32 rows a wave and streaming loads, at heads of 256 by tiles of 32 keys; else 64 rows a wave, at heads of
@@ -143,8 +144,15 @@ __device__ __forceinline__ void run_piece(ParamsAt at_p, unsigned char* lds, con
     const uint32_t pshift = p.shift - (KT == 64 ? 6 : 5);
     const uint32_t* row = reinterpret_cast<const uint32_t*>(x.table);
     const uint32_t t0 = uniform(ks / KT), tlast = uniform(t0 + nt - 1), npages = uniform(p.pages);
-    const auto page_of = [&](uint32_t t) { return uniform(row[min(t, tlast) >> pshift]); };
-    const uint32_t pg0 = page_of(t0), pg1 = page_of(t0 + 1), pg2 = page_of(t0 + 2), pg3 = page_of(t0 + 3);
+    uint32_t pg0, pg1, pg2, pg3;
+    const auto entry_of = [&](uint32_t t) { return uniform(min(t0 + t, tlast) >> pshift); };
+    if (x.items) {
+        const auto page_of = [&](uint32_t t) { return (uint32_t)__builtin_amdgcn_readlane(x.first_pages, entry_of(t)); };
+        pg0 = page_of(0), pg1 = page_of(1), pg2 = page_of(2), pg3 = page_of(3);
+    } else {
+        const auto page_of = [&](uint32_t t) { return uniform(row[entry_of(t)]); };
+        pg0 = page_of(0), pg1 = page_of(1), pg2 = page_of(2), pg3 = page_of(3);
+    }
     const uint64_t ent = uniform64(x.table);
     const uint32_t pstride = uniform(p.page_bytes), pmask = uniform((1u << pshift) - 1), s_pshift = uniform(pshift);
 
@@ -277,6 +285,11 @@ __global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams q)
     // blockIdx.x is the XCD: ranges side by side on one, a range's column blocks too (kItems: the kv head)
     const uint32_t range = q.how == kItems ? blockIdx.z : blockIdx.x * gridDim.z + blockIdx.z, cb = blockIdx.y;
 
+    // kItems: the tiles begin with the first page, whose number needs no length, so it is loaded beside the lengths (one token
+    // over 391 rows 11.1 -> 10.7 us).
+    uint32_t first_pages = 0;
+    if (q.how == kItems)
+        first_pages = q.table[(size_t)blockIdx.z * q.max_pages + min(lane, q.max_pages - 1)];
     uint32_t here[2] = {0, 0};
     u32x4 done = u32x4{kNone, 0, 0, 0};
     const ParamsAt at_p = (ParamsAt)__builtin_amdgcn_kernarg_segment_ptr();
@@ -289,6 +302,7 @@ __global__ __launch_bounds__(256, 1) void paged_rows(const PagedParams q)
         x.v = static_cast<const T*>(p.v) + ((size_t)at.kvh << p.shift) * D;
         x.table = reinterpret_cast<uint64_t>(p.table + (size_t)at.b * p.max_pages);
         x.ta = at.ta, x.tb = at.tb, x.rows = at.rows, x.p0 = at.p0, x.keys = at.keys, x.seen = at.seen;
+        x.items = p.how == kItems, x.first_pages = first_pages;
         x.o = static_cast<TO*>(p.o) + (size_t)at.row0 * p.width + (size_t)h * D;
         x.o_row = p.width * sizeof(TO), x.o_head = D * sizeof(TO), x.l_head = p.rows;
         x.l = p.lse ? p.lse + (size_t)h * p.rows + at.row0 : nullptr;
