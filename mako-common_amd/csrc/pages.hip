@@ -436,6 +436,8 @@ struct ForkParams {
 // New sequence i, by `threads` threads.
 __device__ __forceinline__ void fork_row(const ForkParams& p, uint32_t i, uint32_t thread, uint32_t threads)
 {
+    const uint32_t* old = p.table + (size_t)i * p.max_pages;
+    const uint32_t was0 = thread < p.max_pages ? old[thread] : kNoPage;  // (beside the parent's load)
     const uint32_t cap = p.max_pages << p.shift;
     const uint32_t src = p.parent ? p.parent[i] : i;
     uint32_t c = 0;
@@ -445,10 +447,9 @@ __device__ __forceinline__ void fork_row(const ForkParams& p, uint32_t i, uint32
     if (thread == 0)
         p.ctx_out[i] = c;
     const uint32_t* from = p.table + (size_t)(src < p.batch ? src : i) * p.max_pages;
-    const uint32_t* old = p.table + (size_t)i * p.max_pages;
     for (uint32_t j = thread; j < p.max_pages; j += threads) {
-        const uint32_t was = old[j];
-        uint32_t e = j < kept ? from[j] : kNoPage;
+        const uint32_t was = j == thread ? was0 : old[j];
+        uint32_t e = j < kept ? src == i ? was : from[j] : kNoPage;
         if (e >= p.pages)
             e = kNoPage;
         p.table_out[(size_t)i * p.max_pages + j] = e;
