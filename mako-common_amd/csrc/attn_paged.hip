@@ -436,17 +436,18 @@ struct Plan {
 
 constexpr uint32_t kFewMerged = 16;  // (row, head) pairs a range up to which paged_merge parts an item's pieces
 
-// Whole items and no second launch up to this many tiles a sequence: 11, where a merge joins more rows 17, and more the
-// nearer the items come to one a workgroup. (With a workgroup an item of sequences that are one item each: 0.4 to 0.6 us less a
-// call than by looking for its range; more items than workgroups are better spread by ranges.) us split / direct, single tokens, 32 heads of 128 over 8: 8 items of 8 tiles 15.6 /
-// 12.7, of 12 16.2 / 15.9, of 16 16.3 / 18.9; 64 of 12 15.9 / 16.4; 128 of 16 21.6 / 20.4, of 26 27.2 / 28.8; 256 of 33 48 / 46.
-// 16 heads of 256 over 2: 8 items of 8 17.8 / 16.4, of 12 18.0 / 20.5; 128 of 33 63 / 62. 256 rows of 32 heads: 32 items of 16
-// 28.8 / 27.7, of 24 31.5 / 36.8; 128 of 24 41 / 37. A workgroup takes its item's tiles one after the other whatever the
-// others' lengths, so the limit also bounds what one long sequence among short ones costs.
+// Whole items and no second launch up to this many tiles a sequence: 13, where a merge joins more rows 20, and more the
+// nearer the items come to one a workgroup. us split / whole, sequences of one length. Single tokens, 32 heads of 128 over 8: 8
+// items of 12 tiles 16.3 / 14.9, of 16 16.4 / 17.9; 64 of 12 15.9 / 15.6, of 16 17.7 / 18.7; 128 of 20 25.6 / 23.7, of 33 35.6 /
+// 34.5; 512 of 33 93 / 91. 16 heads of 256 over 2: 8 of 12 21.4 / 20.1, of 16 21.8 / 24.3; 64 of 16 28.2 / 26.4. 64 rows of 32
+// heads: 8 items of 16 32.2 / 28.5, of 24 36.0 / 37.7; 256 rows: 128 of 24 44 / 40. A workgroup takes its item's tiles one after
+// the other whatever the others' lengths, so the limit also bounds what one long sequence among short ones costs.
+// (A workgroup an item, where sequences are one item each: 0.4 to 0.6 us less a call than looking for its range; more items
+// than workgroups are better spread by ranges.)
 uint32_t direct_tiles(uint64_t items, uint32_t ranges, bool many)
 {
     const uint64_t x = std::min<uint64_t>(items * 30 / ranges, 30);
-    return (many ? 17 : 11) + (x > 7 ? (uint32_t)x - 7 : 0);
+    return (many ? 20 : 13) + (x > 7 ? (uint32_t)x - 7 : 0);
 }
 
 uint32_t item_heads(const mako_paged_args* a)
