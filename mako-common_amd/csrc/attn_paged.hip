@@ -258,7 +258,9 @@ __device__ __forceinline__ bool hidden_not_finite(ParamsAt at_p, unsigned char* 
 {
     const auto& p = *params_here(at_p);
     constexpr uint32_t kExp = __is_same(T, __bf16) ? 0x7f807f80u : 0x7c007c00u;
-    const uint32_t lo = max(at.p0 + 1, 64 * at.ta), hi = min(at.keys, 64 * at.tb), n = hi > lo ? (hi - lo) * (D / 8) : 0u;
+    const uint32_t lo = max(at.p0 + 1, 64 * at.ta), hi = min(at.keys, 64 * at.tb), n = (hi - lo) * (D / 8);
+    if (hi <= lo)
+        return false;
     const uint32_t* row = p.table + (size_t)at.b * p.max_pages;
     uint32_t finite = 0x80008000u;  // the upper bits of (the exponent's complement + 0x7fff) are 0 where that is 0
     for (uint32_t i = threadIdx.x; i < n; i += 256) {
