@@ -376,15 +376,16 @@ int mako_pages_write(const mako_pages_args* a, const void* kd, const void* vd, c
  * Pages for the new rows: each entry of sequence b's table row that rows ctx_len[b] .. ctx_len[b] + n - 1 fall into (n:
  * starts[b + 1] - starts[b]) gets a free page where it has none, in the order of sequences and rows, the free pages of the
  * lowest numbers first. A last page that is partly filled and that others hold too is not written to: the sequence gets a
- * page of its own there with its rows copied, in all layers (of sequences that append to one page which nobody else
- * holds, the last one keeps it, whether the others get theirs or not). refs_out: 1 for the pages given, one holder fewer
- * for the pages left. When the free pages run out, the later entries get none; ctx_out[b] is the number of rows that have
- * room (ctx_len[b] + n, or fewer): rows from it on are not to be written (mako_pages_write's end). A sequence's entries
- * behind its last row should name no page, as reserve and fork leave them: rows are taken back by mako_pages_fork (keep);
- * where ctx_len alone is lowered, whole pages that are named already are written to whoever else holds them. k and v [layers][pages][kv_heads][page][dim], or both NULL where no page
- * can be shared or the caller copies. table_out may be table, refs_out refs and ctx_out ctx_len (where mako_pages_write and
- * mako_attn_paged still get the rows before); with other arrays the call can be made again. At most 4096 sequences.
- * workspace: at least mako_pages_reserve_workspace(a) bytes, 16-byte aligned.
+ * page of its own there with its rows copied, in all layers (of sequences that append to one page which nobody else holds,
+ * the last one keeps it, unless one of the others gets no page for its copy and has rows where the last one's new rows would
+ * go: then the last one gets no room either). refs_out: 1 for the pages given, one holder fewer for the pages left. When the
+ * free pages run out, the later entries get none; ctx_out[b] is the number of rows that have room (ctx_len[b] + n, or fewer):
+ * rows from it on are not to be written (mako_pages_write's end). A sequence's entries behind its last row should name no
+ * page, as reserve and fork leave them: rows are taken back by mako_pages_fork (keep); where ctx_len alone is lowered, whole
+ * pages that are named already are written to whoever else holds them. k and v [layers][pages][kv_heads][page][dim], or both
+ * NULL where no page can be shared or the caller copies. table_out may be table, refs_out refs and ctx_out ctx_len (where
+ * mako_pages_write and mako_attn_paged still get the rows before); with other arrays the call can be made again. At most
+ * 4096 sequences. workspace: at least mako_pages_reserve_workspace(a) bytes, 16-byte aligned.
  */
 size_t mako_pages_reserve_workspace(const mako_pages_args* a);
 int mako_pages_reserve(const mako_pages_args* a, const uint32_t* table, const uint32_t* refs, const uint32_t* starts,

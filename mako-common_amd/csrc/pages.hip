@@ -217,7 +217,9 @@ struct ReserveParams {
 __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
 {
     __shared__ uint32_t s_key[kSlots], s_cnt[kSlots], s_last[kSlots];  // pages that are appended to and shared
-    __shared__ uint32_t s_need[kMaxSeqs];  // a sequence's entries, then the sum before it; bit 31: it copies its last page
+    // a sequence's entries, then the sum before it; kCopies: it copies its last page; kKeeps: it keeps one that others copy
+    __shared__ uint32_t s_need[kMaxSeqs];
+    constexpr uint32_t kCopies = 1u << 31, kKeeps = 1u << 30;
     __shared__ uint32_t s_list[kListHere];  // the list's first entries
     __shared__ uint32_t s_wave[kPlan / 64];
     __shared__ uint32_t s_any, s_moves;
@@ -297,14 +299,19 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
         }
         __syncthreads();
     }
-    // Whether sequence b copies its last page: unless all of its holders append to it and b is the last of them.
-    const auto copies = [&](uint32_t b, const Seq& s) __attribute__((always_inline)) {
-        if (s.page == kNoPage)
-            return false;
-        uint32_t i = slot_of(s.page);
-        while (s_key[i] != s.page)
+    const auto slot_with = [&](uint32_t e) __attribute__((always_inline)) {
+        uint32_t i = slot_of(e);
+        while (s_key[i] != e && s_key[i] != kNoPage)  // (e is there; were it not, a slot is free)
             i = (i + 1) % kSlots;
-        return s.held > s_cnt[i] || s_last[i] != b;
+        return i;
+    };
+    // What sequence b does with a last page that is shared: it copies it, unless all of its holders append to it and b is the
+    // last of them, who keeps it.
+    const auto shared = [&](uint32_t b, const Seq& s) __attribute__((always_inline)) {
+        if (s.page == kNoPage)
+            return 0u;
+        const uint32_t i = slot_with(s.page);
+        return s.held > s_cnt[i] || s_last[i] != b ? kCopies : kKeeps;
     };
 
     // A sequence's entries without a page, in the order of their rows: few by its thread, many by its wave.
@@ -313,8 +320,9 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
         const uint32_t b = b0 + tid;
         const Seq s = seq(b);
         const Window& w = s.w;
-        const bool copy = copies(b, s), few = w.last - w.first <= kFew;
-        uint32_t need = copy ? 1u : 0u;
+        const uint32_t how = shared(b, s);
+        const bool few = w.last - w.first <= kFew;
+        uint32_t need = how == kCopies ? 1u : 0u;
         #pragma unroll
         for (uint32_t i = 0; i < kFew; ++i)
             need += few && w.first + i < w.last && s.e[i] >= p.pages ? 1u : 0u;
@@ -330,7 +338,7 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
         uint32_t total;
         const uint32_t before = scan_threads(need, s_wave, total);
         if (b < p.batch)
-            s_need[b] = (carry + before) | (copy ? 1u << 31 : 0u);
+            s_need[b] = ((carry + before) & (kKeeps - 1)) | how;
         carry += total;
     }
     const uint32_t want = min(carry, p.list_max);
@@ -357,7 +365,13 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
         found += total;
     }
     found = min(found, want);
-    __syncthreads();  // the list, and every read of refs, before their writes
+    // Where the free pages run out, a sequence may stay on a shared page that another one, whose new rows would go where it has
+    // rows of its own, was to keep: s_cnt becomes the rows of those whose copy of a page fails.
+    const bool runs_out = any && found < carry;
+    if (runs_out)
+        for (uint32_t i = tid; i < kSlots; i += kPlan)
+            s_cnt[i] = 0;
+    __syncthreads();  // the list, s_cnt, and every read of refs, before their writes
 
     for (uint32_t b0 = 0; b0 < p.batch; b0 += kPlan) {
         const uint32_t b = b0 + tid;
@@ -365,9 +379,16 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
         const Seq s = seq(b);
         const Window& w = s.w;
         const bool few = w.last - w.first <= kFew;
-        const uint32_t prefix = b < p.batch ? s_need[b] & 0x7fffffffu : 0u;
-        const bool copy = b < p.batch && s_need[b] >> 31;
+        const uint32_t need = b < p.batch ? s_need[b] : 0u, prefix = need & (kKeeps - 1);
+        const bool copy = need & kCopies;
         uint32_t fail = kNoPage;  // the first entry that gets none
+        if (runs_out) {  // (those that copy a page come before the one that keeps it: in this round of sequences, or an earlier one)
+            if (copy && prefix >= found)
+                atomicMax(&s_cnt[slot_with(s.e[0])], w.c & in_page);
+            __syncthreads();
+            if ((need & kKeeps) && s_cnt[slot_with(s.e[0])] > (w.c & in_page))
+                fail = w.first;
+        }
         // entry j of sequence x, now old, takes the idx-th page; cp: in place of its shared page of rows [0, part)
         const auto give = [&](uint32_t x, uint32_t j, uint32_t idx, uint32_t old, bool cp, uint32_t part) __attribute__((always_inline)) {
             const uint32_t page = idx < kListHere ? s_list[idx] : p.list[idx];
@@ -414,7 +435,7 @@ __global__ __launch_bounds__(kPlan) void reserve_plan(const ReserveParams p)
                     none = j0 + (uint32_t)__builtin_ctzll(lack);
                 idx += (uint32_t)__popcll(all);
             }
-            fail = lane == l ? none : fail;
+            fail = lane == l ? min(fail, none) : fail;
         }
         if (b < p.batch)
             p.ctx_out[b] = fail == kNoPage ? w.end : max(w.c, fail << p.shift);
