@@ -143,7 +143,8 @@ __device__ __forceinline__ void run_piece(ParamsAt at_p, unsigned char* lds, con
     const u32x4 lrs = rsrc_of(x.l, x.l ? (hs * x.l_head + x.rows) * 4 : 0);
     const uint32_t has_lse = scalar(x.l ? 1u : 0u);
     const float c = __builtin_bit_cast(float, uniform(__builtin_bit_cast(uint32_t, p.scale_log2)));
-    const uint32_t s_nt = uniform(nt), s_ntw = uniform(ntw), s_lmin = uniform(lmin), kn = uniform(n_keys * 2 * D);
+    const uint32_t s_nt = uniform(nt), s_ntw = uniform(ntw), s_lmin = uniform(lmin);
+    const uint32_t kn = uniform(n_keys * 2 * D);  // (mod 2^32: the streams take the last tile's bytes from it)
     const uint64_t kb = reinterpret_cast<uint64_t>(x.k), vb = reinterpret_cast<uint64_t>(x.v);
     const uint32_t kb0 = uniform((uint32_t)kb), kb1 = uniform((uint32_t)(kb >> 32) & 0xffffu);
     const uint32_t vb0 = uniform((uint32_t)vb), vb1 = uniform((uint32_t)(vb >> 32) & 0xffffu);

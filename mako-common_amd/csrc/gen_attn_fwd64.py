@@ -166,7 +166,7 @@ MAPV = "v184"           # the output row map[q0 + lane] (-1: dropped)
 # tile's number in the sequence and %[tlast] the last one's (no entry past its page is read).
 PAGED = False
 SPG = "s65"             # page of the tile the next staging loads
-SREM = "s58"           # bytes of K (of V) from that tile to the end of the keys
+SREM = "s58"           # bytes of K (of V) of the last tile, 0 once that is staged
 STN = "s59"            # that tile's number in the sequence
 # Its form for few rows (body(..., rows=32)): a wave owns 32 rows, one row block, so a tile is half the products and half the
 # softmax against the same staging; tiles come by streaming loads, as few workgroups read them again.
@@ -273,14 +273,21 @@ def dma_groups():
     return groups, ops
 
 
+def last_tile_bytes(rem):
+    """Paged: rem = the bytes of the last tile's keys. %[kn] is the bytes of all the piece's, mod 2^32: a piece may have more, so
+    nothing is counted down from it (a tile's bytes divide 2^32)."""
+    return [f"s_sub_u32 {rem}, %[kn], 1", f"s_and_b32 {rem}, {rem}, {2 * D * KT - 1:#x}", f"s_add_u32 {rem}, {rem}, 1"]
+
+
 def page_source(page, rem, tile, t, lo, hi):
-    """Paged: K's descriptor at the tile `tile` of page `page`, `rem` bytes long (none where there is no page); (lo, hi) keep
-    the tile's offset in the pool."""
+    """Paged: K's descriptor at the tile `tile` of page `page`: a tile's bytes, `rem` from the last tile on (none where there
+    is no page); (lo, hi) keep the tile's offset in the pool."""
     return [f"s_and_b32 {t}, {tile}, %[pmask]", f"s_lshl_b32 {t}, {t}, {(2 * D * KT).bit_length() - 1}",
             f"s_mul_i32 {lo}, {page}, %[pstride]", f"s_mul_hi_u32 {hi}, {page}, %[pstride]",
             f"s_add_u32 {lo}, {lo}, {t}", f"s_addc_u32 {hi}, {hi}, 0",
             f"s_add_u32 {KRS[0]}, %[kb0], {lo}", f"s_addc_u32 {KRS[1]}, %[kb1], {hi}",
-            f"s_cmp_lt_u32 {page}, %[npages]", f"s_cselect_b32 {KRS[2]}, {rem}, 0"]
+            f"s_cmp_lt_u32 {tile}, %[tlast]", f"s_cselect_b32 {KRS[2]}, {2 * D * KT:#x}, {rem}",
+            f"s_cmp_lt_u32 {page}, %[npages]", f"s_cselect_b32 {KRS[2]}, {KRS[2]}, 0"]
 
 
 def value_source(lo, hi):
@@ -289,7 +296,7 @@ def value_source(lo, hi):
 
 
 def page_advance(rem, tile):
-    return [f"s_sub_u32 {rem}, {rem}, {2 * D * KT:#x}", f"s_cselect_b32 {rem}, 0, {rem}", f"s_add_u32 {tile}, {tile}, 1"]
+    return [f"s_cmp_lt_u32 {tile}, %[tlast]", f"s_cselect_b32 {rem}, {rem}, 0", f"s_add_u32 {tile}, {tile}, 1"]
 
 
 def page_load(page, tile, t):
@@ -818,7 +825,8 @@ def body_of(in_dtype, out_dtype):
             e(f"s_mov_b32 {r[2]}, %[{pre}n]")
         e(f"s_mov_b32 {r[3]}, 0x20000")
     if PAGED:
-        e(f"s_mov_b32 {SREM}, %[kn]")
+        for op in last_tile_bytes(SREM):
+            e(op)
         e(f"s_mov_b32 {STN}, %[t0]")
         e(f"s_mov_b32 {SPG}, %[pg0]")
     e(f"s_mov_b32 {SBW}, 0")

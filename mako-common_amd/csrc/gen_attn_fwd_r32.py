@@ -78,7 +78,7 @@ CLOBBER_S_PAGED = (58, 100)
 # and V(j + 1) takes the offset that K(j + 1) was loaded from.
 PAGED = False
 SPG = "s86"        # page of the K tile the next staging loads
-SREM = "s96"       # bytes of K from that tile to the end of the keys
+SREM = "s96"       # bytes of K of the last tile, 0 once that is staged
 STN = "s97"        # that tile's number in the sequence
 SLO, SHI = "s58", "s59"   # offset in the pool of the K tile staged last
 
@@ -480,7 +480,8 @@ def body_of(in_dtype, out_dtype):
             e(f"s_mov_b32 {r[2]}, %[{pre}n]")
         e(f"s_mov_b32 {r[3]}, 0x20000")
     if PAGED:
-        e(f"s_mov_b32 {SREM}, %[kn]")
+        for op in G.last_tile_bytes(SREM):
+            e(op)
         e(f"s_mov_b32 {STN}, %[t0]")
         e(f"s_mov_b32 {SPG}, %[pg0]")
     for r, v in ((SKRT, K_TILE), (SVRT, V_TILE), (SKT, K_TILE), (SVT, V_TILE)):
