@@ -326,7 +326,9 @@ int mako_cache_evict(const mako_evict_args* a, mako_dtype in, void* k, void* v, 
  * by new row, lse [heads][rows] (may be NULL); rows of o and lse that are no sequence's are left as they were, and so are a
  * sequence's from max_new on. max_new bounds the new rows of a sequence and max_ctx the rows it holds with them
  * (max_ctx <= max_pages * page): cache rows from max_ctx on are not seen, and a loose bound costs time and workspace only. A
- * page that the table does not name reads as rows of zeros. What pages hold behind a sequence's last row, and pages that its
+ * page that the table does not name reads as rows of zeros. A new row that got no room (at or past mako_pages_reserve's
+ * ctx_out, so not written) gets a result of no meaning, which is to be dropped: its position may lie in a page that it shares,
+ * with the rows of another holder there, or of nobody. What pages hold behind a sequence's last row, and pages that its
  * table does not name in it, have no part, whatever they hold, nor has a new row in the rows before it (infinities and NaN
  * too; blocks of up to 256 rows that meet a v of their own that is not finite are computed a second time, row by row).
  * dim 64, 128 or 256. Precision as mako_attn_fwd: P rounded to the input type for P V, sums and lse of the f32

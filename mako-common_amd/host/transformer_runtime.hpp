@@ -142,8 +142,8 @@ protected:
     // each), in `rows` rows; q_pad and d_pad as in attention_tree.
     //
     // attention_paged: q [heads][q_pad][dim], o [rows][heads * dim], opt.lse [heads][rows]; row i of sequence b sees the
-    // cache rows up to ctx_len[b] + i, its own. max_new bounds a sequence's new rows, max_ctx its rows with them. Scratch
-    // "attn_paged".
+    // cache rows up to ctx_len[b] + i, its own; rows from `end` on get results of no meaning. max_new bounds a sequence's new
+    // rows, max_ctx its rows with them. Scratch "attn_paged".
     void attention_paged(gpu::Encoder*& enc, gpu::Buffer* q, const PagedCache& c, uint32_t layer, gpu::Buffer* starts,
                          gpu::Buffer* o, uint32_t rows, uint32_t heads, uint32_t max_new, uint32_t max_ctx,
                          const AttnOptions& opt = {}, uint32_t q_pad = 0);

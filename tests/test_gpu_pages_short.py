@@ -1,4 +1,5 @@
-"""A pool of pages that runs out, on the GPU: who gets room among sequences of unlike lengths in one page."""
+"""A pool of pages that runs out, on the GPU: who gets room among sequences of unlike lengths in one page, and a serving loop
+that makes its steps again once pages are free."""
 import random
 
 import pytest
@@ -7,7 +8,9 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import mako_attn as M  # noqa: E402
+import pages_ref as R  # noqa: E402
 from test_gpu_paged import gen, ints, space  # noqa: E402
+from test_gpu_pages_run import ALL, Server  # noqa: E402
 
 
 def room(table, refs, ctx, new, page):
@@ -87,3 +90,62 @@ def test_no_row_of_another_sequence_is_written(batch, beams, most, spare, in_pla
         got = rows(pool, to)
         assert torch.equal(torch.where(before, got, 0), torch.where(before, rows(old, old_t), 0))
         assert torch.equal(torch.where(fresh, got, 0), torch.where(fresh, d[:, nth].transpose(0, 1), 0))
+
+
+class Short(Server):
+    def step_in(self, new, what):
+        """A step in a pool that may run out: new rows that have room, and their attention; returns the rows left."""
+        lens = [x[0].shape[2] for x in self.sim]
+        want = room(self.table.tolist(), self.refs.tolist(), lens, new, self.page)
+        tiles, starts = self.tiles(sum(new)), [sum(new[:b]) for b in range(self.B + 1)]
+        plan = self.prepare(sum(new), max(new), max(c + n for c, n in zip(lens, new)))
+        self.launch(plan, tiles, ints(starts))
+        torch.cuda.synchronize()
+        assert self.ctx.tolist() == want, what
+        got = [e - c for c, e in zip(lens, want)]
+        for b, n in enumerate(got):
+            for x in range(2):
+                rows = torch.stack([t[1 + x][:, starts[b]:starts[b] + n] for t in tiles])
+                self.sim[b][x] = torch.cat([self.sim[b][x], rows], 2)
+        self.check_rows(what)
+        a, o, lse, _ = plan
+        pool = [torch.zeros((self.L, self.B, self.KV, self.cap, self.D), dtype=self.dt, device="cuda") for _ in range(2)]
+        for b in range(self.B):
+            for x in range(2):
+                pool[x][:, b, :, :want[b]] = self.sim[b][x]
+        for l, (q, _, _) in enumerate(tiles):
+            res = R.attention(q, pool[0][l], pool[1][l], [[b] for b in range(self.B)], lens, got, starts, scale=a.scale,
+                              max_ctx=a.max_ctx, max_new=a.max_new, out_dtype=o.dtype)
+            for b, s0, n, out, out_l, tol, ltol in res:
+                assert ((o[l, s0:s0 + n].double().view(n, self.H, self.D) - out).abs() <= tol).all(), (what, l, b)
+                assert ((lse[l, :, s0:s0 + n].t().double() - out_l).abs() <= ltol).all(), (what, l, b)
+        return [n - m for n, m in zip(new, got)]
+
+    def check_rows(self, what):
+        """What the pages hold of every sequence is its rows (a last chunk may hold pages behind them)."""
+        table = self.table.tolist()
+        for b, row in enumerate(table):
+            n = self.sim[b][0].shape[2]
+            held = -(-n // self.page)
+            assert all(0 <= e < self.pages for e in row[:held]), (what, b)
+            for x, pool in enumerate((self.k, self.v)):
+                if held:
+                    rows = pool[:, row[:held]].transpose(1, 2).reshape(self.L, self.KV, held * self.page, self.D)[:, :, :n]
+                    assert torch.equal(rows, self.sim[b][x]), (what, b)
+
+
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(8, 2, 128, "bf16"), (4, 4, 64, "f16"), (8, 1, 256, "bf16")])
+def test_steps_made_again(heads, kv, dim, dtype):
+    """Beams of unlike lengths over one page, then steps that find too few pages; ends of other sequences free some."""
+    s = Short(dim, batch=6, heads=heads, kv=kv, dim=dim, page=64, pages=9, cap=320, layers=2, dtype=dtype)
+    assert s.step_in([114, 0, 0, 0, 130, 90], "prompts") == [0] * 6  # 2, 3 and 2 pages
+    s.fork([0, 0, 0, 0, 4, 5], [114, 94, 107, 70, ALL, ALL], "beams")  # of one page: 50, 30, 43 and 6 rows
+    # two free pages: the first two beams copy, the third gets none and the last would write over its rows
+    assert s.step_in([1, 1, 1, 1, 0, 0], "two pages") == [0, 0, 1, 1, 0, 0]
+    assert s.step_in([0, 0, 1, 1, 0, 0], "none") == [0, 0, 1, 1, 0, 0]
+    assert s.step_in([20, 1, 40, 90, 1, 1], "none, some with room in their pages")[:4] == [7, 0, 40, 90]
+    s.fork([0, 1, 2, 3, 6, 5], [ALL] * 4 + [0, ALL], "one ends")  # three pages
+    assert s.step_in([7, 0, 40, 90, 0, 0], "three pages")[:4] == [0, 0, 0, 32]
+    s.fork([0, 6, 2, 3, 6, 6], [ALL, 0, ALL, ALL, 0, 0], "more end")
+    assert s.step_in([1, 0, 1, 32, 100, 0], "room for all") == [0] * 6
+    s.check_pages("the end")
