@@ -14,7 +14,10 @@
 //   (heads of 256: 128 / hq): one workgroup's four waves, 64 (32) columns each. A wave has one head; of eight, two side by
 //   side, since a second workgroup on the same keys costs their read again (16 heads of 256 over 2, a step of 16 sequences,
 //   605 MB: 143 us with two workgroups of four heads, 103 us with one of eight; 32 heads of 128 over 4 149 and 103 us).
-//   Larger groups take further workgroups (column blocks), beside each other on an XCD, whose L2 the second read hits.
+//   Larger groups, and those that 8, 4 or 2 do not divide, take further workgroups (column blocks), beside each other on an XCD.
+//   Each reads the item's K and V again, which bounds single tokens: a step of 16 with 32 or 64 heads over 8 167-198 us, with
+//   24 over 8 (three readings) 336-373, with 40 over 8 (five) 534-593; 28 over 4 (seven, of half the bytes) 401-443, 64 over 4
+//   (two) 156-171.
 // * Items of half the rows or fewer take a stream of 32 columns a wave with streaming loads (heads of 256, in calls of such
 //   items alone: tiles of 32 keys, three of them in flight).
 // * Lengths are known on the device only, so every workgroup works out its share of the work (paged_split.hpp): ranges of
@@ -24,11 +27,16 @@
 //   Contexts that are too short for a second launch (max_ctx) take whole items and none.
 // * A piece of several rows ends with a look at the v that some of its rows do not see (hidden_not_finite).
 //
-// us a call on one MI355X, 32 heads of 128 over 8: one token over 391 rows (16 heads) 10.7; 16 single tokens over 1.21 GB 184
-// (6.5 TB/s); 11 single tokens beside two chunks of up to 1333 rows, contexts up to 12001, 201-206 (880 TFLOP/s); 512 rows
-// behind 32256 207-219 (1050 to 1100 TFLOP/s). 16 heads of 256 over 2: 16 single tokens over 605 MB 103 (5.9 TB/s), four chunks
-// of up to 300 rows behind up to 16000 156-159 (975 TFLOP/s). paged_merge: 14-17 us of kernel for 57 MB of pieces, 5 for the
-// single tokens'.
+// P meets V in the input type, as in the prefill streams: a second product for what that leaves off would be half as many matrix
+// instructions again. Outputs are off by 2.9e-4 (f16) and 2.3e-3 (bf16) of their size, where rounded ones are by 2.1e-4 and 1.7e-3.
+//
+// us a call on one MI355X, 32 heads of 128 over 8: one token over 391 rows (16 heads) 10.8 (with max_ctx past 832, and so a join,
+// 15); 16 single tokens over 1.02 to 1.21 GB 159-187 (6.4 to 6.5 TB/s); 11 single tokens beside two chunks of up to 1333 rows,
+// contexts up to 12001, 210-272 over four sets of lengths (800 to 870 TFLOP/s); 512 rows behind 32256 218-233 (1050 to 1110);
+// a prompt of 4096 rows 112 (865), of 1531 25-28. 16 heads of 256 over 2: 16 single tokens over 605 MB 103 (5.9 TB/s), four
+// chunks of up to 300 rows behind up to 16000 163-207 (930 to 960), a prompt of 4096 rows 113 (855). 16 heads of 64 over 16: 16
+// single tokens over up to 640 MB 88-103 (6.0 to 6.2 TB/s). paged_merge: 14-18 us of kernel for 57 MB of pieces (heads of 256
+// 12), 5 for the single tokens'.
 #include <algorithm>
 
 #include "attn_paged_asm.inc"

@@ -2,21 +2,22 @@
 // and the compaction of the pool. All counts are on the device; what a launch is sized by are the arguments' bounds.
 //
 // Figures: us of kernel on one MI355X. What bounds the small calls is their chain of dependent loads and the launch; a pass of
-// the smallest kernel takes 6.3 us of a stream's time with its host call.
+// the smallest kernel takes 5.7 to 6.4 us with its host call (2.2 in a graph).
 //
 // * pages_write: a wave a new row. Its sequence is found by counting the starts up to it (64 at a time, a ballot), its page
 //   by one load of the table; the row's 16-byte chunks of all kv heads, k and v, are loaded before either has come. 64 single
-//   rows of 8 heads of 128 2.8-3.3 us; a long prompt's (12.6 MB read, and written) 6.8-7.7.
+//   rows of 8 heads of 128 2.9-3.3 us; a long prompt's (12.6 MB read, and written) 7.0-7.5.
 // * reserve_plan, one workgroup: the entries that need a page are counted a sequence (a thread each, a wave where a sequence
 //   brings many), summed over the sequences, and the free pages looked for from the lowest number on until there are enough,
 //   so the look ends early in a pool that is kept compact. Sequences that append to one shared page meet in a hash table in
 //   LDS, by counts and maxima, which the order of the threads does not change. copy_pages then copies the shared pages' rows.
-//   64 sequences' step 4.8 us; 64 beams of 16 prompts 6.0, and 5.0 for the copies.
+//   64 sequences' step 4.8-5.1 us; 64 beams of 16 prompts 5.9-6.1, and 3.7-4.6 for the copies. Where the pages run out, the
+//   sequences that did not get the copy of a shared page are looked at once more: nobody writes where one of them has rows.
 // * fork_rows: a workgroup a new sequence; the holders' counts change by integer atomics, only where old and new entry differ.
-//   1024 sequences of up to 129 pages 3.8 us after the copies' 2.6; fork_small 3.9-4.2 for 64 beams.
+//   1024 sequences of up to 128 pages 3.1-3.6 us after the copies' 2.2-2.5; fork_small 4.0-4.2 for 64 beams.
 // * compact_plan, one workgroup: used pages counted, then holes and sources ranked by one pass of sums over the threads; a
 //   source meets its hole by rank, as the holes all lie before it. compact_move copies the pages and renumbers the tables:
-//   4096 pages of two layers 7.8 us, then 201-208 (1.07 GB at 5.1 TB/s, a large copy's rate); 512 pages 5.4 and 10.5.
+//   4096 pages of two layers 7.8-8.2 us, then 202-209 (1.07 GB at 5.1 TB/s, a large copy's rate); 512 pages 5.4-5.7 and 9-11.
 #include <algorithm>
 
 #include "pages_common.hpp"
@@ -32,7 +33,7 @@ constexpr uint32_t kMaxSeqs = 4096;   // sequences that reserve_plan takes
 constexpr uint32_t kSlots = 2 * kMaxSeqs;
 constexpr uint32_t kListHere = 2048;  // free pages that reserve_plan lists in LDS
 constexpr uint32_t kLook = 8;         // refs a thread looks at a round
-constexpr uint64_t kForkSmall = 4096; // table entries that one workgroup forks alone (64 x 32: 6.7 us a pass, by rows 9.3)
+constexpr uint64_t kForkSmall = 4096; // table entries that one workgroup forks alone (64 x 32: 6.4 us a pass, by rows 9.0)
 constexpr uint32_t kFew = 2;          // entries of a sequence that one thread goes through alone
 
 // ---- write ---------------------------------------------------------------------------------------------------------
@@ -138,7 +139,7 @@ __device__ __forceinline__ void load_refs(const uint32_t* refs, uint32_t p, uint
 }
 
 // Arrays that a call copies before it changes the copies: by the planning workgroup itself where they are short
-// (kCopyInPlan words; with a launch 64 sequences' reservation among 4096 pages takes 2.1 us more), else by copy_words.
+// (kCopyInPlan words; with a launch 64 sequences' reservation among 4096 pages takes 2.3 us more), else by copy_words.
 struct CopyWords {
     const uint32_t* from[3];
     uint32_t* to[3];
