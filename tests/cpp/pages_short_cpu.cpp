@@ -232,11 +232,11 @@ int main()
 {
     bool good = two(50, 30, 1, {50, 30}) && two(50, 30, 2, {51, 31}) && two(50, 50, 1, {50, 51}) && two(50, 49, 1, {50, 49}) &&
                 two(30, 50, 1, {30, 51}) && two(64, 30, 1, {64, 30}) && two(64, 30, 2, {65, 30}) && two(64, 30, 3, {65, 31});
-    for (uint32_t round = 0; good && round < 8; ++round) {
+    for (uint32_t round = 0; good && round < 3; ++round) {
         const uint32_t batch = 2 + upto(38);
-        good &= loop(batch, batch / 2 + upto(2 * batch), 12, round % 2 ? 3 : 90);
+        good &= loop(batch, batch / 2 + upto(2 * batch), 9, round % 2 ? 3 : 90);
     }
-    good = good && loop(1100, 900, 5, 40) && loop(2100, 1700, 5, 2);
+    good = good && loop(1030, 700, 4, 4);
     std::puts(good ? "all passed" : "FAILED");
     return good ? 0 : 1;
 }

@@ -5,10 +5,10 @@ import pytest
 import paged_run as R
 
 
-@pytest.mark.parametrize("past", [1, 64, 100, 4096])
+@pytest.mark.parametrize("past", [1, 100])
 @pytest.mark.parametrize("d,rows,kt", [(64, 64, 64), (64, 32, 64), (128, 64, 64), (128, 32, 64), (256, 64, 64), (256, 32, 32)])
 def test_first_tiles(d, rows, kt, past, monkeypatch):
-    """A piece of 2^32 bytes of K and `past` keys, in whose first five tiles of 64 keys the waves' rows end."""
+    """A piece of 2^32 bytes of K and `past` keys, in whose first three tiles of 64 keys the waves' products end."""
     class Emu(R.Emu):
         def run_wg(self, waves):
             for w in waves:
@@ -18,20 +18,20 @@ def test_first_tiles(d, rows, kt, past, monkeypatch):
             super().run_wg(waves)
 
     monkeypatch.setattr(R, "Emu", Emu)
-    r = R.run(heads=4, kv=1, n=3, ctx=900, page=64, d=d, wave_rows=rows, cut=(0, 5), seed=3)
+    r = R.run(heads=1, kv=1, n=3, ctx=900, page=64, d=d, wave_rows=rows, cut=(0, 3), seed=3)
     assert r["out_bad"] == 0 and r["lse_bad"] == 0 and r["early_reads"] == 0, r
 
 
 @pytest.mark.parametrize("d,rows,kt", [(64, 64, 64), (64, 32, 64), (128, 64, 64), (128, 32, 64), (256, 64, 64), (256, 32, 32)])
-@pytest.mark.parametrize("keys", [1, 31, 32, 33, 63])
+@pytest.mark.parametrize("keys", [1, 33])
 def test_last_tiles(d, rows, kt, keys, monkeypatch):
-    """The last tiles of a piece, of `keys` keys in the last one, whose count has passed 2^32 bytes: five tiles from there on."""
+    """The last tiles of a piece, of `keys` keys in the last one, whose count has passed 2^32 bytes: three tiles from there on."""
     class Emu(R.Emu):
         def run_wg(self, waves):
             for w in waves:
-                assert int(w.s[R.SREG["kn"]]) == (4 * 64 + keys) * 2 * d  # (2^32 bytes before them leave it)
+                assert int(w.s[R.SREG["kn"]]) == (2 * 64 + keys) * 2 * d  # (2^32 bytes before them leave it)
             super().run_wg(waves)
 
     monkeypatch.setattr(R, "Emu", Emu)
-    r = R.run(heads=4, kv=1, n=1, ctx=8 * 64 + keys - 1, page=64, d=d, wave_rows=rows, cut=(4, 9), seed=3)
+    r = R.run(heads=1, kv=1, n=1, ctx=8 * 64 + keys - 1, page=64, d=d, wave_rows=rows, cut=(6, 9), seed=3)
     assert r["out_bad"] == 0 and r["lse_bad"] == 0 and r["early_reads"] == 0, r
